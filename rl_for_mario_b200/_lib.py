@@ -1,4 +1,4 @@
-"""ctypes binding of the C-ABI library (include/dt_attn.h).
+"""ctypes binding of the C-ABI library (include/dt_attn.h, include/dt_train.h).
 
 The library is loaded from ``rl_for_mario_b200/_native/libdt_attn_sm100.so``.
 There is no fallback: if the library is missing every call raises
@@ -26,9 +26,10 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
 _U = ctypes.c_uint32
 
-# Exported symbol -> (restype, argtypes).  Kept in the order of include/dt_attn.h.
+# Exported symbol -> (restype, argtypes).  Kept in the order of include/dt_attn.h, then include/dt_train.h.
 SIGNATURES = {
     "dt_version": (_I, []),
     "dt_last_error": (ctypes.c_char_p, []),
@@ -56,6 +57,16 @@ SIGNATURES = {
     "dt_nes_set_actions": (_I, [_P, _I, _P, _P, _I, _P]),
     "dt_nes_observe": (_I, [_P, _I, _P, _P, _I, _P]),
     "dt_nes_env_update": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _U, _P, _U, _P]),
+    "dt_attn_train_forward": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _L, _L, _L, _L, _L, _L, _L, _L, _L,
+                                   _L, _L, _L, _F, _D, _P, _U, _I, _P]),
+    "dt_attn_train_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _F, _D, _P,
+                                    _U, _I, _P]),
+    "dt_residual_norm_forward": (_I, [_P, _L, _P, _L, _P, _L, _L, _P, _P, _P, _P, _P, _L, _I, _F, _F, _D, _P, _U, _I,
+                                      _P]),
+    "dt_residual_norm_workspace": (_L, [_L, _I, _L, _I]),
+    "dt_residual_norm_backward": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                       _L, _L, _I, _F, _F, _D, _P, _U, _I, _P]),
+    "dt_dropout": (_I, [_P, _L, _P, _L, _P, _L, _L, _I, _D, _P, _U, _I, _P]),
 }
 
 

@@ -133,6 +133,27 @@ int encode_pages(CUtensorMap* map, const void* base, bool is16, int D, uint64_t 
 
 }  // namespace
 
+namespace dtk {
+
+int api_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int api_device(int** status, int* cc_major, int* num_sms) {
+  int dev = 0;
+  const int rc = device_setup(&dev, status);
+  if (rc) return rc;
+  *cc_major = g_cc_major[dev];
+  *num_sms = g_num_sms[dev];
+  return DT_OK;
+}
+
+}  // namespace dtk
+
 extern "C" {
 
 int dt_version(void) { return (0 << 16) | 1; }

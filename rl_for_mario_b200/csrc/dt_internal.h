@@ -189,6 +189,85 @@ cudaError_t launch_decode_sm100(const DecodeParams& prm, const CUtensorMap& kmap
                                 bool bf16, int grid, cudaStream_t stream);
 
 
+// ---- training operators (capi_train.cu) ----
+
+// Error text and device lookup of the C ABI (capi.cu): api_fail records the
+// message for dt_last_error and returns the code; api_device gives the current
+// device's status word, major compute capability and SM count.
+int api_fail(int code, const char* fmt, ...);
+int api_device(int** status, int* cc_major, int* num_sms);
+
+struct DropoutParams {
+  const void* x;
+  const void* residual;  // or null
+  void* y;
+  long long x_stride, res_stride, y_stride;  // of rows, in elements
+  long long rows;
+  int cols;
+  const long long* rng;  // (seed, step)
+  uint32_t threshold, site;
+  float inv_keep;
+};
+cudaError_t launch_dropout_sm100(const DropoutParams& p, int dtype, int num_sms, cudaStream_t st);
+
+struct ResidualNormParams {
+  const void* x;
+  const void* residual;  // or null
+  const void* gate;      // or null: 1
+  const void* w_pre;
+  const void* w_post;  // or null: no norm of x
+  void* h;             // forward outputs, rows of H without gaps
+  void* n;
+  float* stats;    // [M, 2] reciprocal roots: post, pre
+  const void* dh;  // backward inputs, either may be null: zero
+  const void* dn;
+  void* dx;  // backward outputs
+  void* dresidual;
+  void* dw_pre;
+  void* dw_post;
+  void* dgate;
+  float* part_pre;  // [blocks, H] partial sums
+  float* part_post;
+  float* part_gate;  // [chunks, H]
+  long long x_stride, res_stride, gate_stride, dh_stride, dn_stride;
+  long long M, gate_rows;  // rows that share one row of the gate
+  long long chunks, chunk_rows, chunks_per_span, span_rows;
+  int H, wpr;
+  const long long* rng;
+  uint32_t threshold, site;  // threshold 0: no dropout
+  float inv_keep, alpha, eps;
+};
+struct ResidualNormPlan {
+  long long chunks, chunk_rows, chunks_per_span, span_rows, grid;
+};
+ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, int num_sms);
+cudaError_t launch_residual_norm_fwd_sm100(ResidualNormParams p, int dtype, int num_sms, cudaStream_t st);
+cudaError_t launch_residual_norm_bwd_sm100(ResidualNormParams p, const ResidualNormPlan& plan, int dtype,
+                                           cudaStream_t st);
+
+struct AttnTrainParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;            // forward output, backward input
+  float* lse;         // [B, Hq, S], log2 units; +inf for a row without keys
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* delta;            // [B, Hq, S]
+  const int32_t* pad_len;  // [B] or null
+  long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh;
+  long long do_sb, do_ss, do_sh, dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
+  int B, S, Hq, Hkv, R;
+  float scale;
+  const long long* rng;
+  uint32_t threshold, site;  // threshold 0: no dropout
+  float inv_keep;
+};
+cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, int D, bool bf16, int num_sms, cudaStream_t st);
+cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, int D, bool bf16, int num_sms, cudaStream_t st);
+
 // Batched NES emulation (nes_sm100.cu).  op: 0 run frames, 1 reset, 2 buttons,
 // 3 observation, 4 environment bookkeeping.  Unused fields may be left zero.
 struct NesLaunch {

@@ -1,0 +1,63 @@
+// The dropout generator of the training operators: a counter-based mask that
+// is never stored.  Forward and backward evaluate the same function of
+// (seed, step, site, element), so a mask costs arithmetic and no memory.
+//
+// Philox4x32 with seven rounds (Salmon, Moraes, Dror, Shaw, "Parallel random
+// numbers: as easy as 1, 2, 3", SC 2011: seven is the fewest rounds of this
+// width that pass BigCrush).  key = the 64-bit seed, counter = (block low,
+// block high, step, site).  One call gives eight 16-bit words, one for each of
+// eight consecutive elements of a row; element (row, col) of a tensor whose
+// rows have n columns uses word col % 8 of block row * ceil(n / 8) + col / 8.
+// An element stays iff its word >= round(p * 65536), so p is met to 2^-17 and
+// survivors are scaled by the exact reciprocal of the rounded rate.
+#pragma once
+
+#include <cstdint>
+
+namespace dtk {
+
+struct DropKey {
+  uint32_t k0, k1, step, site;
+};
+
+// rng points at two 64-bit words, (seed, step); read on the device so that a
+// captured graph sees the step of its replay.
+__device__ __forceinline__ DropKey drop_key(const long long* __restrict__ rng, uint32_t site) {
+  const unsigned long long seed = (unsigned long long)__ldg(rng), step = (unsigned long long)__ldg(rng + 1);
+  return DropKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)step, site};
+}
+
+__device__ __forceinline__ uint4 philox7(const DropKey& k, unsigned long long block) {
+  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = k.step, c3 = k.site;
+  uint32_t k0 = k.k0, k1 = k.k1;
+#pragma unroll
+  for (int r = 0; r < 7; ++r) {
+    const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// Bit i set: element i of the block stays.  threshold in [1, 65535].
+__device__ __forceinline__ uint32_t keep_bits(const DropKey& k, unsigned long long block, uint32_t threshold) {
+  const uint4 w = philox7(k, block);
+  // The high word of x stays iff x >= threshold << 16; the low one is moved up first.
+  const uint32_t th = threshold << 16;
+  uint32_t m = 0;
+  m |= (w.x << 16) >= th ? 1u : 0u;
+  m |= w.x >= th ? 2u : 0u;
+  m |= (w.y << 16) >= th ? 4u : 0u;
+  m |= w.y >= th ? 8u : 0u;
+  m |= (w.z << 16) >= th ? 16u : 0u;
+  m |= w.z >= th ? 32u : 0u;
+  m |= (w.w << 16) >= th ? 64u : 0u;
+  m |= w.w >= th ? 128u : 0u;
+  return m;
+}
+
+}  // namespace dtk

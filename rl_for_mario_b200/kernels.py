@@ -504,3 +504,292 @@ def rmsnorm_qkv(x: Tensor, w_fused: Tensor, eps: float, out: Optional[Tensor] = 
                                          rope_cols, head_dim, _dtype_code(x), _stream_ptr(x.device))
     _lib.check("dt_rmsnorm_qkv_rope", rc)
     return out
+
+
+# ------------------------------------------------------------------ training operators
+def _same_device(first: Tensor, *ts: Optional[Tensor]) -> torch.device:
+    """The device that every tensor is on (CUDA)."""
+    _require_cuda(first, *ts)
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors are on different devices ({first.device} and {t.device})")
+    return first.device
+
+
+class _On:
+    """Makes ``device`` current around a launch when it is not (the library
+    launches on the current device)."""
+
+    __slots__ = ("want", "had")
+
+    def __init__(self, device: torch.device):
+        self.want = device.index
+
+    def __enter__(self):
+        self.had = torch.cuda.current_device()
+        if self.had != self.want:
+            torch.cuda.set_device(self.want)
+
+    def __exit__(self, *exc):
+        if self.had != self.want:
+            torch.cuda.set_device(self.had)
+
+
+def _check_dropout(p: float, rng: Optional[Tensor], site: int) -> float:
+    """The dropout arguments shared by the training operators; returns p as a float.
+
+    ``rng``: int64 [2] device tensor (seed, step), see training.DropoutState;
+    ``site``: a number of its own for each place of a model that drops."""
+    p = float(p)
+    if not 0.0 <= p < 1.0 or round(p * 65536) >= 65536:
+        raise ValueError(f"dropout p must lie in [0, 1), below 1 - 2^-17 (got {p})")
+    if p > 0.0:
+        if rng is None:
+            raise ValueError("dropout needs rng, an int64 [2] device tensor (seed, step)")
+        if rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
+            raise ValueError("rng must be a contiguous int64 tensor of shape [2] (seed, step)")
+    if not 0 <= int(site) < 2 ** 32:
+        raise ValueError(f"site must lie in [0, 2^32) (got {site})")
+    return p
+
+
+def _rows16(t: Tensor) -> Tensor:
+    """t itself when the attention kernels can read it ([B, S, H, D], contiguous D, strides
+    multiples of 8, 16-byte aligned), else a contiguous copy."""
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % 8 == 0 for s in t.stride()[:3]):
+        return t
+    return t.contiguous()
+
+
+def _check_attn_train(q: Tensor, k: Tensor, v: Tensor, pad_len: Optional[Tensor], scale: Optional[float]):
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("attn_train takes q [B, S, Hq, D] and k, v [B, S, Hkv, D]")
+    B, S, Hq, D = q.shape
+    Hkv = k.shape[2]
+    if k.shape != (B, S, Hkv, D) or v.shape != k.shape:
+        raise ValueError(f"k/v shapes {tuple(k.shape)}, {tuple(v.shape)} do not match q {tuple(q.shape)}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError("q, k, v must share a dtype")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"attn_train takes bf16 or fp16 (got {q.dtype})")
+    if pad_len is not None:
+        if pad_len.shape != (B,):
+            raise ValueError(f"pad_len must be [{B}] (got {tuple(pad_len.shape)})")
+        pad_len = pad_len.to(torch.int32).contiguous()
+    if scale is not None and not scale > 0:
+        raise ValueError(f"scale must be positive (got {scale})")
+    return pad_len
+
+
+def attn_train_forward(q: Tensor, k: Tensor, v: Tensor, pad_len: Optional[Tensor] = None,
+                       scale: Optional[float] = None, p: float = 0.0, rng: Optional[Tensor] = None,
+                       site: int = 0) -> Tuple[Tensor, Tensor]:
+    """Causal GQA attention for training: q [B,S,Hq,D], k/v [B,S,Hkv,D] (rotated, bf16 / fp16) ->
+    (out [B,S,Hq,D], lse [B,Hq,S] fp32, the backward call's input).
+
+    pad_len [B] int32: leading padding positions.  Their rows of out are zeros and they pass no
+    gradient (attn_prefill, the inference form, gives them the reference's mean of V).  p, rng,
+    site: dropout on the attention weights, see _check_dropout."""
+    dev = _same_device(q, k, v, pad_len, rng)
+    pad_len = _check_attn_train(q, k, v, pad_len, scale)
+    p = _check_dropout(p, rng, site)
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    B, S, Hq, D = q.shape
+    Hkv = k.shape[2]
+    out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, Hq, S), dtype=torch.float32, device=dev)
+    if out.numel() == 0:
+        return out, lse
+    with _On(dev):
+        rc = _lib.load().dt_attn_train_forward(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(pad_len), B, S, Hq, Hkv, D, *q.stride()[:3],
+            *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], float(scale) if scale is not None else 0.0, p,
+            _ptr(rng), int(site), _dtype_code(q), _stream_ptr(dev))
+    _lib.check("dt_attn_train_forward", rc)
+    return out, lse
+
+
+def attn_train_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,
+                        pad_len: Optional[Tensor] = None, scale: Optional[float] = None, p: float = 0.0,
+                        rng: Optional[Tensor] = None, site: int = 0,
+                        grads: Optional[Tuple[Tensor, Tensor, Tensor]] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """Gradient of attn_train_forward: (dq, dk, dv) from dout and the forward call's arguments and
+    results (the same rng contents, site and p).  ``grads``: tensors to write dq, dk and dv into
+    (for instance the parts of one [B, S, Hq + 2 Hkv, D] gradient)."""
+    dev = _same_device(q, k, v, dout, out, lse, pad_len, rng)
+    pad_len = _check_attn_train(q, k, v, pad_len, scale)
+    p = _check_dropout(p, rng, site)
+    B, S, Hq, D = q.shape
+    Hkv = k.shape[2]
+    if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:
+        raise ValueError("dout and out must have q's shape and dtype")
+    if lse.shape != (B, Hq, S) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError("lse must be the forward call's [B, Hq, S] fp32 tensor")
+    q, k, v, dout, out = (_rows16(t) for t in (q, k, v, dout, out))
+    if grads is None:
+        grads = (torch.empty((B, S, Hq, D), dtype=q.dtype, device=dev),
+                 torch.empty((B, S, Hkv, D), dtype=q.dtype, device=dev),
+                 torch.empty((B, S, Hkv, D), dtype=q.dtype, device=dev))
+    dq, dk, dv = grads
+    _same_device(q, dq, dk, dv)
+    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if t.shape != like.shape or t.dtype != q.dtype or (t.numel() and _rows16(t) is not t):
+            raise ValueError(f"{name} must be a {tuple(like.shape)} {q.dtype} tensor with contiguous D, 16-byte aligned "
+                             "rows and strides that are multiples of 8")
+    if dq.numel() == 0:
+        return dq, dk, dv
+    delta = torch.empty((B, Hq, S), dtype=torch.float32, device=dev)
+    strides = [s for t in (q, k, v, out, dout, dq, dk, dv) for s in t.stride()[:3]]
+    with _On(dev):
+        rc = _lib.load().dt_attn_train_backward(
+            _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(delta), _ptr(dq), _ptr(dk), _ptr(dv),
+            _ptr(pad_len), B, S, Hq, Hkv, D, (_lib._L * 24)(*strides), float(scale) if scale is not None else 0.0, p,
+            _ptr(rng), int(site), _dtype_code(q), _stream_ptr(dev))
+    _lib.check("dt_attn_train_backward", rc)
+    return dq, dk, dv
+
+
+def _rows2d(t: Tensor) -> Tensor:
+    """t as a [rows, K] view with a contiguous last dimension (a copy when no view exists)."""
+    t2 = t.reshape(-1, t.shape[-1])
+    return t2 if t2.stride(1) == 1 or t2.shape[1] == 1 else t2.contiguous()
+
+
+def _gate_rows(gate: Optional[Tensor], x: Tensor) -> Tuple[Optional[Tensor], int]:
+    """The gate as [G, H] rows and the number of consecutive rows of x that share each: a gate of
+    shape [H], x's own shape, or x's shape with trailing ones before H ([B, 1, H] for [B, S, H])."""
+    if gate is None:
+        return None, 0
+    H = x.shape[-1]
+    lead = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape[:-1])
+    if gate.dim() > x.dim() or gate.shape[-1] != H:
+        raise ValueError(f"gate {tuple(gate.shape)} does not broadcast to x {tuple(x.shape)}")
+    shared, shares = 1, False
+    for g, n in zip(lead, x.shape[:-1]):
+        if g == n and not (shares and n != 1):
+            continue
+        if g != 1:
+            raise ValueError(f"gate {tuple(gate.shape)} must be x's shape {tuple(x.shape)} with ones in trailing places "
+                             "before the last")
+        shares = True
+        shared *= n
+    return _rows2d(gate), shared
+
+
+def _check_residual_norm(x, residual, pre_weight, post_weight, gate):
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have a last dimension")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+    for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
+        if w is not None and (w.shape != x.shape[-1:] or not w.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous [{x.shape[-1]}] tensor")
+    for name, t in (("residual", residual), ("pre_weight", pre_weight), ("post_weight", post_weight), ("gate", gate)):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError(f"{name} must have x's dtype {x.dtype} (got {t.dtype})")
+
+
+def residual_norm_forward(x: Tensor, residual: Optional[Tensor], pre_weight: Tensor, eps: float,
+                          post_weight: Optional[Tensor] = None, gate: Optional[Tensor] = None, alpha: float = 1.0,
+                          p: float = 0.0, rng: Optional[Tensor] = None, site: int = 0) -> Tuple[Tensor, Tensor, Tensor]:
+    """What stands between two products of a block, in one pass over x [..., H]:
+
+        u = RMSNorm(x) * post_weight         (u = x without post_weight)
+        h = residual + alpha * gate * dropout(u)
+        n = RMSNorm(h) * pre_weight
+
+    Returns (h, n, stats); stats [rows, 2] fp32 is the backward call's input.  ``gate``: [H], x's
+    shape, or x's shape with ones in trailing places before H (a gate of each sample).  bf16, fp16
+    or fp32, H <= 8192; fp32 arithmetic, each output rounded once, n from the unrounded h."""
+    dev = _same_device(x, residual, pre_weight, post_weight, gate, rng)
+    _check_residual_norm(x, residual, pre_weight, post_weight, gate)
+    p = _check_dropout(p, rng, site)
+    g2, gate_rows = _gate_rows(gate, x)
+    x2 = _rows2d(x)
+    r2 = None if residual is None else _rows2d(residual)
+    M, H = x2.shape
+    h, n = torch.empty(x.shape, dtype=x.dtype, device=dev), torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((M, 2), dtype=torch.float32, device=dev)
+    if M == 0:
+        return h, n, stats
+    with _On(dev):
+        rc = _lib.load().dt_residual_norm_forward(
+            _ptr(x2), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(g2),
+            0 if g2 is None else g2.stride(0), gate_rows, _ptr(pre_weight), _ptr(post_weight), _ptr(h), _ptr(n),
+            _ptr(stats), M, H, float(alpha), float(eps), p, _ptr(rng), int(site), _dtype_code(x), _stream_ptr(dev))
+    _lib.check("dt_residual_norm_forward", rc)
+    return h, n, stats
+
+
+def residual_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], x: Tensor, residual: Optional[Tensor],
+                           pre_weight: Tensor, stats: Tensor, post_weight: Optional[Tensor] = None,
+                           gate: Optional[Tensor] = None, alpha: float = 1.0, p: float = 0.0,
+                           rng: Optional[Tensor] = None, site: int = 0):
+    """Gradient of residual_norm_forward from dh and dn (either may be None: zero):
+    (dx, dresidual, dpre_weight, dpost_weight, dgate); the last two are None without their inputs.
+    Sums over rows are fp32 and in a fixed order."""
+    dev = _same_device(x, dh, dn, residual, pre_weight, post_weight, gate, stats, rng)
+    _check_residual_norm(x, residual, pre_weight, post_weight, gate)
+    p = _check_dropout(p, rng, site)
+    for name, t in (("dh", dh), ("dn", dn)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{name} must have x's shape and dtype")
+    g2, gate_rows = _gate_rows(gate, x)
+    x2 = _rows2d(x)
+    M, H = x2.shape
+    if stats.shape != (M, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError("stats must be the forward call's [rows, 2] fp32 tensor")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dres = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dpost = None if post_weight is None else torch.empty_like(post_weight)
+    dgate = None if gate is None else torch.empty(gate.shape, dtype=x.dtype, device=dev)
+    if M == 0 or (dh is None and dn is None):
+        for t in (dx, dres, dpost, dgate):
+            if t is not None:
+                t.zero_()
+        return dx, dres, torch.zeros_like(pre_weight), dpost, dgate
+    dpre = torch.zeros_like(pre_weight) if dn is None else torch.empty_like(pre_weight)
+    r2, dh2, dn2 = (None if t is None else _rows2d(t) for t in (residual, dh, dn))
+    lib = _lib.load()
+    with _On(dev):
+        size = lib.dt_residual_norm_workspace(M, H, gate_rows, 0 if post_weight is None else 1)
+        if size < 0:
+            _lib.check("dt_residual_norm_workspace", -size)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        rc = lib.dt_residual_norm_backward(
+            _ptr(dh2), 0 if dh2 is None else dh2.stride(0), _ptr(dn2), 0 if dn2 is None else dn2.stride(0), _ptr(x2),
+            x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(g2), 0 if g2 is None else g2.stride(0),
+            gate_rows, _ptr(pre_weight), _ptr(post_weight), _ptr(stats), _ptr(dx), _ptr(dres), _ptr(dpre), _ptr(dpost),
+            _ptr(dgate), _ptr(ws), size, M, H, float(alpha), 0.0, p, _ptr(rng), int(site), _dtype_code(x),
+            _stream_ptr(dev))
+    _lib.check("dt_residual_norm_backward", rc)
+    return dx, dres, dpre, dpost, dgate
+
+
+def dropout_forward(x: Tensor, p: float, rng: Optional[Tensor], site: int = 0,
+                    residual: Optional[Tensor] = None) -> Tensor:
+    """residual + dropout(x) (residual None: dropout(x)) with a mask that is a function of rng, site
+    and each element's place in x [..., H] and is never stored.  bf16, fp16 or fp32."""
+    dev = _same_device(x, rng, residual)
+    if x.dim() < 1 or x.dtype not in _DTYPES:
+        raise TypeError(f"dropout takes bf16, fp16 or fp32 tensors of one or more dimensions (got {x.dtype})")
+    p = _check_dropout(p, rng, site)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("residual must have x's shape and dtype")
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if x.numel() == 0:
+        return y
+    x2, r2 = _rows2d(x), None if residual is None else _rows2d(residual)
+    M, H = x2.shape
+    with _On(dev):
+        rc = _lib.load().dt_dropout(_ptr(x2), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(y), H, M,
+                                    H, p, _ptr(rng), int(site), _dtype_code(x), _stream_ptr(dev))
+    _lib.check("dt_dropout", rc)
+    return y
+
+
+def dropout_backward(dy: Tensor, p: float, rng: Optional[Tensor], site: int = 0) -> Tensor:
+    """Gradient of dropout_forward with respect to x (its residual's gradient is dy itself)."""
+    return dropout_forward(dy, p, rng, site)

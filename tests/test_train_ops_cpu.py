@@ -1,0 +1,123 @@
+"""Refusals of the training operators that need no GPU: entry points and wrappers check their
+arguments before any device work.  And the generator's published properties on the CPU."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import train_ref as ref
+
+
+def test_entry_points_refuse_bad_arguments_without_a_gpu():
+    from rl_for_mario_b200 import _lib
+
+    lib = _lib.load()
+    s12, a = [256, 64, 64] * 4, 4096  # any aligned non-null address: nothing is read before the device check
+
+    def fwd(q=a, S=8, Hq=4, Hkv=2, D=32, strides=s12, p=0.0, rng=None, dtype=0, B=1):
+        return lib.dt_attn_train_forward(q, a, a, a, a, None, B, S, Hq, Hkv, D, *strides, 0.0, p, rng, 0, dtype, None)
+
+    cases = [(dict(q=None), "null", _lib.DT_ERR_INVALID), (dict(S=0), "positive", _lib.DT_ERR_INVALID),
+             (dict(Hkv=3), "divisible", _lib.DT_ERR_INVALID), (dict(D=48), "head_dim", _lib.DT_ERR_UNSUPPORTED),
+             (dict(dtype=2), "dtype", _lib.DT_ERR_UNSUPPORTED), (dict(q=a + 2), "aligned", _lib.DT_ERR_INVALID),
+             (dict(strides=[257] + s12[1:]), "multiple of 8", _lib.DT_ERR_INVALID),
+             (dict(strides=[0] + s12[1:]), "multiple of 8", _lib.DT_ERR_INVALID),
+             (dict(p=1.0), "p must lie", _lib.DT_ERR_INVALID), (dict(p=-0.1), "p must lie", _lib.DT_ERR_INVALID),
+             (dict(p=float("nan")), "p must lie", _lib.DT_ERR_INVALID),
+             (dict(p=0.999995), "rounds to 1", _lib.DT_ERR_INVALID), (dict(p=0.1), "null rng", _lib.DT_ERR_INVALID),
+             (dict(p=0.1, rng=a + 4), "8-byte", _lib.DT_ERR_INVALID),
+             (dict(B=1 << 30, S=1 << 20), "too many", _lib.DT_ERR_UNSUPPORTED)]
+    for kw, text, code in cases:
+        assert fwd(**kw) == code and text.encode() in lib.dt_last_error(), kw
+    s24 = (_lib._L * 24)(*([256, 64, 64] * 8))
+    assert lib.dt_attn_train_backward(a, a, a, a, a, a, None, a, a, a, None, 1, 8, 4, 2, 32, s24, 0.0, 0.0, None, 0, 0,
+                                      None) == _lib.DT_ERR_INVALID
+    assert lib.dt_attn_train_backward(a, a, a, a, a, a, a, a + 8, a, a, None, 1, 8, 4, 2, 32, s24, 0.0, 0.0, None, 0,
+                                      0, None) == _lib.DT_ERR_INVALID
+
+    def norm(x=a, w=a, gate=None, gate_rows=0, M=4, H=8, dtype=0, h=a, p=0.0):
+        return lib.dt_residual_norm_forward(x, 8, a, 8, gate, 8, gate_rows, w, None, h, a, a, M, H, 1.0, 1e-5, p, None,
+                                            0, dtype, None)
+
+    for kw in (dict(x=None), dict(w=None), dict(h=None), dict(M=0), dict(H=0), dict(gate=a, gate_rows=3),
+               dict(gate=a, gate_rows=0), dict(x=a + 1), dict(p=0.1), dict(dtype=1, x=a + 1)):
+        assert norm(**kw) == _lib.DT_ERR_INVALID, kw
+    assert norm(H=8193) == _lib.DT_ERR_UNSUPPORTED and norm(dtype=5) == _lib.DT_ERR_UNSUPPORTED
+    assert lib.dt_residual_norm_workspace(4, 8193, 0, 0) < 0 and lib.dt_residual_norm_workspace(4, 8, 3, 0) < 0
+    assert lib.dt_residual_norm_backward(None, 8, None, 8, a, 8, a, 8, None, 0, 0, a, None, a, a, a, a, None, None, a,
+                                         1 << 20, 4, 8, 1.0, 0.0, 0.0, None, 0, 0, None) == _lib.DT_ERR_INVALID
+    for kw in (dict(x=None), dict(y=None), dict(rows=0), dict(cols=0), dict(x=a + 1)):
+        d = dict(x=a, y=a, rows=4, cols=8, **{})
+        d.update(kw)
+        assert lib.dt_dropout(d["x"], 8, None, 0, d["y"], 8, d["rows"], d["cols"], 0.0, None, 0, 0,
+                              None) == _lib.DT_ERR_INVALID, kw
+
+
+def test_wrappers_refuse_cpu_tensors():
+    from rl_for_mario_b200 import kernels
+
+    q, k = torch.zeros(1, 4, 4, 32, dtype=torch.bfloat16), torch.zeros(1, 4, 2, 32, dtype=torch.bfloat16)
+    x, w = torch.zeros(2, 8), torch.ones(8)
+    with pytest.raises(ValueError, match="CUDA"):
+        kernels.attn_train_forward(q, k, k)
+    with pytest.raises(ValueError, match="CUDA"):
+        kernels.attn_train_backward(q, q, k, k, q, torch.zeros(1, 4, 4))
+    with pytest.raises(ValueError, match="CUDA"):
+        kernels.residual_norm_forward(x, x, w, 1e-5)
+    with pytest.raises(ValueError, match="CUDA"):
+        kernels.residual_norm_backward(x, x, x, x, w, torch.zeros(2, 2))
+    with pytest.raises(ValueError, match="CUDA"):
+        kernels.dropout_forward(x, 0.1, torch.zeros(2, dtype=torch.int64))
+
+
+def test_argument_checks_on_the_host():
+    from rl_for_mario_b200 import kernels as K
+
+    x = torch.zeros(2, 3, 8)
+    assert K._gate_rows(None, x) == (None, 0)
+    for shape, rows, shared in (((8,), 1, 6), ((1, 8), 1, 6), ((2, 1, 8), 2, 3), ((1, 1, 8), 1, 6), ((2, 3, 8), 6, 1)):
+        g, s = K._gate_rows(torch.zeros(shape), x)
+        assert tuple(g.shape) == (rows, 8) and s == shared
+    for shape in ((3, 8), (1, 3, 8), (7,), (1, 2, 3, 8), (2, 2, 8)):
+        with pytest.raises(ValueError, match="gate"):
+            K._gate_rows(torch.zeros(shape), x)
+    one = torch.zeros(1, 3, 8)
+    assert K._gate_rows(torch.zeros(1, 1, 8), one)[1] == 3 and K._gate_rows(torch.zeros(3, 8), one)[1] == 1
+    with pytest.raises(TypeError, match="dtype"):
+        K._check_residual_norm(x, x.bfloat16(), torch.ones(8), None, None)
+    with pytest.raises(ValueError, match="residual"):
+        K._check_residual_norm(x, x[:1], torch.ones(8), None, None)
+    with pytest.raises(ValueError, match="pre_weight"):
+        K._check_residual_norm(x, None, torch.ones(7), None, None)
+    rng = torch.zeros(2, dtype=torch.int64)
+    assert K._check_dropout(0, None, 0) == 0.0 and K._check_dropout(0.5, rng, 2 ** 32 - 1) == 0.5
+    for p, r, site in ((1.0, rng, 0), (-0.1, rng, 0), (float("nan"), rng, 0), (0.1, None, 0), (0.1, rng.int(), 0),
+                       (0.1, rng[:1], 0), (0.1, rng, -1), (0.1, rng, 2 ** 32), (0.999995, rng, 0)):
+        with pytest.raises(ValueError):
+            K._check_dropout(p, r, site)
+    q, k = torch.zeros(1, 4, 4, 32, dtype=torch.bfloat16), torch.zeros(1, 4, 2, 32, dtype=torch.bfloat16)
+    with pytest.raises(TypeError, match="bf16"):
+        K._check_attn_train(q.float(), k.float(), k.float(), None, None)
+    with pytest.raises(ValueError, match="pad_len"):
+        K._check_attn_train(q, k, k, torch.zeros(2), None)
+    with pytest.raises(ValueError, match="scale"):
+        K._check_attn_train(q, k, k, None, 0.0)
+    with pytest.raises(ValueError, match="shapes"):
+        K._check_attn_train(q, k, k[:, :3], None, None)
+
+
+def test_generator_words():
+    """Every word takes each half equally often, blocks differ in every counter and key word, and the
+    64-bit multiplication agrees with Python's integers."""
+    w = ref.philox_words(np.arange(1 << 14, dtype=np.uint64), 12345, 6, 7)
+    # 2^14 draws a word: six standard deviations of a fair bit.
+    assert (np.abs((w >= 32768).mean(0) - 0.5) <= 6 * 0.5 / 128).all()
+    base = ref.philox_words(np.array([5], dtype=np.uint64), 1, 2, 3)
+    for args in ((6, 1, 2, 3), (5 + (1 << 32), 1, 2, 3), (5, 2, 2, 3), (5, 1 + (1 << 32), 2, 3), (5, 1, 3, 3),
+                 (5, 1, 2, 4)):
+        assert not np.array_equal(base, ref.philox_words(np.array([args[0]], dtype=np.uint64), *args[1:]))
+    c, k = [5, 0, 2, 3], [1, 0]
+    for _ in range(7):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    assert base[0].tolist() == [h for v in c for h in (v & 0xFFFF, v >> 16)]
