@@ -60,6 +60,17 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
                            const int64_t* rng, uint32_t site, int dtype, void* stream);
 
 /*
+ * Gradient of the RoPE that dt_qkv_rope applies to the q and k heads, in place
+ * on the gradient of its output: columns [0, rope_cols) of g [rows, N] (row
+ * stride in elements), groups of head_dim (32 or 64), row r rotated back by
+ * table row (r mod seq_len) of cos / sin ([>= seq_len, head_dim] fp32).  bf16 or
+ * fp16; stride and rope_cols multiples of 8 and head_dim, g 16-byte and cos /
+ * sin 8-byte aligned with an even row stride.
+ */
+int dt_rope_grad(void* g, int64_t g_stride, int64_t rows, const float* cos_tab, const float* sin_tab,
+                 int64_t cos_stride, int cos_rows, int seq_len, int rope_cols, int head_dim, int dtype, void* stream);
+
+/*
  * Residual add with the norms before and after it, a gate and dropout:
  *   u = x * rsqrt(mean(x^2) + eps) * w_post    (u = x when w_post is null)
  *   h = residual + alpha * gate * dropout(u)   (residual null: 0; gate null: 1)

@@ -61,6 +61,7 @@ SIGNATURES = {
                                    _L, _L, _L, _F, _D, _P, _U, _I, _P]),
     "dt_attn_train_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _F, _D, _P,
                                     _U, _I, _P]),
+    "dt_rope_grad": (_I, [_P, _L, _L, _P, _P, _L, _I, _I, _I, _I, _I, _P]),
     "dt_residual_norm_forward": (_I, [_P, _L, _P, _L, _P, _L, _L, _P, _P, _P, _P, _P, _L, _I, _F, _F, _D, _P, _U, _I,
                                       _P]),
     "dt_residual_norm_workspace": (_L, [_L, _I, _L, _I]),

@@ -22,6 +22,11 @@ accumulation); fp32 inputs run on the fp32 kernels (CUDA cores, fp32
 throughout) unless ``compute_dtype`` selects bf16/fp16 tensor-core compute, in
 which case Q/K/V are cast for the kernels and the result is cast back.  There
 is no CPU path: CPU inputs raise.
+
+The kernels above have no gradient.  ``fuse_training()`` switches forward() to
+the training operators (training.py) whenever autograd is on and no cache takes
+part: same projections and RoPE, attention with its gradient, and dropout on
+the attention weights and on the output while the module is in training mode.
 """
 from __future__ import annotations
 
@@ -30,7 +35,7 @@ from typing import Optional, Tuple
 import torch
 from torch import nn
 
-from . import kernels
+from . import kernels, training
 from .cache import LayerKV, dense_layer
 
 Tensor = torch.Tensor
@@ -66,6 +71,12 @@ class FastDTAttention(nn.Module):
         object.__setattr__(self, "_fused_norm", None)
         object.__setattr__(self, "_fused_w", None)
         object.__setattr__(self, "_fused_key", None)
+        # Training form (fuse_training): off, the module's own generator, and the
+        # number that tells this module's dropout from other modules'.
+        self.train_form = False
+        self.train_seed = 0
+        self.train_site = 0
+        object.__setattr__(self, "_dropout_state", None)
 
     @classmethod
     def from_reference(cls, ref_attn: nn.Module, config, **kw) -> "FastDTAttention":
@@ -155,6 +166,57 @@ class FastDTAttention(nn.Module):
         xv = self.v_proj(x).view(bsz, seq_len, Hkv, D).to(kd)
         return xq, xk, xv, False
 
+    # ----------------------------------------------------------------- training
+    def fuse_training(self, on: bool = True, seed: int = 0, site: int = 0) -> "FastDTAttention":
+        """Runs forward() on the training operators whenever autograd is on and no cache takes part
+        (bf16 / fp16 compute).  ``seed``: of the module's own dropout generator; ``site``: the first of
+        two dropout sites (attention weights, output), which modules that share a seed keep apart.
+
+        Rows of padded positions come out of the attention as zeros there and pass no gradient (the
+        inference kernels give them the reference's mean of V)."""
+        self.train_form, self.train_seed, self.train_site = bool(on), int(seed), int(site)
+        object.__setattr__(self, "_dropout_state", None)
+        return self
+
+    def dropout_state(self) -> "training.DropoutState":
+        """The module's own generator (made on its device when first asked for)."""
+        dev = self.q_proj.weight.device
+        if self._dropout_state is None or self._dropout_state.state.device != dev:
+            object.__setattr__(self, "_dropout_state", training.DropoutState(self.train_seed, dev))
+        return self._dropout_state
+
+    def attend_training(self, x: Tensor, position_embeddings: Tuple[Tensor, Tensor], pad_len: Optional[Tensor],
+                        rng: Optional[Tensor]) -> Tensor:
+        """Projections, attention and o_proj of the training form, without the dropout of the output."""
+        kd = self._kernel_dtype(x)
+        if kd == torch.float32:
+            raise TypeError("the training form of FastDTAttention computes in bf16 or fp16: convert the model or give "
+                            "compute_dtype")
+        if self.rope_rounding != "fp32":
+            raise ValueError("the training form rotates q and k in fp32: rope_rounding must be 'fp32'")
+        B, S, _ = x.shape
+        Hq, Hkv, D = self.n_local_heads, self.n_local_kv_heads, self.head_dim
+        cos, sin = position_embeddings
+        p = self.dropout if self.training else 0.0
+        ws = (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
+        if (kd == x.dtype == ws[0].dtype and D in (32, 64) and x.shape[-1] % 8 == 0 and x.data_ptr() % 16 == 0
+                and x.stride(-1) == 1 and not torch.is_autocast_enabled()
+                and all(m.bias is None for m in (self.q_proj, self.k_proj, self.v_proj))):
+            qkv = training.qkv_rope(x, torch.cat(ws), cos, sin, (Hq + Hkv) * D, D)
+            out = training.attention_qkv(qkv.view(B, S, Hq + 2 * Hkv, D), Hq, Hkv, pad_len, p=p, rng=rng,
+                                         site=self.train_site)
+        else:
+            def rotate(t):
+                t = t.float()
+                half = torch.cat((-t[..., D // 2:], t[..., :D // 2]), -1)
+                return (t * cos[:S, None].float() + half * sin[:S, None].float()).to(kd)
+
+            q = rotate(self.q_proj(x).view(B, S, Hq, D))
+            k = rotate(self.k_proj(x).view(B, S, Hkv, D))
+            v = self.v_proj(x).view(B, S, Hkv, D).to(kd)
+            out = training.attention(q, k, v, pad_len, p=p, rng=rng, site=self.train_site)
+        return self.o_proj(out.reshape(B, S, Hq * D).to(x.dtype))
+
     # ------------------------------------------------------------------ forward
     def forward(self, x: Tensor, position_embeddings: Tuple[Tensor, Tensor],
                 past_key_value=None, use_cache: bool = False, attention_mask: Optional[Tensor] = None,
@@ -166,6 +228,15 @@ class FastDTAttention(nn.Module):
         if not x.is_cuda:
             raise ValueError("FastDTAttention runs on CUDA only (no CPU path)")
         bsz, seq_len, _ = x.shape
+        if self.train_form and torch.is_grad_enabled() and past_key_value is None and not use_cache:
+            p = self.dropout if self.training else 0.0
+            rng = self.dropout_state().draw() if p > 0 else None
+            if raw_input:
+                x = self._fused_norm(x)
+            y = self.attend_training(x, position_embeddings, self._pad_len(attention_mask, seq_len), rng)
+            if p > 0:
+                return training.dropout(y, p, rng, self.train_site + 1, residual), None
+            return (y if residual is None else residual + y), None
         kd = self._kernel_dtype(x)
         cos, sin = position_embeddings
         xq, xk, xv, rotated = self._project(x, kd, raw_input, (cos, sin))

@@ -162,6 +162,32 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
       dtk::launch_attn_train_bwd_sm100(a, D, dtype == DT_DTYPE_BF16, sms, static_cast<cudaStream_t>(stream)), fn);
 }
 
+int dt_rope_grad(void* g, int64_t g_stride, int64_t rows, const float* cos_tab, const float* sin_tab,
+                 int64_t cos_stride, int cos_rows, int seq_len, int rope_cols, int head_dim, int dtype, void* stream) {
+  const char* fn = "dt_rope_grad";
+  Range range(fn);
+  if (!g || !cos_tab || !sin_tab) return api_fail(DT_ERR_INVALID, "%s: null g/cos/sin pointer", fn);
+  if (rows < 1 || seq_len < 1) return api_fail(DT_ERR_INVALID, "%s: sizes must be positive", fn);
+  if (head_dim != 32 && head_dim != 64)
+    return api_fail(DT_ERR_UNSUPPORTED, "%s: head_dim %d not in {32, 64}", fn, head_dim);
+  if (dtype != DT_DTYPE_BF16 && dtype != DT_DTYPE_FP16)
+    return api_fail(DT_ERR_UNSUPPORTED, "%s: dtype %d not supported (bf16 or fp16)", fn, dtype);
+  if (rope_cols < head_dim || rope_cols % head_dim || g_stride < rope_cols || g_stride % 8 || !aligned16(g))
+    return api_fail(DT_ERR_INVALID, "%s: rope_cols %d / row stride %lld / alignment", fn, rope_cols,
+                    (long long)g_stride);
+  if (cos_rows < seq_len || cos_stride < head_dim || cos_stride % 2 ||
+      ((reinterpret_cast<uintptr_t>(cos_tab) | reinterpret_cast<uintptr_t>(sin_tab)) & 7))
+    return api_fail(DT_ERR_INVALID, "%s: cos/sin need %d rows of %d, 8-byte aligned", fn, seq_len, head_dim);
+  int sms = 0;
+  const int rc = need_sm100(fn, &sms);
+  if (rc) return rc;
+  dtk::RopeGradParams a{};
+  a.x = g, a.cos = cos_tab, a.sin = sin_tab, a.stride = g_stride, a.rows = rows, a.cs_stride = cos_stride;
+  a.rope_cols = rope_cols, a.head_dim = head_dim, a.seq_len = seq_len;
+  return cuda_status(dtk::launch_rope_grad_sm100(a, dtype == DT_DTYPE_BF16, sms, static_cast<cudaStream_t>(stream)),
+                     fn);
+}
+
 int64_t dt_residual_norm_workspace(int64_t M, int H, int64_t gate_rows, int has_post) {
   if (M < 1 || H < 1 || H > kMaxHidden || gate_rows < 0 || (gate_rows > 0 && M % gate_rows != 0))
     return -api_fail(DT_ERR_INVALID, "dt_residual_norm_workspace: bad sizes (M=%lld H=%d gate_rows=%lld)", (long long)M,

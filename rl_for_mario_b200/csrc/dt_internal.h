@@ -210,6 +210,15 @@ struct DropoutParams {
 };
 cudaError_t launch_dropout_sm100(const DropoutParams& p, int dtype, int num_sms, cudaStream_t st);
 
+struct RopeGradParams {
+  void* x;  // [rows, >= rope_cols], rotated back in place
+  const float* cos;
+  const float* sin;
+  long long stride, rows, cs_stride;
+  int rope_cols, head_dim, seq_len;
+};
+cudaError_t launch_rope_grad_sm100(const RopeGradParams& p, bool bf16, int num_sms, cudaStream_t st);
+
 struct ResidualNormParams {
   const void* x;
   const void* residual;  // or null

@@ -21,7 +21,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import kernels
+from . import kernels, training
 from .attention import FastDTAttention
 from .cache import LayerKV, PagedKVCache
 
@@ -138,6 +138,18 @@ class DTBlock(nn.Module):
                 and (not self.training or mlp.dropout.p == 0) and inter % 64 == 0 and inter >= 128
                 and h.shape[-1] % 8 == 0 and not (torch.is_grad_enabled() and h.requires_grad))
 
+    def forward_training(self, h: Tensor, n: Tensor, position_embeddings, pad_len: Optional[Tensor],
+                         rng: Optional[Tensor], next_norm: RMSNorm) -> Tuple[Tensor, Tensor]:
+        """The block on the training operators: ``h`` is the residual stream and ``n`` its
+        input_layernorm; returns the stream behind the block and ``next_norm`` of it.  Each residual
+        add is one kernel with the dropout before it and the norm behind it."""
+        attn, mlp, post = self.self_attn, self.mlp, self.post_attention_layernorm
+        p = mlp.dropout.p if self.training else 0.0
+        y = attn.attend_training(n, position_embeddings, pad_len, rng)
+        h, n = training.residual_norm(y, h, post.weight, post.eps, p=p, rng=rng, site=attn.train_site + 1)
+        y = mlp.down_proj(F.silu(mlp.gate_proj(n)) * mlp.up_proj(n))
+        return training.residual_norm(y, h, next_norm.weight, next_norm.eps, p=p, rng=rng, site=attn.train_site + 2)
+
     def forward(self, hidden_states, position_embeddings, past_key_value=None, use_cache=False,
                 attention_mask=None, _owns_input: bool = False):
         """``_owns_input``: the caller (the backbone's layer loop) owns
@@ -188,6 +200,10 @@ class MarioStateEncoder(nn.Module):
         conv0, conv1, conv2, lin = self.cnn[0], self.cnn[2], self.cnn[4], self.cnn[7]
         dt = conv0.weight.dtype
         s = states.reshape(B * T, C, H, W)
+        if self.train_form and torch.is_grad_enabled():
+            # Autograd's own convolutions: the kernels below have no gradient.
+            x = s.to(dt)
+            return self.cnn(torch.where(x.amax() > 1.0, x / 255.0, x)).reshape(B, T, -1)
         cl = torch.channels_last
         if (conv0.in_channels == 4 and conv0.out_channels == 32 and conv0.kernel_size == (8, 8)
                 and conv0.stride == (4, 4) and conv0.padding == (0, 0) and conv0.bias is not None
@@ -264,6 +280,7 @@ class MarioStateEncoder(nn.Module):
             return F.linear(x.permute(0, 2, 3, 1).reshape(n, -1), lw, lin.bias).reshape(B, T, -1)
         return lin(x.contiguous().flatten(1)).reshape(B, T, -1)
 
+    train_form = False
     _fused_conv = True
     # True: layers 2 and 3 on the library's fused tensor-core kernel
     # (dt_encoder_conv23) when the shapes are the Nature-DQN ones on 84 x 84
@@ -326,6 +343,10 @@ class DTBackbone(nn.Module):
 
     def embed(self, states, actions, returns_to_go, timesteps) -> Tensor:
         """Token embeddings interleaved (R, s, a) -> [B, 3T, H] after embed_norm (:401-420)."""
+        return self.dropout(self.embed_norm(self.embed_tokens(states, actions, returns_to_go, timesteps)))
+
+    def embed_tokens(self, states, actions, returns_to_go, timesteps) -> Tensor:
+        """Token embeddings interleaved (R, s, a) -> [B, 3T, H] before embed_norm (:401-419)."""
         cfg = self.config
         B, T = states.shape[0], states.shape[1]
         ts = timesteps.clamp(0, cfg.max_ep_len - 1).long()
@@ -333,8 +354,7 @@ class DTBackbone(nn.Module):
         se = self.state_encoder(states) + te
         re = self.embed_return(returns_to_go.unsqueeze(-1).to(self.embed_return.weight.dtype)) + te
         ae = self.embed_action(actions.long().clamp(0, cfg.act_dim - 1)) + te
-        h = torch.stack((re, se, ae), dim=2).reshape(B, 3 * T, cfg.hidden_size)
-        return self.dropout(self.embed_norm(h))
+        return torch.stack((re, se, ae), dim=2).reshape(B, 3 * T, cfg.hidden_size)
 
     def forward(self, states, actions, returns_to_go, timesteps, attention_mask=None, past_key_values=None,
                 use_cache=False):
@@ -352,13 +372,48 @@ class DTBackbone(nn.Module):
             raise ValueError("timesteps must be [B,T]")
         if T > cfg.context_len:
             raise ValueError(f"seq_len={T} exceeds context_len={cfg.context_len}")
+        if attention_mask is not None and attention_mask.shape != (B, T):
+            raise ValueError(f"attention_mask must be [B,T], got {tuple(attention_mask.shape)}")
+        if self.train_form and torch.is_grad_enabled() and past_key_values is None and not use_cache:
+            pad = None
+            if attention_mask is not None:
+                pad = 3 * kernels.pad_len_from_mask(attention_mask, T)
+            return self.run_training(self.embed_tokens(states, actions, returns_to_go, timesteps), pad)
         h = self.embed(states, actions, returns_to_go, timesteps)
         mask3 = None
         if attention_mask is not None:
-            if attention_mask.shape != (B, T):
-                raise ValueError(f"attention_mask must be [B,T], got {tuple(attention_mask.shape)}")
             mask3 = torch.stack((attention_mask,) * 3, dim=2).reshape(B, 3 * T).to(h.dtype)
         return self.run_layers(h, mask3, past_key_values, use_cache, _owns_h=True)
+
+    train_form = False
+    train_seed = 0
+    _dropout_state: Optional[training.DropoutState] = None
+
+    def dropout_state(self) -> training.DropoutState:
+        """Seed and step of the training form's dropout (made on the model's device when first asked for)."""
+        dev = self.norm.weight.device
+        if self._dropout_state is None or self._dropout_state.state.device != dev:
+            self._dropout_state = training.DropoutState(self.train_seed, dev)
+        return self._dropout_state
+
+    def run_training(self, tokens: Tensor, pad_len: Optional[Tensor] = None):
+        """embed_norm, layers and final norm (:420, :435-461) on the training operators: tokens
+        [B, S, H] before embed_norm, pad_len [B] leading padding tokens; returns what run_layers does."""
+        cfg = self.config
+        B, S = tokens.shape[0], tokens.shape[1]
+        if S > self.freqs_cos.shape[0]:
+            raise ValueError(f"{S} positions exceed max_position_embeddings {self.freqs_cos.shape[0]}")
+        pe = (self.freqs_cos[:S].float(), self.freqs_sin[:S].float())
+        p = self.dropout.p if self.training else 0.0
+        rng = self.dropout_state().draw() if p > 0 else None
+        first = self.layers[0].input_layernorm if len(self.layers) else self.norm
+        h, n = training.residual_norm(tokens, None, first.weight, first.eps, post_weight=self.embed_norm.weight, p=p,
+                                      rng=rng, site=0)
+        for i, layer in enumerate(self.layers):
+            last = i + 1 == len(self.layers)
+            h, n = layer.forward_training(h, n, pe, pad_len, rng,
+                                          self.norm if last else self.layers[i + 1].input_layernorm)
+        return n.view(B, S // 3, 3, cfg.hidden_size), [None] * len(self.layers)
 
     def run_layers(self, h, mask3=None, past_key_values=None, use_cache=False, flat: bool = False,
                    _owns_h: bool = False):
@@ -412,6 +467,22 @@ class MarioDT(nn.Module):
         """Fuses every block's input RMSNorm into its Q/K/V projection kernel."""
         for layer in self.model.layers:
             layer.fuse_norm(on)
+        return self
+
+    def fuse_training(self, on: bool = True, seed: int = 0) -> "MarioDT":
+        """Trains a bf16 / fp16 model on the training operators (training.py): with autograd on and
+        no cache, forward() runs attention with its gradient, every residual add as one kernel with
+        the dropout before it and the norm behind it, and dropout whose masks are never stored, from
+        a generator of ``seed`` (model.dropout_state(), to be saved with a checkpoint).  Without
+        autograd (validation, act()) the inference kernels run as before.
+
+        Padded positions (attention_mask 0) attend to nothing and pass no gradient through the
+        attention; give them action_targets of -100, as their logits mean nothing."""
+        self.model.train_form = self.model.state_encoder.train_form = bool(on)
+        self.model.train_seed = int(seed)
+        self.model._dropout_state = None
+        for i, layer in enumerate(self.model.layers):
+            layer.self_attn.fuse_training(on, seed, 1 + 3 * i)  # three sites a block; 0 is the embedding's
         return self
 
     def reference_rounding(self, on: bool = True) -> "MarioDT":

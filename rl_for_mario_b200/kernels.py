@@ -649,6 +649,27 @@ def attn_train_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tens
     return dq, dk, dv
 
 
+def rope_grad_(g: Tensor, cos: Tensor, sin: Tensor, rope_cols: int, head_dim: int) -> Tensor:
+    """Gradient of qkv_rope's rotation, in place: g [B, S, N] (the gradient of its output, contiguous)
+    has its first rope_cols columns (the q and k heads) rotated back by table rows 0 .. S - 1."""
+    dev = _same_device(g, cos, sin)
+    if g.dim() != 3 or not g.is_contiguous():
+        raise ValueError("rope_grad_ needs a contiguous [B, S, N] gradient")
+    if not 0 < rope_cols <= g.shape[2]:
+        raise ValueError(f"rope_cols {rope_cols} outside 1..{g.shape[2]}")
+    if g.numel() == 0:
+        return g
+    cos, sin = _prep_tables(cos, sin)
+    if cos.shape[-1] != head_dim or sin.shape != cos.shape:
+        raise ValueError(f"cos / sin must be [rows, {head_dim}] tables")
+    with _On(dev):
+        rc = _lib.load().dt_rope_grad(_ptr(g), g.stride(1), g.shape[0] * g.shape[1], _ptr(cos), _ptr(sin),
+                                      cos.stride(0), cos.shape[0], g.shape[1], int(rope_cols), int(head_dim),
+                                      _dtype_code(g), _stream_ptr(dev))
+    _lib.check("dt_rope_grad", rc)
+    return g
+
+
 def _rows2d(t: Tensor) -> Tensor:
     """t as a [rows, K] view with a contiguous last dimension (a copy when no view exists)."""
     t2 = t.reshape(-1, t.shape[-1])
