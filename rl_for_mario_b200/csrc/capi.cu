@@ -152,6 +152,11 @@ int api_device(int** status, int* cc_major, int* num_sms) {
   return DT_OK;
 }
 
+int api_encode_bshd(CUtensorMap* map, const void* base, bool bf16, int B, int S, int H, int D, int64_t sb, int64_t ss,
+                    int64_t sh, uint32_t box_h, uint32_t box_s, const char* name) {
+  return encode_bshd(map, base, bf16, B, S, H, D, sb, ss, sh, box_h, box_s, name);
+}
+
 }  // namespace dtk
 
 extern "C" {

@@ -27,11 +27,12 @@ int cuda_status(cudaError_t e, const char* what) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-int need_sm100(const char* fn, int* num_sms) {
+int need_sm100(const char* fn, int* num_sms, int** status_out = nullptr) {
   int* status = nullptr;
   int cc = 0;
   const int rc = dtk::api_device(&status, &cc, num_sms);
   if (rc) return rc;
+  if (status_out) *status_out = status;
   if (cc != 10) return api_fail(DT_ERR_UNSUPPORTED, "%s: needs an sm_100 GPU (current device is cc %d.x)", fn, cc);
   return DT_OK;
 }
@@ -120,7 +121,7 @@ int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, 
   dtk::AttnTrainParams a{};
   if ((rc = rate(fn, p, rng, &a.threshold, &a.inv_keep))) return rc;
   int sms = 0;
-  if ((rc = need_sm100(fn, &sms))) return rc;
+  if ((rc = need_sm100(fn, &sms, &a.status))) return rc;
   a.q = q, a.k = k, a.v = v, a.o = o, a.lse = lse, a.pad_len = pad_len;
   a.q_sb = q_sb, a.q_ss = q_ss, a.q_sh = q_sh, a.k_sb = k_sb, a.k_ss = k_ss, a.k_sh = k_sh;
   a.v_sb = v_sb, a.v_ss = v_ss, a.v_sh = v_sh, a.o_sb = o_sb, a.o_ss = o_ss, a.o_sh = o_sh;
@@ -128,8 +129,14 @@ int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, 
   a.scale = scale > 0.f ? scale : 1.0f / sqrtf((float)D);
   a.rng = reinterpret_cast<const long long*>(rng);
   a.site = site;
-  return cuda_status(
-      dtk::launch_attn_train_fwd_sm100(a, D, dtype == DT_DTYPE_BF16, sms, static_cast<cudaStream_t>(stream)), fn);
+  a.HC = a.R < 64 ? a.R : 64;
+  const bool bf16 = dtype == DT_DTYPE_BF16;
+  dtk::AttnTrainMaps m;
+  if ((rc = dtk::api_encode_bshd(&m.q_tile, q, bf16, B, S, Hq, D, q_sb, q_ss, q_sh, a.HC, 128 / a.HC, "q")) ||
+      (rc = dtk::api_encode_bshd(&m.k_blk, k, bf16, B, S, Hkv, D, k_sb, k_ss, k_sh, 1, 64, "k")) ||
+      (rc = dtk::api_encode_bshd(&m.v_blk, v, bf16, B, S, Hkv, D, v_sb, v_ss, v_sh, 1, 64, "v")))
+    return rc;
+  return cuda_status(dtk::launch_attn_train_fwd_tc_sm100(a, m, D, bf16, static_cast<cudaStream_t>(stream)), fn);
 }
 
 int dt_attn_train_backward(const void* dout, const void* q, const void* k, const void* v, const void* o,
@@ -147,7 +154,7 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
   dtk::AttnTrainParams a{};
   if ((rc = rate(fn, p, rng, &a.threshold, &a.inv_keep))) return rc;
   int sms = 0;
-  if ((rc = need_sm100(fn, &sms))) return rc;
+  if ((rc = need_sm100(fn, &sms, &a.status))) return rc;
   a.q = q, a.k = k, a.v = v, a.o = const_cast<void*>(o), a.lse = const_cast<float*>(lse), a.pad_len = pad_len;
   a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
   long long* const to[24] = {&a.q_sb,  &a.q_ss,  &a.q_sh,  &a.k_sb,  &a.k_ss,  &a.k_sh,  &a.v_sb,  &a.v_ss,
@@ -158,8 +165,21 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
   a.scale = scale > 0.f ? scale : 1.0f / sqrtf((float)D);
   a.rng = reinterpret_cast<const long long*>(rng);
   a.site = site;
-  return cuda_status(
-      dtk::launch_attn_train_bwd_sm100(a, D, dtype == DT_DTYPE_BF16, sms, static_cast<cudaStream_t>(stream)), fn);
+  a.HC = a.R < 64 ? a.R : 64;
+  const bool bf16 = dtype == DT_DTYPE_BF16;
+  dtk::AttnTrainMaps m;
+  const uint32_t hc = (uint32_t)a.HC;
+  if ((rc = dtk::api_encode_bshd(&m.q_tile, q, bf16, B, S, Hq, D, a.q_sb, a.q_ss, a.q_sh, hc, 128 / hc, "q")) ||
+      (rc = dtk::api_encode_bshd(&m.q_blk, q, bf16, B, S, Hq, D, a.q_sb, a.q_ss, a.q_sh, hc, 64 / hc, "q")) ||
+      (rc = dtk::api_encode_bshd(&m.do_tile, dout, bf16, B, S, Hq, D, a.do_sb, a.do_ss, a.do_sh, hc, 128 / hc,
+                                 "dout")) ||
+      (rc = dtk::api_encode_bshd(&m.do_blk, dout, bf16, B, S, Hq, D, a.do_sb, a.do_ss, a.do_sh, hc, 64 / hc, "dout")) ||
+      (rc = dtk::api_encode_bshd(&m.k_tile, k, bf16, B, S, Hkv, D, a.k_sb, a.k_ss, a.k_sh, 1, 128, "k")) ||
+      (rc = dtk::api_encode_bshd(&m.k_blk, k, bf16, B, S, Hkv, D, a.k_sb, a.k_ss, a.k_sh, 1, 64, "k")) ||
+      (rc = dtk::api_encode_bshd(&m.v_tile, v, bf16, B, S, Hkv, D, a.v_sb, a.v_ss, a.v_sh, 1, 128, "v")) ||
+      (rc = dtk::api_encode_bshd(&m.v_blk, v, bf16, B, S, Hkv, D, a.v_sb, a.v_ss, a.v_sh, 1, 64, "v")))
+    return rc;
+  return cuda_status(dtk::launch_attn_train_bwd_tc_sm100(a, m, D, bf16, static_cast<cudaStream_t>(stream)), fn);
 }
 
 int dt_rope_grad(void* g, int64_t g_stride, int64_t rows, const float* cos_tab, const float* sin_tab,

@@ -196,6 +196,9 @@ cudaError_t launch_decode_sm100(const DecodeParams& prm, const CUtensorMap& kmap
 // device's status word, major compute capability and SM count.
 int api_fail(int code, const char* fmt, ...);
 int api_device(int** status, int* cc_major, int* num_sms);
+// Tensor map over a 16-bit [B, S, H, D] tensor (element strides), boxes of box_s positions of box_h heads.
+int api_encode_bshd(CUtensorMap* map, const void* base, bool bf16, int B, int S, int H, int D, int64_t sb, int64_t ss,
+                    int64_t sh, uint32_t box_h, uint32_t box_s, const char* name);
 
 struct DropoutParams {
   const void* x;
@@ -269,11 +272,22 @@ struct AttnTrainParams {
   long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh;
   long long do_sb, do_ss, do_sh, dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
   int B, S, Hq, Hkv, R;
+  int HC;       // query heads packed into a tile: min(R, 64)
+  int* status;  // device status word
   float scale;
   const long long* rng;
   uint32_t threshold, site;  // threshold 0: no dropout
   float inv_keep;
 };
+// TMA maps over [B, S, H, D]: tiles of 128 rows and blocks of 64, of packed
+// (position, head) rows for q and dout, of positions of one head for k and v.
+struct AttnTrainMaps {
+  CUtensorMap q_tile, do_tile, q_blk, do_blk, k_tile, v_tile, k_blk, v_blk;
+};
+cudaError_t launch_attn_train_fwd_tc_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
+                                           cudaStream_t st);
+cudaError_t launch_attn_train_bwd_tc_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
+                                           cudaStream_t st);
 cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, int D, bool bf16, int num_sms, cudaStream_t st);
 cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, int D, bool bf16, int num_sms, cudaStream_t st);
 

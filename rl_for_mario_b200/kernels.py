@@ -5,7 +5,9 @@ library itself never allocates), and launches on torch's current CUDA stream.
 """
 from __future__ import annotations
 
+import functools
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -26,7 +28,7 @@ def _dtype_code(t: Tensor) -> int:
 
 
 def _stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # current_stream(device).cuda_stream, without its objects
 
 
 def _ptr(t: Optional[Tensor]) -> Optional[int]:
@@ -507,32 +509,37 @@ def rmsnorm_qkv(x: Tensor, w_fused: Tensor, eps: float, out: Optional[Tensor] = 
 
 
 # ------------------------------------------------------------------ training operators
+#
+# A training step makes many small calls, and at small sizes the host's time for
+# one (some 20 us) is the whole of it: these wrappers look at each tensor once
+# and create no object that the call does not need.
 def _same_device(first: Tensor, *ts: Optional[Tensor]) -> torch.device:
     """The device that every tensor is on (CUDA)."""
-    _require_cuda(first, *ts)
+    dev = first.device
+    if dev.type != "cuda":
+        _require_cuda(first)
     for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors are on different devices ({first.device} and {t.device})")
-    return first.device
+        if t is not None and t.device != dev:
+            _require_cuda(t)
+            raise ValueError(f"tensors are on different devices ({dev} and {t.device})")
+    return dev
 
 
-class _On:
-    """Makes ``device`` current around a launch when it is not (the library
-    launches on the current device)."""
-
-    __slots__ = ("want", "had")
-
-    def __init__(self, device: torch.device):
-        self.want = device.index
-
-    def __enter__(self):
-        self.had = torch.cuda.current_device()
-        if self.had != self.want:
-            torch.cuda.set_device(self.want)
-
-    def __exit__(self, *exc):
-        if self.had != self.want:
-            torch.cuda.set_device(self.had)
+def _launch(name: str, dev: torch.device, *args) -> None:
+    """Calls the entry point on the device's current stream (its last argument), with the device
+    current: the library launches there."""
+    fn = getattr(_lib.load(), name)
+    had = torch._C._cuda_getDevice()
+    if had == dev.index:
+        rc = fn(*args, _stream_ptr(dev))
+    else:
+        torch.cuda.set_device(dev)
+        try:
+            rc = fn(*args, _stream_ptr(dev))
+        finally:
+            torch.cuda.set_device(had)
+    if rc:
+        _lib.check(name, rc)
 
 
 def _check_dropout(p: float, rng: Optional[Tensor], site: int) -> float:
@@ -541,44 +548,53 @@ def _check_dropout(p: float, rng: Optional[Tensor], site: int) -> float:
     ``rng``: int64 [2] device tensor (seed, step), see training.DropoutState;
     ``site``: a number of its own for each place of a model that drops."""
     p = float(p)
-    if not 0.0 <= p < 1.0 or round(p * 65536) >= 65536:
-        raise ValueError(f"dropout p must lie in [0, 1), below 1 - 2^-17 (got {p})")
-    if p > 0.0:
+    if p != 0.0:
+        if not 0.0 <= p < 1.0 or round(p * 65536) >= 65536:
+            raise ValueError(f"dropout p must lie in [0, 1), below 1 - 2^-17 (got {p})")
         if rng is None:
             raise ValueError("dropout needs rng, an int64 [2] device tensor (seed, step)")
-        if rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
-            raise ValueError("rng must be a contiguous int64 tensor of shape [2] (seed, step)")
-    if not 0 <= int(site) < 2 ** 32:
+    if rng is not None and (rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous()):
+        raise ValueError("rng must be a contiguous int64 tensor of shape [2] (seed, step)")
+    if not 0 <= site < 2 ** 32:
         raise ValueError(f"site must lie in [0, 2^32) (got {site})")
     return p
 
 
-def _rows16(t: Tensor) -> Tensor:
-    """t itself when the attention kernels can read it ([B, S, H, D], contiguous D, strides
-    multiples of 8, 16-byte aligned), else a contiguous copy."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % 8 == 0 for s in t.stride()[:3]):
-        return t
-    return t.contiguous()
+def _rows16(t: Tensor) -> Tuple[Tensor, Tuple[int, int, int]]:
+    """t when the attention kernels can read it ([B, S, H, D], contiguous D, strides multiples of 8,
+    16-byte aligned), else a contiguous copy, and its first three strides."""
+    b, s, h, d = t.stride()
+    if d != 1 or (b | s | h) % 8 or b <= 0 or s <= 0 or h <= 0 or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        _, s, h, d = t.shape  # by its shape: the stride of a dimension of one element may be anything
+        return t, (s * h * d, h * d, d)
+    return t, (b, s, h)
 
 
 def _check_attn_train(q: Tensor, k: Tensor, v: Tensor, pad_len: Optional[Tensor], scale: Optional[float]):
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("attn_train takes q [B, S, Hq, D] and k, v [B, S, Hkv, D]")
     B, S, Hq, D = q.shape
-    Hkv = k.shape[2]
-    if k.shape != (B, S, Hkv, D) or v.shape != k.shape:
+    kshape = k.shape
+    if kshape != (B, S, kshape[2], D) or v.shape != kshape:
         raise ValueError(f"k/v shapes {tuple(k.shape)}, {tuple(v.shape)} do not match q {tuple(q.shape)}")
-    if not (q.dtype == k.dtype == v.dtype):
+    if D not in (32, 64):
+        raise ValueError(f"head_dim must be 32 or 64 (got {D})")
+    dt = q.dtype
+    if not (dt == k.dtype == v.dtype):
         raise TypeError("q, k, v must share a dtype")
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"attn_train takes bf16 or fp16 (got {q.dtype})")
+    if dt not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"attn_train takes bf16 or fp16 (got {dt})")
     if pad_len is not None:
         if pad_len.shape != (B,):
             raise ValueError(f"pad_len must be [{B}] (got {tuple(pad_len.shape)})")
-        pad_len = pad_len.to(torch.int32).contiguous()
+        if pad_len.dtype != torch.int32 or not pad_len.is_contiguous():
+            pad_len = pad_len.to(torch.int32).contiguous()
     if scale is not None and not scale > 0:
         raise ValueError(f"scale must be positive (got {scale})")
-    return pad_len
+    return pad_len, B, S, Hq, kshape[2], D
 
 
 def attn_train_forward(q: Tensor, k: Tensor, v: Tensor, pad_len: Optional[Tensor] = None,
@@ -591,22 +607,19 @@ def attn_train_forward(q: Tensor, k: Tensor, v: Tensor, pad_len: Optional[Tensor
     gradient (attn_prefill, the inference form, gives them the reference's mean of V).  p, rng,
     site: dropout on the attention weights, see _check_dropout."""
     dev = _same_device(q, k, v, pad_len, rng)
-    pad_len = _check_attn_train(q, k, v, pad_len, scale)
+    pad_len, B, S, Hq, Hkv, D = _check_attn_train(q, k, v, pad_len, scale)
     p = _check_dropout(p, rng, site)
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    B, S, Hq, D = q.shape
-    Hkv = k.shape[2]
+    (q, qs), (k, ks), (v, vs) = _rows16(q), _rows16(k), _rows16(v)
     out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=dev)
     lse = torch.empty((B, Hq, S), dtype=torch.float32, device=dev)
-    if out.numel() == 0:
-        return out, lse
-    with _On(dev):
-        rc = _lib.load().dt_attn_train_forward(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(pad_len), B, S, Hq, Hkv, D, *q.stride()[:3],
-            *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], float(scale) if scale is not None else 0.0, p,
-            _ptr(rng), int(site), _dtype_code(q), _stream_ptr(dev))
-    _lib.check("dt_attn_train_forward", rc)
+    if out.numel():
+        _launch("dt_attn_train_forward", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                _ptr(pad_len), B, S, Hq, Hkv, D, *qs, *ks, *vs, S * Hq * D, Hq * D, D, scale or 0.0, p, _ptr(rng), site,
+                _dtype_code(q))
     return out, lse
+
+
+_PACK24 = struct.Struct("24q")
 
 
 def attn_train_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,
@@ -617,35 +630,34 @@ def attn_train_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tens
     results (the same rng contents, site and p).  ``grads``: tensors to write dq, dk and dv into
     (for instance the parts of one [B, S, Hq + 2 Hkv, D] gradient)."""
     dev = _same_device(q, k, v, dout, out, lse, pad_len, rng)
-    pad_len = _check_attn_train(q, k, v, pad_len, scale)
+    pad_len, B, S, Hq, Hkv, D = _check_attn_train(q, k, v, pad_len, scale)
     p = _check_dropout(p, rng, site)
-    B, S, Hq, D = q.shape
-    Hkv = k.shape[2]
-    if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:
+    dt = q.dtype
+    if dout.shape != q.shape or out.shape != q.shape or dout.dtype != dt or out.dtype != dt:
         raise ValueError("dout and out must have q's shape and dtype")
     if lse.shape != (B, Hq, S) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError("lse must be the forward call's [B, Hq, S] fp32 tensor")
-    q, k, v, dout, out = (_rows16(t) for t in (q, k, v, dout, out))
+    (q, qs), (k, ks), (v, vs), (dout, dos), (out, os) = (_rows16(t) for t in (q, k, v, dout, out))
     if grads is None:
-        grads = (torch.empty((B, S, Hq, D), dtype=q.dtype, device=dev),
-                 torch.empty((B, S, Hkv, D), dtype=q.dtype, device=dev),
-                 torch.empty((B, S, Hkv, D), dtype=q.dtype, device=dev))
-    dq, dk, dv = grads
-    _same_device(q, dq, dk, dv)
-    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        if t.shape != like.shape or t.dtype != q.dtype or (t.numel() and _rows16(t) is not t):
-            raise ValueError(f"{name} must be a {tuple(like.shape)} {q.dtype} tensor with contiguous D, 16-byte aligned "
-                             "rows and strides that are multiples of 8")
-    if dq.numel() == 0:
-        return dq, dk, dv
-    delta = torch.empty((B, Hq, S), dtype=torch.float32, device=dev)
-    strides = [s for t in (q, k, v, out, dout, dq, dk, dv) for s in t.stride()[:3]]
-    with _On(dev):
-        rc = _lib.load().dt_attn_train_backward(
-            _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(delta), _ptr(dq), _ptr(dk), _ptr(dv),
-            _ptr(pad_len), B, S, Hq, Hkv, D, (_lib._L * 24)(*strides), float(scale) if scale is not None else 0.0, p,
-            _ptr(rng), int(site), _dtype_code(q), _stream_ptr(dev))
-    _lib.check("dt_attn_train_backward", rc)
+        dq = torch.empty((B, S, Hq, D), dtype=dt, device=dev)
+        dk = torch.empty((B, S, Hkv, D), dtype=dt, device=dev)
+        dv = torch.empty((B, S, Hkv, D), dtype=dt, device=dev)
+        gs = (S * Hq * D, Hq * D, D) + 2 * (S * Hkv * D, Hkv * D, D)
+    else:
+        dq, dk, dv = grads
+        _same_device(q, dq, dk, dv)
+        gs = ()
+        for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+            if t.shape != like.shape or t.dtype != dt or (t.numel() and _rows16(t)[0] is not t):
+                raise ValueError(f"{name} must be a {tuple(like.shape)} {dt} tensor with contiguous D, 16-byte aligned "
+                                 "rows and strides that are multiples of 8")
+            gs += t.stride()[:3]
+    if dq.numel():
+        delta = torch.empty((B, Hq, S), dtype=torch.float32, device=dev)
+        _launch("dt_attn_train_backward", dev, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                out.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                _ptr(pad_len), B, S, Hq, Hkv, D, _PACK24.pack(*qs, *ks, *vs, *os, *dos, *gs), scale or 0.0, p,
+                _ptr(rng), site, _dtype_code(q))
     return dq, dk, dv
 
 
@@ -662,29 +674,28 @@ def rope_grad_(g: Tensor, cos: Tensor, sin: Tensor, rope_cols: int, head_dim: in
     cos, sin = _prep_tables(cos, sin)
     if cos.shape[-1] != head_dim or sin.shape != cos.shape:
         raise ValueError(f"cos / sin must be [rows, {head_dim}] tables")
-    with _On(dev):
-        rc = _lib.load().dt_rope_grad(_ptr(g), g.stride(1), g.shape[0] * g.shape[1], _ptr(cos), _ptr(sin),
-                                      cos.stride(0), cos.shape[0], g.shape[1], int(rope_cols), int(head_dim),
-                                      _dtype_code(g), _stream_ptr(dev))
-    _lib.check("dt_rope_grad", rc)
+    _launch("dt_rope_grad", dev, _ptr(g), g.stride(1), g.shape[0] * g.shape[1], _ptr(cos), _ptr(sin), cos.stride(0),
+            cos.shape[0], g.shape[1], int(rope_cols), int(head_dim), _dtype_code(g))
     return g
 
 
-def _rows2d(t: Tensor) -> Tensor:
-    """t as a [rows, K] view with a contiguous last dimension (a copy when no view exists)."""
-    t2 = t.reshape(-1, t.shape[-1])
-    return t2 if t2.stride(1) == 1 or t2.shape[1] == 1 else t2.contiguous()
+def _rows2d(t: Tensor) -> Tuple[Tensor, int]:
+    """t as [rows, K] with a contiguous last dimension (a copy when no view exists), and its row stride."""
+    K = t.shape[-1]
+    if t.is_contiguous():
+        return t, K
+    t2 = t.reshape(-1, K)
+    if t2.stride(1) != 1 and K != 1:
+        t2 = t2.contiguous()
+    return t2, t2.stride(0)
 
 
-def _gate_rows(gate: Optional[Tensor], x: Tensor) -> Tuple[Optional[Tensor], int]:
-    """The gate as [G, H] rows and the number of consecutive rows of x that share each: a gate of
-    shape [H], x's own shape, or x's shape with trailing ones before H ([B, 1, H] for [B, S, H])."""
-    if gate is None:
-        return None, 0
-    H = x.shape[-1]
-    lead = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape[:-1])
-    if gate.dim() > x.dim() or gate.shape[-1] != H:
+def _gate_rows(gate: Tensor, x: Tensor) -> int:
+    """The number of consecutive rows of x that share each row of the gate: a gate of shape [H], x's
+    own shape, or x's shape with trailing ones before H ([B, 1, H] for [B, S, H])."""
+    if gate.dim() > x.dim() or gate.dim() < 1 or gate.shape[-1] != x.shape[-1]:
         raise ValueError(f"gate {tuple(gate.shape)} does not broadcast to x {tuple(x.shape)}")
+    lead = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape[:-1])
     shared, shares = 1, False
     for g, n in zip(lead, x.shape[:-1]):
         if g == n and not (shares and n != 1):
@@ -694,22 +705,24 @@ def _gate_rows(gate: Optional[Tensor], x: Tensor) -> Tuple[Optional[Tensor], int
                              "before the last")
         shares = True
         shared *= n
-    return _rows2d(gate), shared
+    return shared
 
 
 def _check_residual_norm(x, residual, pre_weight, post_weight, gate):
-    if x.dim() < 1 or x.shape[-1] < 1:
+    dt, shape = x.dtype, x.shape
+    if x.dim() < 1 or shape[-1] < 1:
         raise ValueError("x must have a last dimension")
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"unsupported dtype {x.dtype}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
-    for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
-        if w is not None and (w.shape != x.shape[-1:] or not w.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous [{x.shape[-1]}] tensor")
-    for name, t in (("residual", residual), ("pre_weight", pre_weight), ("post_weight", post_weight), ("gate", gate)):
-        if t is not None and t.dtype != x.dtype:
-            raise TypeError(f"{name} must have x's dtype {x.dtype} (got {t.dtype})")
+    if dt not in _DTYPES:
+        raise TypeError(f"unsupported dtype {dt}")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(shape)}")
+    if pre_weight.shape != shape[-1:] or not pre_weight.is_contiguous():
+        raise ValueError(f"pre_weight must be a contiguous [{shape[-1]}] tensor")
+    if post_weight is not None and (post_weight.shape != shape[-1:] or not post_weight.is_contiguous()):
+        raise ValueError(f"post_weight must be a contiguous [{shape[-1]}] tensor")
+    for t in (residual, pre_weight, post_weight, gate):
+        if t is not None and t.dtype != dt:
+            raise TypeError(f"residual, weights and gate must have x's dtype {dt} (got {t.dtype})")
 
 
 def residual_norm_forward(x: Tensor, residual: Optional[Tensor], pre_weight: Tensor, eps: float,
@@ -727,21 +740,32 @@ def residual_norm_forward(x: Tensor, residual: Optional[Tensor], pre_weight: Ten
     dev = _same_device(x, residual, pre_weight, post_weight, gate, rng)
     _check_residual_norm(x, residual, pre_weight, post_weight, gate)
     p = _check_dropout(p, rng, site)
-    g2, gate_rows = _gate_rows(gate, x)
-    x2 = _rows2d(x)
-    r2 = None if residual is None else _rows2d(residual)
-    M, H = x2.shape
-    h, n = torch.empty(x.shape, dtype=x.dtype, device=dev), torch.empty(x.shape, dtype=x.dtype, device=dev)
+    H = x.shape[-1]
+    M = x.numel() // H
+    x2, xs = _rows2d(x)
+    r2, rs = (None, 0) if residual is None else _rows2d(residual)
+    g2, gs, gate_rows = None, 0, 0
+    if gate is not None:
+        gate_rows = _gate_rows(gate, x)
+        g2, gs = _rows2d(gate)
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    n = torch.empty(x.shape, dtype=x.dtype, device=dev)
     stats = torch.empty((M, 2), dtype=torch.float32, device=dev)
-    if M == 0:
-        return h, n, stats
-    with _On(dev):
-        rc = _lib.load().dt_residual_norm_forward(
-            _ptr(x2), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(g2),
-            0 if g2 is None else g2.stride(0), gate_rows, _ptr(pre_weight), _ptr(post_weight), _ptr(h), _ptr(n),
-            _ptr(stats), M, H, float(alpha), float(eps), p, _ptr(rng), int(site), _dtype_code(x), _stream_ptr(dev))
-    _lib.check("dt_residual_norm_forward", rc)
+    if M:
+        _launch("dt_residual_norm_forward", dev, x2.data_ptr(), xs, _ptr(r2), rs, _ptr(g2), gs, gate_rows,
+                pre_weight.data_ptr(), _ptr(post_weight), h.data_ptr(), n.data_ptr(), stats.data_ptr(), M, H, alpha,
+                eps, p, _ptr(rng), site, _dtype_code(x))
     return h, n, stats
+
+
+@functools.lru_cache(maxsize=1024)
+def _residual_norm_workspace(M: int, H: int, gate_rows: int, post: int, device: int) -> int:
+    """Bytes of scratch of residual_norm_backward (a rule on sizes and the device's SM count)."""
+    with torch.cuda.device(device):
+        size = _lib.load().dt_residual_norm_workspace(M, H, gate_rows, post)
+    if size < 0:
+        _lib.check("dt_residual_norm_workspace", -size)
+    return size
 
 
 def residual_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], x: Tensor, residual: Optional[Tensor],
@@ -754,38 +778,36 @@ def residual_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], x: Tensor
     dev = _same_device(x, dh, dn, residual, pre_weight, post_weight, gate, stats, rng)
     _check_residual_norm(x, residual, pre_weight, post_weight, gate)
     p = _check_dropout(p, rng, site)
-    for name, t in (("dh", dh), ("dn", dn)):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
-            raise ValueError(f"{name} must have x's shape and dtype")
-    g2, gate_rows = _gate_rows(gate, x)
-    x2 = _rows2d(x)
-    M, H = x2.shape
+    shape, dt = x.shape, x.dtype
+    for t in (dh, dn):
+        if t is not None and (t.shape != shape or t.dtype != dt):
+            raise ValueError("dh and dn must have x's shape and dtype")
+    H = shape[-1]
+    M = x.numel() // H
     if stats.shape != (M, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError("stats must be the forward call's [rows, 2] fp32 tensor")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dres = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dpost = None if post_weight is None else torch.empty_like(post_weight)
-    dgate = None if gate is None else torch.empty(gate.shape, dtype=x.dtype, device=dev)
+    gate_rows = 0 if gate is None else _gate_rows(gate, x)
+    dx = torch.empty(shape, dtype=dt, device=dev)
+    dres = torch.empty(shape, dtype=dt, device=dev)
+    dpost = None if post_weight is None else torch.empty(H, dtype=dt, device=dev)
+    dgate = None if gate is None else torch.empty(gate.shape, dtype=dt, device=dev)
     if M == 0 or (dh is None and dn is None):
         for t in (dx, dres, dpost, dgate):
             if t is not None:
                 t.zero_()
         return dx, dres, torch.zeros_like(pre_weight), dpost, dgate
-    dpre = torch.zeros_like(pre_weight) if dn is None else torch.empty_like(pre_weight)
-    r2, dh2, dn2 = (None if t is None else _rows2d(t) for t in (residual, dh, dn))
-    lib = _lib.load()
-    with _On(dev):
-        size = lib.dt_residual_norm_workspace(M, H, gate_rows, 0 if post_weight is None else 1)
-        if size < 0:
-            _lib.check("dt_residual_norm_workspace", -size)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        rc = lib.dt_residual_norm_backward(
-            _ptr(dh2), 0 if dh2 is None else dh2.stride(0), _ptr(dn2), 0 if dn2 is None else dn2.stride(0), _ptr(x2),
-            x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(g2), 0 if g2 is None else g2.stride(0),
-            gate_rows, _ptr(pre_weight), _ptr(post_weight), _ptr(stats), _ptr(dx), _ptr(dres), _ptr(dpre), _ptr(dpost),
-            _ptr(dgate), _ptr(ws), size, M, H, float(alpha), 0.0, p, _ptr(rng), int(site), _dtype_code(x),
-            _stream_ptr(dev))
-    _lib.check("dt_residual_norm_backward", rc)
+    dpre = torch.empty(H, dtype=dt, device=dev) if dn is not None else torch.zeros(H, dtype=dt, device=dev)
+    x2, xs = _rows2d(x)
+    r2, rs = (None, 0) if residual is None else _rows2d(residual)
+    g2, gs = (None, 0) if gate is None else _rows2d(gate)
+    dh2, dhs = (None, 0) if dh is None else _rows2d(dh)
+    dn2, dns = (None, 0) if dn is None else _rows2d(dn)
+    size = _residual_norm_workspace(M, H, gate_rows, 0 if post_weight is None else 1, dev.index)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _launch("dt_residual_norm_backward", dev, _ptr(dh2), dhs, _ptr(dn2), dns, x2.data_ptr(), xs, _ptr(r2), rs,
+            _ptr(g2), gs, gate_rows, pre_weight.data_ptr(), _ptr(post_weight), stats.data_ptr(), dx.data_ptr(),
+            dres.data_ptr(), dpre.data_ptr(), _ptr(dpost), _ptr(dgate), ws.data_ptr(), size, M, H, alpha, 0.0, p,
+            _ptr(rng), site, _dtype_code(x))
     return dx, dres, dpre, dpost, dgate
 
 
@@ -800,14 +822,13 @@ def dropout_forward(x: Tensor, p: float, rng: Optional[Tensor], site: int = 0,
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have x's shape and dtype")
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    if x.numel() == 0:
-        return y
-    x2, r2 = _rows2d(x), None if residual is None else _rows2d(residual)
-    M, H = x2.shape
-    with _On(dev):
-        rc = _lib.load().dt_dropout(_ptr(x2), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(y), H, M,
-                                    H, p, _ptr(rng), int(site), _dtype_code(x), _stream_ptr(dev))
-    _lib.check("dt_dropout", rc)
+    n = y.numel()
+    if n:
+        H = x.shape[-1]
+        x2, xs = _rows2d(x)
+        r2, rs = (None, 0) if residual is None else _rows2d(residual)
+        _launch("dt_dropout", dev, x2.data_ptr(), xs, _ptr(r2), rs, y.data_ptr(), H, n // H, H, p, _ptr(rng), site,
+                _dtype_code(x))
     return y
 
 

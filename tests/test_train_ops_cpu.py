@@ -73,15 +73,13 @@ def test_argument_checks_on_the_host():
     from rl_for_mario_b200 import kernels as K
 
     x = torch.zeros(2, 3, 8)
-    assert K._gate_rows(None, x) == (None, 0)
-    for shape, rows, shared in (((8,), 1, 6), ((1, 8), 1, 6), ((2, 1, 8), 2, 3), ((1, 1, 8), 1, 6), ((2, 3, 8), 6, 1)):
-        g, s = K._gate_rows(torch.zeros(shape), x)
-        assert tuple(g.shape) == (rows, 8) and s == shared
+    for shape, shared in (((8,), 6), ((1, 8), 6), ((2, 1, 8), 3), ((1, 1, 8), 6), ((2, 3, 8), 1)):
+        assert K._gate_rows(torch.zeros(shape), x) == shared
     for shape in ((3, 8), (1, 3, 8), (7,), (1, 2, 3, 8), (2, 2, 8)):
         with pytest.raises(ValueError, match="gate"):
             K._gate_rows(torch.zeros(shape), x)
     one = torch.zeros(1, 3, 8)
-    assert K._gate_rows(torch.zeros(1, 1, 8), one)[1] == 3 and K._gate_rows(torch.zeros(3, 8), one)[1] == 1
+    assert K._gate_rows(torch.zeros(1, 1, 8), one) == 3 and K._gate_rows(torch.zeros(3, 8), one) == 1
     with pytest.raises(TypeError, match="dtype"):
         K._check_residual_norm(x, x.bfloat16(), torch.ones(8), None, None)
     with pytest.raises(ValueError, match="residual"):
