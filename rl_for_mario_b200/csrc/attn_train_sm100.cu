@@ -1,563 +1,1323 @@
-// Causal grouped-query attention for training, with its gradient.
+// Causal grouped-query attention for training, with its gradient, on the tcgen05
+// tensor cores.
 //
 // For a query row q >= pad of head h (KV head g = h / R) and keys j in pad..q:
-//   s_j = scale q . k_j,   P_j = exp(s_j) / sum exp,   O = sum_j m_j P_j v_j / (1 - p)
-// with m the dropout mask (philox.cuh).  Rows q < pad see no key: O = 0, no
-// gradient.  Backward, with m' = m / (1 - p):
+//   s_j = scale q . k_j,   P_j = exp(s_j) / sum exp,   O = sum_j m'_j P_j v_j
+// with m' = m / (1 - p), m the dropout mask (philox.cuh).  Rows q < pad see no
+// key: O = 0, no gradient.  Backward:
 //   dV_j = sum_q m' P dO,   dP_j = m' dO . v_j,   delta = sum_j P_j dP_j = O . dO
 //   dS_j = P_j (dP_j - delta),   dq = scale sum_j dS_j k_j,   dk_j = scale sum_q dS_j q
-// The forward pass keeps log2 sum exp2 of each row (base-2 logarithm of the
-// softmax's denominator), so the backward passes form P again from one product.
+// The forward pass keeps log2 of each row's softmax denominator (base 2), so the
+// backward passes form P again from one product.
 //
-// Two backward kernels: one walks the keys of 64 query rows (delta and dq), one
-// walks the query rows of all R heads behind 64 keys (dk and dv).  Each sum has
-// one owner, so there are no atomics and every run gives the same bits; the
-// price is that S and dP are formed twice.
+// Two backward kernels: one walks the keys of a tile of query rows (delta, dq),
+// one walks the query rows behind a tile of keys (dk, dv).  Each sum has one
+// owner: no atomics, the same bits every run; the price is that S and dP are
+// formed twice.
 //
 // Rounding: P and dS enter the second products in the inputs' 16-bit type, as
 // the tensor cores take both operands in one type; sums, softmax statistics
 // and delta are fp32.  A row with a single key has a constant softmax: its dS
-// is set to exactly zero.  Where a row's keys lie in one tile delta is the sum
+// is set to exactly zero.  Where a tile's keys are one block, delta is the sum
 // over the unrounded P dP; beyond, it is O . dO with the stored O.
-#include "attn_train_common.cuh"
+//
+// Geometry.  A tile of 128 query rows packs (position, head) pairs of the HC
+// query heads that share a KV head (head fastest), so a group's K and V are
+// fetched once and a short sequence still fills an MMA; HC = R up to 64 heads,
+// else chunks of 64.  Tiles of query rows start at the first unpadded position,
+// blocks and tiles of keys at the multiple of 8 before it (where a block of the
+// dropout generator starts): padding costs nothing, and the up to seven padded
+// keys of a first block are zeroed in shared memory, so what stands there never
+// meets a product (a NaN times a zero weight would be a NaN).
+//
+// Persistent CTAs, two on each SM.  One thread loads tiles and blocks by TMA, one
+// issues the MMAs; the other warps are the element-wise part, one thread per row
+// (forward) or two (backward).  Per block of 64:
+//   forward   S = Q K^T             P -> TMEM, O += P V
+//   dq        S = Q K^T, dP = dO V^T    dS -> TMEM, dQ += dS K
+//   dk, dv    S^T = K Q^T, dP^T = V dO^T    P^T, dS^T -> TMEM, dV += P^T dO, dK += dS^T Q
+// The left operand of every second product goes back to tensor memory, the
+// right one is the shared-memory tile as TMA left it, read row-major ("MN
+// major").  The next block's scores are issued as soon as this block's are in
+// registers (forward, dq: the weights have columns of their own); for dk and dv
+// the 512 columns do not hold both, so P^T lies over S^T and dS^T over dP^T, and
+// the two halves of a block alternate: while the threads form dS^T of a block,
+// dV += P^T dO and the next S^T run, and during the next exponentials
+// dK += dS^T Q and the next dP^T.  MMAs of one thread execute in order, which is
+// what lets a block's scores be issued behind the products that still read the
+// previous block's weights in the same columns.
+//
+// What bounds it: an MMA of N = 64 costs about 50 cycles whatever its K, so at
+// head_dim 64 a 128 x 64 block takes 400 (forward), 600 (dq) and 800 (dk, dv)
+// tensor cycles, about as long as its element-wise part (one exponential, and
+// with dropout an eighth of a generator call, for each score).
+#include <utility>
+
+#include "dt_common.cuh"
+#include "dt_internal.h"
+#include "philox.cuh"
+#include "prefill_common.cuh"
 
 namespace dtk {
 
 namespace {
 
-constexpr int kT = 64;        // query rows and keys of a tile
-constexpr int kThreads = 128;
+template <int I>
+struct Int {
+  static constexpr int value = I;
+};
 
+constexpr int kRows = 128;   // rows of a tile
+constexpr int kBlk = 64;     // rows of a block of the other axis
+constexpr int kMaxStages = 4;
+constexpr int kPerSm = 2;       // CTAs on an SM: each takes half of its tensor memory
+constexpr uint32_t kCols = 256;
+constexpr int kFwdBufs = 2;     // score buffers of the forward kernel
+constexpr int kGroupUnits = 128;  // units scheduled together (their K / V stay in L2)
 
-// Keep bits of a warp's 16 query rows x 64 keys: lane l holds 32 bits, blocks
-// 4 (l / 16) .. + 4 of row l % 16.
-__device__ __forceinline__ uint32_t keep_rows(const DropKey& key, unsigned long long row_block0, unsigned per_row,
-                                              int lane, uint32_t threshold) {
-  const unsigned long long b = row_block0 + (unsigned long long)(lane & 15) * per_row + (lane >> 4) * 4;
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m |= keep_bits(key, b + i, threshold) << (8 * i);
-  return m;
+template <int D>
+struct TcShape {
+  static constexpr int ROWB = D * 2;
+  static constexpr uint32_t LAYOUT = D == 64 ? kSw128 : kSw64;
+  static constexpr int SBO = 8 * ROWB;
+  static constexpr int TILE = kRows * ROWB;
+  static constexpr int BLK = kBlk * ROWB;
+  static constexpr int NCH = ROWB / 16;
+  // Tile buffers of the backward kernels and blocks in flight: what the memory of two CTAs allows.
+  static constexpr int BWD_TILES = D == 64 ? 1 : 2;
+  static constexpr int DQ_STAGES = D == 64 ? 3 : 4;
+  static constexpr int STAGES = 4;
+};
+
+// An item as the loading thread hands it to the element-wise warps.
+constexpr int kItems = 8;
+struct alignas(16) Item {
+  int nblk, pad, heads, tile;  // blocks (-1: no more items); heads of the chunk
+  int first, origin, per, chunk0;  // rows: p0, kb; keys: q0, k0 and blocks of a chunk of heads
+  long long row;   // of lse, delta and the dropout rows: sample and first head, position 0
+  long long out, out2;  // element offsets of the outputs at that sample and head, position 0
+};
+
+// Barriers and small shared state behind the tiles.
+struct TcShared {
+  uint64_t tile_full[2], tile_empty[2], blk_full[kMaxStages], blk_empty[kMaxStages];
+  uint64_t s_full[2], s_read[2], dp_full, p_full, ds_full, w_done, o_empty, drain;
+  uint64_t item_full[kItems], item_empty[kItems];
+  Item item[kItems];  // the items under way
+  int2 tile_meta[8];  // blocks and padded keys of the tiles under way (0 blocks: no more tiles)
+  uint32_t tmem;
+  int abort;
+};
+
+// How a kernel's items are numbered: units in groups, inside a group the tiles
+// with the most work first (longest_last: a unit's last tile has the most blocks).
+struct Grid {
+  int units, tiles, items, chunks;
+  FastDiv by_tiles, by_chunks, by_kv;
+};
+struct TcItem {
+  int unit, tile;
+};
+__device__ __forceinline__ TcItem tc_item(const Grid& gr, int i, bool longest_last) {
+  static_assert(kGroupUnits == 128, "shifts below");
+  const int grp = gr.by_tiles(i >> 7);
+  const int j = i - grp * (kGroupUnits * gr.tiles);
+  const int gu = min(kGroupUnits, gr.units - grp * kGroupUnits);
+  const int t = gu == kGroupUnits ? j >> 7 : j / gu;
+  return TcItem{grp * kGroupUnits + (j - t * gu), longest_last ? gr.tiles - 1 - t : t};
 }
 
-template <int D, bool BF16, bool DROP>
-__global__ void __launch_bounds__(kThreads) attn_train_fwd_kernel(const AttnTrainParams p, int ntiles) {
-  constexpr int TB = kT * D * 2;
-  __shared__ __align__(1024) uint8_t smem[5 * TB];
-  const uint32_t sq = smem_u32(smem), sk = sq + TB, sv = sq + 3 * TB;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
-  const int qt = ntiles - 1 - (int)(blockIdx.x % (unsigned)ntiles);
-  const unsigned bh = blockIdx.x / (unsigned)ntiles;
-  const int b = (int)(bh / (unsigned)p.Hq), h = (int)(bh % (unsigned)p.Hq), g = h / p.R;
-  const int S = p.S, q0 = qt * kT;
-  const int pad = p.pad_len ? min(max(__ldg(p.pad_len + b), 0), S) : 0;
-  const int q_end = min(S, q0 + kT);
-  uint16_t* o = static_cast<uint16_t*>(p.o) + b * p.o_sb + h * p.o_sh;
-  float* lse = p.lse + ((long long)b * p.Hq + h) * S;
-  using E = Elem<BF16>;
+// The k-th item of this CTA: rounds of one item for each CTA, every other one
+// backwards, so that a CTA with a heavy item gets a light one next.
+__device__ __forceinline__ int nth_item(int k, int n_items) {
+  const long long i = (long long)k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  return (int)min(i, (long long)n_items);
+}
 
-  float acc[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const float c2 = p.scale * 1.4426950408889634f;
+// A tile of query rows: sample b, KV head g, the chunk of HC query heads from h0
+// on, positions p0 .. p0 + PT, and the key blocks kb + 64 j, j < nblk.
+struct QTile {
+  static constexpr bool kRowTiles = true;
+  int b, g, h0, heads, pad, p0, kb, nblk, tile, zero;  // zero: padded keys of the first block
+};
+// A tile of keys k0 .. k0 + 128 of KV head g and the blocks of PT positions (from
+// q0 on: earlier queries see none of these keys) x chunks of heads behind it.
+struct KTile {
+  static constexpr bool kRowTiles = false;
+  int b, g, pad, k0, q0, per, nblk, tile, zero;
+};
 
-  if (q_end > pad) {
-    const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_sb + h * p.q_sh;
-    const uint16_t* k = static_cast<const uint16_t*>(p.k) + b * p.k_sb + g * p.k_sh;
-    const uint16_t* v = static_cast<const uint16_t*>(p.v) + b * p.v_sb + g * p.v_sh;
-    DropKey key{};
-    const unsigned per_row = (unsigned)(S + 7) >> 3;
-    unsigned long long blk = 0;
-    if constexpr (DROP) {
-      key = drop_key(p.rng, p.site);
-      blk = ((unsigned long long)bh * (unsigned)S + (unsigned)(q0 + warp * 16)) * per_row;
-    }
-    const int kt0 = pad / kT;
-    load_tile<D, kT, kThreads>(sq, q, p.q_ss, q0, pad, S, tid);
-    load_tile<D, kT, kThreads>(sk, k, p.k_ss, kt0 * kT, pad, S, tid);
-    load_tile<D, kT, kThreads>(sv, v, p.v_ss, kt0 * kT, pad, S, tid);
-    cp_async_commit();
-    uint32_t qa[D / 16][4];
-    for (int kt = kt0; kt <= qt; ++kt) {
-      const int buf = (kt - kt0) & 1;
-      cp_async_wait<0>();
-      __syncthreads();
-      if (kt < qt) {
-        load_tile<D, kT, kThreads>(sk + (buf ^ 1) * TB, k, p.k_ss, (kt + 1) * kT, pad, S, tid);
-        load_tile<D, kT, kThreads>(sv + (buf ^ 1) * TB, v, p.v_ss, (kt + 1) * kT, pad, S, tid);
-        cp_async_commit();
-      }
-      if (kt == kt0)
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) frag_a<D>(sq, warp * 16, 2 * i, lane, qa[i]);
-      float s[8][4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t bb[4];
-          frag_b<D>(sk + buf * TB, 16 * j, 2 * i, lane, bb);
-          mma16816<BF16>(s[2 * j], qa[i], bb[0], bb[1]);
-          mma16816<BF16>(s[2 * j + 1], qa[i], bb[2], bb[3]);
-        }
-      if (kt == qt || kt * kT < pad) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int kk = kt * kT + 8 * j + 2 * t4 + (e & 1), qq = q0 + warp * 16 + g8 + (e >> 1) * 8;
-            if (kk > qq || kk < pad) s[j][e] = -INFINITY;
-          }
-      }
-      float mu[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float x = m[r];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x = fmaxf(x, fmaxf(s[j][2 * r], s[j][2 * r + 1]) * c2);
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        mu[r] = x == -INFINITY ? 0.f : x;
-        const float f = ex2_approx(m[r] - mu[r]);
-        m[r] = x;
-        l[r] *= f;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          acc[i][2 * r] *= f;
-          acc[i][2 * r + 1] *= f;
-        }
-      }
-      uint32_t keep = 0xffffffffu;
-      if constexpr (DROP) keep = keep_rows(key, blk + (unsigned)kt * (kT / 8), per_row, lane, p.threshold);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float x0 = ex2_approx(fmaf(s[j][2 * r], c2, -mu[r])), x1 = ex2_approx(fmaf(s[j][2 * r + 1], c2, -mu[r]));
-          l[r] += x0 + x1;
-          if constexpr (DROP) {
-            const uint32_t bits = __shfl_sync(0xffffffffu, keep, g8 + 8 * r + (j >> 2) * 16) >> ((j & 3) * 8 + 2 * t4);
-            s[j][2 * r] = bits & 1u ? x0 : 0.f;
-            s[j][2 * r + 1] = bits & 2u ? x1 : 0.f;
-          } else {
-            s[j][2 * r] = x0;
-            s[j][2 * r + 1] = x1;
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t a[4] = {E::from_f2(s[2 * j][0], s[2 * j][1]), E::from_f2(s[2 * j][2], s[2 * j][3]),
-                               E::from_f2(s[2 * j + 1][0], s[2 * j + 1][1]),
-                               E::from_f2(s[2 * j + 1][2], s[2 * j + 1][3])};
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t bb[4];
-          frag_bt<D>(sv + buf * TB, 16 * j, 2 * i, lane, bb);
-          mma16816<BF16>(acc[2 * i], a, bb[0], bb[1]);
-          mma16816<BF16>(acc[2 * i + 1], a, bb[2], bb[3]);
-        }
-      }
-    }
+// The CTA's items in order; the padding of the next one is on its way while one is
+// worked on.
+template <class T>
+struct Items {
+  struct Head {
+    int i, b, g, chunk, tile, pad;
+  };
+  static constexpr bool kRowTiles = T::kRowTiles;
+  int k = 0;
+  Head next;
+  __device__ __forceinline__ Items(const AttnTrainParams& p, const Grid& gr) { fetch(p, gr); }
+  __device__ __forceinline__ void fetch(const AttnTrainParams& p, const Grid& gr) {
+    next.i = nth_item(k++, gr.items);
+    if (next.i >= gr.items) return;
+    const TcItem it = tc_item(gr, next.i, kRowTiles);
+    const int bg = kRowTiles ? gr.by_chunks(it.unit) : it.unit;
+    next.chunk = it.unit - bg * (kRowTiles ? gr.chunks : 1);
+    next.b = gr.by_kv(bg);
+    next.g = bg - next.b * p.Hkv;
+    next.tile = it.tile;
+    next.pad = p.pad_len ? __ldg(p.pad_len + next.b) : 0;
   }
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = q0 + warp * 16 + g8 + 8 * r;
-    float sum = l[r];
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    if (row >= S) continue;
-    const float inv = sum > 0.f ? p.inv_keep / sum : 0.f;
-    if (t4 == 0) lse[row] = sum > 0.f ? m[r] + log2f(sum) : INFINITY;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-      *reinterpret_cast<uint32_t*>(o + row * p.o_ss + 8 * i + 2 * t4) =
-          E::from_f2(acc[i][2 * r] * inv, acc[i][2 * r + 1] * inv);
+  // False behind the last item.
+  __device__ __forceinline__ bool get(const AttnTrainParams& p, const Grid& gr, T& t) {
+    if (next.i >= gr.items) return false;
+    const Head h = next;
+    fetch(p, gr);
+    t.b = h.b;
+    t.g = h.g;
+    t.pad = min(max(h.pad, 0), p.S);
+    t.tile = h.tile;
+    if constexpr (kRowTiles) {
+      t.h0 = h.g * p.R + h.chunk * p.HC;
+      t.heads = min(p.HC, p.R - h.chunk * p.HC);
+      t.p0 = t.pad + h.tile * p.PT128;
+      t.kb = t.pad & ~7;
+      t.nblk = t.p0 < p.S ? (min(t.p0 + p.PT128, p.S) - 1 - t.kb) / kBlk + 1 : 0;
+      t.zero = t.pad - t.kb;
+    } else {
+      t.k0 = (t.pad & ~7) + h.tile * kRows;
+      t.q0 = max(t.k0, t.pad);
+      t.per = t.q0 < p.S ? p.by_pt64(p.S - t.q0 + p.PT64 - 1) : 0;
+      t.nblk = t.per * gr.chunks;
+      t.zero = 0;
+    }
+    return true;
+  }
+};
+
+// Whether the phase with this parity has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status));
+}
+
+// Zeros rows [rows, total) of `count` tiles of `bytes` bytes each (the rows that
+// TMA never fills when the packed heads leave some over).
+template <int ROWB>
+__device__ __forceinline__ void zero_rows(uint8_t* tiles, int count, int bytes, int rows, int total, int tid,
+                                          int threads) {
+  const int per = (total - rows) * (ROWB / 16);
+  for (int e = tid; e < count * per; e += threads) {
+    const int t = e / per, rem = e - t * per;
+    *reinterpret_cast<uint4*>(tiles + t * bytes + rows * ROWB + rem * 16) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
-// delta and dq of 64 query rows of one head.
-template <int D, bool BF16, bool DROP>
-__global__ void __launch_bounds__(kThreads) attn_train_dq_kernel(const AttnTrainParams p, int ntiles) {
-  constexpr int TB = kT * D * 2;
-  __shared__ __align__(1024) uint8_t smem[5 * TB];
-  __shared__ float sdelta[kT];
-  const uint32_t sq = smem_u32(smem), sk = sq + TB, sv = sq + 3 * TB;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
-  const int qt = ntiles - 1 - (int)(blockIdx.x % (unsigned)ntiles);
-  const unsigned bh = blockIdx.x / (unsigned)ntiles;
-  const int b = (int)(bh / (unsigned)p.Hq), h = (int)(bh % (unsigned)p.Hq), g = h / p.R;
-  const int S = p.S, q0 = qt * kT;
-  const int pad = p.pad_len ? min(max(__ldg(p.pad_len + b), 0), S) : 0;
-  const int q_end = min(S, q0 + kT);
-  uint16_t* dq = static_cast<uint16_t*>(p.dq) + b * p.dq_sb + h * p.dq_sh;
+// Eight fp32 values, scaled, as 16 bytes.
+template <bool BF16>
+__device__ __forceinline__ uint4 pack8(const uint32_t* v, float f) {
   using E = Elem<BF16>;
+  return make_uint4(E::from_f2(__uint_as_float(v[0]) * f, __uint_as_float(v[1]) * f),
+                    E::from_f2(__uint_as_float(v[2]) * f, __uint_as_float(v[3]) * f),
+                    E::from_f2(__uint_as_float(v[4]) * f, __uint_as_float(v[5]) * f),
+                    E::from_f2(__uint_as_float(v[6]) * f, __uint_as_float(v[7]) * f));
+}
 
-  float acc[D / 8][4];
+// Scores of one tile against one block: D[128 x 64] = A[128 x D] B[64 x D]^T.
+template <int D>
+__device__ __forceinline__ void issue_scores(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i)
+  for (int kk = 0; kk < D / 16; ++kk) umma_f16_ss(tmem_d, a + 2 * kk, b + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+}
+// D[128 x D] += A[128 x 64] B[64 x D] with A in tensor memory: its first 32 columns
+// in 16 columns of 32 bits, the others half_step columns further.
+template <int D>
+__device__ __forceinline__ void issue_weights(uint32_t tmem_d, uint32_t tmem_a, uint32_t half_step, uint64_t b,
+                                              uint32_t idesc, bool accumulate) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+  for (int kk = 0; kk < kBlk / 16; ++kk)
+    umma_f16_ts(tmem_d, tmem_a + (uint32_t)(kk >> 1) * half_step + (uint32_t)((kk & 1) * 8),
+                b + (uint64_t)(kk * 16 * TcShape<D>::ROWB >> 4), idesc, (accumulate || kk > 0) ? 1u : 0u);
+}
 
-  if (q_end > pad) {
-    const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_sb + h * p.q_sh;
-    const uint16_t* k = static_cast<const uint16_t*>(p.k) + b * p.k_sb + g * p.k_sh;
-    const uint16_t* v = static_cast<const uint16_t*>(p.v) + b * p.v_sb + g * p.v_sh;
-    const uint16_t* dout = static_cast<const uint16_t*>(p.dout) + b * p.do_sb + h * p.do_sh;
+__device__ __forceinline__ void tc_init(TcShared* sh, int warps) {
+  for (int i = 0; i < 2; ++i) {
+    mbar_init(&sh->tile_full[i], 1);
+    mbar_init(&sh->tile_empty[i], 1);
+    mbar_init(&sh->s_full[i], 1);
+    mbar_init(&sh->s_read[i], warps);
+  }
+  for (int i = 0; i < kMaxStages; ++i) {
+    mbar_init(&sh->blk_full[i], 1);
+    mbar_init(&sh->blk_empty[i], 1);
+  }
+  for (int i = 0; i < kItems; ++i) {
+    mbar_init(&sh->item_full[i], 1);
+    mbar_init(&sh->item_empty[i], warps);
+  }
+  mbar_init(&sh->dp_full, 1);
+  mbar_init(&sh->p_full, warps);
+  mbar_init(&sh->ds_full, warps);
+  mbar_init(&sh->w_done, 1);
+  mbar_init(&sh->o_empty, warps);
+  mbar_init(&sh->drain, 1);
+  sh->abort = 0;
+  fence_mbar_init();
+}
+
+// The loading thread, the same for the three kernels: the tiles and blocks of the
+// CTA's items in order, each into the next of TB tile buffers and STAGES stages,
+// and each item's numbers into the ring that the element-wise warps read.
+template <int TB, int STAGES, class T, class Describe, class LoadTile, class LoadBlk>
+__device__ __forceinline__ void load_all(TcShared* sh, const AttnTrainParams& p, const Grid& gr, Describe describe,
+                                         LoadTile load_tile, LoadBlk load_blk) {
+  volatile int* abort = &sh->abort;
+  Items<T> items(p, gr);
+  T t;
+  int blocks = 0, tiles = 0, n = 0;
+  bool ok = true, more = true;
+  while (more) {
+    more = items.get(p, gr, t);
+    const int slot = n % kItems;
+    if (!(ok = mbar_wait(&sh->item_empty[slot], ((n / kItems) & 1) ^ 1, abort, p.status))) break;
+    if (more)
+      describe(t, sh->item[slot]);
+    else
+      sh->item[slot].nblk = -1;
+    mbar_arrive(&sh->item_full[slot]);
+    ++n;
+    if (!more || t.nblk == 0) continue;
+    if (!(ok = mbar_wait(&sh->tile_empty[tiles % TB], ((tiles / TB) & 1) ^ 1, abort, p.status))) break;
+    sh->tile_meta[tiles & 7] = make_int2(t.nblk, t.zero);
+    load_tile(t, tiles % TB);
+    ++tiles;
+    for (int j = 0; j < t.nblk; ++j, ++blocks) {
+      const int st = blocks % STAGES;
+      if (!(ok = mbar_wait(&sh->blk_empty[st], ((blocks / STAGES) & 1) ^ 1, abort, p.status))) break;
+      load_blk(t, j, st);
+    }
+    if (!ok) break;
+  }
+  // Every copy must have landed before the CTA may end: after an error nobody else waits for them.
+  for (int q = max(0, tiles - TB); q < tiles; ++q) mbar_wait(&sh->tile_full[q % TB], (q / TB) & 1, nullptr, nullptr);
+  for (int q = max(0, blocks - STAGES); q < blocks; ++q)
+    mbar_wait(&sh->blk_full[q % STAGES], (q / STAGES) & 1, nullptr, nullptr);
+  if (ok && mbar_wait(&sh->tile_empty[tiles % TB], ((tiles / TB) & 1) ^ 1, abort, p.status)) {
+    sh->tile_meta[tiles & 7] = make_int2(0, 0);
+    mbar_arrive(&sh->tile_full[tiles % TB]);
+  }
+}
+
+// The thread that issues the MMAs of the forward and dq kernels: SB score
+// buffers, weights in columns of their own.
+template <int SB, int TB, int STAGES, class Prepare, class Scores, class Weights>
+__device__ __forceinline__ void issue_rows(TcShared* sh, int* status, Prepare prepare, Scores scores, Weights weights) {
+  volatile int* abort = &sh->abort;
+  int sblk = 0, stile = 0, sj = 0, sn = 0;  // next scores: block, tile, block within it, the tile's blocks
+  bool ok = true, end = false;
+  // Issues the next scores; without `wait` only if their operands are there.
+  auto next_scores = [&](bool wait) {
+    const int tb = stile % TB, st = sblk % STAGES;
+    if (sj == 0) {
+      if (!wait && !mbar_test(&sh->tile_full[tb], (stile / TB) & 1)) return;
+      if (!(ok = mbar_wait(&sh->tile_full[tb], (stile / TB) & 1, abort, status))) return;
+      sn = sh->tile_meta[stile & 7].x;
+      if (sn == 0) {
+        end = true;
+        return;
+      }
+    }
+    if (!wait && !mbar_test(&sh->blk_full[st], (sblk / STAGES) & 1)) return;
+    if (!(ok = mbar_wait(&sh->blk_full[st], (sblk / STAGES) & 1, abort, status))) return;
+    if (sj == 0) prepare(sh->tile_meta[stile & 7].y, st);
+    tc_fence_after();
+    scores(tb, st, sblk % SB);
+    umma_commit(&sh->s_full[sblk % SB]);
+    ++sblk;
+    if (++sj == sn) {
+      umma_commit(&sh->tile_empty[tb]);
+      sj = 0;
+      ++stile;
+    }
+  };
+  int tiles = 0, j = 0, n = 0;  // the block whose weights come next: tile, block within it, the tile's blocks
+  for (int blk = 0; ok; ++blk) {
+    while (ok && !end && sblk <= blk) next_scores(true);
+    if (!ok || sblk <= blk) break;
+    if (SB > 1 && !end && sblk < blk + SB) next_scores(false);
+    // The scores of this block being in registers, their buffer takes the next ones.
+    if (!ok || !(ok = mbar_wait(&sh->s_read[blk % SB], (blk / SB) & 1, abort, status))) break;
+    if (!end && sblk == blk + SB) next_scores(false);
+    if (!ok || !(ok = mbar_wait(&sh->p_full, blk & 1, abort, status))) break;
+    if (j == 0) {
+      n = sh->tile_meta[tiles & 7].x;
+      if (tiles > 0 && !(ok = mbar_wait(&sh->o_empty, (tiles - 1) & 1, abort, status))) break;
+    }
+    tc_fence_after();
+    weights(blk % STAGES, j > 0);
+    umma_commit(&sh->w_done);
+    umma_commit(&sh->blk_empty[blk % STAGES]);
+    if (++j == n) {
+      j = 0;
+      ++tiles;
+    }
+  }
+  umma_commit(&sh->drain);
+  mbar_wait(&sh->drain, 0, nullptr, nullptr);
+}
+
+// The same for the dk, dv kernel: weights over their scores, the two halves of a
+// block in turn.
+template <int TB, int STAGES, class ScoresA, class ScoresB, class WeightsA, class WeightsB>
+__device__ __forceinline__ void issue_keys(TcShared* sh, int* status, ScoresA scores_a, ScoresB scores_b,
+                                           WeightsA weights_a, WeightsB weights_b) {
+  volatile int* abort = &sh->abort;
+  int a_blk = 0, a_tile = 0, a_j = 0, a_n = 0;  // next scores of the first half
+  int b_blk = 0, b_tile = 0, b_j = 0;           // and of the second
+  bool ok = true, end = false;
+  auto next_a = [&](bool wait) {
+    const int tb = a_tile % TB, st = a_blk % STAGES;
+    if (a_j == 0) {
+      if (!wait && !mbar_test(&sh->tile_full[tb], (a_tile / TB) & 1)) return;
+      if (!(ok = mbar_wait(&sh->tile_full[tb], (a_tile / TB) & 1, abort, status))) return;
+      a_n = sh->tile_meta[a_tile & 7].x;
+      if (a_n == 0) {
+        end = true;
+        return;
+      }
+    }
+    if (!wait && !mbar_test(&sh->blk_full[st], (a_blk / STAGES) & 1)) return;
+    if (!(ok = mbar_wait(&sh->blk_full[st], (a_blk / STAGES) & 1, abort, status))) return;
+    tc_fence_after();
+    scores_a(tb, st);
+    umma_commit(&sh->s_full[0]);
+    ++a_blk;
+    if (++a_j == a_n) {
+      a_j = 0;
+      ++a_tile;
+    }
+  };
+  auto next_b = [&]() {  // behind next_a of the same block, whose waits it shares
+    scores_b(b_tile % TB, b_blk % STAGES);
+    umma_commit(&sh->dp_full);
+    ++b_blk;
+    if (++b_j == sh->tile_meta[b_tile & 7].x) {
+      umma_commit(&sh->tile_empty[b_tile % TB]);
+      b_j = 0;
+      ++b_tile;
+    }
+  };
+  int tiles = 0, j = 0, n = 0;
+  for (int blk = 0; ok; ++blk) {
+    while (ok && !end && a_blk <= blk) next_a(true);
+    if (!ok || a_blk <= blk) break;
+    if (b_blk <= blk) next_b();
+    if (!(ok = mbar_wait(&sh->p_full, blk & 1, abort, status))) break;
+    if (j == 0) {
+      n = sh->tile_meta[tiles & 7].x;
+      if (tiles > 0 && !(ok = mbar_wait(&sh->o_empty, (tiles - 1) & 1, abort, status))) break;
+    }
+    tc_fence_after();
+    weights_a(blk % STAGES, j > 0);
+    if (!end) next_a(false);
+    if (!ok || !(ok = mbar_wait(&sh->ds_full, blk & 1, abort, status))) break;
+    tc_fence_after();
+    weights_b(blk % STAGES, j > 0);
+    umma_commit(&sh->blk_empty[blk % STAGES]);
+    if (++j == n) {
+      umma_commit(&sh->w_done);
+      j = 0;
+      ++tiles;
+    }
+    if (b_blk < a_blk) next_b();
+  }
+  umma_commit(&sh->drain);
+  mbar_wait(&sh->drain, 0, nullptr, nullptr);
+}
+
+// The element-wise warps' side of the item ring.
+struct ItemReader {
+  TcShared* sh;
+  volatile int* abort;
+  int* status;
+  int n = 0;
+  __device__ __forceinline__ const Item* get(bool& ok) {  // the next item
+    ok = warp_wait(&sh->item_full[n % kItems], (n / kItems) & 1, abort, status);
+    return &sh->item[n % kItems];
+  }
+  __device__ __forceinline__ void next() {  // done with it (one lane of each warp says so)
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->item_empty[n % kItems]);
+    ++n;
+  }
+};
+
+// Zeros the rows of a first block that lie before the padding's end (key block
+// origin a multiple of 8), in both tensors of stage st.
+template <int D>
+__device__ __forceinline__ void zero_padded_keys(uint8_t* ring_a, uint8_t* ring_b, int st, int count) {
+  using SH = TcShape<D>;
+  if (count == 0) return;
+  for (int e = 0; e < count * SH::NCH; ++e) {
+    *reinterpret_cast<uint4*>(ring_a + st * SH::BLK + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+    *reinterpret_cast<uint4*>(ring_b + st * SH::BLK + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  fence_proxy_async_smem();
+}
+
+// ---------------------------------------------------------------- forward
+constexpr int kFwdThreads = 192;  // a warpgroup of rows, the MMA warp, the loading warp
+
+template <int D>
+struct FwdSmem {
+  using SH = TcShape<D>;
+  static constexpr int OFF_K = 2 * SH::TILE;
+  static constexpr int OFF_V = OFF_K + SH::STAGES * SH::BLK;
+  static constexpr int OFF_SH = OFF_V + SH::STAGES * SH::BLK;
+  static constexpr int BYTES = OFF_SH + (int)sizeof(TcShared) + 1024;
+  static_assert(kPerSm * (BYTES + 1024) <= 228 * 1024, "CTAs of an SM share its memory");
+};
+
+template <int D, bool BF16, bool DROP>
+__global__ void __launch_bounds__(kFwdThreads, kPerSm)
+    attn_train_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                             const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnTrainParams p,
+                             const __grid_constant__ Grid gr) {
+  using SH = TcShape<D>;
+  using SM = FwdSmem<D>;
+  using E = Elem<BF16>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TcShared* sh = reinterpret_cast<TcShared*>(smem + SM::OFF_SH);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int S = p.S, PT = p.PT128, rows = PT * p.HC;
+
+  if (tid == 0) tc_init(sh, 4);
+  if (warp == 4) {
+    tmem_alloc(&sh->tmem, kCols);
+    tmem_relinquish();
+  }
+  zero_rows<SH::ROWB>(smem, 2, SH::TILE, rows, kRows, tid, kFwdThreads);
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // Columns: scores (one or two buffers), weights, O.
+  const uint32_t t_s = sh->tmem, t_p = t_s + kFwdBufs * kBlk, t_o = t_p + kBlk / 2;
+  volatile int* abort = &sh->abort;
+
+  if (tid == 128) {
+    const uint64_t qd = umma_smem_desc(smem_u32(smem), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t kd = umma_smem_desc(smem_u32(smem + SM::OFF_K), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t vd = umma_smem_desc(smem_u32(smem + SM::OFF_V), SH::BLK, SH::SBO, SH::LAYOUT);
+    const uint32_t id_s = umma_idesc_f16(BF16, kRows, kBlk, 0, 0), id_o = umma_idesc_f16(BF16, kRows, D, 0, 1);
+    issue_rows<kFwdBufs, 2, SH::STAGES>(
+        sh, p.status,
+        [&](int zero, int st) { zero_padded_keys<D>(smem + SM::OFF_K, smem + SM::OFF_V, st, zero); },
+        [&](int tb, int st, int sb) {
+          issue_scores<D>(t_s + (uint32_t)(sb * kBlk), qd + (uint64_t)((tb * SH::TILE) >> 4),
+                          kd + (uint64_t)((st * SH::BLK) >> 4), id_s);
+        },
+        [&](int st, bool acc) { issue_weights<D>(t_o, t_p, 16, vd + (uint64_t)((st * SH::BLK) >> 4), id_o, acc); });
+  } else if (tid == 160) {
+    load_all<2, SH::STAGES, QTile>(
+        sh, p, gr,
+        [&](const QTile& t, Item& it) {
+          it.nblk = t.nblk, it.pad = t.pad, it.heads = t.heads, it.tile = t.tile;
+          it.first = t.p0, it.origin = t.kb;
+          it.row = ((long long)t.b * p.Hq + t.h0) * S;
+          it.out = t.b * p.o_sb + t.h0 * p.o_sh;
+        },
+        [&](const QTile& t, int tb) {
+          mbar_arrive_expect_tx(&sh->tile_full[tb], (uint32_t)(rows * SH::ROWB));
+          tma_load_4d(smem + tb * SH::TILE, &tmQ, &sh->tile_full[tb], 0, t.h0, t.p0, t.b);
+        },
+        [&](const QTile& t, int j, int st) {
+          mbar_arrive_expect_tx(&sh->blk_full[st], 2u * SH::BLK);
+          tma_load_4d(smem + SM::OFF_K + st * SH::BLK, &tmK, &sh->blk_full[st], 0, t.g, t.kb + j * kBlk, t.b);
+          tma_load_4d(smem + SM::OFF_V + st * SH::BLK, &tmV, &sh->blk_full[st], 0, t.g, t.kb + j * kBlk, t.b);
+        });
+  } else if (warp < 4) {
+    const int r = tid, head = r % p.HC, rpos = r / p.HC;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    const uint32_t tp = t_p + lane_off, to = t_o + lane_off;
     const float c2 = p.scale * 1.4426950408889634f;
-    const int kt0 = pad / kT;
-    const bool one_tile = kt0 == qt;
-    // Q and dO pass through the second K / V buffers into registers.
-    load_tile<D, kT, kThreads>(sk + TB, q, p.q_ss, q0, pad, S, tid);
-    load_tile<D, kT, kThreads>(sv + TB, dout, p.do_ss, q0, pad, S, tid);
-    load_tile<D, kT, kThreads>(sk, k, p.k_ss, kt0 * kT, pad, S, tid);
-    load_tile<D, kT, kThreads>(sv, v, p.v_ss, kt0 * kT, pad, S, tid);
-    cp_async_commit();
-    const long long row0 = (long long)bh * S;
-    if (!one_tile) {
-      // delta = O . dO, two threads a row.
-      const uint16_t* o = static_cast<const uint16_t*>(p.o) + b * p.o_sb + h * p.o_sh;
-      const int r = tid >> 1, row = q0 + r;
-      float d = 0.f;
-      if (row >= pad && row < S) {
-        const uint4* po = reinterpret_cast<const uint4*>(o + row * p.o_ss + (tid & 1) * (D / 2));
-        const uint4* pd = reinterpret_cast<const uint4*>(dout + row * p.do_ss + (tid & 1) * (D / 2));
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint4 a = __ldg(po + i), c = __ldg(pd + i);
-          const uint32_t au[4] = {a.x, a.y, a.z, a.w}, cu[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 x = E::to_f2(au[e]), y = E::to_f2(cu[e]);
-            d = fmaf(x.x, y.x, fmaf(x.y, y.y, d));
-          }
-        }
-      }
-      d += __shfl_xor_sync(0xffffffffu, d, 1);
-      if (!(tid & 1)) {
-        sdelta[r] = d;
-        if (row < S) p.delta[row0 + row] = d;
-      }
-    }
-    DropKey key{};
     const unsigned per_row = (unsigned)(S + 7) >> 3;
-    unsigned long long blk = 0;
-    if constexpr (DROP) {
-      key = drop_key(p.rng, p.site);
-      blk = ((unsigned long long)bh * (unsigned)S + (unsigned)(q0 + warp * 16)) * per_row;
-    }
-    float ls[2], delta[2];
+    const uint32_t th = p.threshold << 16;
+    DropKey key{};
+    if constexpr (DROP) key = drop_key(p.rng, p.site);
+    int blk = 0;
+    bool ok = true;
+    ItemReader items{sh, abort, p.status};
+    // The finished tile: its O is read behind the next tile's first exponentials, when its last P V has long been done.
+    struct {
+      bool live, valid;
+      long long row;
+      uint16_t* out;
+      float m, l;
+    } fin{};
+    auto finish = [&]() {
+      fin.live = false;
+      uint32_t o[D];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      // A row with one key (row == pad) has no gradient: P is taken as 0.
-      const int row = q0 + warp * 16 + g8 + 8 * r;
-      ls[r] = row < S && row != pad ? __ldg(p.lse + row0 + row) : INFINITY;
-    }
-    cp_async_wait<0>();
-    __syncthreads();
-    uint32_t qa[D / 16][4], da[D / 16][4];
+      for (int c = 0; c < D; c += 32) tmem_ld32_async(to + c, *reinterpret_cast<uint32_t(*)[32]>(o + c));
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      frag_a<D>(sk + TB, warp * 16, 2 * i, lane, qa[i]);
-      frag_a<D>(sv + TB, warp * 16, 2 * i, lane, da[i]);
-    }
-    delta[0] = sdelta[warp * 16 + g8];
-    delta[1] = sdelta[warp * 16 + g8 + 8];
-    for (int kt = kt0; kt <= qt; ++kt) {
-      const int buf = (kt - kt0) & 1;
-      cp_async_wait<0>();
-      __syncthreads();
-      if (kt < qt) {
-        load_tile<D, kT, kThreads>(sk + (buf ^ 1) * TB, k, p.k_ss, (kt + 1) * kT, pad, S, tid);
-        load_tile<D, kT, kThreads>(sv + (buf ^ 1) * TB, v, p.v_ss, (kt + 1) * kT, pad, S, tid);
-        cp_async_commit();
-      }
-      float s[8][4], dp[8][4];
+      for (int c = 0; c < D; c += 32) tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(o + c));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->o_empty);
+      if (fin.valid) {
+        const float inv = p.inv_keep / fin.l;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = dp[j][e] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t bb[4];
-          frag_b<D>(sk + buf * TB, 16 * j, 2 * i, lane, bb);
-          mma16816<BF16>(s[2 * j], qa[i], bb[0], bb[1]);
-          mma16816<BF16>(s[2 * j + 1], qa[i], bb[2], bb[3]);
-          frag_b<D>(sv + buf * TB, 16 * j, 2 * i, lane, bb);
-          mma16816<BF16>(dp[2 * j], da[i], bb[0], bb[1]);
-          mma16816<BF16>(dp[2 * j + 1], da[i], bb[2], bb[3]);
-        }
-      if (kt == qt || kt * kT < pad) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int kk = kt * kT + 8 * j + 2 * t4 + (e & 1), qq = q0 + warp * 16 + g8 + (e >> 1) * 8;
-            if (kk > qq || kk < pad) s[j][e] = -INFINITY;
-          }
-      }
-      if constexpr (DROP) {
-        const uint32_t keep = keep_rows(key, blk + (unsigned)kt * (kT / 8), per_row, lane, p.threshold);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint32_t bits = __shfl_sync(0xffffffffu, keep, g8 + 8 * r + (j >> 2) * 16) >> ((j & 3) * 8 + 2 * t4);
-            dp[j][2 * r] = bits & 1u ? dp[j][2 * r] * p.inv_keep : 0.f;
-            dp[j][2 * r + 1] = bits & 2u ? dp[j][2 * r + 1] * p.inv_keep : 0.f;
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = ex2_approx(fmaf(s[j][e], c2, -ls[e >> 1]));
-      if (one_tile) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float d = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) d = fmaf(s[j][2 * r], dp[j][2 * r], fmaf(s[j][2 * r + 1], dp[j][2 * r + 1], d));
-          d += __shfl_xor_sync(0xffffffffu, d, 1);
-          d += __shfl_xor_sync(0xffffffffu, d, 2);
-          delta[r] = d;
-          const int row = q0 + warp * 16 + g8 + 8 * r;
-          if (t4 == 0 && row < S) p.delta[row0 + row] = d;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] *= dp[j][e] - delta[e >> 1];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t a[4] = {E::from_f2(s[2 * j][0], s[2 * j][1]), E::from_f2(s[2 * j][2], s[2 * j][3]),
-                               E::from_f2(s[2 * j + 1][0], s[2 * j + 1][1]),
-                               E::from_f2(s[2 * j + 1][2], s[2 * j + 1][3])};
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t bb[4];
-          frag_bt<D>(sk + buf * TB, 16 * j, 2 * i, lane, bb);
-          mma16816<BF16>(acc[2 * i], a, bb[0], bb[1]);
-          mma16816<BF16>(acc[2 * i + 1], a, bb[2], bb[3]);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = q0 + warp * 16 + g8 + 8 * r;
-    if (row >= S) continue;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-      *reinterpret_cast<uint32_t*>(dq + row * p.dq_ss + 8 * i + 2 * t4) =
-          E::from_f2(acc[i][2 * r] * p.scale, acc[i][2 * r + 1] * p.scale);
-  }
-}
-
-// dk and dv of 64 keys of one KV head, over the R query heads that share it.
-// The products are formed transposed (keys as rows), so P^T and dS^T are the
-// left operands of dV and dK where they stand in registers.
-template <int D, bool BF16, bool DROP>
-__global__ void __launch_bounds__(kThreads) attn_train_dkv_kernel(const AttnTrainParams p, int ntiles) {
-  constexpr int TB = kT * D * 2;
-  __shared__ __align__(1024) uint8_t smem[4 * TB];
-  __shared__ float slse[2][kT], sdelta[2][kT];
-  const uint32_t sq = smem_u32(smem), sd = sq + 2 * TB;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
-  const int kt = (int)(blockIdx.x % (unsigned)ntiles);
-  const unsigned bg = blockIdx.x / (unsigned)ntiles;
-  const int b = (int)(bg / (unsigned)p.Hkv), g = (int)(bg % (unsigned)p.Hkv);
-  const int S = p.S, k0 = kt * kT;
-  const int pad = p.pad_len ? min(max(__ldg(p.pad_len + b), 0), S) : 0;
-  uint16_t* dk = static_cast<uint16_t*>(p.dk) + b * p.dk_sb + g * p.dk_sh;
-  uint16_t* dv = static_cast<uint16_t*>(p.dv) + b * p.dv_sb + g * p.dv_sh;
-  using E = Elem<BF16>;
-
-  float ak[D / 8][4], av[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ak[i][e] = av[i][e] = 0.f;
-
-  if (min(S, k0 + kT) > pad) {
-    const uint16_t* k = static_cast<const uint16_t*>(p.k) + b * p.k_sb + g * p.k_sh;
-    const uint16_t* v = static_cast<const uint16_t*>(p.v) + b * p.v_sb + g * p.v_sh;
-    const float c2 = p.scale * 1.4426950408889634f;
-    const int nq = ntiles - kt, items = nq * p.R;  // (head of the group, query tile) pairs, tiles fastest
-    // K and V pass through the second buffers into registers.
-    load_tile<D, kT, kThreads>(sq + TB, k, p.k_ss, k0, pad, S, tid);
-    load_tile<D, kT, kThreads>(sd + TB, v, p.v_ss, k0, pad, S, tid);
-    auto fetch = [&](int item, int buf) {
-      const int h = g * p.R + item / nq, q0 = (kt + item % nq) * kT;
-      load_tile<D, kT, kThreads>(sq + buf * TB, static_cast<const uint16_t*>(p.q) + b * p.q_sb + h * p.q_sh, p.q_ss, q0,
-                                 pad, S, tid);
-      load_tile<D, kT, kThreads>(sd + buf * TB, static_cast<const uint16_t*>(p.dout) + b * p.do_sb + h * p.do_sh,
-                                 p.do_ss, q0, pad, S, tid);
-      cp_async_commit();
-      if (tid < kT) {
-        const int row = q0 + tid;
-        const long long at = ((long long)b * p.Hq + h) * S + row;
-        const bool ok = row < S && row >= pad;
-        slse[buf][tid] = ok ? __ldg(p.lse + at) : INFINITY;
-        sdelta[buf][tid] = ok ? __ldg(p.delta + at) : 0.f;
+        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(fin.out + c) = pack8<BF16>(o + c, inv);
+        p.lse[fin.row] = fin.m + log2f(fin.l);
       }
     };
-    fetch(0, 0);
+    while (true) {
+      const Item* it = items.get(ok);
+      if (!ok) break;
+      const int nblk = it->nblk, pad = it->pad, kb = it->origin, pos = it->first + rpos;
+      if (nblk < 0) break;
+      const bool mine = r < rows && head < it->heads, valid = mine && pos < S;
+      const long long row = it->row + (long long)head * S + pos;
+      uint16_t* out = static_cast<uint16_t*>(p.o) + it->out + head * p.o_sh;
+      // This tile's share of the padded rows: zeros, each thread the row of its place.
+      const int pz = it->tile * PT + rpos;
+      if (mine && pz < pad) {
+#pragma unroll
+        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + pz * p.o_ss + c) = make_uint4(0u, 0u, 0u, 0u);
+        p.lse[row - pos + pz] = INFINITY;
+      }
+      items.next();
+      const unsigned long long row_block = (unsigned long long)row * per_row;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nblk; ++j, ++blk) {
+        const int sb = blk % kFwdBufs;
+        if (!(ok = warp_wait(&sh->s_full[sb], (blk / kFwdBufs) & 1, abort, p.status))) break;
+        tc_fence_after();
+        const uint32_t ts = t_s + (uint32_t)(sb * kBlk) + lane_off;
+        const int k0 = kb + j * kBlk;
+        // Keys lo .. see - 1 of the block are the row's (a row without a query takes them all: it is not stored).
+        const int see = valid ? pos - k0 + 1 : kBlk, lo = j == 0 ? pad - kb : 0;
+        uint32_t s0[32], s1[32];
+        tmem_ld32_async(ts, s0);
+        tmem_ld32_async(ts + 32, s1);
+        tmem_wait_ld(s0);
+        tmem_wait_ld(s1);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->s_read[sb]);
+        if (lo > 0) {
+#pragma unroll
+          for (int i = 0; i < 7; ++i)
+            if (i < lo) s0[i] = 0xff800000u;
+        }
+        if (__any_sync(0xffffffffu, see < kBlk)) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i >= see) s0[i] = 0xff800000u;
+            if (i + 32 >= see) s1[i] = 0xff800000u;
+          }
+        }
+        float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          x0 = fmax3(x0, __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
+          x1 = fmax3(x1, __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
+        }
+        const float top = fmaxf(x0, x1) * c2;
+        // The reference maximum moves only when a weight would pass 2^8; then O and l are
+        // scaled by an exact power of two (P <= 256 is as exact in 16 bits as P <= 1).
+        float f = 1.f;
+        if (m == -INFINITY) {
+          m = top;
+        } else if (top > m + 8.f) {
+          const float k = ceilf(top - m);
+          m += k;
+          f = exp2f(-k);
+          l *= f;
+        }
+        const float mm = m == -INFINITY ? 0.f : m;
+        const float2 c2v = make_float2(c2, c2), nm = make_float2(-mm, -mm);
+        auto half = [&](uint32_t (&s)[32], int c) {  // leaves the packed weights in s[0 .. 16)
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int b8 = 0; b8 < 4; ++b8) {
+            uint4 w8;
+            if constexpr (DROP) w8 = philox7(key, row_block + (unsigned)((k0 + 32 * c) / 8 + b8));
+            auto two = [&](auto I) {
+              constexpr int e = decltype(I)::value;
+              const int i = 8 * b8 + e;
+              const float2 x = ffma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2v, nm);
+              float2 w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              sum = fadd2(sum, w);
+              if constexpr (DROP) {
+                w.x = stays<e>(w8, th) ? w.x : 0.f;
+                w.y = stays<e + 1>(w8, th) ? w.y : 0.f;
+              }
+              s[i >> 1] = E::from_f2(w.x, w.y);
+            };
+            two(Int<0>{});
+            two(Int<2>{});
+            two(Int<4>{});
+            two(Int<6>{});
+          }
+          l += sum.x + sum.y;
+        };
+        half(s0, 0);
+        if (__any_sync(0xffffffffu, see > 32)) {
+          half(s1, 1);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s1[i] = 0u;
+        }
+        // The previous P V must be done before its weights are overwritten, or O scaled.
+        if (blk > 0 && !(ok = warp_wait(&sh->w_done, (blk - 1) & 1, abort, p.status))) break;
+        tc_fence_after();
+        if (fin.live) finish();
+        if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld16_u(to + c, o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(to + c, o);
+          }
+        }
+        tmem_st16(tp, *reinterpret_cast<uint32_t(*)[16]>(s0));
+        tmem_st16(tp + 16, *reinterpret_cast<uint32_t(*)[16]>(s1));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->p_full);
+      }
+      if (!ok) break;
+      if (nblk > 0) {
+        fin.live = true;
+        fin.valid = valid;
+        fin.row = row;
+        fin.out = out + pos * p.o_ss;
+        fin.m = m;
+        fin.l = l;
+      }
+    }
+    if (ok && fin.live && warp_wait(&sh->w_done, (blk - 1) & 1, abort, p.status)) {
+      tc_fence_after();
+      finish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(sh->tmem, kCols);
+  }
+}
+
+// ---------------------------------------------------------------- dq
+constexpr int kBwdThreads = 320;  // two warpgroups (half of a block's columns each), the MMA warp, the loading warp
+
+template <int D, bool DQ>
+struct BwdSmem {
+  using SH = TcShape<D>;
+  static constexpr int STAGES = DQ ? SH::DQ_STAGES : SH::STAGES;
+  static constexpr int OFF_B = SH::BWD_TILES * SH::TILE;                // second tensor's tiles
+  static constexpr int OFF_O = 2 * SH::BWD_TILES * SH::TILE;            // O's tiles (dq)
+  static constexpr int OFF_C = OFF_O + (DQ ? SH::BWD_TILES * SH::TILE : 0);  // first ring
+  static constexpr int OFF_E = OFF_C + STAGES * SH::BLK;                // second ring
+  static constexpr int OFF_X = OFF_E + STAGES * SH::BLK;                // 4 KB of rows' scalars
+  static constexpr int OFF_SH = OFF_X + 4096;
+  static constexpr int NEED = OFF_SH + (int)sizeof(TcShared) + 1024;
+  // Above a third of the SM's shared memory: two CTAs' 256 columns fill its tensor memory.
+  static constexpr int BYTES = NEED > 78 * 1024 ? NEED : 78 * 1024;
+  static_assert(kPerSm * (BYTES + 1024) <= 228 * 1024, "CTAs of an SM share its memory");
+};
+
+template <int D, bool BF16, bool DROP>
+__global__ void __launch_bounds__(kBwdThreads, kPerSm)
+    attn_train_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                            const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmK,
+                            const __grid_constant__ CUtensorMap tmV,
+                            const __grid_constant__ AttnTrainParams p, const __grid_constant__ Grid gr) {
+  using SH = TcShape<D>;
+  using SM = BwdSmem<D, true>;
+  using E = Elem<BF16>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TcShared* sh = reinterpret_cast<TcShared*>(smem + SM::OFF_SH);
+  float* xrow = reinterpret_cast<float*>(smem + SM::OFF_X);  // [2 items][2 halves][128] of delta
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int S = p.S, PT = p.PT128, rows = PT * p.HC;
+
+  if (tid == 0) tc_init(sh, 8);
+  if (warp == 8) {
+    tmem_alloc(&sh->tmem, kCols);
+    tmem_relinquish();
+  }
+  zero_rows<SH::ROWB>(smem, 2 * SH::BWD_TILES, SH::TILE, rows, kRows, tid, kBwdThreads);
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // Columns: S, dP, dS, dQ.
+  const uint32_t t_s = sh->tmem, t_dp = t_s + kBlk, t_ds = t_dp + kBlk, t_dq = t_ds + kBlk / 2;
+  volatile int* abort = &sh->abort;
+
+  if (tid == 256) {
+    const uint64_t qd = umma_smem_desc(smem_u32(smem), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t dd = umma_smem_desc(smem_u32(smem + SM::OFF_B), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t kd = umma_smem_desc(smem_u32(smem + SM::OFF_C), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t vd = umma_smem_desc(smem_u32(smem + SM::OFF_E), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t kt = umma_smem_desc(smem_u32(smem + SM::OFF_C), SH::BLK, SH::SBO, SH::LAYOUT);
+    const uint32_t id_s = umma_idesc_f16(BF16, kRows, kBlk, 0, 0), id_o = umma_idesc_f16(BF16, kRows, D, 0, 1);
+    issue_rows<1, SH::BWD_TILES, SH::DQ_STAGES>(
+        sh, p.status,
+        [&](int zero, int st) { zero_padded_keys<D>(smem + SM::OFF_C, smem + SM::OFF_E, st, zero); },
+        [&](int tb, int st, int) {
+          const uint64_t ta = (uint64_t)((tb * SH::TILE) >> 4), sa = (uint64_t)((st * SH::BLK) >> 4);
+          issue_scores<D>(t_s, qd + ta, kd + sa, id_s);
+          issue_scores<D>(t_dp, dd + ta, vd + sa, id_s);
+        },
+        [&](int st, bool acc) { issue_weights<D>(t_dq, t_ds, 16, kt + (uint64_t)((st * SH::BLK) >> 4), id_o, acc); });
+  } else if (tid == 288) {
+    load_all<SH::BWD_TILES, SH::DQ_STAGES, QTile>(
+        sh, p, gr,
+        [&](const QTile& t, Item& it) {
+          it.nblk = t.nblk, it.pad = t.pad, it.heads = t.heads, it.tile = t.tile;
+          it.first = t.p0, it.origin = t.kb;
+          it.row = ((long long)t.b * p.Hq + t.h0) * S;
+          it.out = t.b * p.dq_sb + t.h0 * p.dq_sh;
+        },
+        [&](const QTile& t, int tb) {
+          mbar_arrive_expect_tx(&sh->tile_full[tb], 3u * (uint32_t)(rows * SH::ROWB));
+          tma_load_4d(smem + tb * SH::TILE, &tmQ, &sh->tile_full[tb], 0, t.h0, t.p0, t.b);
+          tma_load_4d(smem + SM::OFF_B + tb * SH::TILE, &tmDO, &sh->tile_full[tb], 0, t.h0, t.p0, t.b);
+          tma_load_4d(smem + SM::OFF_O + tb * SH::TILE, &tmO, &sh->tile_full[tb], 0, t.h0, t.p0, t.b);
+        },
+        [&](const QTile& t, int j, int st) {
+          mbar_arrive_expect_tx(&sh->blk_full[st], 2u * SH::BLK);
+          tma_load_4d(smem + SM::OFF_C + st * SH::BLK, &tmK, &sh->blk_full[st], 0, t.g, t.kb + j * kBlk, t.b);
+          tma_load_4d(smem + SM::OFF_E + st * SH::BLK, &tmV, &sh->blk_full[st], 0, t.g, t.kb + j * kBlk, t.b);
+        });
+  } else if (warp < 8) {
+    const int half = warp >> 2, wq = warp & 3, r = wq * 32 + lane;
+    const int head = r % p.HC, rpos = r / p.HC;
+    const uint32_t lane_off = (uint32_t)(wq * 32) << 16;
+    const uint32_t ts = t_s + lane_off + 32 * half, tdp = t_dp + lane_off + 32 * half;
+    const uint32_t tds = t_ds + lane_off + 16 * half;
+    const float c2 = p.scale * 1.4426950408889634f;
+    const unsigned per_row = (unsigned)(S + 7) >> 3;
+    const uint32_t th = p.threshold << 16;
+    DropKey key{};
+    if constexpr (DROP) key = drop_key(p.rng, p.site);
+    int blk = 0, done = 0;
+    bool ok = true;
+    ItemReader items{sh, abort, p.status};
+    // The finished tile: its dQ is read behind the next tile's first weights.
+    uint16_t* fin_out = nullptr;
+    bool fin = false;
+    auto finish = [&]() {
+      fin = false;
+      uint32_t o[D / 2];
+#pragma unroll
+      for (int c = 0; c < D / 2; c += 16)
+        tmem_ld16_u(t_dq + lane_off + half * (D / 2) + c, *reinterpret_cast<uint32_t(*)[16]>(o + c));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->o_empty);
+      if (fin_out)
+#pragma unroll
+        for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(fin_out + c) = pack8<BF16>(o + c, p.scale);
+    };
+    while (true) {
+      const Item* it = items.get(ok);
+      if (!ok) break;
+      const int nblk = it->nblk, pad = it->pad, kb = it->origin, pos = it->first + rpos;
+      if (nblk < 0) break;
+      const bool mine = r < rows && head < it->heads, valid = mine && pos < S;
+      const long long row = it->row + (long long)head * S + pos;
+      // A row with a single key (pos == pad) has no gradient: its P is taken as 0.
+      const float ls = valid && pos != pad ? __ldg(p.lse + row) : INFINITY;
+      uint16_t* out = static_cast<uint16_t*>(p.dq) + it->out + head * p.dq_sh + half * (D / 2);
+      const int pz = it->tile * PT + rpos;
+      if (mine && pz < pad) {
+#pragma unroll
+        for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(out + pz * p.dq_ss + c) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      items.next();
+      out += pos * p.dq_ss;
+      const unsigned long long row_block = (unsigned long long)row * per_row;
+      float delta = 0.f;
+      float* xr = xrow + (done & 1) * 2 * kRows;  // the other half may still be read for the previous item
+      if (nblk > 1) {
+        // delta = O . dO: each of the row's two threads takes half of the columns.
+        const int tb = done % SH::BWD_TILES;
+        if ((ok = warp_wait(&sh->tile_full[tb], (done / SH::BWD_TILES) & 1, abort, p.status))) {
+          float d = 0.f;
+#pragma unroll
+          for (int c = 0; c < SH::NCH / 2; ++c) {
+            const uint32_t at = swz<SH::ROWB>(r, half * (SH::NCH / 2) + c) + tb * SH::TILE;
+            const uint4 o = *reinterpret_cast<const uint4*>(smem + SM::OFF_O + at);
+            const uint4 g = *reinterpret_cast<const uint4*>(smem + SM::OFF_B + at);
+            const uint32_t a[4] = {o.x, o.y, o.z, o.w}, y[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 fa = E::to_f2(a[e]), fy = E::to_f2(y[e]);
+              d = fmaf(fa.x, fy.x, fmaf(fa.y, fy.y, d));
+            }
+          }
+          xr[half * kRows + r] = d;
+        }
+        ok = named_bar_and(1, 256, ok);
+        if (!ok) break;
+        delta = xr[r] + xr[kRows + r];
+        if (half == 0 && valid) p.delta[row] = delta;
+      }
+      for (int j = 0; j < nblk; ++j, ++blk) {
+        if (!(ok = warp_wait(&sh->s_full[0], blk & 1, abort, p.status))) {
+          if (nblk == 1) named_bar_and(1, 256, false);  // the others may wait there
+          break;
+        }
+        tc_fence_after();
+        const int k0 = kb + j * kBlk + 32 * half;
+        const int see = valid ? pos - k0 + 1 : 32, lo = j == 0 && half == 0 ? pad - kb : 0;
+        const bool any = __any_sync(0xffffffffu, see > 0), edge = __any_sync(0xffffffffu, see < 32);
+        // Columns c0 .. c0 + 16: P into w, dP (dropped, not yet scaled by 1 / (1 - p)) into d.
+        auto chunk = [&](int c0, uint32_t (&w)[16], uint32_t (&d)[16]) {
+          tmem_ld16_u(ts + c0, w);
+          tmem_ld16_u(tdp + c0, d);
+          if (c0 == 0 && lo > 0) {
+#pragma unroll
+            for (int c = 0; c < 7; ++c)
+              if (c < lo) w[c] = 0xff800000u;
+          }
+          if (edge) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              if (c + c0 >= see) w[c] = 0xff800000u;
+          }
+          if constexpr (DROP) {
+#pragma unroll
+            for (int b8 = 0; b8 < 2; ++b8) {
+              const uint4 w8 = philox7(key, row_block + (unsigned)((k0 + c0) / 8 + b8));
+              auto one = [&](auto I) {
+                constexpr int e = decltype(I)::value;
+                d[8 * b8 + e] = stays<e>(w8, th) ? d[8 * b8 + e] : 0u;
+              };
+              one(Int<0>{}), one(Int<1>{}), one(Int<2>{}), one(Int<3>{});
+              one(Int<4>{}), one(Int<5>{}), one(Int<6>{}), one(Int<7>{});
+            }
+          }
+          const float2 c2v = make_float2(c2, c2), nl = make_float2(-ls, -ls);
+#pragma unroll
+          for (int c = 0; c < 16; c += 2) {
+            const float2 x = ffma2(make_float2(__uint_as_float(w[c]), __uint_as_float(w[c + 1])), c2v, nl);
+            w[c] = __float_as_uint(ex2_approx(x.x));
+            w[c + 1] = __float_as_uint(ex2_approx(x.y));
+          }
+        };
+        if (nblk == 1) {
+          // All keys of these rows are here: delta from the unrounded terms.
+          float s = 0.f;
+          if (any) {
+#pragma unroll
+            for (int c0 = 0; c0 < 32; c0 += 16) {
+              uint32_t w[16], d[16];
+              chunk(c0, w, d);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) s = fmaf(__uint_as_float(w[c]), __uint_as_float(d[c]), s);
+            }
+          }
+          xr[half * kRows + r] = s * p.inv_keep;
+          if (!(ok = named_bar_and(1, 256, true))) break;
+          delta = xr[r] + xr[kRows + r];
+          if (half == 0 && valid) p.delta[row] = delta;
+        }
+        uint32_t pk[16];
+        if (any) {
+          const float2 ik = make_float2(p.inv_keep, p.inv_keep), nd = make_float2(-delta, -delta);
+#pragma unroll
+          for (int c0 = 0; c0 < 32; c0 += 16) {
+            uint32_t w[16], d[16];
+            chunk(c0, w, d);
+            if (c0 == 16) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh->s_read[0]);
+            }
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) {
+              const float2 g = make_float2(__uint_as_float(d[c]), __uint_as_float(d[c + 1]));
+              const float2 x = fmul2(make_float2(__uint_as_float(w[c]), __uint_as_float(w[c + 1])),
+                                     DROP ? ffma2(g, ik, nd) : fadd2(g, nd));
+              pk[(c0 + c) >> 1] = E::from_f2(x.x, x.y);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) pk[c] = 0u;
+          if (lane == 0) mbar_arrive(&sh->s_read[0]);
+        }
+        if (blk > 0 && !(ok = warp_wait(&sh->w_done, (blk - 1) & 1, abort, p.status))) break;
+        tc_fence_after();
+        if (fin) finish();
+        tmem_st16(tds, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->p_full);
+      }
+      if (!ok) break;
+      if (nblk > 0) {
+        ++done;
+        fin = true;
+        fin_out = valid ? out : nullptr;
+      }
+    }
+    if (ok && fin && warp_wait(&sh->w_done, (blk - 1) & 1, abort, p.status)) {
+      tc_fence_after();
+      finish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(sh->tmem, kCols);
+  }
+}
+
+// ---------------------------------------------------------------- dk, dv
+template <int D, bool BF16, bool DROP>
+__global__ void __launch_bounds__(kBwdThreads, kPerSm)
+    attn_train_dkv_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                             const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                             const __grid_constant__ AttnTrainParams p, const __grid_constant__ Grid gr) {
+  using SH = TcShape<D>;
+  using SM = BwdSmem<D, false>;
+  using E = Elem<BF16>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TcShared* sh = reinterpret_cast<TcShared*>(smem + SM::OFF_SH);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int S = p.S, PT = p.PT64, rows = PT * p.HC;
+
+  if (tid == 0) tc_init(sh, 8);
+  if (warp == 8) {
+    tmem_alloc(&sh->tmem, kCols);
+    tmem_relinquish();
+  }
+  zero_rows<SH::ROWB>(smem + SM::OFF_C, 2 * SH::STAGES, SH::BLK, rows, kBlk, tid, kBwdThreads);
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t t_s = sh->tmem, t_dp = sh->tmem + 64, t_dv = sh->tmem + 128, t_dk = sh->tmem + 128 + D;
+  volatile int* abort = &sh->abort;
+
+  if (tid == 256) {
+    const uint64_t kd = umma_smem_desc(smem_u32(smem), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t vd = umma_smem_desc(smem_u32(smem + SM::OFF_B), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t qd = umma_smem_desc(smem_u32(smem + SM::OFF_C), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t dd = umma_smem_desc(smem_u32(smem + SM::OFF_E), 16, SH::SBO, SH::LAYOUT);
+    const uint64_t qt = umma_smem_desc(smem_u32(smem + SM::OFF_C), SH::BLK, SH::SBO, SH::LAYOUT);
+    const uint64_t dt = umma_smem_desc(smem_u32(smem + SM::OFF_E), SH::BLK, SH::SBO, SH::LAYOUT);
+    const uint32_t id_s = umma_idesc_f16(BF16, kRows, kBlk, 0, 0), id_o = umma_idesc_f16(BF16, kRows, D, 0, 1);
+    auto tile_at = [](int tb) { return (uint64_t)((tb * SH::TILE) >> 4); };
+    auto blk_at = [](int st) { return (uint64_t)((st * SH::BLK) >> 4); };
+    issue_keys<SH::BWD_TILES, SH::STAGES>(
+        sh, p.status,
+        [&](int tb, int st) { issue_scores<D>(t_s, kd + tile_at(tb), qd + blk_at(st), id_s); },
+        [&](int tb, int st) { issue_scores<D>(t_dp, vd + tile_at(tb), dd + blk_at(st), id_s); },
+        [&](int st, bool acc) { issue_weights<D>(t_dv, t_s, 32, dt + blk_at(st), id_o, acc); },
+        [&](int st, bool acc) { issue_weights<D>(t_dk, t_dp, 32, qt + blk_at(st), id_o, acc); });
+  } else if (tid == 288) {
+    load_all<SH::BWD_TILES, SH::STAGES, KTile>(
+        sh, p, gr,
+        [&](const KTile& t, Item& it) {
+          it.nblk = t.nblk, it.pad = t.pad, it.tile = t.tile;
+          it.first = t.q0, it.origin = t.k0, it.per = t.per;
+          it.row = ((long long)t.b * p.Hq + t.g * p.R) * S;
+          it.out = t.b * p.dv_sb + t.g * p.dv_sh;
+          it.out2 = t.b * p.dk_sb + t.g * p.dk_sh;
+        },
+        [&](const KTile& t, int tb) {
+          mbar_arrive_expect_tx(&sh->tile_full[tb], 2u * SH::TILE);
+          tma_load_4d(smem + tb * SH::TILE, &tmK, &sh->tile_full[tb], 0, t.g, t.k0, t.b);
+          tma_load_4d(smem + SM::OFF_B + tb * SH::TILE, &tmV, &sh->tile_full[tb], 0, t.g, t.k0, t.b);
+        },
+        [&](const KTile& t, int j, int st) {
+          const int c = gr.chunks > 1 ? j / t.per : 0, h0 = t.g * p.R + c * p.HC, q0 = t.q0 + (j - c * t.per) * PT;
+          mbar_arrive_expect_tx(&sh->blk_full[st], 2u * (uint32_t)(rows * SH::ROWB));
+          tma_load_4d(smem + SM::OFF_C + st * SH::BLK, &tmQ, &sh->blk_full[st], 0, h0, q0, t.b);
+          tma_load_4d(smem + SM::OFF_E + st * SH::BLK, &tmDO, &sh->blk_full[st], 0, h0, q0, t.b);
+        });
+  } else if (warp < 8) {
+    const int half = warp >> 2, wq = warp & 3;
+    const uint32_t lane_off = (uint32_t)(wq * 32) << 16, lane_bit = 1u << lane;
+    const uint32_t ts = t_s + lane_off + 32 * half, tdp = t_dp + lane_off + 32 * half;
+    const float c2 = p.scale * 1.4426950408889634f;
     DropKey key{};
     const unsigned per_row = (unsigned)(S + 7) >> 3;
     if constexpr (DROP) key = drop_key(p.rng, p.site);
-    cp_async_wait<0>();
-    __syncthreads();
-    uint32_t ka[D / 16][4], va[D / 16][4];
+    // Scalars of the warp's 32 columns (query rows): lane l fetches those of column l.
+    float2* x_ld = reinterpret_cast<float2*>(smem + SM::OFF_X) + warp * 32;               // lse, delta
+    uint32_t* x_keep = reinterpret_cast<uint32_t*>(smem + SM::OFF_X + 2048) + warp * 32;  // keep bits of the warp's keys
+    int* x_pos = reinterpret_cast<int*>(smem + SM::OFF_X + 3072) + warp * 32;
+    const int col = 32 * half + lane, chead = col % p.HC, cpos = col / p.HC;
+    const int last_pos = min(32 * half + 31, rows - 1) / p.HC;
+    int blk = 0, done = 0;
+    bool ok = true;
+    ItemReader items{sh, abort, p.status};
+    // The finished tile: dv (first warpgroup) or dk (second) is read behind the next tile's first weights.
+    uint16_t* fin_out = nullptr;
+    bool fin = false;
+    auto finish = [&]() {
+      fin = false;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      frag_a<D>(sq + TB, warp * 16, 2 * i, lane, ka[i]);
-      frag_a<D>(sd + TB, warp * 16, 2 * i, lane, va[i]);
-    }
-    for (int item = 0; item < items; ++item) {
-      const int buf = item & 1;
-      const int qt = kt + item % nq, q0 = qt * kT;
-      cp_async_wait<0>();
-      __syncthreads();
-      if (item + 1 < items) fetch(item + 1, buf ^ 1);
-      uint32_t keep = 0xffffffffu;
-      if constexpr (DROP) {
-        // Lane l: the two blocks of the warp's 16 keys in query rows l (low half) and l + 32 (high half).
-        const unsigned h = (unsigned)(g * p.R + item / nq);
-        const unsigned long long row = ((unsigned long long)b * (unsigned)p.Hq + h) * (unsigned)S + (unsigned)(q0 + lane);
-        const unsigned long long blk = row * per_row + (unsigned)(k0 / 8 + warp * 2);
-        const unsigned long long far = blk + 32ull * per_row;
-        keep = keep_bits(key, blk, p.threshold) | keep_bits(key, blk + 1, p.threshold) << 8 |
-               keep_bits(key, far, p.threshold) << 16 | keep_bits(key, far + 1, p.threshold) << 24;
-      }
-      const bool edge = qt == kt || k0 < pad;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float s[4][4], dp[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][e] = dp[j][e] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t bb[4];
-            frag_b<D>(sq + buf * TB, half * 32 + 16 * j, 2 * i, lane, bb);
-            mma16816<BF16>(s[2 * j], ka[i], bb[0], bb[1]);
-            mma16816<BF16>(s[2 * j + 1], ka[i], bb[2], bb[3]);
-            frag_b<D>(sd + buf * TB, half * 32 + 16 * j, 2 * i, lane, bb);
-            mma16816<BF16>(dp[2 * j], va[i], bb[0], bb[1]);
-            mma16816<BF16>(dp[2 * j + 1], va[i], bb[2], bb[3]);
-          }
-        uint32_t pa[2][4], sa[2][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col = half * 32 + 8 * j + 2 * t4;
-          const float2 ls = *reinterpret_cast<const float2*>(&slse[buf][col]);
-          const float2 dl = *reinterpret_cast<const float2*>(&sdelta[buf][col]);
-          uint32_t bits0 = 0, bits1 = 0;
-          if constexpr (DROP) {
-            bits0 = __shfl_sync(0xffffffffu, keep, 8 * j + 2 * t4) >> (16 * half + g8);
-            bits1 = __shfl_sync(0xffffffffu, keep, 8 * j + 2 * t4 + 1) >> (16 * half + g8);
-          }
-          float pd[4], ds[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float lq = e & 1 ? ls.y : ls.x, de = e & 1 ? dl.y : dl.x;
-            float x = ex2_approx(fmaf(s[j][e], c2, -lq));
-            float y = dp[j][e];
-            bool single = false;
-            if (edge) {
-              const int kk = k0 + warp * 16 + g8 + (e >> 1) * 8, qq = q0 + col + (e & 1);
-              if (kk > qq || kk < pad) x = 0.f;
-              single = qq == pad;
-            }
-            pd[e] = x;
-            if constexpr (DROP) {
-              const bool stays = ((e & 1 ? bits1 : bits0) >> ((e >> 1) * 8)) & 1u;
-              pd[e] = stays ? x : 0.f;
-              y = stays ? y * p.inv_keep : 0.f;
-            }
-            ds[e] = single ? 0.f : x * (y - de);
-          }
-          pa[j >> 1][(j & 1) * 2] = E::from_f2(pd[0], pd[1]);
-          pa[j >> 1][(j & 1) * 2 + 1] = E::from_f2(pd[2], pd[3]);
-          sa[j >> 1][(j & 1) * 2] = E::from_f2(ds[0], ds[1]);
-          sa[j >> 1][(j & 1) * 2 + 1] = E::from_f2(ds[2], ds[3]);
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_ld32_async((half ? t_dk : t_dv) + lane_off + c, o);
+        tmem_wait_ld(o);
+        if (c + 32 == D) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->o_empty);
         }
+        if (fin_out)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t bb[4];
-            frag_bt<D>(sd + buf * TB, half * 32 + 16 * j, 2 * i, lane, bb);
-            mma16816<BF16>(av[2 * i], pa[j], bb[0], bb[1]);
-            mma16816<BF16>(av[2 * i + 1], pa[j], bb[2], bb[3]);
-            frag_bt<D>(sq + buf * TB, half * 32 + 16 * j, 2 * i, lane, bb);
-            mma16816<BF16>(ak[2 * i], sa[j], bb[0], bb[1]);
-            mma16816<BF16>(ak[2 * i + 1], sa[j], bb[2], bb[3]);
-          }
+          for (int e = 0; e < 32; e += 8)
+            *reinterpret_cast<uint4*>(fin_out + c + e) = pack8<BF16>(o + e, half ? p.scale : p.inv_keep);
       }
+    };
+    while (true) {
+      const Item* it = items.get(ok);
+      if (!ok) break;
+      const int nblk = it->nblk, pad = it->pad, per = it->per, first = it->first;
+      if (nblk < 0) break;
+      const int key0 = it->origin + wq * 32, kk = key0 + lane;  // the warp's keys, the thread's
+      const long long row_at = it->row;
+      uint16_t* out = half ? static_cast<uint16_t*>(p.dk) + it->out2 : static_cast<uint16_t*>(p.dv) + it->out;
+      const long long out_ss = half ? p.dk_ss : p.dv_ss;
+      const int pz = it->tile * kRows + wq * 32 + lane;
+      if (pz < pad) {
+#pragma unroll
+        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + pz * out_ss + c) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      items.next();
+      // Query row of the thread's column in block j, or -1; and its lse and delta.
+      auto row_of = [&](int j) -> long long {
+        const int chunk = gr.chunks > 1 ? j / per : 0, pos = first + (j - chunk * per) * PT + cpos;
+        const bool ok_row = j < nblk && col < rows && chunk * p.HC + chead < p.R && pos < S;
+        return ok_row ? row_at + (long long)(chunk * p.HC + chead) * S + pos : -1;
+      };
+      auto scalars_of = [&](long long row) {
+        return row >= 0 ? make_float2(__ldg(p.lse + row), __ldg(p.delta + row)) : make_float2(INFINITY, 0.f);
+      };
+      long long row = row_of(0);
+      float2 ld = scalars_of(row);
+      for (int j = 0; j < nblk; ++j, ++blk) {
+        const int chunk = gr.chunks > 1 ? j / per : 0, q0 = first + (j - chunk * per) * PT;
+        const int pos = q0 + cpos;
+        // The warp's last position against its first key: nothing to do where every query comes before every key.
+        const int last = q0 + last_pos;
+        const bool any = last >= key0;
+        uint32_t keep = 0;
+        if constexpr (DROP) {
+          if (any) {
+            const unsigned long long b0 = (unsigned long long)row * per_row + (unsigned)(key0 >> 3);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) keep |= keep_bits(key, b0 + c, p.threshold) << (8 * c);
+          }
+        }
+        __syncwarp();
+        x_ld[lane] = ld;
+        if constexpr (DROP) x_keep[lane] = keep;
+        x_pos[lane] = pos;
+        __syncwarp();
+        // The next block's scalars: on their way while this one is worked on.
+        row = row_of(j + 1);
+        ld = scalars_of(row);
+        if (!(ok = warp_wait(&sh->s_full[0], blk & 1, abort, p.status))) break;
+        tc_fence_after();
+        uint32_t s[32];
+        if (any) {
+          tmem_ld32_async(ts, s);
+          tmem_wait_ld(s);
+          // Only blocks on the diagonal hold queries before a key.
+          if (q0 < key0 + 31) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (kk > x_pos[c]) s[c] = 0xff800000u;
+          }
+          uint32_t pw[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const float4 a = *reinterpret_cast<const float4*>(x_ld + c);  // lse, delta of two columns
+            const float w0 = ex2_approx(fmaf(__uint_as_float(s[c]), c2, -a.x));
+            const float w1 = ex2_approx(fmaf(__uint_as_float(s[c + 1]), c2, -a.z));
+            s[c] = __float_as_uint(w0);
+            s[c + 1] = __float_as_uint(w1);
+            if constexpr (DROP) {
+              const uint2 kb = *reinterpret_cast<const uint2*>(x_keep + c);
+              pw[c >> 1] = E::from_f2(kb.x & lane_bit ? w0 : 0.f, kb.y & lane_bit ? w1 : 0.f);
+            } else {
+              pw[c >> 1] = E::from_f2(w0, w1);
+            }
+          }
+          if (fin) {
+            if (!(ok = warp_wait(&sh->w_done, (done - 1) & 1, abort, p.status))) break;
+            tc_fence_after();
+            finish();
+          }
+          tmem_st16(ts, pw);
+        } else {
+          if (fin) {
+            if (!(ok = warp_wait(&sh->w_done, (done - 1) & 1, abort, p.status))) break;
+            tc_fence_after();
+            finish();
+          }
+          uint32_t z[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) z[c] = 0u;
+          tmem_st16(ts, z);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->p_full);
+        if (!(ok = warp_wait(&sh->dp_full, blk & 1, abort, p.status))) break;
+        tc_fence_after();
+        if (any) {
+          // The row with a single key (position pad) has no dS.
+          if (q0 == pad) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (x_pos[c] == pad) s[c] = 0u;
+          }
+#pragma unroll
+          for (int c0 = 0; c0 < 32; c0 += 16) {
+            uint32_t dp[16];
+            tmem_ld16_u(tdp + c0, dp);
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) {
+              const float4 a = *reinterpret_cast<const float4*>(x_ld + c0 + c);
+              float d0 = __uint_as_float(dp[c]), d1 = __uint_as_float(dp[c + 1]);
+              if constexpr (DROP) {
+                const uint2 kb = *reinterpret_cast<const uint2*>(x_keep + c0 + c);
+                d0 = fmaf(kb.x & lane_bit ? d0 : 0.f, p.inv_keep, -a.y);
+                d1 = fmaf(kb.y & lane_bit ? d1 : 0.f, p.inv_keep, -a.w);
+              } else {
+                d0 -= a.y;
+                d1 -= a.w;
+              }
+              s[(c0 + c) >> 1] = E::from_f2(__uint_as_float(s[c0 + c]) * d0, __uint_as_float(s[c0 + c + 1]) * d1);
+            }
+          }
+          tmem_st16(tdp, *reinterpret_cast<uint32_t(*)[16]>(s));
+        } else {
+          uint32_t z[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) z[c] = 0u;
+          tmem_st16(tdp, z);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->ds_full);
+      }
+      if (!ok) break;
+      if (nblk > 0) {
+        ++done;
+        fin = true;
+        fin_out = kk >= pad && kk < S ? out + kk * out_ss : nullptr;
+      }
+    }
+    if (ok && fin && warp_wait(&sh->w_done, (done - 1) & 1, abort, p.status)) {
+      tc_fence_after();
+      finish();
     }
   }
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = k0 + warp * 16 + g8 + 8 * r;
-    if (row >= S) continue;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      *reinterpret_cast<uint32_t*>(dk + row * p.dk_ss + 8 * i + 2 * t4) =
-          E::from_f2(ak[i][2 * r] * p.scale, ak[i][2 * r + 1] * p.scale);
-      *reinterpret_cast<uint32_t*>(dv + row * p.dv_ss + 8 * i + 2 * t4) =
-          E::from_f2(av[i][2 * r] * p.inv_keep, av[i][2 * r + 1] * p.inv_keep);
-    }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(sh->tmem, kCols);
   }
 }
 
+Grid make_grid(const AttnTrainParams& p, int units, int tiles) {
+  const int chunks = (p.R + p.HC - 1) / p.HC;
+  return Grid{units, tiles, units * tiles, chunks, FastDiv((uint32_t)tiles), FastDiv((uint32_t)chunks),
+              FastDiv((uint32_t)p.Hkv)};
+}
+Grid grid_rows(const AttnTrainParams& p) {
+  return make_grid(p, p.B * p.Hkv * ((p.R + p.HC - 1) / p.HC), (p.S + p.PT128 - 1) / p.PT128);
+}
+Grid grid_keys(const AttnTrainParams& p) { return make_grid(p, p.B * p.Hkv, (p.S + kRows - 1) / kRows); }
+unsigned ctas(const Grid& gr, int num_sms, int per_sm) {
+  const int most = num_sms * per_sm;
+  return (unsigned)(gr.items < most ? gr.items : most);
+}
+
 template <int D, bool BF16, bool DROP>
-cudaError_t fwd(const AttnTrainParams& p, cudaStream_t st) {
-  const int nt = (p.S + kT - 1) / kT;
-  attn_train_fwd_kernel<D, BF16, DROP><<<(unsigned)((long long)nt * p.B * p.Hq), kThreads, 0, st>>>(p, nt);
+cudaError_t run_fwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sms, cudaStream_t st) {
+  auto kern = attn_train_fwd_tc_kernel<D, BF16, DROP>;
+  const cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kern), FwdSmem<D>::BYTES);
+  if (e != cudaSuccess) return e;
+  const Grid gr = grid_rows(p);
+  kern<<<ctas(gr, num_sms, kPerSm), kFwdThreads, FwdSmem<D>::BYTES, st>>>(m.q_tile, m.k_blk, m.v_blk, p,
+                                                                                          gr);
   return cudaGetLastError();
 }
 template <int D, bool BF16, bool DROP>
-cudaError_t bwd(const AttnTrainParams& p, cudaStream_t st) {
-  const int nt = (p.S + kT - 1) / kT;
-  attn_train_dq_kernel<D, BF16, DROP><<<(unsigned)((long long)nt * p.B * p.Hq), kThreads, 0, st>>>(p, nt);
-  const cudaError_t e = cudaGetLastError();
+cudaError_t run_bwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sms, cudaStream_t st) {
+  auto kq = attn_train_dq_tc_kernel<D, BF16, DROP>;
+  auto kk = attn_train_dkv_tc_kernel<D, BF16, DROP>;
+  cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kq), BwdSmem<D, true>::BYTES);
   if (e != cudaSuccess) return e;
-  attn_train_dkv_kernel<D, BF16, DROP><<<(unsigned)((long long)nt * p.B * p.Hkv), kThreads, 0, st>>>(p, nt);
+  if ((e = smem_limit_once(reinterpret_cast<const void*>(kk), BwdSmem<D, false>::BYTES)) != cudaSuccess) return e;
+  const Grid gq = grid_rows(p), gk = grid_keys(p);
+  kq<<<ctas(gq, num_sms, kPerSm), kBwdThreads, BwdSmem<D, true>::BYTES, st>>>(m.q_tile, m.do_tile, m.o_tile, m.k_blk,
+                                                                              m.v_blk, p, gq);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  kk<<<ctas(gk, num_sms, kPerSm), kBwdThreads, BwdSmem<D, false>::BYTES, st>>>(m.k_tile, m.v_tile, m.q_blk, m.do_blk, p, gk);
   return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, int D, bool bf16, int num_sms, cudaStream_t st) {
+cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
+                                        int num_sms, cudaStream_t st) {
   const bool drop = p.threshold != 0;
   if (D == 32)
-    return bf16 ? (drop ? fwd<32, true, true>(p, st) : fwd<32, true, false>(p, st))
-                : (drop ? fwd<32, false, true>(p, st) : fwd<32, false, false>(p, st));
-  return bf16 ? (drop ? fwd<64, true, true>(p, st) : fwd<64, true, false>(p, st))
-              : (drop ? fwd<64, false, true>(p, st) : fwd<64, false, false>(p, st));
+    return bf16 ? (drop ? run_fwd<32, true, true>(p, m, num_sms, st) : run_fwd<32, true, false>(p, m, num_sms, st))
+                : (drop ? run_fwd<32, false, true>(p, m, num_sms, st) : run_fwd<32, false, false>(p, m, num_sms, st));
+  return bf16 ? (drop ? run_fwd<64, true, true>(p, m, num_sms, st) : run_fwd<64, true, false>(p, m, num_sms, st))
+              : (drop ? run_fwd<64, false, true>(p, m, num_sms, st) : run_fwd<64, false, false>(p, m, num_sms, st));
 }
 
-cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, int D, bool bf16, int num_sms, cudaStream_t st) {
+cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
+                                        int num_sms, cudaStream_t st) {
   const bool drop = p.threshold != 0;
   if (D == 32)
-    return bf16 ? (drop ? bwd<32, true, true>(p, st) : bwd<32, true, false>(p, st))
-                : (drop ? bwd<32, false, true>(p, st) : bwd<32, false, false>(p, st));
-  return bf16 ? (drop ? bwd<64, true, true>(p, st) : bwd<64, true, false>(p, st))
-              : (drop ? bwd<64, false, true>(p, st) : bwd<64, false, false>(p, st));
+    return bf16 ? (drop ? run_bwd<32, true, true>(p, m, num_sms, st) : run_bwd<32, true, false>(p, m, num_sms, st))
+                : (drop ? run_bwd<32, false, true>(p, m, num_sms, st) : run_bwd<32, false, false>(p, m, num_sms, st));
+  return bf16 ? (drop ? run_bwd<64, true, true>(p, m, num_sms, st) : run_bwd<64, true, false>(p, m, num_sms, st))
+              : (drop ? run_bwd<64, false, true>(p, m, num_sms, st) : run_bwd<64, false, false>(p, m, num_sms, st));
 }
 
 }  // namespace dtk

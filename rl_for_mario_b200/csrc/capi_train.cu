@@ -70,7 +70,7 @@ int check_attn(const char* fn, int B, int S, int Hq, int Hkv, int D, const int64
     if (strides[i] <= 0 || strides[i] % 8 != 0)
       return api_fail(DT_ERR_INVALID, "%s: stride #%d (%lld) must be a positive multiple of 8", fn, i,
                       (long long)strides[i]);
-  if ((long long)((S + 63) / 64) * B * Hq > 0x7fffffffLL)
+  if ((long long)((S + 63) / 64) * B * Hq > 0x3fffffffLL)
     return api_fail(DT_ERR_UNSUPPORTED, "%s: too many query tiles (B=%d S=%d Hq=%d)", fn, B, S, Hq);
   return DT_OK;
 }
@@ -130,13 +130,14 @@ int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, 
   a.rng = reinterpret_cast<const long long*>(rng);
   a.site = site;
   a.HC = a.R < 64 ? a.R : 64;
+  a.PT128 = 128 / a.HC, a.PT64 = 64 / a.HC, a.by_pt64 = dtk::FastDiv((uint32_t)a.PT64);
   const bool bf16 = dtype == DT_DTYPE_BF16;
   dtk::AttnTrainMaps m;
   if ((rc = dtk::api_encode_bshd(&m.q_tile, q, bf16, B, S, Hq, D, q_sb, q_ss, q_sh, a.HC, 128 / a.HC, "q")) ||
       (rc = dtk::api_encode_bshd(&m.k_blk, k, bf16, B, S, Hkv, D, k_sb, k_ss, k_sh, 1, 64, "k")) ||
       (rc = dtk::api_encode_bshd(&m.v_blk, v, bf16, B, S, Hkv, D, v_sb, v_ss, v_sh, 1, 64, "v")))
     return rc;
-  return cuda_status(dtk::launch_attn_train_fwd_tc_sm100(a, m, D, bf16, static_cast<cudaStream_t>(stream)), fn);
+  return cuda_status(dtk::launch_attn_train_fwd_sm100(a, m, D, bf16, sms, static_cast<cudaStream_t>(stream)), fn);
 }
 
 int dt_attn_train_backward(const void* dout, const void* q, const void* k, const void* v, const void* o,
@@ -166,6 +167,7 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
   a.rng = reinterpret_cast<const long long*>(rng);
   a.site = site;
   a.HC = a.R < 64 ? a.R : 64;
+  a.PT128 = 128 / a.HC, a.PT64 = 64 / a.HC, a.by_pt64 = dtk::FastDiv((uint32_t)a.PT64);
   const bool bf16 = dtype == DT_DTYPE_BF16;
   dtk::AttnTrainMaps m;
   const uint32_t hc = (uint32_t)a.HC;
@@ -173,13 +175,14 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
       (rc = dtk::api_encode_bshd(&m.q_blk, q, bf16, B, S, Hq, D, a.q_sb, a.q_ss, a.q_sh, hc, 64 / hc, "q")) ||
       (rc = dtk::api_encode_bshd(&m.do_tile, dout, bf16, B, S, Hq, D, a.do_sb, a.do_ss, a.do_sh, hc, 128 / hc,
                                  "dout")) ||
+      (rc = dtk::api_encode_bshd(&m.o_tile, o, bf16, B, S, Hq, D, a.o_sb, a.o_ss, a.o_sh, hc, 128 / hc, "o")) ||
       (rc = dtk::api_encode_bshd(&m.do_blk, dout, bf16, B, S, Hq, D, a.do_sb, a.do_ss, a.do_sh, hc, 64 / hc, "dout")) ||
       (rc = dtk::api_encode_bshd(&m.k_tile, k, bf16, B, S, Hkv, D, a.k_sb, a.k_ss, a.k_sh, 1, 128, "k")) ||
       (rc = dtk::api_encode_bshd(&m.k_blk, k, bf16, B, S, Hkv, D, a.k_sb, a.k_ss, a.k_sh, 1, 64, "k")) ||
       (rc = dtk::api_encode_bshd(&m.v_tile, v, bf16, B, S, Hkv, D, a.v_sb, a.v_ss, a.v_sh, 1, 128, "v")) ||
       (rc = dtk::api_encode_bshd(&m.v_blk, v, bf16, B, S, Hkv, D, a.v_sb, a.v_ss, a.v_sh, 1, 64, "v")))
     return rc;
-  return cuda_status(dtk::launch_attn_train_bwd_tc_sm100(a, m, D, bf16, static_cast<cudaStream_t>(stream)), fn);
+  return cuda_status(dtk::launch_attn_train_bwd_sm100(a, m, D, bf16, sms, static_cast<cudaStream_t>(stream)), fn);
 }
 
 int dt_rope_grad(void* g, int64_t g_stride, int64_t rows, const float* cos_tab, const float* sin_tab,

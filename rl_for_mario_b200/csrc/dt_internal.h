@@ -257,6 +257,25 @@ cudaError_t launch_residual_norm_fwd_sm100(ResidualNormParams p, int dtype, int 
 cudaError_t launch_residual_norm_bwd_sm100(ResidualNormParams p, const ResidualNormPlan& plan, int dtype,
                                            cudaStream_t st);
 
+// Division of n < 2^31 by a fixed divisor: a multiplication and a shift, prepared
+// on the host.  With 2^b the first power of two >= d, m = ceil(2^(31 + b) / d) is
+// off by less than one part in 2^31, so n m >> (31 + b) is floor(n / d).
+struct FastDiv {
+  uint32_t d = 1, m = 0, s = 0;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div) {
+    uint32_t b = 0;
+    while ((1ull << b) < div) ++b;
+    s = b ? b - 1 : 0;
+    m = (uint32_t)(((1ull << (31 + b)) + div - 1) / div);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int operator()(int n) const {
+    return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> s);
+  }
+#endif
+};
+
 struct AttnTrainParams {
   const void* q;
   const void* k;
@@ -273,6 +292,8 @@ struct AttnTrainParams {
   long long do_sb, do_ss, do_sh, dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
   int B, S, Hq, Hkv, R;
   int HC;       // query heads packed into a tile: min(R, 64)
+  int PT128, PT64;  // positions of a tile of 128 packed rows and of a block of 64
+  FastDiv by_pt64;
   int* status;  // device status word
   float scale;
   const long long* rng;
@@ -282,14 +303,12 @@ struct AttnTrainParams {
 // TMA maps over [B, S, H, D]: tiles of 128 rows and blocks of 64, of packed
 // (position, head) rows for q and dout, of positions of one head for k and v.
 struct AttnTrainMaps {
-  CUtensorMap q_tile, do_tile, q_blk, do_blk, k_tile, v_tile, k_blk, v_blk;
+  CUtensorMap q_tile, do_tile, o_tile, q_blk, do_blk, k_tile, v_tile, k_blk, v_blk;
 };
-cudaError_t launch_attn_train_fwd_tc_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
-                                           cudaStream_t st);
-cudaError_t launch_attn_train_bwd_tc_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
-                                           cudaStream_t st);
-cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, int D, bool bf16, int num_sms, cudaStream_t st);
-cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, int D, bool bf16, int num_sms, cudaStream_t st);
+cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
+                                        int num_sms, cudaStream_t st);
+cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
+                                        int num_sms, cudaStream_t st);
 
 // Batched NES emulation (nes_sm100.cu).  op: 0 run frames, 1 reset, 2 buttons,
 // 3 observation, 4 environment bookkeeping.  Unused fields may be left zero.

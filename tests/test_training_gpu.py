@@ -12,6 +12,17 @@ from oracle import train_ref as ref
 EPS = 1e-5
 
 
+@pytest.fixture(autouse=True)
+def no_device_error(request):
+    """No kernel of a test reports a wait that ran out."""
+    yield
+    if "gpu" in request.keywords and torch.cuda.is_available():
+        from rl_for_mario_b200.kernels import device_status
+
+        torch.cuda.synchronize()
+        assert device_status() == 0
+
+
 def small_model(dtype, dropout=0.1, hidden=128, heads=4, kv_heads=2, layers=2, context=8, seed=0):
     from rl_for_mario_b200.dt_model import DTConfig, MarioDT
 
