@@ -235,21 +235,56 @@ __device__ __forceinline__ uint4 pack8(const uint32_t* v, float f) {
                     E::from_f2(__uint_as_float(v[6]) * f, __uint_as_float(v[7]) * f));
 }
 
-// Scores of one tile against one block: D[128 x 64] = A[128 x D] B[64 x D]^T.
+// Shared-memory matrix descriptors: the address is in the low word, so a thread
+// that issues MMAs adds to 32 bits and joins the words in the instruction.
+struct Desc {
+  uint32_t lo, hi;
+  __device__ __forceinline__ Desc(const void* tile, uint32_t lbo, uint32_t sbo, uint32_t layout) {
+    const uint64_t d = umma_smem_desc(smem_u32(tile), lbo, sbo, layout);
+    lo = (uint32_t)d;
+    hi = (uint32_t)(d >> 32);
+  }
+};
+template <bool FIRST>
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                       uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(tmem_d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(FIRST ? 0 : 1)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tmov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Scores of one tile against one block: D[128 x 64] = A[128 x D] B[64 x D]^T; a_at and
+// b_at move the descriptors to a tile buffer and a stage.
 template <int D>
-__device__ __forceinline__ void issue_scores(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc) {
+__device__ __forceinline__ void issue_scores(uint32_t tmem_d, const Desc& a, uint32_t a_at, const Desc& b,
+                                             uint32_t b_at, uint32_t idesc) {
+  const uint32_t al = a.lo + a_at, bl = b.lo + b_at;
+  mma_ss<true>(tmem_d, al, a.hi, bl, b.hi, idesc);
 #pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk) umma_f16_ss(tmem_d, a + 2 * kk, b + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+  for (int kk = 1; kk < D / 16; ++kk) mma_ss<false>(tmem_d, al + 2 * kk, a.hi, bl + 2 * kk, b.hi, idesc);
 }
 // D[128 x D] += A[128 x 64] B[64 x D] with A in tensor memory: its first 32 columns
 // in 16 columns of 32 bits, the others half_step columns further.
 template <int D>
-__device__ __forceinline__ void issue_weights(uint32_t tmem_d, uint32_t tmem_a, uint32_t half_step, uint64_t b,
-                                              uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void issue_weights(uint32_t tmem_d, uint32_t tmem_a, uint32_t half_step, const Desc& b,
+                                              uint32_t b_at, uint32_t idesc, bool accumulate) {
+  const uint32_t bl = b.lo + b_at;
 #pragma unroll
   for (int kk = 0; kk < kBlk / 16; ++kk)
-    umma_f16_ts(tmem_d, tmem_a + (uint32_t)(kk >> 1) * half_step + (uint32_t)((kk & 1) * 8),
-                b + (uint64_t)(kk * 16 * TcShape<D>::ROWB >> 4), idesc, (accumulate || kk > 0) ? 1u : 0u);
+    mma_ts(tmem_d, tmem_a + (uint32_t)(kk >> 1) * half_step + (uint32_t)((kk & 1) * 8),
+           bl + (uint32_t)(kk * 16 * TcShape<D>::ROWB >> 4), b.hi, idesc, kk > 0 ? 1u : (uint32_t)accumulate);
 }
 
 __device__ __forceinline__ void tc_init(TcShared* sh, int warps) {
@@ -519,18 +554,18 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
   volatile int* abort = &sh->abort;
 
   if (tid == 128) {
-    const uint64_t qd = umma_smem_desc(smem_u32(smem), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t kd = umma_smem_desc(smem_u32(smem + SM::OFF_K), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t vd = umma_smem_desc(smem_u32(smem + SM::OFF_V), SH::BLK, SH::SBO, SH::LAYOUT);
+    const Desc qd(smem, 16, SH::SBO, SH::LAYOUT);
+    const Desc kd(smem + SM::OFF_K, 16, SH::SBO, SH::LAYOUT);
+    const Desc vd(smem + SM::OFF_V, SH::BLK, SH::SBO, SH::LAYOUT);
     const uint32_t id_s = umma_idesc_f16(BF16, kRows, kBlk, 0, 0), id_o = umma_idesc_f16(BF16, kRows, D, 0, 1);
     issue_rows<kFwdBufs, 2, SH::STAGES>(
         sh, p.status,
         [&](int zero, int st) { zero_padded_keys<D>(smem + SM::OFF_K, smem + SM::OFF_V, st, zero); },
         [&](int tb, int st, int sb) {
-          issue_scores<D>(t_s + (uint32_t)(sb * kBlk), qd + (uint64_t)((tb * SH::TILE) >> 4),
-                          kd + (uint64_t)((st * SH::BLK) >> 4), id_s);
+          issue_scores<D>(t_s + (uint32_t)(sb * kBlk), qd, (uint32_t)(tb * (SH::TILE >> 4)), kd,
+                          (uint32_t)(st * (SH::BLK >> 4)), id_s);
         },
-        [&](int st, bool acc) { issue_weights<D>(t_o, t_p, 16, vd + (uint64_t)((st * SH::BLK) >> 4), id_o, acc); });
+        [&](int st, bool acc) { issue_weights<D>(t_o, t_p, 16, vd, (uint32_t)(st * (SH::BLK >> 4)), id_o, acc); });
   } else if (tid == 160) {
     load_all<2, SH::STAGES, QTile>(
         sh, p, gr,
@@ -555,7 +590,7 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
     const uint32_t tp = t_p + lane_off, to = t_o + lane_off;
     const float c2 = p.scale * 1.4426950408889634f;
     const unsigned per_row = (unsigned)(S + 7) >> 3;
-    const uint32_t th = p.threshold << 16;
+    const uint32_t t2 = p.threshold * 0x10001u;
     DropKey key{};
     if constexpr (DROP) key = drop_key(p.rng, p.site);
     int blk = 0;
@@ -655,24 +690,19 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int b8 = 0; b8 < 4; ++b8) {
-            uint4 w8;
+            uint4 w8{};
             if constexpr (DROP) w8 = philox7(key, row_block + (unsigned)((k0 + 32 * c) / 8 + b8));
-            auto two = [&](auto I) {
-              constexpr int e = decltype(I)::value;
-              const int i = 8 * b8 + e;
+            const uint32_t words[4] = {w8.x, w8.y, w8.z, w8.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 8 * b8 + 2 * e;
               const float2 x = ffma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2v, nm);
-              float2 w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              const float2 w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
               sum = fadd2(sum, w);
-              if constexpr (DROP) {
-                w.x = stays<e>(w8, th) ? w.x : 0.f;
-                w.y = stays<e + 1>(w8, th) ? w.y : 0.f;
-              }
               s[i >> 1] = E::from_f2(w.x, w.y);
-            };
-            two(Int<0>{});
-            two(Int<2>{});
-            two(Int<4>{});
-            two(Int<6>{});
+              // Dropped halves of the packed pair are cleared: a flag times 0xffff is its half's mask.
+              if constexpr (DROP) s[i >> 1] &= ~(drop_flags(words[e], t2) * 0xffffu);
+            }
           }
           l += sum.x + sum.y;
         };
@@ -777,21 +807,21 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
   volatile int* abort = &sh->abort;
 
   if (tid == 256) {
-    const uint64_t qd = umma_smem_desc(smem_u32(smem), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t dd = umma_smem_desc(smem_u32(smem + SM::OFF_B), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t kd = umma_smem_desc(smem_u32(smem + SM::OFF_C), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t vd = umma_smem_desc(smem_u32(smem + SM::OFF_E), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t kt = umma_smem_desc(smem_u32(smem + SM::OFF_C), SH::BLK, SH::SBO, SH::LAYOUT);
+    const Desc qd(smem, 16, SH::SBO, SH::LAYOUT);
+    const Desc dd(smem + SM::OFF_B, 16, SH::SBO, SH::LAYOUT);
+    const Desc kd(smem + SM::OFF_C, 16, SH::SBO, SH::LAYOUT);
+    const Desc vd(smem + SM::OFF_E, 16, SH::SBO, SH::LAYOUT);
+    const Desc kt(smem + SM::OFF_C, SH::BLK, SH::SBO, SH::LAYOUT);
     const uint32_t id_s = umma_idesc_f16(BF16, kRows, kBlk, 0, 0), id_o = umma_idesc_f16(BF16, kRows, D, 0, 1);
     issue_rows<1, SH::BWD_TILES, SH::DQ_STAGES>(
         sh, p.status,
         [&](int zero, int st) { zero_padded_keys<D>(smem + SM::OFF_C, smem + SM::OFF_E, st, zero); },
         [&](int tb, int st, int) {
-          const uint64_t ta = (uint64_t)((tb * SH::TILE) >> 4), sa = (uint64_t)((st * SH::BLK) >> 4);
-          issue_scores<D>(t_s, qd + ta, kd + sa, id_s);
-          issue_scores<D>(t_dp, dd + ta, vd + sa, id_s);
+          const uint32_t ta = (uint32_t)(tb * (SH::TILE >> 4)), sa = (uint32_t)(st * (SH::BLK >> 4));
+          issue_scores<D>(t_s, qd, ta, kd, sa, id_s);
+          issue_scores<D>(t_dp, dd, ta, vd, sa, id_s);
         },
-        [&](int st, bool acc) { issue_weights<D>(t_dq, t_ds, 16, kt + (uint64_t)((st * SH::BLK) >> 4), id_o, acc); });
+        [&](int st, bool acc) { issue_weights<D>(t_dq, t_ds, 16, kt, (uint32_t)(st * (SH::BLK >> 4)), id_o, acc); });
   } else if (tid == 288) {
     load_all<SH::BWD_TILES, SH::DQ_STAGES, QTile>(
         sh, p, gr,
@@ -1029,21 +1059,21 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
   volatile int* abort = &sh->abort;
 
   if (tid == 256) {
-    const uint64_t kd = umma_smem_desc(smem_u32(smem), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t vd = umma_smem_desc(smem_u32(smem + SM::OFF_B), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t qd = umma_smem_desc(smem_u32(smem + SM::OFF_C), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t dd = umma_smem_desc(smem_u32(smem + SM::OFF_E), 16, SH::SBO, SH::LAYOUT);
-    const uint64_t qt = umma_smem_desc(smem_u32(smem + SM::OFF_C), SH::BLK, SH::SBO, SH::LAYOUT);
-    const uint64_t dt = umma_smem_desc(smem_u32(smem + SM::OFF_E), SH::BLK, SH::SBO, SH::LAYOUT);
+    const Desc kd(smem, 16, SH::SBO, SH::LAYOUT);
+    const Desc vd(smem + SM::OFF_B, 16, SH::SBO, SH::LAYOUT);
+    const Desc qd(smem + SM::OFF_C, 16, SH::SBO, SH::LAYOUT);
+    const Desc dd(smem + SM::OFF_E, 16, SH::SBO, SH::LAYOUT);
+    const Desc qt(smem + SM::OFF_C, SH::BLK, SH::SBO, SH::LAYOUT);
+    const Desc dt(smem + SM::OFF_E, SH::BLK, SH::SBO, SH::LAYOUT);
     const uint32_t id_s = umma_idesc_f16(BF16, kRows, kBlk, 0, 0), id_o = umma_idesc_f16(BF16, kRows, D, 0, 1);
-    auto tile_at = [](int tb) { return (uint64_t)((tb * SH::TILE) >> 4); };
-    auto blk_at = [](int st) { return (uint64_t)((st * SH::BLK) >> 4); };
+    auto tile_at = [](int tb) { return (uint32_t)(tb * (SH::TILE >> 4)); };
+    auto blk_at = [](int st) { return (uint32_t)(st * (SH::BLK >> 4)); };
     issue_keys<SH::BWD_TILES, SH::STAGES>(
         sh, p.status,
-        [&](int tb, int st) { issue_scores<D>(t_s, kd + tile_at(tb), qd + blk_at(st), id_s); },
-        [&](int tb, int st) { issue_scores<D>(t_dp, vd + tile_at(tb), dd + blk_at(st), id_s); },
-        [&](int st, bool acc) { issue_weights<D>(t_dv, t_s, 32, dt + blk_at(st), id_o, acc); },
-        [&](int st, bool acc) { issue_weights<D>(t_dk, t_dp, 32, qt + blk_at(st), id_o, acc); });
+        [&](int tb, int st) { issue_scores<D>(t_s, kd, tile_at(tb), qd, blk_at(st), id_s); },
+        [&](int tb, int st) { issue_scores<D>(t_dp, vd, tile_at(tb), dd, blk_at(st), id_s); },
+        [&](int st, bool acc) { issue_weights<D>(t_dv, t_s, 32, dt, blk_at(st), id_o, acc); },
+        [&](int st, bool acc) { issue_weights<D>(t_dk, t_dp, 32, qt, blk_at(st), id_o, acc); });
   } else if (tid == 288) {
     load_all<SH::BWD_TILES, SH::STAGES, KTile>(
         sh, p, gr,
@@ -1067,22 +1097,24 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         });
   } else if (warp < 8) {
     const int half = warp >> 2, wq = warp & 3;
-    const uint32_t lane_off = (uint32_t)(wq * 32) << 16, lane_bit = 1u << lane;
+    const uint32_t lane_off = (uint32_t)(wq * 32) << 16, lane_bit = drop_bit(lane);
     const uint32_t ts = t_s + lane_off + 32 * half, tdp = t_dp + lane_off + 32 * half;
     const float c2 = p.scale * 1.4426950408889634f;
+    const float2 c2v = make_float2(c2, c2), ik = make_float2(p.inv_keep, p.inv_keep);
     DropKey key{};
     const unsigned per_row = (unsigned)(S + 7) >> 3;
     if constexpr (DROP) key = drop_key(p.rng, p.site);
-    // Scalars of the warp's 32 columns (query rows): lane l fetches those of column l.
-    float2* x_ld = reinterpret_cast<float2*>(smem + SM::OFF_X) + warp * 32;               // lse, delta
-    uint32_t* x_keep = reinterpret_cast<uint32_t*>(smem + SM::OFF_X + 2048) + warp * 32;  // keep bits of the warp's keys
+    // Scalars of the warp's 32 columns (query rows): lane l fetches those of column l; 4-byte arrays read in pairs.
+    float* x_nl = reinterpret_cast<float*>(smem + SM::OFF_X) + warp * 32;                 // -lse
+    float* x_nd = reinterpret_cast<float*>(smem + SM::OFF_X + 1024) + warp * 32;          // -delta
+    uint32_t* x_drop = reinterpret_cast<uint32_t*>(smem + SM::OFF_X + 2048) + warp * 32;  // drop flags of the warp's keys
     int* x_pos = reinterpret_cast<int*>(smem + SM::OFF_X + 3072) + warp * 32;
     const int col = 32 * half + lane, chead = col % p.HC, cpos = col / p.HC;
     const int last_pos = min(32 * half + 31, rows - 1) / p.HC;
     int blk = 0, done = 0;
     bool ok = true;
     ItemReader items{sh, abort, p.status};
-    // The finished tile: dv (first warpgroup) or dk (second) is read behind the next tile's first weights.
+    // The finished tile: dv (first warpgroup) or dk (second) is read when the next tile's first scores are there.
     uint16_t* fin_out = nullptr;
     bool fin = false;
     auto finish = [&]() {
@@ -1118,41 +1150,46 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + pz * out_ss + c) = make_uint4(0u, 0u, 0u, 0u);
       }
       items.next();
-      // Query row of the thread's column in block j, or -1; and its lse and delta.
-      auto row_of = [&](int j) -> long long {
-        const int chunk = gr.chunks > 1 ? j / per : 0, pos = first + (j - chunk * per) * PT + cpos;
-        const bool ok_row = j < nblk && col < rows && chunk * p.HC + chead < p.R && pos < S;
-        return ok_row ? row_at + (long long)(chunk * p.HC + chead) * S + pos : -1;
+      // Position and row of the thread's column in the block whose scalars are fetched next, and those scalars.
+      int npos = first + cpos;
+      long long nrow = row_at + (long long)chead * S + npos;
+      float nl = -INFINITY, nd = 0.f;
+      auto fetch = [&](int j) {
+        if (gr.chunks > 1 && j > 0 && j % per == 0) {  // the next chunk of heads, from the first position again
+          npos = first + cpos;
+          nrow = row_at + (long long)(j / per * p.HC + chead) * S + npos;
+        }
+        const bool there = j < nblk && col < rows && npos < S && (gr.chunks == 1 || j / per * p.HC + chead < p.R);
+        nl = there ? -__ldg(p.lse + nrow) : -INFINITY;
+        nd = there ? -__ldg(p.delta + nrow) : 0.f;
       };
-      auto scalars_of = [&](long long row) {
-        return row >= 0 ? make_float2(__ldg(p.lse + row), __ldg(p.delta + row)) : make_float2(INFINITY, 0.f);
-      };
-      long long row = row_of(0);
-      float2 ld = scalars_of(row);
+      fetch(0);
       for (int j = 0; j < nblk; ++j, ++blk) {
-        const int chunk = gr.chunks > 1 ? j / per : 0, q0 = first + (j - chunk * per) * PT;
-        const int pos = q0 + cpos;
+        const int pos = npos, q0 = pos - cpos;
+        const long long row = nrow;
         // The warp's last position against its first key: nothing to do where every query comes before every key.
-        const int last = q0 + last_pos;
-        const bool any = last >= key0;
-        uint32_t keep = 0;
+        const bool any = q0 + last_pos >= key0;
+        uint32_t drop = 0;
         if constexpr (DROP) {
-          if (any) {
-            const unsigned long long b0 = (unsigned long long)row * per_row + (unsigned)(key0 >> 3);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) keep |= keep_bits(key, b0 + c, p.threshold) << (8 * c);
-          }
+          if (any) drop = drop_word(key, (unsigned long long)row * per_row + (unsigned)(key0 >> 3), p.threshold);
         }
         __syncwarp();
-        x_ld[lane] = ld;
-        if constexpr (DROP) x_keep[lane] = keep;
+        x_nl[lane] = nl;
+        x_nd[lane] = nd;
+        if constexpr (DROP) x_drop[lane] = drop;
         x_pos[lane] = pos;
         __syncwarp();
         // The next block's scalars: on their way while this one is worked on.
-        row = row_of(j + 1);
-        ld = scalars_of(row);
+        npos += PT;
+        nrow += PT;
+        fetch(j + 1);
         if (!(ok = warp_wait(&sh->s_full[0], blk & 1, abort, p.status))) break;
         tc_fence_after();
+        if (fin) {
+          if (!(ok = warp_wait(&sh->w_done, (done - 1) & 1, abort, p.status))) break;
+          tc_fence_after();
+          finish();
+        }
         uint32_t s[32];
         if (any) {
           tmem_ld32_async(ts, s);
@@ -1163,37 +1200,31 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
             for (int c = 0; c < 32; ++c)
               if (kk > x_pos[c]) s[c] = 0xff800000u;
           }
-          uint32_t pw[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const float4 a = *reinterpret_cast<const float4*>(x_ld + c);  // lse, delta of two columns
-            const float w0 = ex2_approx(fmaf(__uint_as_float(s[c]), c2, -a.x));
-            const float w1 = ex2_approx(fmaf(__uint_as_float(s[c + 1]), c2, -a.z));
-            s[c] = __float_as_uint(w0);
-            s[c + 1] = __float_as_uint(w1);
-            if constexpr (DROP) {
-              const uint2 kb = *reinterpret_cast<const uint2*>(x_keep + c);
-              pw[c >> 1] = E::from_f2(kb.x & lane_bit ? w0 : 0.f, kb.y & lane_bit ? w1 : 0.f);
-            } else {
-              pw[c >> 1] = E::from_f2(w0, w1);
+          for (int c0 = 0; c0 < 32; c0 += 16) {
+            uint32_t pw[8];
+#pragma unroll
+            for (int c = c0; c < c0 + 16; c += 2) {
+              const float2 x = ffma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2v,
+                                     *reinterpret_cast<const float2*>(x_nl + c));
+              const float w0 = ex2_approx(x.x), w1 = ex2_approx(x.y);
+              s[c] = __float_as_uint(w0);
+              s[c + 1] = __float_as_uint(w1);
+              if constexpr (DROP) {
+                const uint2 db = *reinterpret_cast<const uint2*>(x_drop + c);
+                pw[(c - c0) >> 1] = E::from_f2(db.x & lane_bit ? 0.f : w0, db.y & lane_bit ? 0.f : w1);
+              } else {
+                pw[(c - c0) >> 1] = E::from_f2(w0, w1);
+              }
             }
+            tmem_st8(ts + (c0 >> 1), pw);
           }
-          if (fin) {
-            if (!(ok = warp_wait(&sh->w_done, (done - 1) & 1, abort, p.status))) break;
-            tc_fence_after();
-            finish();
-          }
-          tmem_st16(ts, pw);
         } else {
-          if (fin) {
-            if (!(ok = warp_wait(&sh->w_done, (done - 1) & 1, abort, p.status))) break;
-            tc_fence_after();
-            finish();
-          }
-          uint32_t z[16];
+          uint32_t z[8];
 #pragma unroll
-          for (int c = 0; c < 16; ++c) z[c] = 0u;
-          tmem_st16(ts, z);
+          for (int c = 0; c < 8; ++c) z[c] = 0u;
+          tmem_st8(ts, z);
+          tmem_st8(ts + 8, z);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -1214,17 +1245,16 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
             tmem_ld16_u(tdp + c0, dp);
 #pragma unroll
             for (int c = 0; c < 16; c += 2) {
-              const float4 a = *reinterpret_cast<const float4*>(x_ld + c0 + c);
-              float d0 = __uint_as_float(dp[c]), d1 = __uint_as_float(dp[c + 1]);
+              const float2 md = *reinterpret_cast<const float2*>(x_nd + c0 + c);
+              float2 d = make_float2(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1]));
               if constexpr (DROP) {
-                const uint2 kb = *reinterpret_cast<const uint2*>(x_keep + c0 + c);
-                d0 = fmaf(kb.x & lane_bit ? d0 : 0.f, p.inv_keep, -a.y);
-                d1 = fmaf(kb.y & lane_bit ? d1 : 0.f, p.inv_keep, -a.w);
+                const uint2 db = *reinterpret_cast<const uint2*>(x_drop + c0 + c);
+                d = ffma2(make_float2(db.x & lane_bit ? 0.f : d.x, db.y & lane_bit ? 0.f : d.y), ik, md);
               } else {
-                d0 -= a.y;
-                d1 -= a.w;
+                d = fadd2(d, md);
               }
-              s[(c0 + c) >> 1] = E::from_f2(__uint_as_float(s[c0 + c]) * d0, __uint_as_float(s[c0 + c + 1]) * d1);
+              d = fmul2(make_float2(__uint_as_float(s[c0 + c]), __uint_as_float(s[c0 + c + 1])), d);
+              s[(c0 + c) >> 1] = E::from_f2(d.x, d.y);
             }
           }
           tmem_st16(tdp, *reinterpret_cast<uint32_t(*)[16]>(s));

@@ -53,20 +53,37 @@ __device__ __forceinline__ bool stays(const uint4& w, uint32_t threshold_hi) {
   return (I & 1 ? x : x << 16) >= threshold_hi;
 }
 
-// Bit i set: element i of the block stays.  threshold in [1, 65535].
+// Drop flags of a block's eight elements in four words: bit 0 of word i is set when
+// element 2 i is dropped, bit 16 when element 2 i + 1 is.  Both halves of a word at
+// once: max(w, t) - w is 0 in a half that stays (w >= t), min with 1 makes a flag of
+// the rest.  t2 = threshold * 0x10001.
+__device__ __forceinline__ uint32_t drop_flags(uint32_t w, uint32_t t2) {
+  return __vminu2(__vmaxu2(w, t2) - w, 0x00010001u);
+}
+
+// Bit i set: element i of the block stays.
 __device__ __forceinline__ uint32_t keep_bits(const DropKey& k, unsigned long long block, uint32_t threshold) {
   const uint4 w = philox7(k, block);
-  const uint32_t th = threshold << 16;
-  uint32_t m = 0;
-  m |= stays<0>(w, th) ? 1u : 0u;
-  m |= stays<1>(w, th) ? 2u : 0u;
-  m |= stays<2>(w, th) ? 4u : 0u;
-  m |= stays<3>(w, th) ? 8u : 0u;
-  m |= stays<4>(w, th) ? 16u : 0u;
-  m |= stays<5>(w, th) ? 32u : 0u;
-  m |= stays<6>(w, th) ? 64u : 0u;
-  m |= stays<7>(w, th) ? 128u : 0u;
-  return m;
+  const uint32_t t2 = threshold * 0x10001u;
+  // Even elements' flags in bits 0, 2, 4, 6, odd ones' in bits 16, 18, 20, 22, then one above the other.
+  const uint32_t d = drop_flags(w.x, t2) + drop_flags(w.y, t2) * 4u + drop_flags(w.z, t2) * 16u + drop_flags(w.w, t2) * 64u;
+  return ~(d | d >> 15) & 0xffu;
+}
+
+// The flags of four blocks (32 elements) in one word, a set bit for a dropped one:
+// element e of block b is bit (e & 1) * 16 + 4 b + e / 2 (drop_bit).
+__device__ __forceinline__ uint32_t drop_word(const DropKey& k, unsigned long long block, uint32_t threshold) {
+  const uint32_t t2 = threshold * 0x10001u;
+  uint32_t r = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const uint4 w = philox7(k, block + b);
+    r += (drop_flags(w.x, t2) + drop_flags(w.y, t2) * 2u + drop_flags(w.z, t2) * 4u + drop_flags(w.w, t2) * 8u) << (4 * b);
+  }
+  return r;
+}
+__device__ __forceinline__ uint32_t drop_bit(int element) {  // 0 .. 31
+  return 1u << ((element & 1) * 16 + (element >> 3) * 4 + ((element & 7) >> 1));
 }
 
 }  // namespace dtk
