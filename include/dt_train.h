@@ -50,14 +50,19 @@ int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, 
 /*
  * Gradient of dt_attn_train_forward: dq [B, S, Hq, D], dk, dv [B, S, Hkv, D]
  * (summed over the query heads that share a KV head) from dout and the forward
- * call's inputs, o and lse.  delta [B, Hq, S] fp32 is scratch.  strides holds
- * the (batch, position, head) strides of q, k, v, o, dout, dq, dk and dv in
- * that order, 24 values.  Deterministic: each sum has one owner.
+ * call's inputs, o and lse.  strides holds the (batch, position, head) strides
+ * of q, k, v, o, dout, dq, dk and dv in that order, 24 values.  workspace:
+ * dt_attn_train_workspace bytes, 16-byte aligned.  Deterministic: every sum is
+ * taken in a fixed order.
  */
 int dt_attn_train_backward(const void* dout, const void* q, const void* k, const void* v, const void* o,
-                           const float* lse, float* delta, void* dq, void* dk, void* dv, const int32_t* pad_len, int B,
-                           int S, int Hq, int Hkv, int D, const int64_t* strides, float scale, double p,
-                           const int64_t* rng, uint32_t site, int dtype, void* stream);
+                           const float* lse, void* dq, void* dk, void* dv, const int32_t* pad_len, void* workspace,
+                           int64_t workspace_bytes, int B, int S, int Hq, int Hkv, int D, const int64_t* strides,
+                           float scale, double p, const int64_t* rng, uint32_t site, int dtype, void* stream);
+
+/* Bytes of scratch that dt_attn_train_backward needs on the current device;
+ * negative on an error. */
+int64_t dt_attn_train_workspace(int B, int S, int Hq, int Hkv, int D);
 
 /*
  * Gradient of the RoPE that dt_qkv_rope applies to the q and k heads, in place

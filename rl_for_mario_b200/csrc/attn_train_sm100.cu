@@ -13,7 +13,8 @@
 // Two backward kernels: one walks the keys of a tile of query rows (delta, dq),
 // one walks the query rows behind a tile of keys (dk, dv).  Each sum has one
 // owner: no atomics, the same bits every run; the price is that S and dP are
-// formed twice.
+// formed twice.  When the tiles of keys are too few for the GPU, the rows behind
+// each are dealt out to several CTAs whose fp32 sums a third kernel adds in order.
 //
 // Rounding: P and dS enter the second products in the inputs' 16-bit type, as
 // the tensor cores take both operands in one type; sums, softmax statistics
@@ -93,9 +94,9 @@ struct TcShape {
 constexpr int kItems = 8;
 struct alignas(16) Item {
   int nblk, pad, heads, tile;  // blocks (-1: no more items); heads of the chunk
-  int first, origin, per, chunk0;  // rows: p0, kb; keys: q0, k0 and blocks of a chunk of heads
+  int first, origin, per, split;  // rows: p0, kb; keys: q0, k0, blocks of a chunk of heads, the first block
   long long row;   // of lse, delta and the dropout rows: sample and first head, position 0
-  long long out, out2;  // element offsets of the outputs at that sample and head, position 0
+  long long out, out2, part;  // element offsets of the outputs at that sample and head, position 0; rows of partial sums
 };
 
 // Barriers and small shared state behind the tiles.
@@ -112,8 +113,8 @@ struct TcShared {
 // How a kernel's items are numbered: units in groups, inside a group the tiles
 // with the most work first (longest_last: a unit's last tile has the most blocks).
 struct Grid {
-  int units, tiles, items, chunks;
-  FastDiv by_tiles, by_chunks, by_kv;
+  int units, tiles, items, chunks, splits;  // chunks of a group's heads; CTAs that share a tile of keys
+  FastDiv by_tiles, by_parts, by_kv;        // parts of a unit: chunks (rows) or splits (keys)
 };
 struct TcItem {
   int unit, tile;
@@ -144,7 +145,7 @@ struct QTile {
 // q0 on: earlier queries see none of these keys) x chunks of heads behind it.
 struct KTile {
   static constexpr bool kRowTiles = false;
-  int b, g, pad, k0, q0, per, nblk, tile, zero;
+  int b, g, pad, k0, q0, per, nblk, tile, zero, split;  // its blocks are split, split + splits, ...
 };
 
 // The CTA's items in order; the padding of the next one is on its way while one is
@@ -152,7 +153,7 @@ struct KTile {
 template <class T>
 struct Items {
   struct Head {
-    int i, b, g, chunk, tile, pad;
+    int i, b, g, part, tile, pad;
   };
   static constexpr bool kRowTiles = T::kRowTiles;
   int k = 0;
@@ -162,8 +163,8 @@ struct Items {
     next.i = nth_item(k++, gr.items);
     if (next.i >= gr.items) return;
     const TcItem it = tc_item(gr, next.i, kRowTiles);
-    const int bg = kRowTiles ? gr.by_chunks(it.unit) : it.unit;
-    next.chunk = it.unit - bg * (kRowTiles ? gr.chunks : 1);
+    const int bg = gr.by_parts(it.unit);
+    next.part = it.unit - bg * (kRowTiles ? gr.chunks : gr.splits);
     next.b = gr.by_kv(bg);
     next.g = bg - next.b * p.Hkv;
     next.tile = it.tile;
@@ -179,8 +180,8 @@ struct Items {
     t.pad = min(max(h.pad, 0), p.S);
     t.tile = h.tile;
     if constexpr (kRowTiles) {
-      t.h0 = h.g * p.R + h.chunk * p.HC;
-      t.heads = min(p.HC, p.R - h.chunk * p.HC);
+      t.h0 = h.g * p.R + h.part * p.HC;
+      t.heads = min(p.HC, p.R - h.part * p.HC);
       t.p0 = t.pad + h.tile * p.PT128;
       t.kb = t.pad & ~7;
       t.nblk = t.p0 < p.S ? (min(t.p0 + p.PT128, p.S) - 1 - t.kb) / kBlk + 1 : 0;
@@ -189,7 +190,8 @@ struct Items {
       t.k0 = (t.pad & ~7) + h.tile * kRows;
       t.q0 = max(t.k0, t.pad);
       t.per = t.q0 < p.S ? p.by_pt64(p.S - t.q0 + p.PT64 - 1) : 0;
-      t.nblk = t.per * gr.chunks;
+      t.split = h.part;
+      t.nblk = gr.splits == 1 ? t.per * gr.chunks : max(0, t.per - h.part + gr.splits - 1) / gr.splits;
       t.zero = 0;
     }
     return true;
@@ -209,6 +211,9 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+__device__ __forceinline__ bool warp_test(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_test(bar, parity));
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status));
 }
@@ -249,19 +254,26 @@ template <bool FIRST>
 __device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
                                        uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\telect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %6, 0;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(tmem_d),
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(tmem_d),
       "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(FIRST ? 0 : 1)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
                                        uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\telect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %5, 0;\n\tmov.b64 db, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(tmem_d),
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(tmem_d),
       "r"(tmem_a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
       : "memory");
 }
 
@@ -366,23 +378,23 @@ __device__ __forceinline__ void issue_rows(TcShared* sh, int* status, Prepare pr
   auto next_scores = [&](bool wait) {
     const int tb = stile % TB, st = sblk % STAGES;
     if (sj == 0) {
-      if (!wait && !mbar_test(&sh->tile_full[tb], (stile / TB) & 1)) return;
-      if (!(ok = mbar_wait(&sh->tile_full[tb], (stile / TB) & 1, abort, status))) return;
+      if (!wait && !warp_test(&sh->tile_full[tb], (stile / TB) & 1)) return;
+      if (!(ok = warp_wait(&sh->tile_full[tb], (stile / TB) & 1, abort, status))) return;
       sn = sh->tile_meta[stile & 7].x;
       if (sn == 0) {
         end = true;
         return;
       }
     }
-    if (!wait && !mbar_test(&sh->blk_full[st], (sblk / STAGES) & 1)) return;
-    if (!(ok = mbar_wait(&sh->blk_full[st], (sblk / STAGES) & 1, abort, status))) return;
+    if (!wait && !warp_test(&sh->blk_full[st], (sblk / STAGES) & 1)) return;
+    if (!(ok = warp_wait(&sh->blk_full[st], (sblk / STAGES) & 1, abort, status))) return;
     if (sj == 0) prepare(sh->tile_meta[stile & 7].y, st);
     tc_fence_after();
     scores(tb, st, sblk % SB);
-    umma_commit(&sh->s_full[sblk % SB]);
+    commit(&sh->s_full[sblk % SB]);
     ++sblk;
     if (++sj == sn) {
-      umma_commit(&sh->tile_empty[tb]);
+      commit(&sh->tile_empty[tb]);
       sj = 0;
       ++stile;
     }
@@ -393,24 +405,24 @@ __device__ __forceinline__ void issue_rows(TcShared* sh, int* status, Prepare pr
     if (!ok || sblk <= blk) break;
     if (SB > 1 && !end && sblk < blk + SB) next_scores(false);
     // The scores of this block being in registers, their buffer takes the next ones.
-    if (!ok || !(ok = mbar_wait(&sh->s_read[blk % SB], (blk / SB) & 1, abort, status))) break;
+    if (!ok || !(ok = warp_wait(&sh->s_read[blk % SB], (blk / SB) & 1, abort, status))) break;
     if (!end && sblk == blk + SB) next_scores(false);
-    if (!ok || !(ok = mbar_wait(&sh->p_full, blk & 1, abort, status))) break;
+    if (!ok || !(ok = warp_wait(&sh->p_full, blk & 1, abort, status))) break;
     if (j == 0) {
       n = sh->tile_meta[tiles & 7].x;
-      if (tiles > 0 && !(ok = mbar_wait(&sh->o_empty, (tiles - 1) & 1, abort, status))) break;
+      if (tiles > 0 && !(ok = warp_wait(&sh->o_empty, (tiles - 1) & 1, abort, status))) break;
     }
     tc_fence_after();
     weights(blk % STAGES, j > 0);
-    umma_commit(&sh->w_done);
-    umma_commit(&sh->blk_empty[blk % STAGES]);
+    commit(&sh->w_done);
+    commit(&sh->blk_empty[blk % STAGES]);
     if (++j == n) {
       j = 0;
       ++tiles;
     }
   }
-  umma_commit(&sh->drain);
-  mbar_wait(&sh->drain, 0, nullptr, nullptr);
+  commit(&sh->drain);
+  warp_wait(&sh->drain, 0, nullptr, nullptr);
 }
 
 // The same for the dk, dv kernel: weights over their scores, the two halves of a
@@ -425,19 +437,19 @@ __device__ __forceinline__ void issue_keys(TcShared* sh, int* status, ScoresA sc
   auto next_a = [&](bool wait) {
     const int tb = a_tile % TB, st = a_blk % STAGES;
     if (a_j == 0) {
-      if (!wait && !mbar_test(&sh->tile_full[tb], (a_tile / TB) & 1)) return;
-      if (!(ok = mbar_wait(&sh->tile_full[tb], (a_tile / TB) & 1, abort, status))) return;
+      if (!wait && !warp_test(&sh->tile_full[tb], (a_tile / TB) & 1)) return;
+      if (!(ok = warp_wait(&sh->tile_full[tb], (a_tile / TB) & 1, abort, status))) return;
       a_n = sh->tile_meta[a_tile & 7].x;
       if (a_n == 0) {
         end = true;
         return;
       }
     }
-    if (!wait && !mbar_test(&sh->blk_full[st], (a_blk / STAGES) & 1)) return;
-    if (!(ok = mbar_wait(&sh->blk_full[st], (a_blk / STAGES) & 1, abort, status))) return;
+    if (!wait && !warp_test(&sh->blk_full[st], (a_blk / STAGES) & 1)) return;
+    if (!(ok = warp_wait(&sh->blk_full[st], (a_blk / STAGES) & 1, abort, status))) return;
     tc_fence_after();
     scores_a(tb, st);
-    umma_commit(&sh->s_full[0]);
+    commit(&sh->s_full[0]);
     ++a_blk;
     if (++a_j == a_n) {
       a_j = 0;
@@ -446,10 +458,10 @@ __device__ __forceinline__ void issue_keys(TcShared* sh, int* status, ScoresA sc
   };
   auto next_b = [&]() {  // behind next_a of the same block, whose waits it shares
     scores_b(b_tile % TB, b_blk % STAGES);
-    umma_commit(&sh->dp_full);
+    commit(&sh->dp_full);
     ++b_blk;
     if (++b_j == sh->tile_meta[b_tile & 7].x) {
-      umma_commit(&sh->tile_empty[b_tile % TB]);
+      commit(&sh->tile_empty[b_tile % TB]);
       b_j = 0;
       ++b_tile;
     }
@@ -459,27 +471,27 @@ __device__ __forceinline__ void issue_keys(TcShared* sh, int* status, ScoresA sc
     while (ok && !end && a_blk <= blk) next_a(true);
     if (!ok || a_blk <= blk) break;
     if (b_blk <= blk) next_b();
-    if (!(ok = mbar_wait(&sh->p_full, blk & 1, abort, status))) break;
+    if (!(ok = warp_wait(&sh->p_full, blk & 1, abort, status))) break;
     if (j == 0) {
       n = sh->tile_meta[tiles & 7].x;
-      if (tiles > 0 && !(ok = mbar_wait(&sh->o_empty, (tiles - 1) & 1, abort, status))) break;
+      if (tiles > 0 && !(ok = warp_wait(&sh->o_empty, (tiles - 1) & 1, abort, status))) break;
     }
     tc_fence_after();
     weights_a(blk % STAGES, j > 0);
     if (!end) next_a(false);
-    if (!ok || !(ok = mbar_wait(&sh->ds_full, blk & 1, abort, status))) break;
+    if (!ok || !(ok = warp_wait(&sh->ds_full, blk & 1, abort, status))) break;
     tc_fence_after();
     weights_b(blk % STAGES, j > 0);
-    umma_commit(&sh->blk_empty[blk % STAGES]);
+    commit(&sh->blk_empty[blk % STAGES]);
     if (++j == n) {
-      umma_commit(&sh->w_done);
+      commit(&sh->w_done);
       j = 0;
       ++tiles;
     }
     if (b_blk < a_blk) next_b();
   }
-  umma_commit(&sh->drain);
-  mbar_wait(&sh->drain, 0, nullptr, nullptr);
+  commit(&sh->drain);
+  warp_wait(&sh->drain, 0, nullptr, nullptr);
 }
 
 // The element-wise warps' side of the item ring.
@@ -505,11 +517,12 @@ template <int D>
 __device__ __forceinline__ void zero_padded_keys(uint8_t* ring_a, uint8_t* ring_b, int st, int count) {
   using SH = TcShape<D>;
   if (count == 0) return;
-  for (int e = 0; e < count * SH::NCH; ++e) {
+  for (int e = threadIdx.x & 31; e < count * SH::NCH; e += 32) {
     *reinterpret_cast<uint4*>(ring_a + st * SH::BLK + e * 16) = make_uint4(0u, 0u, 0u, 0u);
     *reinterpret_cast<uint4*>(ring_b + st * SH::BLK + e * 16) = make_uint4(0u, 0u, 0u, 0u);
   }
   fence_proxy_async_smem();
+  __syncwarp();
 }
 
 // ---------------------------------------------------------------- forward
@@ -553,7 +566,7 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
   const uint32_t t_s = sh->tmem, t_p = t_s + kFwdBufs * kBlk, t_o = t_p + kBlk / 2;
   volatile int* abort = &sh->abort;
 
-  if (tid == 128) {
+  if (warp == 4) {
     const Desc qd(smem, 16, SH::SBO, SH::LAYOUT);
     const Desc kd(smem + SM::OFF_K, 16, SH::SBO, SH::LAYOUT);
     const Desc vd(smem + SM::OFF_V, SH::BLK, SH::SBO, SH::LAYOUT);
@@ -806,7 +819,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
   const uint32_t t_s = sh->tmem, t_dp = t_s + kBlk, t_ds = t_dp + kBlk, t_dq = t_ds + kBlk / 2;
   volatile int* abort = &sh->abort;
 
-  if (tid == 256) {
+  if (warp == 8) {
     const Desc qd(smem, 16, SH::SBO, SH::LAYOUT);
     const Desc dd(smem + SM::OFF_B, 16, SH::SBO, SH::LAYOUT);
     const Desc kd(smem + SM::OFF_C, 16, SH::SBO, SH::LAYOUT);
@@ -1058,7 +1071,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
   const uint32_t t_s = sh->tmem, t_dp = sh->tmem + 64, t_dv = sh->tmem + 128, t_dk = sh->tmem + 128 + D;
   volatile int* abort = &sh->abort;
 
-  if (tid == 256) {
+  if (warp == 8) {
     const Desc kd(smem, 16, SH::SBO, SH::LAYOUT);
     const Desc vd(smem + SM::OFF_B, 16, SH::SBO, SH::LAYOUT);
     const Desc qd(smem + SM::OFF_C, 16, SH::SBO, SH::LAYOUT);
@@ -1079,10 +1092,11 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         sh, p, gr,
         [&](const KTile& t, Item& it) {
           it.nblk = t.nblk, it.pad = t.pad, it.tile = t.tile;
-          it.first = t.q0, it.origin = t.k0, it.per = t.per;
+          it.first = t.q0, it.origin = t.k0, it.per = t.per, it.split = t.split;
           it.row = ((long long)t.b * p.Hq + t.g * p.R) * S;
           it.out = t.b * p.dv_sb + t.g * p.dv_sh;
           it.out2 = t.b * p.dk_sb + t.g * p.dk_sh;
+          it.part = (((long long)t.split * 2 * p.B + t.b) * p.Hkv + t.g) * S;
         },
         [&](const KTile& t, int tb) {
           mbar_arrive_expect_tx(&sh->tile_full[tb], 2u * SH::TILE);
@@ -1090,7 +1104,8 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
           tma_load_4d(smem + SM::OFF_B + tb * SH::TILE, &tmV, &sh->tile_full[tb], 0, t.g, t.k0, t.b);
         },
         [&](const KTile& t, int j, int st) {
-          const int c = gr.chunks > 1 ? j / t.per : 0, h0 = t.g * p.R + c * p.HC, q0 = t.q0 + (j - c * t.per) * PT;
+          const int c = gr.chunks > 1 ? j / t.per : 0, h0 = t.g * p.R + c * p.HC;
+          const int q0 = t.q0 + (t.split + j * gr.splits - c * t.per) * PT;
           mbar_arrive_expect_tx(&sh->blk_full[st], 2u * (uint32_t)(rows * SH::ROWB));
           tma_load_4d(smem + SM::OFF_C + st * SH::BLK, &tmQ, &sh->blk_full[st], 0, h0, q0, t.b);
           tma_load_4d(smem + SM::OFF_E + st * SH::BLK, &tmDO, &sh->blk_full[st], 0, h0, q0, t.b);
@@ -1116,6 +1131,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     ItemReader items{sh, abort, p.status};
     // The finished tile: dv (first warpgroup) or dk (second) is read when the next tile's first scores are there.
     uint16_t* fin_out = nullptr;
+    float* fin_part = nullptr;
     bool fin = false;
     auto finish = [&]() {
       fin = false;
@@ -1129,7 +1145,10 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->o_empty);
         }
-        if (fin_out)
+        if (fin_part) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(fin_part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else if (fin_out)
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
             *reinterpret_cast<uint4*>(fin_out + c + e) = pack8<BF16>(o + e, half ? p.scale : p.inv_keep);
@@ -1138,17 +1157,19 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     while (true) {
       const Item* it = items.get(ok);
       if (!ok) break;
-      const int nblk = it->nblk, pad = it->pad, per = it->per, first = it->first;
+      const int nblk = it->nblk, pad = it->pad, per = it->per;
+      const int first = it->first + it->split * PT, step = gr.splits * PT;
       if (nblk < 0) break;
       const int key0 = it->origin + wq * 32, kk = key0 + lane;  // the warp's keys, the thread's
       const long long row_at = it->row;
       uint16_t* out = half ? static_cast<uint16_t*>(p.dk) + it->out2 : static_cast<uint16_t*>(p.dv) + it->out;
       const long long out_ss = half ? p.dk_ss : p.dv_ss;
       const int pz = it->tile * kRows + wq * 32 + lane;
-      if (pz < pad) {
+      if (pz < pad && it->split == 0) {
 #pragma unroll
         for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + pz * out_ss + c) = make_uint4(0u, 0u, 0u, 0u);
       }
+      float* part = gr.splits > 1 ? p.part + (it->part + (half ? (long long)p.B * p.Hkv * S : 0)) * D : nullptr;
       items.next();
       // Position and row of the thread's column in the block whose scalars are fetched next, and those scalars.
       int npos = first + cpos;
@@ -1180,8 +1201,8 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         x_pos[lane] = pos;
         __syncwarp();
         // The next block's scalars: on their way while this one is worked on.
-        npos += PT;
-        nrow += PT;
+        npos += step;
+        nrow += step;
         fetch(j + 1);
         if (!(ok = warp_wait(&sh->s_full[0], blk & 1, abort, p.status))) break;
         tc_fence_after();
@@ -1273,7 +1294,9 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       if (nblk > 0) {
         ++done;
         fin = true;
-        fin_out = kk >= pad && kk < S ? out + kk * out_ss : nullptr;
+        const bool kept = kk >= pad && kk < S;
+        fin_out = kept ? out + kk * out_ss : nullptr;
+        fin_part = kept && part ? part + (long long)kk * D : nullptr;
       }
     }
     if (ok && fin && warp_wait(&sh->w_done, (done - 1) & 1, abort, p.status)) {
@@ -1289,15 +1312,47 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
   }
 }
 
-Grid make_grid(const AttnTrainParams& p, int units, int tiles) {
-  const int chunks = (p.R + p.HC - 1) / p.HC;
-  return Grid{units, tiles, units * tiles, chunks, FastDiv((uint32_t)tiles), FastDiv((uint32_t)chunks),
-              FastDiv((uint32_t)p.Hkv)};
+// Adds the splits' sums of dk and dv in order: eight columns of a row a thread.  A
+// tile has sums from as many splits as it has blocks, at most all.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) attn_train_sum_kernel(const __grid_constant__ AttnTrainParams p, int splits) {
+  constexpr int NC = D / 8;
+  const long long rows = (long long)p.B * p.Hkv * p.S, total = rows * 2 * NC;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const int c = (int)(i % NC) * 8, which = (int)(i / NC % 2);
+    const long long row = i / (2 * NC);
+    const int pos = (int)(row % p.S);
+    const long long bg = row / p.S;
+    const int g = (int)(bg % p.Hkv), b = (int)(bg / p.Hkv), pad = p.pad_len ? min(max(__ldg(p.pad_len + b), 0), p.S) : 0;
+    if (pos < pad) continue;
+    const int k0 = (pad & ~7) + (pos - (pad & ~7)) / kRows * kRows;
+    const int n = min(splits, (p.S - max(k0, pad) + p.PT64 - 1) / p.PT64);
+    const float* src = p.part + (which * rows + row) * D + c;
+    uint32_t s[8];
+    float acc[8] = {};
+    for (int q = 0; q < n; ++q, src += 2 * rows * D) {
+      const float4 x = *reinterpret_cast<const float4*>(src), y = *reinterpret_cast<const float4*>(src + 4);
+      acc[0] += x.x, acc[1] += x.y, acc[2] += x.z, acc[3] += x.w;
+      acc[4] += y.x, acc[5] += y.y, acc[6] += y.z, acc[7] += y.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = __float_as_uint(acc[e]);
+    uint16_t* dst = which ? static_cast<uint16_t*>(p.dk) + b * p.dk_sb + (long long)pos * p.dk_ss + g * p.dk_sh
+                          : static_cast<uint16_t*>(p.dv) + b * p.dv_sb + (long long)pos * p.dv_ss + g * p.dv_sh;
+    *reinterpret_cast<uint4*>(dst + c) = pack8<BF16>(s, which ? p.scale : p.inv_keep);
+  }
+}
+
+Grid make_grid(const AttnTrainParams& p, int units, int tiles, int parts, int splits) {
+  return Grid{units * parts, tiles, units * parts * tiles, (p.R + p.HC - 1) / p.HC, splits, FastDiv((uint32_t)tiles),
+              FastDiv((uint32_t)parts), FastDiv((uint32_t)p.Hkv)};
 }
 Grid grid_rows(const AttnTrainParams& p) {
-  return make_grid(p, p.B * p.Hkv * ((p.R + p.HC - 1) / p.HC), (p.S + p.PT128 - 1) / p.PT128);
+  return make_grid(p, p.B * p.Hkv, (p.S + p.PT128 - 1) / p.PT128, (p.R + p.HC - 1) / p.HC, 1);
 }
-Grid grid_keys(const AttnTrainParams& p) { return make_grid(p, p.B * p.Hkv, (p.S + kRows - 1) / kRows); }
+Grid grid_keys(const AttnTrainParams& p, int splits) {
+  return make_grid(p, p.B * p.Hkv, (p.S + kRows - 1) / kRows, splits, splits);
+}
 unsigned ctas(const Grid& gr, int num_sms, int per_sm) {
   const int most = num_sms * per_sm;
   return (unsigned)(gr.items < most ? gr.items : most);
@@ -1320,15 +1375,31 @@ cudaError_t run_bwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sm
   cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kq), BwdSmem<D, true>::BYTES);
   if (e != cudaSuccess) return e;
   if ((e = smem_limit_once(reinterpret_cast<const void*>(kk), BwdSmem<D, false>::BYTES)) != cudaSuccess) return e;
-  const Grid gq = grid_rows(p), gk = grid_keys(p);
+  const int splits = attn_train_splits(p.B, p.S, p.Hkv, p.R, num_sms);
+  const Grid gq = grid_rows(p), gk = grid_keys(p, splits);
   kq<<<ctas(gq, num_sms, kPerSm), kBwdThreads, BwdSmem<D, true>::BYTES, st>>>(m.q_tile, m.do_tile, m.o_tile, m.k_blk,
                                                                               m.v_blk, p, gq);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   kk<<<ctas(gk, num_sms, kPerSm), kBwdThreads, BwdSmem<D, false>::BYTES, st>>>(m.k_tile, m.v_tile, m.q_blk, m.do_blk, p, gk);
+  if ((e = cudaGetLastError()) != cudaSuccess || splits == 1) return e;
+  const long long blocks = ((long long)p.B * p.Hkv * p.S * 2 * (D / 8) + 255) / 256;
+  attn_train_sum_kernel<D, BF16><<<(unsigned)(blocks < num_sms * 16 ? blocks : num_sms * 16), 256, 0, st>>>(p, splits);
   return cudaGetLastError();
 }
 
 }  // namespace
+
+// CTAs that share the query rows behind one tile of keys: as many as fill the GPU,
+// with four blocks or more for each.  (B 2, S 4000, 8 / 2 heads of 32 has 128 tiles
+// of keys for 296 CTAs.)
+int attn_train_splits(int B, int S, int Hkv, int R, int num_sms) {
+  if (R > 64) return 1;  // chunks of heads: not split
+  const long long items = (long long)B * Hkv * ((S + kRows - 1) / kRows);
+  const int pt = kBlk / R, blocks = (S + pt - 1) / pt;
+  long long n = (long long)kPerSm * num_sms / items;
+  if (n > blocks / 4) n = blocks / 4;
+  return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+}
 
 cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
                                         int num_sms, cudaStream_t st) {

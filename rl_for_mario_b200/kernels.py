@@ -542,6 +542,16 @@ def _launch(name: str, dev: torch.device, *args) -> None:
         _lib.check(name, rc)
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace(name: str, device: int, *sizes: int) -> int:
+    """Bytes of scratch that the entry point ``name`` asks for (a rule on sizes and the device's SM count)."""
+    with torch.cuda.device(device):
+        size = getattr(_lib.load(), name)(*sizes)
+    if size < 0:
+        _lib.check(name, -size)
+    return size
+
+
 def _check_dropout(p: float, rng: Optional[Tensor], site: int) -> float:
     """The dropout arguments shared by the training operators; returns p as a float.
 
@@ -653,10 +663,11 @@ def attn_train_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tens
                                  "rows and strides that are multiples of 8")
             gs += t.stride()[:3]
     if dq.numel():
-        delta = torch.empty((B, Hq, S), dtype=torch.float32, device=dev)
+        size = _workspace("dt_attn_train_workspace", dev.index, B, S, Hq, Hkv, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
         _launch("dt_attn_train_backward", dev, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                out.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                _ptr(pad_len), B, S, Hq, Hkv, D, _PACK24.pack(*qs, *ks, *vs, *os, *dos, *gs), scale or 0.0, p,
+                out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(pad_len),
+                ws.data_ptr(), size, B, S, Hq, Hkv, D, _PACK24.pack(*qs, *ks, *vs, *os, *dos, *gs), scale or 0.0, p,
                 _ptr(rng), site, _dtype_code(q))
     return dq, dk, dv
 
@@ -758,16 +769,6 @@ def residual_norm_forward(x: Tensor, residual: Optional[Tensor], pre_weight: Ten
     return h, n, stats
 
 
-@functools.lru_cache(maxsize=1024)
-def _residual_norm_workspace(M: int, H: int, gate_rows: int, post: int, device: int) -> int:
-    """Bytes of scratch of residual_norm_backward (a rule on sizes and the device's SM count)."""
-    with torch.cuda.device(device):
-        size = _lib.load().dt_residual_norm_workspace(M, H, gate_rows, post)
-    if size < 0:
-        _lib.check("dt_residual_norm_workspace", -size)
-    return size
-
-
 def residual_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], x: Tensor, residual: Optional[Tensor],
                            pre_weight: Tensor, stats: Tensor, post_weight: Optional[Tensor] = None,
                            gate: Optional[Tensor] = None, alpha: float = 1.0, p: float = 0.0,
@@ -802,7 +803,7 @@ def residual_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], x: Tensor
     g2, gs = (None, 0) if gate is None else _rows2d(gate)
     dh2, dhs = (None, 0) if dh is None else _rows2d(dh)
     dn2, dns = (None, 0) if dn is None else _rows2d(dn)
-    size = _residual_norm_workspace(M, H, gate_rows, 0 if post_weight is None else 1, dev.index)
+    size = _workspace("dt_residual_norm_workspace", dev.index, M, H, gate_rows, 0 if post_weight is None else 1)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     _launch("dt_residual_norm_backward", dev, _ptr(dh2), dhs, _ptr(dn2), dns, x2.data_ptr(), xs, _ptr(r2), rs,
             _ptr(g2), gs, gate_rows, pre_weight.data_ptr(), _ptr(post_weight), stats.data_ptr(), dx.data_ptr(),

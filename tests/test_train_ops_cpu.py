@@ -29,10 +29,14 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     for kw, text, code in cases:
         assert fwd(**kw) == code and text.encode() in lib.dt_last_error(), kw
     s24 = (_lib._L * 24)(*([256, 64, 64] * 8))
-    assert lib.dt_attn_train_backward(a, a, a, a, a, a, None, a, a, a, None, 1, 8, 4, 2, 32, s24, 0.0, 0.0, None, 0, 0,
-                                      None) == _lib.DT_ERR_INVALID
-    assert lib.dt_attn_train_backward(a, a, a, a, a, a, a, a + 8, a, a, None, 1, 8, 4, 2, 32, s24, 0.0, 0.0, None, 0,
-                                      0, None) == _lib.DT_ERR_INVALID
+
+    def bwd(dq=a, ws=a, dtype=0):
+        return lib.dt_attn_train_backward(a, a, a, a, a, a, dq, a, a, None, ws, 1 << 20, 1, 8, 4, 2, 32, s24, 0.0, 0.0,
+                                          None, 0, dtype, None)
+
+    assert bwd(ws=None) == _lib.DT_ERR_INVALID and bwd(dq=a + 8) == _lib.DT_ERR_INVALID
+    assert bwd(dtype=2) == _lib.DT_ERR_UNSUPPORTED
+    assert lib.dt_attn_train_workspace(1, 8, 4, 3, 32) < 0 and lib.dt_attn_train_workspace(1, 0, 4, 2, 32) < 0
 
     def norm(x=a, w=a, gate=None, gate_rows=0, M=4, H=8, dtype=0, h=a, p=0.0):
         return lib.dt_residual_norm_forward(x, 8, a, 8, gate, 8, gate_rows, w, None, h, a, a, M, H, 1.0, 1e-5, p, None,
