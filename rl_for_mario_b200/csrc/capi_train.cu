@@ -232,13 +232,16 @@ int dt_rope_grad(void* g, int64_t g_stride, int64_t rows, const float* cos_tab, 
 }
 
 int64_t dt_residual_norm_workspace(int64_t M, int H, int64_t gate_rows, int has_post) {
-  if (M < 1 || H < 1 || H > kMaxHidden || gate_rows < 0 || (gate_rows > 0 && M % gate_rows != 0))
+  if (M < 1 || M > 0x7fffffffLL || H < 1 || H > kMaxHidden || gate_rows < 0 || (gate_rows > 0 && M % gate_rows != 0))
     return -api_fail(DT_ERR_INVALID, "dt_residual_norm_workspace: bad sizes (M=%lld H=%d gate_rows=%lld)", (long long)M,
                      H, (long long)gate_rows);
   int sms = 0;
   const int rc = need_sm100("dt_residual_norm_workspace", &sms);
   if (rc) return -rc;
-  return 4 * part_elems(dtk::residual_norm_plan(M, H, gate_rows, sms), H, gate_rows, has_post != 0);
+  // Alignment decides between two plans when the backward call comes: room for either.
+  const int64_t a = part_elems(dtk::residual_norm_plan(M, H, gate_rows, true, sms), H, gate_rows, has_post != 0);
+  const int64_t b = part_elems(dtk::residual_norm_plan(M, H, gate_rows, false, sms), H, gate_rows, has_post != 0);
+  return 4 * (a > b ? a : b);
 }
 
 static int check_residual_norm(const char* fn, const void* x, const void* w_pre, const void* gate, int64_t gate_rows,
@@ -247,6 +250,7 @@ static int check_residual_norm(const char* fn, const void* x, const void* w_pre,
   if (rc) return rc;
   if ((rc = check_rows(fn, x, M, H, "M", "H"))) return rc;
   if (H > kMaxHidden) return api_fail(DT_ERR_UNSUPPORTED, "%s: H %d above %d", fn, H, kMaxHidden);
+  if (M > 0x7fffffffLL) return api_fail(DT_ERR_UNSUPPORTED, "%s: M %lld above 2^31 - 1", fn, (long long)M);
   if (!w_pre) return api_fail(DT_ERR_INVALID, "%s: null w_pre", fn);
   if (gate && (gate_rows < 1 || M % gate_rows != 0))
     return api_fail(DT_ERR_INVALID, "%s: gate_rows %lld does not divide M %lld", fn, (long long)gate_rows,
@@ -270,7 +274,7 @@ int dt_residual_norm_forward(const void* x, int64_t x_stride, const void* residu
   if ((rc = need_sm100(fn, &sms))) return rc;
   a.x = x, a.residual = residual, a.gate = gate, a.w_pre = w_pre, a.w_post = w_post, a.h = h, a.n = n, a.stats = stats;
   a.x_stride = x_stride, a.res_stride = res_stride, a.gate_stride = gate_stride;
-  a.M = M, a.H = H, a.gate_rows = gate ? gate_rows : 0;
+  a.M = M, a.H = H, a.gate_rows = gate ? gate_rows : 0, a.by_gate = dtk::FastDiv(gate ? (uint32_t)gate_rows : 1u);
   a.alpha = alpha, a.eps = eps, a.rng = reinterpret_cast<const long long*>(rng), a.site = site;
   return cuda_status(dtk::launch_residual_norm_fwd_sm100(a, dtype, sms, static_cast<cudaStream_t>(stream)), fn);
 }
@@ -297,22 +301,22 @@ int dt_residual_norm_backward(const void* dh, int64_t dh_stride, const void* dn,
   if ((rc = need_sm100(fn, &sms))) return rc;
   if (!gate) gate_rows = 0;
   const bool post = w_post != nullptr;
-  const dtk::ResidualNormPlan plan = dtk::residual_norm_plan(M, H, gate_rows, sms);
-  if (workspace_bytes < 4 * part_elems(plan, H, gate_rows, post) || !workspace || !aligned16(workspace))
-    return api_fail(DT_ERR_INVALID, "%s: workspace of %lld bytes is too small, null or not 16-byte aligned", fn,
-                    (long long)workspace_bytes);
   a.x = x, a.residual = residual, a.gate = gate, a.w_pre = w_pre, a.w_post = w_post, a.dh = dh, a.dn = dn;
   a.stats = const_cast<float*>(stats);
   a.dx = dx, a.dresidual = dresidual, a.dw_pre = dw_pre, a.dw_post = dw_post, a.dgate = dgate;
+  a.x_stride = x_stride, a.res_stride = res_stride, a.gate_stride = gate_stride;
+  a.dh_stride = dh_stride, a.dn_stride = dn_stride;
+  a.M = M, a.H = H, a.gate_rows = gate_rows;
+  a.alpha = alpha, a.eps = eps, a.rng = reinterpret_cast<const long long*>(rng), a.site = site;
+  const dtk::ResidualNormPlan plan = dtk::residual_norm_plan(M, H, gate_rows, dtk::residual_norm_ahead(a, dtype), sms);
+  if (workspace_bytes < 4 * part_elems(plan, H, gate_rows, post) || !workspace || !aligned16(workspace))
+    return api_fail(DT_ERR_INVALID, "%s: workspace of %lld bytes is too small, null or not 16-byte aligned", fn,
+                    (long long)workspace_bytes);
   float* part = static_cast<float*>(workspace);
   const int64_t one = plan.grid > 1 ? plan.grid * (int64_t)H : 0, step = (one + 3) / 4 * 4;
   a.part_pre = part;
   a.part_post = part + step;
   a.part_gate = part + (post ? 2 : 1) * step;
-  a.x_stride = x_stride, a.res_stride = res_stride, a.gate_stride = gate_stride;
-  a.dh_stride = dh_stride, a.dn_stride = dn_stride;
-  a.M = M, a.H = H, a.gate_rows = gate_rows;
-  a.alpha = alpha, a.eps = eps, a.rng = reinterpret_cast<const long long*>(rng), a.site = site;
   return cuda_status(dtk::launch_residual_norm_bwd_sm100(a, plan, dtype, static_cast<cudaStream_t>(stream)), fn);
 }
 

@@ -213,6 +213,25 @@ struct DropoutParams {
 };
 cudaError_t launch_dropout_sm100(const DropoutParams& p, int dtype, int num_sms, cudaStream_t st);
 
+// Division of n < 2^31 by a fixed divisor: a multiplication and a shift, prepared
+// on the host.  With 2^b the first power of two >= d, m = ceil(2^(31 + b) / d) is
+// off by less than one part in 2^31, so n m >> (31 + b) is floor(n / d).
+struct FastDiv {
+  uint32_t d = 1, m = 0, s = 0;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div) {
+    uint32_t b = 0;
+    while ((1ull << b) < div) ++b;
+    s = b ? b - 1 : 0;
+    m = (uint32_t)(((1ull << (31 + b)) + div - 1) / div);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int operator()(int n) const {
+    return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> s);
+  }
+#endif
+};
+
 struct RopeGradParams {
   void* x;  // [rows, >= rope_cols], rotated back in place
   const float* cos;
@@ -242,7 +261,8 @@ struct ResidualNormParams {
   float* part_post;
   float* part_gate;  // [chunks, H]
   long long x_stride, res_stride, gate_stride, dh_stride, dn_stride;
-  long long M, gate_rows;  // rows that share one row of the gate
+  long long M, gate_rows;  // M < 2^31; rows that share one row of the gate
+  FastDiv by_gate;
   long long chunks, chunk_rows, chunks_per_span, span_rows;
   int H, wpr;
   const long long* rng;
@@ -251,30 +271,14 @@ struct ResidualNormParams {
 };
 struct ResidualNormPlan {
   long long chunks, chunk_rows, chunks_per_span, span_rows, grid;
+  int groups;  // rows of a block
 };
-ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, int num_sms);
+// ahead: the backward kernel holds rows ahead (residual_norm_ahead says which calls).
+ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, bool ahead, int num_sms);
+bool residual_norm_ahead(const ResidualNormParams& p, int dtype);
 cudaError_t launch_residual_norm_fwd_sm100(ResidualNormParams p, int dtype, int num_sms, cudaStream_t st);
 cudaError_t launch_residual_norm_bwd_sm100(ResidualNormParams p, const ResidualNormPlan& plan, int dtype,
                                            cudaStream_t st);
-
-// Division of n < 2^31 by a fixed divisor: a multiplication and a shift, prepared
-// on the host.  With 2^b the first power of two >= d, m = ceil(2^(31 + b) / d) is
-// off by less than one part in 2^31, so n m >> (31 + b) is floor(n / d).
-struct FastDiv {
-  uint32_t d = 1, m = 0, s = 0;
-  FastDiv() = default;
-  explicit FastDiv(uint32_t div) : d(div) {
-    uint32_t b = 0;
-    while ((1ull << b) < div) ++b;
-    s = b ? b - 1 : 0;
-    m = (uint32_t)(((1ull << (31 + b)) + div - 1) / div);
-  }
-#ifdef __CUDACC__
-  __device__ __forceinline__ int operator()(int n) const {
-    return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> s);
-  }
-#endif
-};
 
 struct AttnTrainParams {
   const void* q;

@@ -6,24 +6,29 @@
 //   h = residual + alpha * g * v
 //   n = h * r_pre * w_pre     r_pre = rsqrt(mean(h^2) + eps)
 //
-// Backward, from dh (the gradient that reaches h past this op) and dn:
-//   t  = dn * w_pre,  c = mean(t * h r_pre)
-//   D  = dh + r_pre (t - h r_pre c)          the gradient of h: d(residual) = D
-//   dg = alpha v D (summed over the rows that share a gate),  dv = alpha g D,  du = m dv / (1 - p)
-//   s  = du * w_post, d(x) = r_post (s - x r_post mean(s * x r_post))     (d(x) = du without a post norm)
-//   dw_pre = sum over rows of dn h r_pre,  dw_post = sum over rows of du x r_post
+// Backward, from dh (the gradient that reaches h past this op) and dn, with
+// h^ = h r_pre and x^ = x r_post:
+//   t  = dn * w_pre,  e = dh + r_pre t,  c = mean(t h^)
+//   D  = e - r_pre c h^                      the gradient of h: d(residual) = D
+//   dg = alpha v D (summed over the rows that share a gate),  du = m alpha g D / (1 - p)
+//   s  = du * w_post, d(x) = r_post (s - x^ c')     (d(x) = du without a post norm)
+//   dw_pre = sum over rows of dn h^,  dw_post = sum over rows of du x^
+// c' = mean(s x^) looks as if it had to wait for c, but s x^ = (alpha g v) D, so
+//   c' = mean(alpha g v e) - r_pre c mean(alpha g v h^),
+// and one sum over the row gives all three means.
 // h is formed again from x and residual in fp32 instead of being read back: the
 // same bytes, and the gradient does not see the rounding of the stored h.
 //
 // Everything between the loads and the stores is fp32; each output is rounded
 // once, and n is the norm of the unrounded h.
 //
-// Bound by HBM.  A row is held by WPR = ceil(H / 256) warps, eight columns a
-// thread, so it is read once and its sums are a shuffle tree plus (WPR > 1)
-// one named barrier; a 256-thread block holds 8 / WPR rows.  The sums over rows
-// stay in registers (a thread owns its columns for every row that it meets),
-// each block writes one partial row of them and a second kernel adds the
-// partial rows in a fixed order: no atomics, the same bits every run.
+// Bound by HBM.  A row is held by one or more warps (WPR), so it is read once and
+// its sums are a shuffle tree plus (WPR > 1) one named barrier; the next row's loads are issued before this row's sums, so
+// they are in flight behind the barriers.  The sums over rows of the backward
+// pass stay in registers (a thread owns its columns for every row that it
+// meets); one block of up to 512 threads on each SM writes one partial row of
+// them and a second kernel adds the partial rows in a fixed order: no atomics,
+// the same bits every run.
 #include "dt_common.cuh"
 #include "dt_internal.h"
 #include "train_common.cuh"
@@ -32,21 +37,62 @@ namespace dtk {
 
 namespace {
 
-// Sum over the row's warps.  Slots alternate between two halves of `red`, so
-// one barrier is enough: a slot is written again two sums later, and the sum
-// between has passed a barrier after every read of it.
-__device__ __forceinline__ float row_sum(float v, float* red, int& turn, int wpr, int w, int lane, int bar) {
+// Whether a thread holds the next row while it works on one: 16-bit vectors only,
+// whose four registers a tensor leave room for it (fp32 rows held ahead spill:
+// 71 us against 49 us without, 4,257 rows of 1,001).
+template <int DT, bool VEC>
+constexpr bool kAhead = VEC && DT != 2;
+
+constexpr int kSums = 3;      // row sums taken together, at most
+constexpr int kMaxGroups = 16;  // rows of a block
+
+// Sums of N values over the row's warps.  Slots alternate between two halves of
+// `red`, so one barrier is enough: a slot is written again two sums later, and the
+// sum between has passed a barrier after every read of it.
+template <int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& turn, int wpr, int w, int lane, int bar) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (wpr == 1) return v;
-  float* slot = red + turn * 32;
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if (wpr == 1) return;
+  float* slot = red + turn * (32 * kSums);
   turn ^= 1;
-  if (lane == 0) slot[w] = v;
+  if (lane == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) slot[w * kSums + i] = v[i];
   named_bar_sync(bar, wpr * 32);
-  v = 0.f;
-  for (int i = 0; i < wpr; ++i) v += slot[i];
-  return v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.f;
+  for (int k = 0; k < wpr; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += slot[k * kSums + i];
 }
+
+// Eight columns as packed pairs (one instruction for two of them: the kernels are
+// as near to the issue rate as to HBM).
+struct F8 {
+  float2 p[4];
+  template <int DT, bool VEC>
+  __device__ __forceinline__ void load(const typename TrainElem<DT>::T* row, int w, int lane, int n) {
+    load8<DT, VEC>(row, w, lane, n, as());
+  }
+  __device__ __forceinline__ float (&as())[8] { return *reinterpret_cast<float(*)[8]>(p); }
+  __device__ __forceinline__ void set(float v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = make_float2(v, v);
+  }
+  // Clears what the mask bits drop (bit i: element i stays).
+  __device__ __forceinline__ void keep(uint32_t m) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i].x = (m >> (2 * i)) & 1u ? p[i].x : 0.f;
+      p[i].y = (m >> (2 * i + 1)) & 1u ? p[i].y : 0.f;
+    }
+  }
+};
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float both_sum(float2 v) { return v.x + v.y; }
 
 struct RowPlace {
   int w, lane, group, groups, bar;
@@ -61,16 +107,18 @@ __device__ __forceinline__ RowPlace place(int wpr, float* red_all) {
   r.w = warp - r.group * wpr;
   r.lane = threadIdx.x & 31;
   r.bar = 1 + r.group;
-  r.red = red_all + r.group * 64;
+  r.red = red_all + r.group * (64 * kSums);  // (only rows of several warps use it: at most 8 of them a block)
   return r;
 }
 
-// MAXT: the block's largest size, 256 for rows of up to 2048 columns (so that the
-// compiler may use more registers), else 1024.
+// A row of H columns is ceil(H / 256) warps' (one warp for rows of up to 1024, four
+// pieces of eight columns a lane, took 127 us where three take 104 us: 96 x 768 rows
+// of 768, both norms and a gate).  The weights come from L1 each time, in favour of
+// the next row's registers.  MAXT: the block's largest size.
 template <int DT, bool VEC, bool POST, bool DROP, int MAXT>
-__global__ void __launch_bounds__(MAXT) residual_norm_fwd_kernel(const ResidualNormParams p) {
+__global__ void __launch_bounds__(MAXT) residual_norm_fwd_kernel(const __grid_constant__ ResidualNormParams p) {
   using T = typename TrainElem<DT>::T;
-  __shared__ float red_all[8 * 64];
+  __shared__ float red_all[8 * 64 * kSums];
   const RowPlace at = place(p.wpr, red_all);
   int turn = 0;
   const int w = at.w, lane = at.lane, H = p.H;
@@ -80,54 +128,74 @@ __global__ void __launch_bounds__(MAXT) residual_norm_fwd_kernel(const ResidualN
   const T* x = static_cast<const T*>(p.x);
   const T* res = static_cast<const T*>(p.residual);
   const T* gate = static_cast<const T*>(p.gate);
-  float wpre[8], wpost[8];
-  load8<DT, VEC>(static_cast<const T*>(p.w_pre), w, lane, H, wpre);
-  if constexpr (POST) load8<DT, VEC>(static_cast<const T*>(p.w_post), w, lane, H, wpost);
+  const T* w_pre = static_cast<const T*>(p.w_pre);
+  const T* w_post = static_cast<const T*>(p.w_post);
   const float inv_h = 1.f / (float)H;
-  for (long long row = (long long)blockIdx.x * at.groups + at.group; row < p.M; row += (long long)gridDim.x * at.groups) {
-    float v[8], h[8], g[8];
-    load8<DT, VEC>(x + row * p.x_stride, w, lane, H, v);
-    if (res)
-      load8<DT, VEC>(res + row * p.res_stride, w, lane, H, h);
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = 0.f;
-    if (gate) {
-      load8<DT, VEC>(gate + (row / p.gate_rows) * p.gate_stride, w, lane, H, g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] *= p.alpha;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = p.alpha;
-    }
+  // What x^ is multiplied with on its way into h: alpha * gate * w_post / (1 - p).  Held, unless the gate's
+  // row changes with the row.
+  const bool fixed_gate = !gate || p.gate_rows == p.M;
+  F8 cw, wpre;
+  auto weigh = [&](long long gate_row) {
+    cw.set(DROP ? p.alpha * p.inv_keep : p.alpha);
+    F8 f;
     if constexpr (POST) {
-      float ss = 0.f;
+      f.load<DT, VEC>(w_post, w, lane, H);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-      ss = row_sum(ss, at.red, turn, p.wpr, w, lane, at.bar);
-      const float r = rsqrtf(fmaf(ss, inv_h, p.eps));
+      for (int i = 0; i < 4; ++i) cw.p[i] = fmul2(cw.p[i], f.p[i]);
+    }
+    if (gate) {
+      f.load<DT, VEC>(gate + gate_row * p.gate_stride, w, lane, H);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cw.p[i] = fmul2(cw.p[i], f.p[i]);
+    }
+  };
+  if (fixed_gate) weigh(0);
+  wpre.load<DT, VEC>(w_pre, w, lane, H);
+  Raw8<DT, VEC> nx, nr;
+  auto fetch = [&](long long row) {
+    if (row >= p.M) return;
+    nx.load(x + row * p.x_stride, w, lane, H);
+    if (res) nr.load(res + row * p.res_stride, w, lane, H);
+  };
+  const long long step = (long long)gridDim.x * at.groups;
+  long long row = (long long)blockIdx.x * at.groups + at.group;
+  if constexpr (kAhead<DT, VEC>) fetch(row);
+  for (; row < p.M; row += step) {
+    F8 v, h;
+    if constexpr (!kAhead<DT, VEC>) fetch(row);
+    nx.get(v.as());
+    if (res)
+      nr.get(h.as());
+    else
+      h.set(0.f);
+    if constexpr (kAhead<DT, VEC>) fetch(row + step);
+    if (!fixed_gate) weigh(p.by_gate((int)row));
+    if constexpr (POST) {
+      float2 q = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q = ffma2(v.p[i], v.p[i], q);
+      float ss[1] = {both_sum(q)};
+      row_sums<1>(ss, at.red, turn, p.wpr, w, lane, at.bar);
+      const float r = rsqrtf(fmaf(ss[0], inv_h, p.eps));
       if (w == 0 && lane == 0) p.stats[2 * row] = r;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= r * wpost[i];
+      for (int i = 0; i < 4; ++i) v.p[i] = fmul2(v.p[i], both(r));
     }
-    if constexpr (DROP) {
-      const uint32_t m = keep8<VEC>(key, (unsigned long long)row * per_row, w, lane, p.threshold);
+    if constexpr (DROP) v.keep(keep8<VEC>(key, (unsigned long long)row * per_row, w, lane, p.threshold));
+    float2 q = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (m >> i) & 1u ? v[i] * p.inv_keep : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      h.p[i] = ffma2(v.p[i], cw.p[i], h.p[i]);
+      q = ffma2(h.p[i], h.p[i], q);
     }
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      h[i] = fmaf(g[i], v[i], h[i]);
-      ss = fmaf(h[i], h[i], ss);
-    }
-    store8<DT, VEC>(static_cast<T*>(p.h) + row * H, w, lane, H, h);
-    ss = row_sum(ss, at.red, turn, p.wpr, w, lane, at.bar);
-    const float r = rsqrtf(fmaf(ss, inv_h, p.eps));
+    store8<DT, VEC>(static_cast<T*>(p.h) + row * H, w, lane, H, h.as());
+    float ss[1] = {both_sum(q)};
+    row_sums<1>(ss, at.red, turn, p.wpr, w, lane, at.bar);
+    const float r = rsqrtf(fmaf(ss[0], inv_h, p.eps));
     if (w == 0 && lane == 0) p.stats[2 * row + 1] = r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] *= r * wpre[i];
-    store8<DT, VEC>(static_cast<T*>(p.n) + row * H, w, lane, H, h);
+    for (int i = 0; i < 4; ++i) h.p[i] = fmul2(fmul2(h.p[i], both(r)), wpre.p[i]);
+    store8<DT, VEC>(static_cast<T*>(p.n) + row * H, w, lane, H, h.as());
   }
 }
 
@@ -166,11 +234,12 @@ __device__ __forceinline__ void flush_row(float (&acc)[8], float* sh, const RowP
 // there is no gate or each row has its own) and these into chunks; a block walks
 // chunks blockIdx.x, blockIdx.x + gridDim.x, ... and flushes the gate's sum at
 // the end of each, the weights' sums at its own end.
+// MAXT: the block's largest size (a bound on the registers a thread may take).
 template <int DT, bool VEC, bool POST, bool DROP, int MAXT>
-__global__ void __launch_bounds__(MAXT) residual_norm_bwd_kernel(const ResidualNormParams p) {
+__global__ void __launch_bounds__(MAXT) residual_norm_bwd_kernel(const __grid_constant__ ResidualNormParams p) {
   using T = typename TrainElem<DT>::T;
-  __shared__ float red_all[8 * 64];
-  __shared__ float sums[7 * 256];
+  __shared__ float red_all[8 * 64 * kSums];
+  __shared__ float sums[(kMaxGroups - 1) * 256];
   const RowPlace at = place(p.wpr, red_all);
   int turn = 0;
   const int w = at.w, lane = at.lane, H = p.H;
@@ -183,152 +252,207 @@ __global__ void __launch_bounds__(MAXT) residual_norm_bwd_kernel(const ResidualN
   const T* dh = static_cast<const T*>(p.dh);
   const T* dn = static_cast<const T*>(p.dn);
   T* dgate = static_cast<T*>(p.dgate);
-  float wpre[8], wpost[8], a_pre[8], a_post[8], a_gate[8];
-  load8<DT, VEC>(static_cast<const T*>(p.w_pre), w, lane, H, wpre);
-  if constexpr (POST) load8<DT, VEC>(static_cast<const T*>(p.w_post), w, lane, H, wpost);
+  const T* w_post = static_cast<const T*>(p.w_post);
+  // cw: alpha * gate * w_post / (1 - p), what x^ is multiplied with on its way into h.  With md the kept part of
+  // D, both d(w_post) and d(gate) are multiples of sum md x^ as long as the gate's row stays: one sum (q) serves.
+  F8 wpre, cw, a_pre, a_post, q;
+  wpre.load<DT, VEC>(static_cast<const T*>(p.w_pre), w, lane, H);
+  a_pre.set(0.f);
+  a_post.set(0.f);
+  q.set(0.f);
+  const float inv_h = 1.f / (float)H, ak = DROP ? p.alpha * p.inv_keep : p.alpha;
+  const bool sum_gate = gate && p.gate_rows > 1, row_gate = gate && p.gate_rows == 1;
+  auto weigh = [&](long long gate_row) {
+    cw.set(ak);
+    F8 f;
+    if constexpr (POST) {
+      f.load<DT, VEC>(w_post, w, lane, H);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a_pre[i] = a_post[i] = a_gate[i] = 0.f;
-  const float inv_h = 1.f / (float)H;
-  const bool sum_gate = gate && p.gate_rows > 1;
+      for (int i = 0; i < 4; ++i) cw.p[i] = fmul2(cw.p[i], f.p[i]);
+    }
+    if (gate) {
+      f.load<DT, VEC>(gate + gate_row * p.gate_stride, w, lane, H);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cw.p[i] = fmul2(cw.p[i], f.p[i]);
+    }
+  };
+  if (!gate) weigh(0);
 
+  Raw8<DT, VEC> nx, nr, nh, nn;
+  float n_post = 1.f, n_pre = 0.f;
+  auto fetch = [&](long long row) {
+    nx.load(x + row * p.x_stride, w, lane, H);
+    if (res) nr.load(res + row * p.res_stride, w, lane, H);
+    if (dh) nh.load(dh + row * p.dh_stride, w, lane, H);
+    if (dn) nn.load(dn + row * p.dn_stride, w, lane, H);
+    if constexpr (POST) n_post = p.stats[2 * row];
+    n_pre = p.stats[2 * row + 1];
+  };
   for (long long chunk = blockIdx.x; chunk < p.chunks; chunk += gridDim.x) {
     const long long span = chunk / p.chunks_per_span;  // the gate's row, when several rows share it
     const long long r0 = span * p.span_rows + (chunk - span * p.chunks_per_span) * p.chunk_rows;
     const long long r1 = min(r0 + p.chunk_rows, (span + 1) * p.span_rows);
-    for (long long row = r0 + at.group; row < r1; row += at.groups) {
-      float xv[8], h[8], g[8], d[8], t[8];
-      load8<DT, VEC>(x + row * p.x_stride, w, lane, H, xv);
+    if (sum_gate) weigh(span);
+    long long row = r0 + at.group;
+    if constexpr (kAhead<DT, VEC>)
+      if (row < r1) fetch(row);
+    for (; row < r1; row += at.groups) {
+      F8 xn, h, e, t;
+      if constexpr (!kAhead<DT, VEC>) fetch(row);
+      nx.get(xn.as());
       if (res)
-        load8<DT, VEC>(res + row * p.res_stride, w, lane, H, h);
+        nr.get(h.as());
       else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = 0.f;
+        h.set(0.f);
       if (dh)
-        load8<DT, VEC>(dh + row * p.dh_stride, w, lane, H, d);
+        nh.get(e.as());
       else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = 0.f;
-      if (dn) load8<DT, VEC>(dn + row * p.dn_stride, w, lane, H, t);
-      if (gate) {
-        load8<DT, VEC>(gate + (sum_gate ? span : row) * p.gate_stride, w, lane, H, g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] *= p.alpha;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = p.alpha;
-      }
-      float v[8];
-      float r_post = 1.f;
-      if constexpr (POST) {
-        r_post = p.stats[2 * row];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) xv[i] *= r_post;  // from here on the normalised x
-      }
+        e.set(0.f);
+      if (dn)
+        nn.get(t.as());
+      else
+        t.set(0.f);
+      const float r_post = n_post, r_pre = n_pre;
+      if constexpr (kAhead<DT, VEC>)
+        if (row + at.groups < r1) fetch(row + at.groups);
+      if (row_gate) weigh(row);
       uint32_t m = 0xffu;
       if constexpr (DROP) m = keep8<VEC>(key, (unsigned long long)row * per_row, w, lane, p.threshold);
+      float2 s0 = make_float2(0.f, 0.f), s1 = s0, s2 = s0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float u = xv[i];
-        if constexpr (POST) u *= wpost[i];
-        if constexpr (DROP) u = (m >> i) & 1u ? u * p.inv_keep : 0.f;
-        v[i] = u;
-      }
-      if (dn) {
-        const float r_pre = p.stats[2 * row + 1];
-        float c = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          h[i] = fmaf(g[i], v[i], h[i]) * r_pre;  // the normalised h
-          a_pre[i] = fmaf(t[i], h[i], a_pre[i]);
-          t[i] *= wpre[i];
-          c = fmaf(t[i], h[i], c);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (POST) xn.p[i] = fmul2(xn.p[i], both(r_post));  // from here on the normalised x
+        float2 gv = fmul2(xn.p[i], cw.p[i]);
+        if constexpr (DROP) {
+          gv.x = (m >> (2 * i)) & 1u ? gv.x : 0.f;
+          gv.y = (m >> (2 * i + 1)) & 1u ? gv.y : 0.f;
         }
-        c = row_sum(c, at.red, turn, p.wpr, w, lane, at.bar) * inv_h;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = fmaf(r_pre, fmaf(-h[i], c, t[i]), d[i]);
-      }
-      if (p.dresidual) store8<DT, VEC>(static_cast<T*>(p.dresidual) + row * H, w, lane, H, d);
-      if (gate) {
-        if (sum_gate) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) a_gate[i] = fmaf(p.alpha * v[i], d[i], a_gate[i]);
-        } else {
-          float dg[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dg[i] = p.alpha * v[i] * d[i];
-          store8<DT, VEC>(dgate + row * H, w, lane, H, dg);
+        h.p[i] = fmul2(fadd2(h.p[i], gv), both(r_pre));  // the normalised h
+        a_pre.p[i] = ffma2(t.p[i], h.p[i], a_pre.p[i]);
+        t.p[i] = fmul2(t.p[i], wpre.p[i]);
+        e.p[i] = ffma2(t.p[i], both(r_pre), e.p[i]);
+        s0 = ffma2(t.p[i], h.p[i], s0);
+        if constexpr (POST) {
+          s1 = ffma2(gv, e.p[i], s1);
+          s2 = ffma2(gv, h.p[i], s2);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        d[i] *= g[i];
-        if constexpr (DROP) d[i] = (m >> i) & 1u ? d[i] * p.inv_keep : 0.f;
-      }
+      float s[3] = {both_sum(s0), both_sum(s1), both_sum(s2)};
       if constexpr (POST) {
-        float c = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a_post[i] = fmaf(d[i], xv[i], a_post[i]);
-          d[i] *= wpost[i];
-          c = fmaf(d[i], xv[i], c);
-        }
-        c = row_sum(c, at.red, turn, p.wpr, w, lane, at.bar) * inv_h;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = r_post * fmaf(-xv[i], c, d[i]);
+        row_sums<3>(s, at.red, turn, p.wpr, w, lane, at.bar);
+      } else {
+        float one[1] = {s[0]};
+        row_sums<1>(one, at.red, turn, p.wpr, w, lane, at.bar);
+        s[0] = one[0];
       }
-      store8<DT, VEC>(static_cast<T*>(p.dx) + row * H, w, lane, H, d);
+      const float rc = r_pre * s[0] * inv_h, c_post = (s[1] - rc * s[2]) * inv_h * r_post;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e.p[i] = ffma2(h.p[i], both(-rc), e.p[i]);  // the gradient of h
+      if (p.dresidual) store8<DT, VEC>(static_cast<T*>(p.dresidual) + row * H, w, lane, H, e.as());
+      if constexpr (DROP) e.keep(m);
+      if (row_gate) {
+        // The gate's row is this row's own.
+        F8 f;
+        f.set(ak);
+        if constexpr (POST) {
+          F8 g;
+          f.load<DT, VEC>(w_post, w, lane, H);
+          g.load<DT, VEC>(gate + row * p.gate_stride, w, lane, H);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f.p[i] = fmul2(f.p[i], both(ak));
+            a_post.p[i] = ffma2(fmul2(g.p[i], both(ak)), fmul2(e.p[i], xn.p[i]), a_post.p[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.p[i] = fmul2(f.p[i], fmul2(xn.p[i], e.p[i]));
+        store8<DT, VEC>(dgate + row * H, w, lane, H, f.as());
+      } else if (POST || sum_gate) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q.p[i] = ffma2(e.p[i], xn.p[i], q.p[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e.p[i] = fmul2(e.p[i], cw.p[i]);
+        if constexpr (POST) e.p[i] = ffma2(e.p[i], both(r_post), fmul2(xn.p[i], both(-c_post)));
+      }
+      store8<DT, VEC>(static_cast<T*>(p.dx) + row * H, w, lane, H, e.as());
     }
     if (sum_gate) {
+      // The span's sum, as the gate's gradient and as a share of the weight's.
+      F8 f;
+      if constexpr (POST) {
+        f.load<DT, VEC>(gate + span * p.gate_stride, w, lane, H);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a_post.p[i] = ffma2(fmul2(f.p[i], both(ak)), q.p[i], a_post.p[i]);
+        f.load<DT, VEC>(w_post, w, lane, H);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q.p[i] = fmul2(q.p[i], fmul2(f.p[i], both(ak)));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q.p[i] = fmul2(q.p[i], both(ak));
+      }
       const bool whole = p.chunks_per_span == 1;
-      flush_row<DT, VEC>(a_gate, sums, at, H, whole ? nullptr : p.part_gate + chunk * H, whole ? dgate + span * H : nullptr);
+      flush_row<DT, VEC>(q.as(), sums, at, H, whole ? nullptr : p.part_gate + chunk * H, whole ? dgate + span * H : nullptr);
     }
+  }
+  if constexpr (POST) {
+    if (!gate)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a_post.p[i] = fmul2(q.p[i], both(ak));
   }
   const bool alone = gridDim.x == 1;
   if (dn)
-    flush_row<DT, VEC>(a_pre, sums, at, H, alone ? nullptr : p.part_pre + (long long)blockIdx.x * H,
+    flush_row<DT, VEC>(a_pre.as(), sums, at, H, alone ? nullptr : p.part_pre + (long long)blockIdx.x * H,
                        static_cast<T*>(p.dw_pre));
   if constexpr (POST)
-    flush_row<DT, VEC>(a_post, sums, at, H, alone ? nullptr : p.part_post + (long long)blockIdx.x * H,
+    flush_row<DT, VEC>(a_post.as(), sums, at, H, alone ? nullptr : p.part_post + (long long)blockIdx.x * H,
                        static_cast<T*>(p.dw_post));
 }
 
-// Adds partial rows: out[j][c] = sum over i < n of part[(j * n + i) * H + c].
-// 32 columns and 16 slices of the rows a block, added in a fixed order.
+// Adds partial rows in a fixed order: out[j][c] = sum over i < n of
+// part[(j * n + i) * H + c].  The weights' gradients have one row of many parts:
+// 32 columns a block, 32 slices of the parts, then a shuffle tree.  So has a
+// gate's when few rows share many parts; else (narrow) a warp takes 32 columns of a row.
 struct SumJob {
   const float* part;
   void* out;
   long long n, rows;  // partial rows of each output row; output rows
 };
 template <int DT>
-__global__ void __launch_bounds__(512) sum_rows_kernel(SumJob a, SumJob b, SumJob c, int H) {
+__global__ void __launch_bounds__(1024) sum_rows_kernel(SumJob w0, SumJob w1, SumJob gate, int H) {
   using T = typename TrainElem<DT>::T;
-  __shared__ float sh[16][33];
-  const SumJob job = blockIdx.z == 0 ? a : blockIdx.z == 1 ? b : c;
+  __shared__ float sh[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + lane;
-  for (long long j = blockIdx.y; j < job.rows; j += gridDim.y) {
-    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-    if (col < H) {
-      const float* q = job.part + j * job.n * H + col;
-      long long i = slice;
-      for (; i + 48 < job.n; i += 64) {
-        s0 += q[i * H];
-        s1 += q[(i + 16) * H];
-        s2 += q[(i + 32) * H];
-        s3 += q[(i + 48) * H];
-      }
-      for (; i < job.n; i += 16) s0 += q[i * H];
-    }
-    sh[slice][lane] = (s0 + s1) + (s2 + s3);
-    __syncthreads();
-    if (slice == 0 && col < H) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s += sh[i][lane];
-      static_cast<T*>(job.out)[j * H + col] = TrainElem<DT>::from_f(s);
-    }
-    __syncthreads();
+  if (blockIdx.y >= 2 && gate.n < 32) {
+    const long long j = (long long)(blockIdx.y - 2) * 32 + slice;
+    if (j >= gate.rows || col >= H) return;
+    const float* q = gate.part + j * gate.n * H + col;
+    float s = 0.f;
+#pragma unroll 4
+    for (long long i = 0; i < gate.n; ++i) s += q[i * H];
+    static_cast<T*>(gate.out)[j * H + col] = TrainElem<DT>::from_f(s);
+    return;
   }
+  SumJob job = blockIdx.y == 0 ? w0 : blockIdx.y == 1 ? w1 : gate;
+  if (!job.part) return;
+  const long long j = blockIdx.y < 2 ? 0 : blockIdx.y - 2;
+  job.part += j * job.n * H;
+  float s = 0.f;
+  if (col < H) {
+    const float* q = job.part + col;
+#pragma unroll 4
+    for (long long i = slice; i < job.n; i += 32) s += q[i * H];
+  }
+  sh[slice][lane] = s;
+  __syncthreads();
+  // Warp k adds column k's slices.
+  s = sh[lane][slice];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0 && blockIdx.x * 32 + slice < H)
+    static_cast<T*>(job.out)[j * H + blockIdx.x * 32 + slice] = TrainElem<DT>::from_f(s);
 }
 
 template <int DT, bool VEC, bool POST>
@@ -348,16 +472,16 @@ cudaError_t launch_fwd(const ResidualNormParams& p, unsigned grid, unsigned bloc
 }
 template <int DT, bool VEC, bool POST>
 cudaError_t launch_bwd(const ResidualNormParams& p, unsigned grid, unsigned block, cudaStream_t st) {
-  if (block > 256) {
+  if (block > 512) {
     if (p.threshold)
       residual_norm_bwd_kernel<DT, VEC, POST, true, 1024><<<grid, block, 0, st>>>(p);
     else
       residual_norm_bwd_kernel<DT, VEC, POST, false, 1024><<<grid, block, 0, st>>>(p);
   } else {
     if (p.threshold)
-      residual_norm_bwd_kernel<DT, VEC, POST, true, 256><<<grid, block, 0, st>>>(p);
+      residual_norm_bwd_kernel<DT, VEC, POST, true, 512><<<grid, block, 0, st>>>(p);
     else
-      residual_norm_bwd_kernel<DT, VEC, POST, false, 256><<<grid, block, 0, st>>>(p);
+      residual_norm_bwd_kernel<DT, VEC, POST, false, 512><<<grid, block, 0, st>>>(p);
   }
   return cudaGetLastError();
 }
@@ -379,21 +503,29 @@ bool can_vector(const ResidualNormParams& p, int dtype, bool bwd) {
 
 }  // namespace
 
-// Warps that hold a row (eight columns a thread), rows that a block holds.
+// Warps that hold a row (eight columns a thread), and rows that a block of up to
+// `warps` warps holds.
 static int rn_wpr(int H) { return (H + 255) / 256; }
-static int rn_groups(int H) { return rn_wpr(H) >= 8 ? 1 : 8 / rn_wpr(H); }
+static int rn_groups(int H, int warps) { return rn_wpr(H) >= warps ? 1 : warps / rn_wpr(H); }
+// Warps of a block: rows held ahead take 128 registers a thread, one block of 16
+// warps fills an SM; the others go without and come as four blocks of 8.
+constexpr int kFwdWarps = 8;
+static int rn_bwd_warps(bool ahead) { return ahead ? 16 : 8; }
 
-// Chunks of the backward pass: about six blocks' worth of work for each SM, never
-// across two spans.  gate_rows: rows that share a row of the gate, 0 without one.
-ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, int num_sms) {
+// Chunks of the backward pass: one for each block that the GPU holds, never across
+// two spans.  gate_rows: rows that share a row of the gate, 0 without one.
+ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, bool ahead, int num_sms) {
   ResidualNormPlan q;
-  const int groups = rn_groups(H);
+  const int groups = rn_groups(H, rn_bwd_warps(ahead)), warps = groups * rn_wpr(H);
+  q.groups = groups;
   q.span_rows = gate_rows > 1 ? gate_rows : M;
   const long long spans = M / q.span_rows;
-  const long long want = (long long)num_sms * (rn_wpr(H) > 8 ? 2 : 6);
+  const int fit = (ahead ? 16 : 32) / warps;
+  const long long want = (long long)num_sms * (fit < 1 ? 1 : fit);
   const long long most = (q.span_rows + groups - 1) / groups;
-  long long per_span = (want + spans - 1) / spans;
+  long long per_span = want / spans;
   if (per_span > most) per_span = most;
+  if (per_span < 1) per_span = 1;
   q.chunk_rows = (q.span_rows + per_span - 1) / per_span;
   q.chunks_per_span = (q.span_rows + q.chunk_rows - 1) / q.chunk_rows;
   q.chunks = spans * q.chunks_per_span;
@@ -403,7 +535,7 @@ ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, int
 
 cudaError_t launch_residual_norm_fwd_sm100(ResidualNormParams p, int dtype, int num_sms, cudaStream_t st) {
   p.wpr = rn_wpr(p.H);
-  const int groups = rn_groups(p.H);
+  const int groups = rn_groups(p.H, kFwdWarps);
   const unsigned block = (unsigned)(p.wpr * groups * 32);
   const long long want = (p.M + groups - 1) / groups, cap = (long long)num_sms * 32;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
@@ -417,10 +549,12 @@ cudaError_t launch_residual_norm_fwd_sm100(ResidualNormParams p, int dtype, int 
 #undef DT_FWD
 }
 
+bool residual_norm_ahead(const ResidualNormParams& p, int dtype) { return dtype != 2 && can_vector(p, dtype, true); }
+
 cudaError_t launch_residual_norm_bwd_sm100(ResidualNormParams p, const ResidualNormPlan& plan, int dtype,
                                            cudaStream_t st) {
   p.wpr = rn_wpr(p.H);
-  const unsigned block = (unsigned)(p.wpr * rn_groups(p.H) * 32), grid = (unsigned)plan.grid;
+  const unsigned block = (unsigned)(p.wpr * plan.groups * 32), grid = (unsigned)plan.grid;
   p.chunks = plan.chunks;
   p.chunk_rows = plan.chunk_rows;
   p.chunks_per_span = plan.chunks_per_span;
@@ -437,20 +571,16 @@ cudaError_t launch_residual_norm_bwd_sm100(ResidualNormParams p, const ResidualN
 #undef DT_BWD
   if (e != cudaSuccess) return e;
   // What the blocks left in parts.
-  SumJob jobs[3];
-  int n = 0;
-  if (grid > 1 && p.dn) jobs[n++] = SumJob{p.part_pre, p.dw_pre, (long long)grid, 1};
-  if (grid > 1 && post) jobs[n++] = SumJob{p.part_post, p.dw_post, (long long)grid, 1};
+  SumJob w0{}, w1{}, gate{};
+  if (grid > 1 && p.dn) w0 = SumJob{p.part_pre, p.dw_pre, (long long)grid, 1};
+  if (grid > 1 && post) w1 = SumJob{p.part_post, p.dw_post, (long long)grid, 1};
   if (sum_gate && plan.chunks_per_span > 1)
-    jobs[n++] = SumJob{p.part_gate, p.dgate, plan.chunks_per_span, plan.chunks / plan.chunks_per_span};
-  if (!n) return cudaSuccess;
-  long long rows = 1;
-  for (int i = 0; i < n; ++i) rows = jobs[i].rows > rows ? jobs[i].rows : rows;
-  for (int i = n; i < 3; ++i) jobs[i] = jobs[0];
-  const dim3 g((unsigned)((p.H + 31) / 32), (unsigned)(rows < 4096 ? rows : 4096), (unsigned)n);
-  if (dtype == 0) sum_rows_kernel<0><<<g, 512, 0, st>>>(jobs[0], jobs[1], jobs[2], p.H);
-  else if (dtype == 1) sum_rows_kernel<1><<<g, 512, 0, st>>>(jobs[0], jobs[1], jobs[2], p.H);
-  else sum_rows_kernel<2><<<g, 512, 0, st>>>(jobs[0], jobs[1], jobs[2], p.H);
+    gate = SumJob{p.part_gate, p.dgate, plan.chunks_per_span, plan.chunks / plan.chunks_per_span};
+  if (!w0.part && !w1.part && !gate.part) return cudaSuccess;
+  const dim3 g((unsigned)((p.H + 31) / 32), (unsigned)(2 + (gate.n < 32 ? (gate.rows + 31) / 32 : gate.rows)));
+  if (dtype == 0) sum_rows_kernel<0><<<g, 1024, 0, st>>>(w0, w1, gate, p.H);
+  else if (dtype == 1) sum_rows_kernel<1><<<g, 1024, 0, st>>>(w0, w1, gate, p.H);
+  else sum_rows_kernel<2><<<g, 1024, 0, st>>>(w0, w1, gate, p.H);
   return cudaGetLastError();
 }
 

@@ -69,6 +69,43 @@ __device__ __forceinline__ void load8(const typename TrainElem<DT>::T* __restric
   }
 }
 
+// The same eight columns as they stand in memory: what a thread holds of a row that
+// it works on later (half the registers of fp32 for 16-bit rows of vectors).
+template <int DT, bool VEC>
+struct Raw8 {
+  using T = typename TrainElem<DT>::T;
+  float v[8];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int w, int lane, int n) {
+    load8<DT, VEC>(row, w, lane, n, v);
+  }
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = v[i];
+  }
+};
+template <int DT>
+struct Raw8Half {
+  using T = typename TrainElem<DT>::T;
+  uint4 u;
+  __device__ __forceinline__ void load(const T* __restrict__ row, int w, int lane, int n) {
+    const int c = (w * 32 + lane) * 8;
+    u = c < n ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+    const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Elem<DT == 0>::to_f2(q[i]);
+      o[2 * i] = f.x;
+      o[2 * i + 1] = f.y;
+    }
+  }
+};
+template <>
+struct Raw8<0, true> : Raw8Half<0> {};
+template <>
+struct Raw8<1, true> : Raw8Half<1> {};
+
 template <int DT, bool VEC>
 __device__ __forceinline__ void store8(typename TrainElem<DT>::T* __restrict__ row, int w, int lane, int n,
                                        const float (&v)[8]) {
