@@ -525,6 +525,11 @@ def _same_device(first: Tensor, *ts: Optional[Tensor]) -> torch.device:
     return dev
 
 
+def _empty_as(t: Tensor) -> Tensor:
+    """A contiguous tensor of t's shape and type (1.5 us on the host; from a shape and a type, 2.4 to 3.3)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _launch(name: str, dev: torch.device, *args) -> None:
     """Calls the entry point on the device's current stream (its last argument), with the device
     current: the library launches there."""
@@ -620,8 +625,8 @@ def attn_train_forward(q: Tensor, k: Tensor, v: Tensor, pad_len: Optional[Tensor
     pad_len, B, S, Hq, Hkv, D = _check_attn_train(q, k, v, pad_len, scale)
     p = _check_dropout(p, rng, site)
     (q, qs), (k, ks), (v, vs) = _rows16(q), _rows16(k), _rows16(v)
-    out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((B, Hq, S), dtype=torch.float32, device=dev)
+    out = _empty_as(q)
+    lse = torch.empty(B, Hq, S, dtype=torch.float32, device=dev)
     if out.numel():
         _launch("dt_attn_train_forward", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
                 _ptr(pad_len), B, S, Hq, Hkv, D, *qs, *ks, *vs, S * Hq * D, Hq * D, D, scale or 0.0, p, _ptr(rng), site,
@@ -649,9 +654,7 @@ def attn_train_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tens
         raise ValueError("lse must be the forward call's [B, Hq, S] fp32 tensor")
     (q, qs), (k, ks), (v, vs), (dout, dos), (out, os) = (_rows16(t) for t in (q, k, v, dout, out))
     if grads is None:
-        dq = torch.empty((B, S, Hq, D), dtype=dt, device=dev)
-        dk = torch.empty((B, S, Hkv, D), dtype=dt, device=dev)
-        dv = torch.empty((B, S, Hkv, D), dtype=dt, device=dev)
+        dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
         gs = (S * Hq * D, Hq * D, D) + 2 * (S * Hkv * D, Hkv * D, D)
     else:
         dq, dk, dv = grads
@@ -759,9 +762,8 @@ def residual_norm_forward(x: Tensor, residual: Optional[Tensor], pre_weight: Ten
     if gate is not None:
         gate_rows = _gate_rows(gate, x)
         g2, gs = _rows2d(gate)
-    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    n = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((M, 2), dtype=torch.float32, device=dev)
+    h, n = _empty_as(x), _empty_as(x)
+    stats = torch.empty(M, 2, dtype=torch.float32, device=dev)
     if M:
         _launch("dt_residual_norm_forward", dev, x2.data_ptr(), xs, _ptr(r2), rs, _ptr(g2), gs, gate_rows,
                 pre_weight.data_ptr(), _ptr(post_weight), h.data_ptr(), n.data_ptr(), stats.data_ptr(), M, H, alpha,
@@ -788,16 +790,15 @@ def residual_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], x: Tensor
     if stats.shape != (M, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError("stats must be the forward call's [rows, 2] fp32 tensor")
     gate_rows = 0 if gate is None else _gate_rows(gate, x)
-    dx = torch.empty(shape, dtype=dt, device=dev)
-    dres = torch.empty(shape, dtype=dt, device=dev)
-    dpost = None if post_weight is None else torch.empty(H, dtype=dt, device=dev)
-    dgate = None if gate is None else torch.empty(gate.shape, dtype=dt, device=dev)
+    dx, dres = _empty_as(x), _empty_as(x)
+    dpost = None if post_weight is None else _empty_as(post_weight)
+    dgate = None if gate is None else _empty_as(gate)
     if M == 0 or (dh is None and dn is None):
         for t in (dx, dres, dpost, dgate):
             if t is not None:
                 t.zero_()
         return dx, dres, torch.zeros_like(pre_weight), dpost, dgate
-    dpre = torch.empty(H, dtype=dt, device=dev) if dn is not None else torch.zeros(H, dtype=dt, device=dev)
+    dpre = torch.zeros_like(pre_weight) if dn is None else _empty_as(pre_weight)
     x2, xs = _rows2d(x)
     r2, rs = (None, 0) if residual is None else _rows2d(residual)
     g2, gs = (None, 0) if gate is None else _rows2d(gate)
@@ -822,7 +823,7 @@ def dropout_forward(x: Tensor, p: float, rng: Optional[Tensor], site: int = 0,
     p = _check_dropout(p, rng, site)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have x's shape and dtype")
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = _empty_as(x)
     n = y.numel()
     if n:
         H = x.shape[-1]
