@@ -60,9 +60,9 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
                            int64_t workspace_bytes, int B, int S, int Hq, int Hkv, int D, const int64_t* strides,
                            float scale, double p, const int64_t* rng, uint32_t site, int dtype, void* stream);
 
-/* Bytes of scratch that dt_attn_train_backward needs on the current device;
- * negative on an error. */
-int64_t dt_attn_train_workspace(int B, int S, int Hq, int Hkv, int D);
+/* Bytes of scratch that dt_attn_train_backward needs on the current device (more
+ * with has_dropout, the p > 0 of its call, than without); negative on an error. */
+int64_t dt_attn_train_workspace(int B, int S, int Hq, int Hkv, int D, int has_dropout);
 
 /*
  * Gradient of the RoPE that dt_qkv_rope applies to the q and k heads, in place

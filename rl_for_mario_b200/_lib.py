@@ -61,7 +61,7 @@ SIGNATURES = {
                                    _L, _L, _L, _F, _D, _P, _U, _I, _P]),
     "dt_attn_train_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P, _F, _D,
                                     _P, _U, _I, _P]),
-    "dt_attn_train_workspace": (_L, [_I, _I, _I, _I, _I]),
+    "dt_attn_train_workspace": (_L, [_I, _I, _I, _I, _I, _I]),
     "dt_rope_grad": (_I, [_P, _L, _L, _P, _P, _L, _I, _I, _I, _I, _I, _P]),
     "dt_residual_norm_forward": (_I, [_P, _L, _P, _L, _P, _L, _L, _P, _P, _P, _P, _P, _L, _I, _F, _F, _D, _P, _U, _I,
                                       _P]),

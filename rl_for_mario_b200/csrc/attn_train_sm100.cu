@@ -63,13 +63,11 @@ namespace dtk {
 
 namespace {
 
-template <int I>
-struct Int {
-  static constexpr int value = I;
-};
-
 constexpr int kRows = 128;   // rows of a tile
 constexpr int kBlk = 64;     // rows of a block of the other axis
+// The dq kernel hands its drop flags on for up to this many positions per head
+// dimension: S / 8 bytes a query row against 2 D of q itself, so at most four times q.
+constexpr int kWordsPerDim = 64;
 constexpr int kMaxStages = 4;
 constexpr int kPerSm = 2;       // CTAs on an SM: each takes half of its tensor memory
 constexpr uint32_t kCols = 256;
@@ -863,9 +861,9 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     const uint32_t tds = t_ds + lane_off + 16 * half;
     const float c2 = p.scale * 1.4426950408889634f;
     const unsigned per_row = (unsigned)(S + 7) >> 3;
-    const uint32_t th = p.threshold << 16;
     DropKey key{};
     if constexpr (DROP) key = drop_key(p.rng, p.site);
+    const long long all_rows = (long long)p.B * p.Hq * S;
     int blk = 0, done = 0;
     bool ok = true;
     ItemReader items{sh, abort, p.status};
@@ -938,6 +936,13 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         const int k0 = kb + j * kBlk + 32 * half;
         const int see = valid ? pos - k0 + 1 : 32, lo = j == 0 && half == 0 ? pad - kb : 0;
         const bool any = __any_sync(0xffffffffu, see > 0), edge = __any_sync(0xffffffffu, see < 32);
+        uint32_t drop = 0;
+        if constexpr (DROP) {
+          if (any) {
+            drop = drop_word(key, row_block + (unsigned)(k0 >> 3), p.threshold);
+            if (p.words && valid) p.words[(2 * j + half) * all_rows + row] = drop;
+          }
+        }
         // Columns c0 .. c0 + 16: P into w, dP (dropped, not yet scaled by 1 / (1 - p)) into d.
         auto chunk = [&](int c0, uint32_t (&w)[16], uint32_t (&d)[16]) {
           tmem_ld16_u(ts + c0, w);
@@ -954,15 +959,8 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
           }
           if constexpr (DROP) {
 #pragma unroll
-            for (int b8 = 0; b8 < 2; ++b8) {
-              const uint4 w8 = philox7(key, row_block + (unsigned)((k0 + c0) / 8 + b8));
-              auto one = [&](auto I) {
-                constexpr int e = decltype(I)::value;
-                d[8 * b8 + e] = stays<e>(w8, th) ? d[8 * b8 + e] : 0u;
-              };
-              one(Int<0>{}), one(Int<1>{}), one(Int<2>{}), one(Int<3>{});
-              one(Int<4>{}), one(Int<5>{}), one(Int<6>{}), one(Int<7>{});
-            }
+            for (int c = 0; c < 16; ++c)
+              if (drop & drop_bit(c0 + c)) d[c] = 0u;
           }
           const float2 c2v = make_float2(c2, c2), nl = make_float2(-ls, -ls);
 #pragma unroll
@@ -1044,7 +1042,8 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
 }
 
 // ---------------------------------------------------------------- dk, dv
-template <int D, bool BF16, bool DROP>
+// WORDS: the drop flags come from the dq kernel (p.words).
+template <int D, bool BF16, bool DROP, bool WORDS>
 __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     attn_train_dkv_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                              const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -1118,7 +1117,8 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     const float2 c2v = make_float2(c2, c2), ik = make_float2(p.inv_keep, p.inv_keep);
     DropKey key{};
     const unsigned per_row = (unsigned)(S + 7) >> 3;
-    if constexpr (DROP) key = drop_key(p.rng, p.site);
+    if constexpr (DROP && !WORDS) key = drop_key(p.rng, p.site);
+    const long long all_rows = (long long)p.B * p.Hq * S;
     // Scalars of the warp's 32 columns (query rows): lane l fetches those of column l; 4-byte arrays read in pairs.
     float* x_nl = reinterpret_cast<float*>(smem + SM::OFF_X) + warp * 32;                 // -lse
     float* x_nd = reinterpret_cast<float*>(smem + SM::OFF_X + 1024) + warp * 32;          // -delta
@@ -1161,10 +1161,11 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       const int first = it->first + it->split * PT, step = gr.splits * PT;
       if (nblk < 0) break;
       const int key0 = it->origin + wq * 32, kk = key0 + lane;  // the warp's keys, the thread's
+      const int it_tile = it->tile;
       const long long row_at = it->row;
       uint16_t* out = half ? static_cast<uint16_t*>(p.dk) + it->out2 : static_cast<uint16_t*>(p.dv) + it->out;
       const long long out_ss = half ? p.dk_ss : p.dv_ss;
-      const int pz = it->tile * kRows + wq * 32 + lane;
+      const int pz = it_tile * kRows + wq * 32 + lane;
       if (pz < pad && it->split == 0) {
 #pragma unroll
         for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + pz * out_ss + c) = make_uint4(0u, 0u, 0u, 0u);
@@ -1175,6 +1176,9 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       int npos = first + cpos;
       long long nrow = row_at + (long long)chead * S + npos;
       float nl = -INFINITY, nd = 0.f;
+      uint32_t nw = 0;
+      const uint32_t* words = nullptr;
+      if constexpr (WORDS) words = p.words + (it_tile * 4 + wq) * all_rows;
       auto fetch = [&](int j) {
         if (gr.chunks > 1 && j > 0 && j % per == 0) {  // the next chunk of heads, from the first position again
           npos = first + cpos;
@@ -1183,6 +1187,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         const bool there = j < nblk && col < rows && npos < S && (gr.chunks == 1 || j / per * p.HC + chead < p.R);
         nl = there ? -__ldg(p.lse + nrow) : -INFINITY;
         nd = there ? -__ldg(p.delta + nrow) : 0.f;
+        if constexpr (WORDS) nw = there && npos >= key0 ? __ldg(words + nrow) : 0u;  // written where a key is seen
       };
       fetch(0);
       for (int j = 0; j < nblk; ++j, ++blk) {
@@ -1190,8 +1195,8 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         const long long row = nrow;
         // The warp's last position against its first key: nothing to do where every query comes before every key.
         const bool any = q0 + last_pos >= key0;
-        uint32_t drop = 0;
-        if constexpr (DROP) {
+        uint32_t drop = nw;
+        if constexpr (DROP && !WORDS) {
           if (any) drop = drop_word(key, (unsigned long long)row * per_row + (unsigned)(key0 >> 3), p.threshold);
         }
         __syncwarp();
@@ -1371,7 +1376,7 @@ cudaError_t run_fwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sm
 template <int D, bool BF16, bool DROP>
 cudaError_t run_bwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sms, cudaStream_t st) {
   auto kq = attn_train_dq_tc_kernel<D, BF16, DROP>;
-  auto kk = attn_train_dkv_tc_kernel<D, BF16, DROP>;
+  auto kk = DROP && p.words ? attn_train_dkv_tc_kernel<D, BF16, DROP, DROP> : attn_train_dkv_tc_kernel<D, BF16, DROP, false>;
   cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kq), BwdSmem<D, true>::BYTES);
   if (e != cudaSuccess) return e;
   if ((e = smem_limit_once(reinterpret_cast<const void*>(kk), BwdSmem<D, false>::BYTES)) != cudaSuccess) return e;
@@ -1399,6 +1404,13 @@ int attn_train_splits(int B, int S, int Hkv, int R, int num_sms) {
   long long n = (long long)kPerSm * num_sms / items;
   if (n > blocks / 4) n = blocks / 4;
   return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+}
+
+// Words of drop flags that the dq kernel hands to the dk, dv kernel, 0 where both
+// generate them.
+long long attn_train_words(int B, int S, int Hq, int D) {
+  if (S > kWordsPerDim * D) return 0;
+  return (long long)B * Hq * S * ((S + kBlk - 1) / kBlk * 2);
 }
 
 cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,

@@ -91,11 +91,15 @@ int check_elem_aligned(const char* fn, int dtype, std::initializer_list<const vo
   return DT_OK;
 }
 
-// The backward pass's scratch: delta, then the partial sums of split tiles of keys.
+// The backward pass's scratch: delta, then the partial sums of split tiles of keys, then the drop flags.
 int64_t delta_elems(int B, int S, int Hq) { return ((int64_t)B * Hq * S + 3) / 4 * 4; }
-int64_t attn_workspace(int B, int S, int Hq, int Hkv, int D, int sms) {
+int64_t attn_part_elems(int B, int S, int Hq, int Hkv, int D, int sms) {
   const int n = dtk::attn_train_splits(B, S, Hkv, Hq / Hkv, sms);
-  return 4 * (delta_elems(B, S, Hq) + (n > 1 ? (int64_t)n * 2 * B * Hkv * S * D : 0));
+  return n > 1 ? (int64_t)n * 2 * B * Hkv * S * D : 0;
+}
+int64_t attn_workspace(int B, int S, int Hq, int Hkv, int D, bool drop, int sms) {
+  return 4 * (delta_elems(B, S, Hq) + attn_part_elems(B, S, Hq, Hkv, D, sms) +
+              (drop ? dtk::attn_train_words(B, S, Hq, D) : 0));
 }
 
 constexpr int kMaxHidden = 8192;  // 32 warps of 256 columns: one block holds a row
@@ -164,12 +168,14 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
   int sms = 0;
   if ((rc = need_sm100(fn, &sms, &a.status))) return rc;
   a.q = q, a.k = k, a.v = v, a.o = const_cast<void*>(o), a.lse = const_cast<float*>(lse), a.pad_len = pad_len;
-  if (workspace_bytes < attn_workspace(B, S, Hq, Hkv, D, sms) || !aligned16(workspace))
+  if (workspace_bytes < attn_workspace(B, S, Hq, Hkv, D, a.threshold != 0, sms) || !aligned16(workspace))
     return api_fail(DT_ERR_INVALID, "%s: workspace of %lld bytes is too small or not 16-byte aligned", fn,
                     (long long)workspace_bytes);
   a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
   a.delta = static_cast<float*>(workspace);
   a.part = a.delta + delta_elems(B, S, Hq);
+  if (a.threshold && dtk::attn_train_words(B, S, Hq, D))
+    a.words = reinterpret_cast<uint32_t*>(a.part + attn_part_elems(B, S, Hq, Hkv, D, sms));
   long long* const to[24] = {&a.q_sb,  &a.q_ss,  &a.q_sh,  &a.k_sb,  &a.k_ss,  &a.k_sh,  &a.v_sb,  &a.v_ss,
                              &a.v_sh,  &a.o_sb,  &a.o_ss,  &a.o_sh,  &a.do_sb, &a.do_ss, &a.do_sh, &a.dq_sb,
                              &a.dq_ss, &a.dq_sh, &a.dk_sb, &a.dk_ss, &a.dk_sh, &a.dv_sb, &a.dv_ss, &a.dv_sh};
@@ -197,12 +203,12 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
   return cuda_status(dtk::launch_attn_train_bwd_sm100(a, m, D, bf16, sms, static_cast<cudaStream_t>(stream)), fn);
 }
 
-int64_t dt_attn_train_workspace(int B, int S, int Hq, int Hkv, int D) {
+int64_t dt_attn_train_workspace(int B, int S, int Hq, int Hkv, int D, int has_dropout) {
   const int64_t s[3] = {8, 8, 8};
   int rc = check_attn("dt_attn_train_workspace", B, S, Hq, Hkv, D, s, 3, DT_DTYPE_BF16);
   int sms = 0;
   if (rc || (rc = need_sm100("dt_attn_train_workspace", &sms))) return -rc;
-  return attn_workspace(B, S, Hq, Hkv, D, sms);
+  return attn_workspace(B, S, Hq, Hkv, D, has_dropout != 0, sms);
 }
 
 int dt_rope_grad(void* g, int64_t g_stride, int64_t rows, const float* cos_tab, const float* sin_tab,

@@ -292,6 +292,9 @@ struct AttnTrainParams {
   void* dv;
   float* delta;            // [B, Hq, S]
   float* part;             // [splits, 2 (dv, dk), B, Hkv, S, D] partial sums when a tile of keys is split
+  // Drop flags from the dq kernel for the dk, dv kernel: [groups of 32 keys, from the first
+  // unpadded position rounded down to 8] x [B, Hq, S] words, or null: generated again.
+  uint32_t* words;
   const int32_t* pad_len;  // [B] or null
   long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh;
   long long do_sb, do_ss, do_sh, dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
@@ -311,6 +314,7 @@ struct AttnTrainMaps {
   CUtensorMap q_tile, do_tile, o_tile, q_blk, do_blk, k_tile, v_tile, k_blk, v_blk;
 };
 int attn_train_splits(int B, int S, int Hkv, int R, int num_sms);
+long long attn_train_words(int B, int S, int Hq, int D);
 cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
                                         int num_sms, cudaStream_t st);
 cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,

@@ -666,7 +666,7 @@ def attn_train_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tens
                                  "rows and strides that are multiples of 8")
             gs += t.stride()[:3]
     if dq.numel():
-        size = _workspace("dt_attn_train_workspace", dev.index, B, S, Hq, Hkv, D)
+        size = _workspace("dt_attn_train_workspace", dev.index, B, S, Hq, Hkv, D, int(p > 0.0))
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         _launch("dt_attn_train_backward", dev, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(pad_len),

@@ -36,7 +36,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
 
     assert bwd(ws=None) == _lib.DT_ERR_INVALID and bwd(dq=a + 8) == _lib.DT_ERR_INVALID
     assert bwd(dtype=2) == _lib.DT_ERR_UNSUPPORTED
-    assert lib.dt_attn_train_workspace(1, 8, 4, 3, 32) < 0 and lib.dt_attn_train_workspace(1, 0, 4, 2, 32) < 0
+    assert lib.dt_attn_train_workspace(1, 8, 4, 3, 32, 0) < 0 and lib.dt_attn_train_workspace(1, 0, 4, 2, 32, 1) < 0
 
     def norm(x=a, w=a, gate=None, gate_rows=0, M=4, H=8, dtype=0, h=a, p=0.0):
         return lib.dt_residual_norm_forward(x, 8, a, 8, gate, 8, gate_rows, w, None, h, a, a, M, H, 1.0, 1e-5, p, None,
