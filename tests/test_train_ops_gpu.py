@@ -114,6 +114,8 @@ ATTN = [
     (200, 33, 5, 1, 32, "each", BF16, 0.1),  # many short units: a CTA walks several, padding on every residue of 8
     (150, 192, 8, 2, 32, "each", BF16, 0.0),
     (40, 130, 6, 2, 64, "each", FP16, 0.2),
+    (1, 2048, 2, 1, 32, [9], BF16, 0.1),  # 64 positions for each of D: the longest whose drop flags are kept
+    (1, 2055, 2, 1, 32, [9], BF16, 0.1),
 ]
 
 
