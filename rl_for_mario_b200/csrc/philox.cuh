@@ -61,6 +61,15 @@ __device__ __forceinline__ uint32_t drop_flags(uint32_t w, uint32_t t2) {
   return __vminu2(__vmaxu2(w, t2) - w, 0x00010001u);
 }
 
+// All ones in the halves of four words whose elements stay (word i: elements 2 i and
+// 2 i + 1): a pair of 16-bit elements is dropped by one AND.
+__device__ __forceinline__ uint4 keep_masks(const DropKey& k, unsigned long long block, uint32_t threshold) {
+  const uint4 w = philox7(k, block);
+  const uint32_t t2 = threshold * 0x10001u;
+  return make_uint4(~(drop_flags(w.x, t2) * 0xffffu), ~(drop_flags(w.y, t2) * 0xffffu),
+                    ~(drop_flags(w.z, t2) * 0xffffu), ~(drop_flags(w.w, t2) * 0xffffu));
+}
+
 // Bit i set: element i of the block stays.
 __device__ __forceinline__ uint32_t keep_bits(const DropKey& k, unsigned long long block, uint32_t threshold) {
   const uint4 w = philox7(k, block);

@@ -69,31 +69,6 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& turn, i
     for (int i = 0; i < N; ++i) v[i] += slot[k * kSums + i];
 }
 
-// Eight columns as packed pairs (one instruction for two of them: the kernels are
-// as near to the issue rate as to HBM).
-struct F8 {
-  float2 p[4];
-  template <int DT, bool VEC>
-  __device__ __forceinline__ void load(const typename TrainElem<DT>::T* row, int w, int lane, int n) {
-    load8<DT, VEC>(row, w, lane, n, as());
-  }
-  __device__ __forceinline__ float (&as())[8] { return *reinterpret_cast<float(*)[8]>(p); }
-  __device__ __forceinline__ void set(float v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = make_float2(v, v);
-  }
-  // Clears what the mask bits drop (bit i: element i stays).
-  __device__ __forceinline__ void keep(uint32_t m) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[i].x = (m >> (2 * i)) & 1u ? p[i].x : 0.f;
-      p[i].y = (m >> (2 * i + 1)) & 1u ? p[i].y : 0.f;
-    }
-  }
-};
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float both_sum(float2 v) { return v.x + v.y; }
-
 struct RowPlace {
   int w, lane, group, groups, bar;
   float* red;

@@ -130,6 +130,31 @@ __device__ __forceinline__ void store8(typename TrainElem<DT>::T* __restrict__ r
   }
 }
 
+// Eight columns as packed pairs (one instruction for two of them: the kernels are
+// as near to the issue rate as to HBM).
+struct F8 {
+  float2 p[4];
+  template <int DT, bool VEC>
+  __device__ __forceinline__ void load(const typename TrainElem<DT>::T* row, int w, int lane, int n) {
+    load8<DT, VEC>(row, w, lane, n, as());
+  }
+  __device__ __forceinline__ float (&as())[8] { return *reinterpret_cast<float(*)[8]>(p); }
+  __device__ __forceinline__ void set(float v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = make_float2(v, v);
+  }
+  // Clears what the mask bits drop (bit i: element i stays).
+  __device__ __forceinline__ void keep(uint32_t m) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i].x = (m >> (2 * i)) & 1u ? p[i].x : 0.f;
+      p[i].y = (m >> (2 * i + 1)) & 1u ? p[i].y : 0.f;
+    }
+  }
+};
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float both_sum(float2 v) { return v.x + v.y; }
+
 // Bit i set: the thread's element i stays.  Every lane computes the block of
 // columns 8 (32 w + lane) ..; without VEC the bits then move to the lanes that
 // own the columns (element j of lane l is bit l % 8 of lane 4 j + l / 8).
