@@ -314,7 +314,7 @@ int dt_residual_norm_backward(const void* dh, int64_t dh_stride, const void* dn,
   a.dh_stride = dh_stride, a.dn_stride = dn_stride;
   a.M = M, a.H = H, a.gate_rows = gate_rows;
   a.alpha = alpha, a.eps = eps, a.rng = reinterpret_cast<const long long*>(rng), a.site = site;
-  const dtk::ResidualNormPlan plan = dtk::residual_norm_plan(M, H, gate_rows, dtk::residual_norm_ahead(a, dtype), sms);
+  const dtk::ResidualNormPlan plan = dtk::residual_norm_plan(M, H, gate_rows, dtk::residual_norm_ring(a, dtype), sms);
   if (workspace_bytes < 4 * part_elems(plan, H, gate_rows, post) || !workspace || !aligned16(workspace))
     return api_fail(DT_ERR_INVALID, "%s: workspace of %lld bytes is too small, null or not 16-byte aligned", fn,
                     (long long)workspace_bytes);

@@ -23,7 +23,8 @@
 // once, and n is the norm of the unrounded h.
 //
 // Bound by HBM.  A row is held by one or more warps (WPR), so it is read once and
-// its sums are a shuffle tree plus (WPR > 1) one named barrier; the next row's loads are issued before this row's sums, so
+// its sums are a shuffle tree plus (WPR > 1) one named barrier; the next rows' loads
+// are issued before this row's sums, so that
 // they are in flight behind the barriers.  The sums over rows of the backward
 // pass stay in registers (a thread owns its columns for every row that it
 // meets); one block of up to 512 threads on each SM writes one partial row of
@@ -37,11 +38,53 @@ namespace dtk {
 
 namespace {
 
-// Whether a thread holds the next row while it works on one: 16-bit vectors only,
-// whose four registers a tensor leave room for it (fp32 rows held ahead spill:
-// 71 us against 49 us without, 4,257 rows of 1,001).
+// 16-bit rows of vectors are fetched before their turn, others where they are used
+// (fp32 rows held ahead take the registers of one block in four: 21 and 30 us
+// against 16 and 27, 4,257 rows of 1,001).
 template <int DT, bool VEC>
 constexpr bool kAhead = VEC && DT != 2;
+
+// The forward pass holds one row ahead in registers (two tensors, four registers
+// each; a ring as below took 90.3 us instead of 88.3, 96 x 768 rows of 768).  The
+// backward pass, with four tensors, has several rows on their way into shared memory
+// (131 us, 137 with one row in registers): each thread copies its own eight columns
+// and reads only those back, so a copy needs no barrier, and what is in flight takes
+// no registers.  kDepth: rows of a ring in a block of MAXT threads.
+constexpr int kRingTensors = 4, kRingBytes = 128 << 10;
+template <int MAXT>
+constexpr int kDepth = kRingBytes / (kRingTensors * 16 * MAXT);
+static_assert(kDepth<512> == 4 && kDepth<1024> == 2);
+
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <int DT>
+struct RowRing {
+  using T = typename TrainElem<DT>::T;
+  uint4* mine;  // the thread's place in the first slot
+  int c, n;     // its first column, the width
+  __device__ __forceinline__ void copy(int slot, const T* __restrict__ row) const {
+    if (c < n)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                       (uint32_t)__cvta_generic_to_shared(mine + slot * blockDim.x)),
+                   "l"(row + c)
+                   : "memory");
+  }
+  // Columns at or past n read as 0.
+  __device__ __forceinline__ void get(int slot, float (&v)[8]) const {
+    const uint4 u = c < n ? mine[slot * blockDim.x] : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Elem<DT == 0>::to_f2(q[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
 
 constexpr int kSums = 3;      // row sums taken together, at most
 constexpr int kMaxGroups = 16;  // rows of a block
@@ -89,9 +132,13 @@ __device__ __forceinline__ RowPlace place(int wpr, float* red_all) {
 // A row of H columns is ceil(H / 256) warps' (one warp for rows of up to 1024, four
 // pieces of eight columns a lane, took 127 us where three take 104 us: 96 x 768 rows
 // of 768, both norms and a gate).  The weights come from L1 each time, in favour of
-// the next row's registers.  MAXT: the block's largest size.
+// the next row's registers.  MAXT: the block's largest size; of blocks of 256, three
+// (rows held ahead) or four have to fit an SM, which caps a thread's registers (96 x
+// 768 rows of 768: 88 us with three, 94 with four, 170 with five; 4,257 fp32 rows of
+// 1,001: 17 us with three, 16 with four).
 template <int DT, bool VEC, bool POST, bool DROP, int MAXT>
-__global__ void __launch_bounds__(MAXT) residual_norm_fwd_kernel(const __grid_constant__ ResidualNormParams p) {
+__global__ void __launch_bounds__(MAXT, MAXT > 256 ? 1 : kAhead<DT, VEC> ? 3 : 4)
+    residual_norm_fwd_kernel(const __grid_constant__ ResidualNormParams p) {
   using T = typename TrainElem<DT>::T;
   __shared__ float red_all[8 * 64 * kSums];
   const RowPlace at = place(p.wpr, red_all);
@@ -137,13 +184,15 @@ __global__ void __launch_bounds__(MAXT) residual_norm_fwd_kernel(const __grid_co
   if constexpr (kAhead<DT, VEC>) fetch(row);
   for (; row < p.M; row += step) {
     F8 v, h;
-    if constexpr (!kAhead<DT, VEC>) fetch(row);
-    nx.get(v.as());
-    if (res)
-      nr.get(h.as());
-    else
-      h.set(0.f);
-    if constexpr (kAhead<DT, VEC>) fetch(row + step);
+    h.set(0.f);
+    if constexpr (kAhead<DT, VEC>) {
+      nx.get(v.as());
+      if (res) nr.get(h.as());
+      fetch(row + step);
+    } else {
+      v.load<DT, VEC>(x + row * p.x_stride, w, lane, H);
+      if (res) h.load<DT, VEC>(res + row * p.res_stride, w, lane, H);
+    }
     if (!fixed_gate) weigh(p.by_gate((int)row));
     if constexpr (POST) {
       float2 q = make_float2(0.f, 0.f);
@@ -211,7 +260,7 @@ __device__ __forceinline__ void flush_row(float (&acc)[8], float* sh, const RowP
 // the end of each, the weights' sums at its own end.
 // MAXT: the block's largest size (a bound on the registers a thread may take).
 template <int DT, bool VEC, bool POST, bool DROP, int MAXT>
-__global__ void __launch_bounds__(MAXT) residual_norm_bwd_kernel(const __grid_constant__ ResidualNormParams p) {
+__global__ void __launch_bounds__(MAXT, 1) residual_norm_bwd_kernel(const __grid_constant__ ResidualNormParams p) {
   using T = typename TrainElem<DT>::T;
   __shared__ float red_all[8 * 64 * kSums];
   __shared__ float sums[(kMaxGroups - 1) * 256];
@@ -253,13 +302,20 @@ __global__ void __launch_bounds__(MAXT) residual_norm_bwd_kernel(const __grid_co
   };
   if (!gate) weigh(0);
 
-  Raw8<DT, VEC> nx, nr, nh, nn;
+  extern __shared__ uint4 ring_smem[];
+  constexpr int DEPTH = kDepth<MAXT>;
+  const RowRing<DT> ring{ring_smem + threadIdx.x, (w * 32 + lane) * 8, H};
+  auto fetch = [&](int stage, long long row, long long end) {
+    if (row < end) {
+      ring.copy(stage * 4, x + row * p.x_stride);
+      if (res) ring.copy(stage * 4 + 1, res + row * p.res_stride);
+      if (dh) ring.copy(stage * 4 + 2, dh + row * p.dh_stride);
+      if (dn) ring.copy(stage * 4 + 3, dn + row * p.dn_stride);
+    }
+    copies_commit();
+  };
   float n_post = 1.f, n_pre = 0.f;
-  auto fetch = [&](long long row) {
-    nx.load(x + row * p.x_stride, w, lane, H);
-    if (res) nr.load(res + row * p.res_stride, w, lane, H);
-    if (dh) nh.load(dh + row * p.dh_stride, w, lane, H);
-    if (dn) nn.load(dn + row * p.dn_stride, w, lane, H);
+  auto fetch_stats = [&](long long row) {
     if constexpr (POST) n_post = p.stats[2 * row];
     n_pre = p.stats[2 * row + 1];
   };
@@ -269,27 +325,32 @@ __global__ void __launch_bounds__(MAXT) residual_norm_bwd_kernel(const __grid_co
     const long long r1 = min(r0 + p.chunk_rows, (span + 1) * p.span_rows);
     if (sum_gate) weigh(span);
     long long row = r0 + at.group;
+    int stage = 0;
+    if (row < r1) fetch_stats(row);
     if constexpr (kAhead<DT, VEC>)
-      if (row < r1) fetch(row);
+#pragma unroll
+      for (int s = 0; s < DEPTH; ++s) fetch(s, row + s * at.groups, r1);
     for (; row < r1; row += at.groups) {
       F8 xn, h, e, t;
-      if constexpr (!kAhead<DT, VEC>) fetch(row);
-      nx.get(xn.as());
-      if (res)
-        nr.get(h.as());
-      else
-        h.set(0.f);
-      if (dh)
-        nh.get(e.as());
-      else
-        e.set(0.f);
-      if (dn)
-        nn.get(t.as());
-      else
-        t.set(0.f);
+      h.set(0.f);
+      e.set(0.f);
+      t.set(0.f);
+      if constexpr (kAhead<DT, VEC>) {
+        copies_wait<DEPTH - 1>();
+        ring.get(stage * 4, xn.as());
+        if (res) ring.get(stage * 4 + 1, h.as());
+        if (dh) ring.get(stage * 4 + 2, e.as());
+        if (dn) ring.get(stage * 4 + 3, t.as());
+        fetch(stage, row + DEPTH * at.groups, r1);
+        stage = stage + 1 == DEPTH ? 0 : stage + 1;
+      } else {
+        xn.load<DT, VEC>(x + row * p.x_stride, w, lane, H);
+        if (res) h.load<DT, VEC>(res + row * p.res_stride, w, lane, H);
+        if (dh) e.load<DT, VEC>(dh + row * p.dh_stride, w, lane, H);
+        if (dn) t.load<DT, VEC>(dn + row * p.dn_stride, w, lane, H);
+      }
       const float r_post = n_post, r_pre = n_pre;
-      if constexpr (kAhead<DT, VEC>)
-        if (row + at.groups < r1) fetch(row + at.groups);
+      if (row + at.groups < r1) fetch_stats(row + at.groups);
       if (row_gate) weigh(row);
       uint32_t m = 0xffu;
       if constexpr (DROP) m = keep8<VEC>(key, (unsigned long long)row * per_row, w, lane, p.threshold);
@@ -430,35 +491,35 @@ __global__ void __launch_bounds__(1024) sum_rows_kernel(SumJob w0, SumJob w1, Su
     static_cast<T*>(job.out)[j * H + blockIdx.x * 32 + slice] = TrainElem<DT>::from_f(s);
 }
 
+template <int DT, bool VEC, bool POST, int MAXT>
+cudaError_t run_fwd(const ResidualNormParams& p, unsigned grid, unsigned block, cudaStream_t st) {
+  if (p.threshold)
+    residual_norm_fwd_kernel<DT, VEC, POST, true, MAXT><<<grid, block, 0, st>>>(p);
+  else
+    residual_norm_fwd_kernel<DT, VEC, POST, false, MAXT><<<grid, block, 0, st>>>(p);
+  return cudaGetLastError();
+}
 template <int DT, bool VEC, bool POST>
 cudaError_t launch_fwd(const ResidualNormParams& p, unsigned grid, unsigned block, cudaStream_t st) {
-  if (block > 256) {
-    if (p.threshold)
-      residual_norm_fwd_kernel<DT, VEC, POST, true, 1024><<<grid, block, 0, st>>>(p);
-    else
-      residual_norm_fwd_kernel<DT, VEC, POST, false, 1024><<<grid, block, 0, st>>>(p);
-  } else {
-    if (p.threshold)
-      residual_norm_fwd_kernel<DT, VEC, POST, true, 256><<<grid, block, 0, st>>>(p);
-    else
-      residual_norm_fwd_kernel<DT, VEC, POST, false, 256><<<grid, block, 0, st>>>(p);
+  return block > 256 ? run_fwd<DT, VEC, POST, 1024>(p, grid, block, st) : run_fwd<DT, VEC, POST, 256>(p, grid, block, st);
+}
+
+template <int DT, bool VEC, bool POST, int MAXT>
+cudaError_t run_bwd(const ResidualNormParams& p, unsigned grid, unsigned block, cudaStream_t st) {
+  auto kern = p.threshold ? residual_norm_bwd_kernel<DT, VEC, POST, true, MAXT>
+                          : residual_norm_bwd_kernel<DT, VEC, POST, false, MAXT>;
+  unsigned smem = 0;
+  if constexpr (kAhead<DT, VEC>) {
+    smem = kDepth<MAXT> * kRingTensors * 16 * block;
+    const cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kern), kRingBytes);
+    if (e != cudaSuccess) return e;
   }
+  kern<<<grid, block, smem, st>>>(p);
   return cudaGetLastError();
 }
 template <int DT, bool VEC, bool POST>
 cudaError_t launch_bwd(const ResidualNormParams& p, unsigned grid, unsigned block, cudaStream_t st) {
-  if (block > 512) {
-    if (p.threshold)
-      residual_norm_bwd_kernel<DT, VEC, POST, true, 1024><<<grid, block, 0, st>>>(p);
-    else
-      residual_norm_bwd_kernel<DT, VEC, POST, false, 1024><<<grid, block, 0, st>>>(p);
-  } else {
-    if (p.threshold)
-      residual_norm_bwd_kernel<DT, VEC, POST, true, 512><<<grid, block, 0, st>>>(p);
-    else
-      residual_norm_bwd_kernel<DT, VEC, POST, false, 512><<<grid, block, 0, st>>>(p);
-  }
-  return cudaGetLastError();
+  return block > 512 ? run_bwd<DT, VEC, POST, 1024>(p, grid, block, st) : run_bwd<DT, VEC, POST, 512>(p, grid, block, st);
 }
 
 // 16-byte accesses need every row on a 16-byte boundary and whole vectors.
@@ -482,20 +543,20 @@ bool can_vector(const ResidualNormParams& p, int dtype, bool bwd) {
 // `warps` warps holds.
 static int rn_wpr(int H) { return (H + 255) / 256; }
 static int rn_groups(int H, int warps) { return rn_wpr(H) >= warps ? 1 : warps / rn_wpr(H); }
-// Warps of a block: rows held ahead take 128 registers a thread, one block of 16
-// warps fills an SM; the others go without and come as four blocks of 8.
+// Warps of a block: with a ring of rows on their way one block of 16 warps fills an
+// SM, without one four blocks of 8.
 constexpr int kFwdWarps = 8;
-static int rn_bwd_warps(bool ahead) { return ahead ? 16 : 8; }
+static int rn_bwd_warps(bool ring) { return ring ? 16 : 8; }
 
 // Chunks of the backward pass: one for each block that the GPU holds, never across
 // two spans.  gate_rows: rows that share a row of the gate, 0 without one.
-ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, bool ahead, int num_sms) {
+ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, bool ring, int num_sms) {
   ResidualNormPlan q;
-  const int groups = rn_groups(H, rn_bwd_warps(ahead)), warps = groups * rn_wpr(H);
+  const int groups = rn_groups(H, rn_bwd_warps(ring)), warps = groups * rn_wpr(H);
   q.groups = groups;
   q.span_rows = gate_rows > 1 ? gate_rows : M;
   const long long spans = M / q.span_rows;
-  const int fit = (ahead ? 16 : 32) / warps;
+  const int fit = (ring ? 16 : 32) / warps;
   const long long want = (long long)num_sms * (fit < 1 ? 1 : fit);
   const long long most = (q.span_rows + groups - 1) / groups;
   long long per_span = want / spans;
@@ -524,7 +585,7 @@ cudaError_t launch_residual_norm_fwd_sm100(ResidualNormParams p, int dtype, int 
 #undef DT_FWD
 }
 
-bool residual_norm_ahead(const ResidualNormParams& p, int dtype) { return dtype != 2 && can_vector(p, dtype, true); }
+bool residual_norm_ring(const ResidualNormParams& p, int dtype) { return dtype != 2 && can_vector(p, dtype, true); }
 
 cudaError_t launch_residual_norm_bwd_sm100(ResidualNormParams p, const ResidualNormPlan& plan, int dtype,
                                            cudaStream_t st) {
