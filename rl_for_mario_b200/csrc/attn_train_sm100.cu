@@ -1111,7 +1111,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         });
   } else if (warp < 8) {
     const int half = warp >> 2, wq = warp & 3;
-    const uint32_t lane_off = (uint32_t)(wq * 32) << 16, lane_bit = drop_bit(lane);
+    const uint32_t lane_off = (uint32_t)(wq * 32) << 16;
     const uint32_t ts = t_s + lane_off + 32 * half, tdp = t_dp + lane_off + 32 * half;
     const float c2 = p.scale * 1.4426950408889634f;
     const float2 c2v = make_float2(c2, c2), ik = make_float2(p.inv_keep, p.inv_keep);
@@ -1119,11 +1119,10 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     const unsigned per_row = (unsigned)(S + 7) >> 3;
     if constexpr (DROP && !WORDS) key = drop_key(p.rng, p.site);
     const long long all_rows = (long long)p.B * p.Hq * S;
-    // Scalars of the warp's 32 columns (query rows): lane l fetches those of column l; 4-byte arrays read in pairs.
+    // Scalars of the warp's 32 columns (query rows): lane l fetches those of column l; 4-byte arrays read in fours.
     float* x_nl = reinterpret_cast<float*>(smem + SM::OFF_X) + warp * 32;                 // -lse
     float* x_nd = reinterpret_cast<float*>(smem + SM::OFF_X + 1024) + warp * 32;          // -delta
-    uint32_t* x_drop = reinterpret_cast<uint32_t*>(smem + SM::OFF_X + 2048) + warp * 32;  // drop flags of the warp's keys
-    int* x_pos = reinterpret_cast<int*>(smem + SM::OFF_X + 3072) + warp * 32;
+    int* x_pos = reinterpret_cast<int*>(smem + SM::OFF_X + 2048) + warp * 32;
     const int col = 32 * half + lane, chead = col % p.HC, cpos = col / p.HC;
     const int last_pos = min(32 * half + 31, rows - 1) / p.HC;
     int blk = 0, done = 0;
@@ -1199,10 +1198,11 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         if constexpr (DROP && !WORDS) {
           if (any) drop = drop_word(key, (unsigned long long)row * per_row + (unsigned)(key0 >> 3), p.threshold);
         }
+        // From the flags of a column's 32 keys to those of the thread's key in 32 columns.
+        if constexpr (DROP) drop = __shfl_sync(0xffffffffu, warp_transpose(drop, lane), drop_place(lane));
         __syncwarp();
         x_nl[lane] = nl;
         x_nd[lane] = nd;
-        if constexpr (DROP) x_drop[lane] = drop;
         x_pos[lane] = pos;
         __syncwarp();
         // The next block's scalars: on their way while this one is worked on.
@@ -1230,17 +1230,19 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
           for (int c0 = 0; c0 < 32; c0 += 16) {
             uint32_t pw[8];
 #pragma unroll
-            for (int c = c0; c < c0 + 16; c += 2) {
-              const float2 x = ffma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2v,
-                                     *reinterpret_cast<const float2*>(x_nl + c));
-              const float w0 = ex2_approx(x.x), w1 = ex2_approx(x.y);
-              s[c] = __float_as_uint(w0);
-              s[c + 1] = __float_as_uint(w1);
-              if constexpr (DROP) {
-                const uint2 db = *reinterpret_cast<const uint2*>(x_drop + c);
-                pw[(c - c0) >> 1] = E::from_f2(db.x & lane_bit ? 0.f : w0, db.y & lane_bit ? 0.f : w1);
-              } else {
-                pw[(c - c0) >> 1] = E::from_f2(w0, w1);
+            for (int c4 = c0; c4 < c0 + 16; c4 += 4) {
+              const float4 nl4 = *reinterpret_cast<const float4*>(x_nl + c4);
+#pragma unroll
+              for (int c = c4; c < c4 + 4; c += 2) {
+                const float2 x = ffma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2v,
+                                       c == c4 ? make_float2(nl4.x, nl4.y) : make_float2(nl4.z, nl4.w));
+                const float w0 = ex2_approx(x.x), w1 = ex2_approx(x.y);
+                s[c] = __float_as_uint(w0);
+                s[c + 1] = __float_as_uint(w1);
+                if constexpr (DROP)
+                  pw[(c - c0) >> 1] = E::from_f2(drop & 1u << c ? 0.f : w0, drop & 2u << c ? 0.f : w1);
+                else
+                  pw[(c - c0) >> 1] = E::from_f2(w0, w1);
               }
             }
             tmem_st8(ts + (c0 >> 1), pw);
@@ -1270,17 +1272,19 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
             uint32_t dp[16];
             tmem_ld16_u(tdp + c0, dp);
 #pragma unroll
-            for (int c = 0; c < 16; c += 2) {
-              const float2 md = *reinterpret_cast<const float2*>(x_nd + c0 + c);
-              float2 d = make_float2(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1]));
-              if constexpr (DROP) {
-                const uint2 db = *reinterpret_cast<const uint2*>(x_drop + c0 + c);
-                d = ffma2(make_float2(db.x & lane_bit ? 0.f : d.x, db.y & lane_bit ? 0.f : d.y), ik, md);
-              } else {
-                d = fadd2(d, md);
+            for (int c4 = 0; c4 < 16; c4 += 4) {
+              const float4 nd4 = *reinterpret_cast<const float4*>(x_nd + c0 + c4);
+#pragma unroll
+              for (int c = c4; c < c4 + 4; c += 2) {
+                const float2 md = c == c4 ? make_float2(nd4.x, nd4.y) : make_float2(nd4.z, nd4.w);
+                float2 d = make_float2(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1]));
+                if constexpr (DROP)
+                  d = ffma2(make_float2(drop & 1u << (c0 + c) ? 0.f : d.x, drop & 2u << (c0 + c) ? 0.f : d.y), ik, md);
+                else
+                  d = fadd2(d, md);
+                d = fmul2(make_float2(__uint_as_float(s[c0 + c]), __uint_as_float(s[c0 + c + 1])), d);
+                s[(c0 + c) >> 1] = E::from_f2(d.x, d.y);
               }
-              d = fmul2(make_float2(__uint_as_float(s[c0 + c]), __uint_as_float(s[c0 + c + 1])), d);
-              s[(c0 + c) >> 1] = E::from_f2(d.x, d.y);
             }
           }
           tmem_st16(tdp, *reinterpret_cast<uint32_t(*)[16]>(s));

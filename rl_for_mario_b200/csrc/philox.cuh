@@ -91,8 +91,22 @@ __device__ __forceinline__ uint32_t drop_word(const DropKey& k, unsigned long lo
   }
   return r;
 }
-__device__ __forceinline__ uint32_t drop_bit(int element) {  // 0 .. 31
-  return 1u << ((element & 1) * 16 + (element >> 3) * 4 + ((element & 7) >> 1));
+__device__ __forceinline__ int drop_place(int element) {  // 0 .. 31
+  return (element & 1) * 16 + (element >> 3) * 4 + ((element & 7) >> 1);
+}
+__device__ __forceinline__ uint32_t drop_bit(int element) { return 1u << drop_place(element); }
+
+// 32 x 32 bits turned over across a warp: bit c of lane b becomes bit b of lane c.
+// Five exchanges of half as many bits each time.
+__device__ __forceinline__ uint32_t warp_transpose(uint32_t x, int lane) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    const uint32_t low = s == 16 ? 0x0000ffffu : s == 8 ? 0x00ff00ffu : s == 4 ? 0x0f0f0f0fu : s == 2 ? 0x33333333u : 0x55555555u;
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, s);
+    // The upper lane of a pair takes the other's upper bits into its lower ones, the lower lane the other way.
+    x = lane & s ? (x & ~low) | (y >> s & low) : (x & low) | (y << s & ~low);
+  }
+  return x;
 }
 
 }  // namespace dtk

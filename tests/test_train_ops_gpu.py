@@ -360,6 +360,8 @@ NORM = [
     ((500, 1, 264), BF16, False, "sample", 0.0, True),
     ((700, 3, 64), BF16, True, "sample", 0.2, True),
     ((9, 192, 256), BF16, False, "none", 0.1, True),
+    ((2, 700, 5000), BF16, True, "channel", 0.1, True),  # rows of more than 16 warps, several for each block
+    ((3, 300, 8192), FP16, True, "sample", 0.0, True),
 ]
 
 
