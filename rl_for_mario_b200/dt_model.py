@@ -144,11 +144,17 @@ class DTBlock(nn.Module):
         input_layernorm; returns the stream behind the block and ``next_norm`` of it.  Each residual
         add is one kernel with the dropout before it and the norm behind it."""
         attn, mlp, post = self.self_attn, self.mlp, self.post_attention_layernorm
-        p = mlp.dropout.p if self.training else 0.0
+        p_attn, p_mlp = self.training_rates()
         y = attn.attend_training(n, position_embeddings, pad_len, rng)
-        h, n = training.residual_norm(y, h, post.weight, post.eps, p=p, rng=rng, site=attn.train_site + 1)
+        h, n = training.residual_norm(y, h, post.weight, post.eps, p=p_attn, rng=rng, site=attn.train_site + 1)
         y = mlp.down_proj(F.silu(mlp.gate_proj(n)) * mlp.up_proj(n))
-        return training.residual_norm(y, h, next_norm.weight, next_norm.eps, p=p, rng=rng, site=attn.train_site + 2)
+        return training.residual_norm(y, h, next_norm.weight, next_norm.eps, p=p_mlp, rng=rng,
+                                      site=attn.train_site + 2)
+
+    def training_rates(self) -> Tuple[float, float]:
+        """Dropout rates in force: of the attention (weights and output) and of the MLP's output."""
+        attn, drop = self.self_attn, self.mlp.dropout
+        return attn.dropout if attn.training else 0.0, drop.p if drop.training else 0.0
 
     def forward(self, hidden_states, position_embeddings, past_key_value=None, use_cache=False,
                 attention_mask=None, _owns_input: bool = False):
@@ -404,8 +410,9 @@ class DTBackbone(nn.Module):
         if S > self.freqs_cos.shape[0]:
             raise ValueError(f"{S} positions exceed max_position_embeddings {self.freqs_cos.shape[0]}")
         pe = (self.freqs_cos[:S].float(), self.freqs_sin[:S].float())
-        p = self.dropout.p if self.training else 0.0
-        rng = self.dropout_state().draw() if p > 0 else None
+        p = self.dropout.p if self.dropout.training else 0.0
+        drops = p > 0 or any(max(layer.training_rates()) > 0 for layer in self.layers)
+        rng = self.dropout_state().draw() if drops else None
         first = self.layers[0].input_layernorm if len(self.layers) else self.norm
         h, n = training.residual_norm(tokens, None, first.weight, first.eps, post_weight=self.embed_norm.weight, p=p,
                                       rng=rng, site=0)

@@ -158,6 +158,30 @@ def test_model_step_reaches_every_parameter(dtype):
 
 
 @pytest.mark.gpu
+def test_every_place_drops_at_its_own_rate():
+    """The embedding's, the attention's and the MLP's rate are read apart: with only one of them above zero the
+    result still depends on the generator's step, and with none it does not."""
+    x = torch.randn(2, 24, 128, generator=torch.Generator().manual_seed(2)).half().cuda()
+
+    def twice(model):
+        return [model.model.run_training(x)[0] for _ in range(2)]
+
+    for place in (0, 1, 2, None):
+        model = small_model(torch.float16, 0.0, 128, 4, 2).train().fuse_training(seed=5)
+        if place == 0:
+            model.model.dropout.p = 0.3
+        for layer in model.model.layers:
+            if place == 1:
+                layer.self_attn.dropout = 0.3
+            if place == 2:
+                layer.mlp.dropout.p = 0.3
+        a, b = twice(model)
+        assert torch.equal(a, b) == (place is None)
+        a, b = twice(model.eval())
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_inference_is_left_alone():
     """Without autograd a model gives the same bits with and without fuse_training(); with autograd and no dropout
     the training form agrees with it to bf16 rounding."""
