@@ -148,7 +148,7 @@ int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, 
       (rc = dtk::api_encode_bshd(&m.k_blk, k, bf16, B, S, Hkv, D, k_sb, k_ss, k_sh, 1, 64, "k")) ||
       (rc = dtk::api_encode_bshd(&m.v_blk, v, bf16, B, S, Hkv, D, v_sb, v_ss, v_sh, 1, 64, "v")))
     return rc;
-  return cuda_status(dtk::launch_attn_train_fwd_sm100(a, m, D, bf16, sms, static_cast<cudaStream_t>(stream)), fn);
+  return cuda_status(dtk::launch_attn_train_fwd_sm100(a, m, D, bf16, static_cast<cudaStream_t>(stream)), fn);
 }
 
 int dt_attn_train_backward(const void* dout, const void* q, const void* k, const void* v, const void* o,

@@ -316,7 +316,7 @@ struct AttnTrainMaps {
 int attn_train_splits(int B, int S, int Hkv, int R, int num_sms);
 long long attn_train_words(int B, int S, int Hq, int D);
 cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
-                                        int num_sms, cudaStream_t st);
+                                        cudaStream_t st);
 cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
                                         int num_sms, cudaStream_t st);
 
