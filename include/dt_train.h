@@ -40,12 +40,20 @@ extern "C" {
  * query s of head h of sample b is (b * Hq + h) * S + s, its columns the keys.
  * lse [B, Hq, S] fp32 receives the base-2 logarithm of each row's softmax
  * denominator (+inf for a row without keys), the backward call's input.
+ * workspace: dt_attn_train_forward_workspace bytes, 16-byte aligned.  Values that
+ * are not finite never leave padding; elsewhere they may reach earlier rows of
+ * their block of 64 positions, as a zero weight times them is not a zero.
  */
 int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* pad_len,
                           int B, int S, int Hq, int Hkv, int D, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                           int64_t k_sb, int64_t k_ss, int64_t k_sh, int64_t v_sb, int64_t v_ss, int64_t v_sh,
-                          int64_t o_sb, int64_t o_ss, int64_t o_sh, float scale, double p, const int64_t* rng,
-                          uint32_t site, int dtype, void* stream);
+                          int64_t o_sb, int64_t o_ss, int64_t o_sh, void* workspace, int64_t workspace_bytes,
+                          float scale, double p, const int64_t* rng, uint32_t site, int dtype, void* stream);
+
+/* Bytes of scratch that dt_attn_train_forward needs on the current device: 0 (then
+ * workspace may be null) unless rows are too few for the GPU and the walk over
+ * their keys is cut; negative on an error. */
+int64_t dt_attn_train_forward_workspace(int B, int S, int Hq, int Hkv, int D);
 
 /*
  * Gradient of dt_attn_train_forward: dq [B, S, Hq, D], dk, dv [B, S, Hkv, D]

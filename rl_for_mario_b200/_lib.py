@@ -58,7 +58,8 @@ SIGNATURES = {
     "dt_nes_observe": (_I, [_P, _I, _P, _P, _I, _P]),
     "dt_nes_env_update": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _U, _P, _U, _P]),
     "dt_attn_train_forward": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _L, _L, _L, _L, _L, _L, _L, _L, _L,
-                                   _L, _L, _L, _F, _D, _P, _U, _I, _P]),
+                                   _L, _L, _L, _P, _L, _F, _D, _P, _U, _I, _P]),
+    "dt_attn_train_forward_workspace": (_L, [_I, _I, _I, _I, _I]),
     "dt_attn_train_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P, _F, _D,
                                     _P, _U, _I, _P]),
     "dt_attn_train_workspace": (_L, [_I, _I, _I, _I, _I, _I]),

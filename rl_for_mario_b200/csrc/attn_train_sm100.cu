@@ -113,8 +113,9 @@ struct TcShared {
 // How a kernel's items are numbered: units in groups, inside a group the tiles
 // with the most work first (longest_last: a unit's last tile has the most blocks).
 struct Grid {
-  int units, tiles, items, chunks, splits;  // chunks of a group's heads; CTAs that share a tile of keys
-  FastDiv by_tiles, by_parts, by_kv;        // parts of a unit: chunks (rows) or splits (keys)
+  int units, tiles, items, chunks, splits;  // chunks of a group's heads; CTAs that share a tile
+  int seg;                                  // tiles of rows: key blocks of a split, at most
+  FastDiv by_tiles, by_parts, by_kv;        // parts of a unit: chunks or splits (never both)
 };
 struct TcItem {
   int unit, tile;
@@ -160,10 +161,12 @@ __device__ __forceinline__ int claim_item(TcShared* sh, int n, volatile int* abo
 }
 
 // A tile of query rows: sample b, KV head g, the chunk of HC query heads from h0
-// on, positions p0 .. p0 + PT, and the key blocks kb + 64 j, j < nblk.
+// on, positions p0 .. p0 + PT, and the key blocks kb + 64 j, j < nblk: all of the
+// tile's, or one segment of them.
 struct QTile {
   static constexpr bool kRowTiles = true;
   int b, g, h0, heads, pad, p0, kb, nblk, tile, zero;  // zero: padded keys of the first block
+  int split, all;                                      // the segment; blocks of the whole tile
 };
 // A tile of keys k0 .. k0 + 128 of KV head g and the blocks of PT positions (from
 // q0 on: earlier queries see none of these keys) x chunks of heads behind it.
@@ -171,6 +174,11 @@ struct KTile {
   static constexpr bool kRowTiles = false;
   int b, g, pad, k0, q0, per, nblk, tile, zero, split;  // its blocks are split, split + splits, ...
 };
+
+// Key blocks that the rows before position `end` of a tile see.
+__device__ __forceinline__ int row_blocks(int end, int pad, int S) {
+  return (min(end, S) - 1 - (pad & ~7)) / kBlk + 1;
+}
 
 // The CTA's items: its own, then what it takes.  Taken no earlier than the loading
 // thread needs it, a few blocks before the MMAs do.
@@ -194,7 +202,7 @@ struct Items {
     struct {
       int b, g, part, tile, pad;
     } h;
-    h.part = it.unit - bg * (kRowTiles ? gr.chunks : gr.splits);
+    h.part = it.unit - bg * (gr.chunks > 1 && kRowTiles ? gr.chunks : gr.splits);
     h.b = gr.by_kv(bg);
     h.g = bg - h.b * p.Hkv;
     h.tile = it.tile;
@@ -204,12 +212,15 @@ struct Items {
     t.pad = min(max(h.pad, 0), p.S);
     t.tile = h.tile;
     if constexpr (kRowTiles) {
-      t.h0 = h.g * p.R + h.part * p.HC;
-      t.heads = min(p.HC, p.R - h.part * p.HC);
+      const int chunk = gr.chunks > 1 ? h.part : 0;
+      t.split = gr.chunks > 1 ? 0 : h.part;
+      t.h0 = h.g * p.R + chunk * p.HC;
+      t.heads = min(p.HC, p.R - chunk * p.HC);
       t.p0 = t.pad + h.tile * p.PT128;
-      t.kb = t.pad & ~7;
-      t.nblk = t.p0 < p.S ? (min(t.p0 + p.PT128, p.S) - 1 - t.kb) / kBlk + 1 : 0;
-      t.zero = t.pad - t.kb;
+      t.all = t.p0 < p.S ? row_blocks(t.p0 + p.PT128, t.pad, p.S) : 0;
+      t.kb = (t.pad & ~7) + t.split * gr.seg * kBlk;
+      t.nblk = max(0, min(gr.seg, t.all - t.split * gr.seg));
+      t.zero = t.split == 0 ? t.pad - t.kb : 0;
     } else {
       t.k0 = (t.pad & ~7) + h.tile * kRows;
       t.q0 = max(t.k0, t.pad);
@@ -615,7 +626,7 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
         sh, p, gr,
         [&](const QTile& t, Item& it) {
           it.nblk = t.nblk, it.pad = t.pad, it.heads = t.heads, it.tile = t.tile;
-          it.first = t.p0, it.origin = t.kb;
+          it.first = t.p0, it.origin = t.kb, it.split = t.split, it.per = t.all;
           it.row = ((long long)t.b * p.Hq + t.h0) * S;
           it.out = t.b * p.o_sb + t.h0 * p.o_sh;
         },
@@ -642,9 +653,9 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
     ItemReader items{sh, abort, p.status};
     // The finished tile: its O is read behind the next tile's first exponentials, when its last P V has long been done.
     struct {
-      bool live, valid;
+      bool live, valid, partial;
       long long row;
-      uint16_t* out;
+      void* out;
       float m, l;
     } fin{};
     auto finish = [&]() {
@@ -657,10 +668,17 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->o_empty);
-      if (fin.valid) {
-        const float inv = p.inv_keep / fin.l;
+      if (fin.valid && fin.partial) {
+        float* out = static_cast<float*>(fin.out);
 #pragma unroll
-        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(fin.out + c) = pack8<BF16>(o + c, inv);
+        for (int c = 0; c < D; c += 4)
+          *reinterpret_cast<uint4*>(out + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+        *reinterpret_cast<float2*>(p.part_ml + 2 * fin.row) = make_float2(fin.m, fin.l);
+      } else if (fin.valid) {
+        const float inv = p.inv_keep / fin.l;
+        uint16_t* out = static_cast<uint16_t*>(fin.out);
+#pragma unroll
+        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = pack8<BF16>(o + c, inv);
         p.lse[fin.row] = fin.m + log2f(fin.l);
       }
     };
@@ -674,7 +692,9 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
       uint16_t* out = static_cast<uint16_t*>(p.o) + it->out + head * p.o_sh;
       // This tile's share of the padded rows: zeros, each thread the row of its place.
       const int pz = it->tile * PT + rpos;
-      if (mine && pz < pad) {
+      const int split = it->split;
+      const bool partial = it->per > gr.seg;
+      if (mine && pz < pad && split == 0) {
 #pragma unroll
         for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + pz * p.o_ss + c) = make_uint4(0u, 0u, 0u, 0u);
         p.lse[row - pos + pz] = INFINITY;
@@ -782,8 +802,9 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
       if (nblk > 0) {
         fin.live = true;
         fin.valid = valid;
-        fin.row = row;
-        fin.out = out + pos * p.o_ss;
+        fin.partial = partial;
+        fin.row = partial ? split * ((long long)p.B * p.Hq * S) + row : row;
+        fin.out = partial ? static_cast<void*>(p.part + fin.row * D) : out + pos * p.o_ss;
         fin.m = m;
         fin.l = l;
       }
@@ -820,7 +841,9 @@ struct BwdSmem {
   static_assert(kPerSm * (BYTES + 1024) <= 228 * 1024, "CTAs of an SM share its memory");
 };
 
-template <int D, bool BF16, bool DROP>
+// CUT: tiles may be cut into segments (a form of its own: its registers spill, 250 us
+// instead of 241 for 96 x 768, 12 / 4 heads of 64, where none is cut).
+template <int D, bool BF16, bool DROP, bool CUT>
 __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     attn_train_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                             const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmK,
@@ -871,7 +894,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         sh, p, gr,
         [&](const QTile& t, Item& it) {
           it.nblk = t.nblk, it.pad = t.pad, it.heads = t.heads, it.tile = t.tile;
-          it.first = t.p0, it.origin = t.kb;
+          it.first = t.p0, it.origin = t.kb, it.split = t.split, it.per = t.all;
           it.row = ((long long)t.b * p.Hq + t.h0) * S;
           it.out = t.b * p.dq_sb + t.h0 * p.dq_sh;
         },
@@ -901,8 +924,8 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     bool ok = true;
     ItemReader items{sh, abort, p.status};
     // The finished tile: its dQ is read behind the next tile's first weights.
-    uint16_t* fin_out = nullptr;
-    bool fin = false;
+    void* fin_out = nullptr;
+    bool fin = false, fin_partial = false;
     auto finish = [&]() {
       fin = false;
       uint32_t o[D / 2];
@@ -912,9 +935,16 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->o_empty);
-      if (fin_out)
+      if (CUT && fin_out && fin_partial) {
+        float* out = static_cast<float*>(fin_out);
 #pragma unroll
-        for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(fin_out + c) = pack8<BF16>(o + c, p.scale);
+        for (int c = 0; c < D / 2; c += 4)
+          *reinterpret_cast<uint4*>(out + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+      } else if (fin_out) {
+        uint16_t* out = static_cast<uint16_t*>(fin_out);
+#pragma unroll
+        for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(out + c) = pack8<BF16>(o + c, p.scale);
+      }
     };
     while (true) {
       const Item* it = items.get(ok);
@@ -927,7 +957,8 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       const float ls = valid && pos != pad ? __ldg(p.lse + row) : INFINITY;
       uint16_t* out = static_cast<uint16_t*>(p.dq) + it->out + head * p.dq_sh + half * (D / 2);
       const int pz = it->tile * PT + rpos;
-      if (mine && pz < pad) {
+      const int split = CUT ? it->split : 0, all = CUT ? it->per : nblk;
+      if (mine && pz < pad && split == 0) {
 #pragma unroll
         for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(out + pz * p.dq_ss + c) = make_uint4(0u, 0u, 0u, 0u);
       }
@@ -936,7 +967,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       const unsigned long long row_block = (unsigned long long)row * per_row;
       float delta = 0.f;
       float* xr = xrow + (done & 1) * 2 * kRows;  // the other half may still be read for the previous item
-      if (nblk > 1) {
+      if (nblk > 0 && all > 1) {
         // delta = O . dO: each of the row's two threads takes half of the columns.
         const int tb = done % SH::BWD_TILES;
         if ((ok = warp_wait(&sh->tile_full[tb], (done / SH::BWD_TILES) & 1, abort, p.status))) {
@@ -958,11 +989,11 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         ok = named_bar_and(1, 256, ok);
         if (!ok) break;
         delta = xr[r] + xr[kRows + r];
-        if (half == 0 && valid) p.delta[row] = delta;
+        if (half == 0 && valid && split == 0) p.delta[row] = delta;
       }
       for (int j = 0; j < nblk; ++j, ++blk) {
         if (!(ok = warp_wait(&sh->s_full[0], blk & 1, abort, p.status))) {
-          if (nblk == 1) named_bar_and(1, 256, false);  // the others may wait there
+          if (all == 1) named_bar_and(1, 256, false);  // the others may wait there
           break;
         }
         tc_fence_after();
@@ -973,7 +1004,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         if constexpr (DROP) {
           if (any) {
             drop = drop_word(key, row_block + (unsigned)(k0 >> 3), p.threshold);
-            if (p.words && valid) p.words[(2 * j + half) * all_rows + row] = drop;
+            if (p.words && valid) p.words[((k0 - (pad & ~7)) >> 5) * all_rows + row] = drop;
           }
         }
         // Columns c0 .. c0 + 16: P into w, dP (dropped, not yet scaled by 1 / (1 - p)) into d.
@@ -1003,7 +1034,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
             w[c + 1] = __float_as_uint(ex2_approx(x.y));
           }
         };
-        if (nblk == 1) {
+        if (all == 1) {
           // All keys of these rows are here: delta from the unrounded terms.
           float s = 0.f;
           if (any) {
@@ -1058,7 +1089,11 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       if (nblk > 0) {
         ++done;
         fin = true;
-        fin_out = valid ? out : nullptr;
+        fin_partial = CUT && all > gr.seg;
+        fin_out = !valid ? nullptr
+                  : fin_partial
+                      ? static_cast<void*>(p.part + (split * all_rows + row) * D + half * (D / 2))
+                      : out;
       }
     }
     if (ok && fin && warp_wait(&sh->w_done, (blk - 1) & 1, abort, p.status)) {
@@ -1385,38 +1420,98 @@ __global__ void __launch_bounds__(256) attn_train_sum_kernel(const __grid_consta
   }
 }
 
-Grid make_grid(const AttnTrainParams& p, int units, int tiles, int parts, int splits) {
-  return Grid{units * parts, tiles, units * parts * tiles, (p.R + p.HC - 1) / p.HC, splits, FastDiv((uint32_t)tiles),
-              FastDiv((uint32_t)parts), FastDiv((uint32_t)p.Hkv)};
+// Joins the segments of the tiles of rows that were cut, eight columns of a row a
+// thread, in order.  Forward: O and the sums l to the largest of the segments'
+// references m, then O / l and lse.  dq: the sum.
+template <int D, bool BF16, bool FWD>
+__global__ void __launch_bounds__(256) attn_train_join_kernel(const __grid_constant__ AttnTrainParams p, int seg) {
+  constexpr int NC = D / 8;
+  const long long rows = (long long)p.B * p.Hq * p.S, total = rows * NC;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const int c = (int)(i % NC) * 8;
+    const long long row = i / NC, bh = row / p.S;
+    const int pos = (int)(row - bh * p.S), b = (int)(bh / p.Hq), h = (int)(bh - (long long)b * p.Hq);
+    const int pad = p.pad_len ? min(max(__ldg(p.pad_len + b), 0), p.S) : 0;
+    if (pos < pad) continue;
+    const int all = row_blocks(pad + ((pos - pad) / p.PT128 + 1) * p.PT128, pad, p.S);
+    if (all <= seg) continue;
+    const int n = (all + seg - 1) / seg;
+    float top = -INFINITY, l = 0.f;
+    if constexpr (FWD)
+      for (int q = 0; q < n; ++q) top = fmaxf(top, p.part_ml[2 * (q * rows + row)]);
+    float acc[8] = {};
+    const float* src = p.part + row * D + c;
+    for (int q = 0; q < n; ++q, src += rows * D) {
+      const float4 x = *reinterpret_cast<const float4*>(src), y = *reinterpret_cast<const float4*>(src + 4);
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      float f = 1.f;
+      if constexpr (FWD) {
+        // A segment without a key of this row (all behind it) has m = -inf and zeros.
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (q * rows + row));
+        f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+        l = fmaf(ml.y, f, l);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(v[e], f, acc[e]);
+    }
+    uint32_t s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = __float_as_uint(acc[e]);
+    if constexpr (FWD) {
+      uint16_t* out = static_cast<uint16_t*>(p.o) + b * p.o_sb + (long long)pos * p.o_ss + h * p.o_sh;
+      *reinterpret_cast<uint4*>(out + c) = pack8<BF16>(s, p.inv_keep / l);
+      if (c == 0) p.lse[row] = top + log2f(l);
+    } else {
+      uint16_t* out = static_cast<uint16_t*>(p.dq) + b * p.dq_sb + (long long)pos * p.dq_ss + h * p.dq_sh;
+      *reinterpret_cast<uint4*>(out + c) = pack8<BF16>(s, p.scale);
+    }
+  }
 }
-Grid grid_rows(const AttnTrainParams& p) {
-  return make_grid(p, p.B * p.Hkv, (p.S + p.PT128 - 1) / p.PT128, (p.R + p.HC - 1) / p.HC, 1);
+
+int row_blocks_most(int S) { return (S + 7 + kBlk - 1) / kBlk; }  // of any tile, whatever the padding
+Grid make_grid(const AttnTrainParams& p, int units, int tiles, int parts, int splits, int seg) {
+  return Grid{units * parts, tiles, units * parts * tiles, (p.R + p.HC - 1) / p.HC, splits, seg,
+              FastDiv((uint32_t)tiles), FastDiv((uint32_t)parts), FastDiv((uint32_t)p.Hkv)};
+}
+Grid grid_rows(const AttnTrainParams& p, int num_sms) {
+  const int chunks = (p.R + p.HC - 1) / p.HC, splits = attn_train_row_splits(p.B, p.S, p.Hkv, p.R, num_sms);
+  return make_grid(p, p.B * p.Hkv, (p.S + p.PT128 - 1) / p.PT128, chunks > 1 ? chunks : splits, splits,
+                   (row_blocks_most(p.S) + splits - 1) / splits);
 }
 Grid grid_keys(const AttnTrainParams& p, int splits) {
-  return make_grid(p, p.B * p.Hkv, (p.S + kRows - 1) / kRows, splits, splits);
+  return make_grid(p, p.B * p.Hkv, (p.S + kRows - 1) / kRows, splits, splits, 0);
 }
-template <int D, bool BF16, bool DROP>
-cudaError_t run_fwd(const AttnTrainParams& p, const AttnTrainMaps& m, cudaStream_t st) {
-  auto kern = attn_train_fwd_tc_kernel<D, BF16, DROP>;
-  const cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kern), FwdSmem<D>::BYTES);
-  if (e != cudaSuccess) return e;
-  const Grid gr = grid_rows(p);
-  kern<<<(unsigned)gr.items, kFwdThreads, FwdSmem<D>::BYTES, st>>>(m.q_tile, m.k_blk, m.v_blk, p,
-                                                                                          gr);
+template <int D, bool BF16, bool FWD>
+cudaError_t join(const AttnTrainParams& p, const Grid& gr, int num_sms, cudaStream_t st) {
+  if (gr.splits == 1) return cudaSuccess;
+  const long long blocks = ((long long)p.B * p.Hq * p.S * (D / 8) + 255) / 256;
+  attn_train_join_kernel<D, BF16, FWD><<<(unsigned)(blocks < num_sms * 16 ? blocks : num_sms * 16), 256, 0, st>>>(p, gr.seg);
   return cudaGetLastError();
 }
 template <int D, bool BF16, bool DROP>
+cudaError_t run_fwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sms, cudaStream_t st) {
+  auto kern = attn_train_fwd_tc_kernel<D, BF16, DROP>;
+  cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kern), FwdSmem<D>::BYTES);
+  if (e != cudaSuccess) return e;
+  const Grid gr = grid_rows(p, num_sms);
+  kern<<<(unsigned)gr.items, kFwdThreads, FwdSmem<D>::BYTES, st>>>(m.q_tile, m.k_blk, m.v_blk, p, gr);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return join<D, BF16, true>(p, gr, num_sms, st);
+}
+template <int D, bool BF16, bool DROP>
 cudaError_t run_bwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sms, cudaStream_t st) {
-  auto kq = attn_train_dq_tc_kernel<D, BF16, DROP>;
+  const Grid gq = grid_rows(p, num_sms);
+  auto kq = gq.splits > 1 ? attn_train_dq_tc_kernel<D, BF16, DROP, true> : attn_train_dq_tc_kernel<D, BF16, DROP, false>;
   auto kk = DROP && p.words ? attn_train_dkv_tc_kernel<D, BF16, DROP, DROP> : attn_train_dkv_tc_kernel<D, BF16, DROP, false>;
   cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kq), BwdSmem<D, true>::BYTES);
   if (e != cudaSuccess) return e;
   if ((e = smem_limit_once(reinterpret_cast<const void*>(kk), BwdSmem<D, false>::BYTES)) != cudaSuccess) return e;
   const int splits = attn_train_splits(p.B, p.S, p.Hkv, p.R, num_sms);
-  const Grid gq = grid_rows(p), gk = grid_keys(p, splits);
+  const Grid gk = grid_keys(p, splits);
   kq<<<(unsigned)gq.items, kBwdThreads, BwdSmem<D, true>::BYTES, st>>>(m.q_tile, m.do_tile, m.o_tile, m.k_blk,
                                                                               m.v_blk, p, gq);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if ((e = join<D, BF16, false>(p, gq, num_sms, st)) != cudaSuccess) return e;
   kk<<<(unsigned)gk.items, kBwdThreads, BwdSmem<D, false>::BYTES, st>>>(m.k_tile, m.v_tile, m.q_blk, m.do_blk, p, gk);
   if ((e = cudaGetLastError()) != cudaSuccess || splits == 1) return e;
   const long long blocks = ((long long)p.B * p.Hkv * p.S * 2 * (D / 8) + 255) / 256;
@@ -1429,14 +1524,26 @@ cudaError_t run_bwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sm
 // CTAs that share the query rows behind one tile of keys.  The first tile of a
 // causal unit has twice the average's rows, so that a few tiles are cut until there
 // are about two items for each CTA of the GPU, with eight blocks or more for each
-// (B 2, S 4000, 8 / 2 heads of 32, 128 tiles for 296 CTAs: 164 us cut in two, 95 us
-// in four, 102 in nine; B 64, S 192, twelve blocks in the longest of 256 tiles:
-// 25 us whole, 36 us with the sum cut in two).
+// (B 2, S 4000, 8 / 2 heads of 32, 128 tiles for 296 CTAs: 166 us cut in two, 120 us
+// in three, 97 us in four and in six; B 64, S 192, twelve blocks in the longest of 256
+// tiles: 24 us whole, 29 us with the sum cut in two).
 int attn_train_splits(int B, int S, int Hkv, int R, int num_sms) {
   if (R > 64) return 1;  // chunks of heads: not split
   const long long items = (long long)B * Hkv * ((S + kRows - 1) / kRows);
   const int pt = kBlk / R, blocks = (S + pt - 1) / pt;
   long long n = 2LL * kPerSm * num_sms / items;
+  if (n > blocks / 8) n = blocks / 8;
+  return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+}
+
+// Segments of the longest tile of query rows' key blocks, each its own item: the same
+// rule for the walk over keys.
+int attn_train_row_splits(int B, int S, int Hkv, int R, int num_sms) {
+  if (R > 64) return 1;
+  const int pt = kRows / R;
+  const long long items = (long long)B * Hkv * ((S + pt - 1) / pt);
+  long long n = 2LL * kPerSm * num_sms / items;
+  const int blocks = row_blocks_most(S);
   if (n > blocks / 8) n = blocks / 8;
   return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
 }
@@ -1449,13 +1556,13 @@ long long attn_train_words(int B, int S, int Hq, int D) {
 }
 
 cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
-                                        cudaStream_t st) {
+                                        int num_sms, cudaStream_t st) {
   const bool drop = p.threshold != 0;
   if (D == 32)
-    return bf16 ? (drop ? run_fwd<32, true, true>(p, m, st) : run_fwd<32, true, false>(p, m, st))
-                : (drop ? run_fwd<32, false, true>(p, m, st) : run_fwd<32, false, false>(p, m, st));
-  return bf16 ? (drop ? run_fwd<64, true, true>(p, m, st) : run_fwd<64, true, false>(p, m, st))
-              : (drop ? run_fwd<64, false, true>(p, m, st) : run_fwd<64, false, false>(p, m, st));
+    return bf16 ? (drop ? run_fwd<32, true, true>(p, m, num_sms, st) : run_fwd<32, true, false>(p, m, num_sms, st))
+                : (drop ? run_fwd<32, false, true>(p, m, num_sms, st) : run_fwd<32, false, false>(p, m, num_sms, st));
+  return bf16 ? (drop ? run_fwd<64, true, true>(p, m, num_sms, st) : run_fwd<64, true, false>(p, m, num_sms, st))
+              : (drop ? run_fwd<64, false, true>(p, m, num_sms, st) : run_fwd<64, false, false>(p, m, num_sms, st));
 }
 
 cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,

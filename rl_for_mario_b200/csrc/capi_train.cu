@@ -93,9 +93,17 @@ int check_elem_aligned(const char* fn, int dtype, std::initializer_list<const vo
 
 // The backward pass's scratch: delta, then the partial sums of split tiles of keys, then the drop flags.
 int64_t delta_elems(int B, int S, int Hq) { return ((int64_t)B * Hq * S + 3) / 4 * 4; }
-int64_t attn_part_elems(int B, int S, int Hq, int Hkv, int D, int sms) {
+int64_t attn_row_part_elems(int B, int S, int Hq, int Hkv, int D, int sms) {
+  const int n = dtk::attn_train_row_splits(B, S, Hkv, Hq / Hkv, sms);
+  return n > 1 ? (int64_t)n * B * Hq * S * D : 0;
+}
+int64_t attn_part_elems(int B, int S, int Hq, int Hkv, int D, int sms) {  // dq's are read before dk's and dv's come
   const int n = dtk::attn_train_splits(B, S, Hkv, Hq / Hkv, sms);
-  return n > 1 ? (int64_t)n * 2 * B * Hkv * S * D : 0;
+  const int64_t keys = n > 1 ? (int64_t)n * 2 * B * Hkv * S * D : 0, rows = attn_row_part_elems(B, S, Hq, Hkv, D, sms);
+  return keys > rows ? keys : rows;
+}
+int64_t attn_forward_workspace(int B, int S, int Hq, int Hkv, int D, int sms) {
+  return attn_row_part_elems(B, S, Hq, Hkv, D, sms) / D * (D + 2) * 4;
 }
 int64_t attn_workspace(int B, int S, int Hq, int Hkv, int D, bool drop, int sms) {
   return 4 * (delta_elems(B, S, Hq) + attn_part_elems(B, S, Hq, Hkv, D, sms) +
@@ -119,8 +127,8 @@ extern "C" {
 int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* pad_len,
                           int B, int S, int Hq, int Hkv, int D, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                           int64_t k_sb, int64_t k_ss, int64_t k_sh, int64_t v_sb, int64_t v_ss, int64_t v_sh,
-                          int64_t o_sb, int64_t o_ss, int64_t o_sh, float scale, double p, const int64_t* rng,
-                          uint32_t site, int dtype, void* stream) {
+                          int64_t o_sb, int64_t o_ss, int64_t o_sh, void* workspace, int64_t workspace_bytes,
+                          float scale, double p, const int64_t* rng, uint32_t site, int dtype, void* stream) {
   const char* fn = "dt_attn_train_forward";
   Range range(fn);
   if (!q || !k || !v || !o || !lse) return api_fail(DT_ERR_INVALID, "%s: null q/k/v/o/lse pointer", fn);
@@ -133,6 +141,12 @@ int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, 
   if ((rc = rate(fn, p, rng, &a.threshold, &a.inv_keep))) return rc;
   int sms = 0;
   if ((rc = need_sm100(fn, &sms, &a.status))) return rc;
+  const int64_t need = attn_forward_workspace(B, S, Hq, Hkv, D, sms);
+  if (need && (workspace_bytes < need || !workspace || !aligned16(workspace)))
+    return api_fail(DT_ERR_INVALID, "%s: workspace of %lld bytes is too small, null or not 16-byte aligned", fn,
+                    (long long)workspace_bytes);
+  a.part = static_cast<float*>(workspace);
+  a.part_ml = a.part + attn_row_part_elems(B, S, Hq, Hkv, D, sms);
   a.q = q, a.k = k, a.v = v, a.o = o, a.lse = lse, a.pad_len = pad_len;
   a.q_sb = q_sb, a.q_ss = q_ss, a.q_sh = q_sh, a.k_sb = k_sb, a.k_ss = k_ss, a.k_sh = k_sh;
   a.v_sb = v_sb, a.v_ss = v_ss, a.v_sh = v_sh, a.o_sb = o_sb, a.o_ss = o_ss, a.o_sh = o_sh;
@@ -148,7 +162,7 @@ int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, 
       (rc = dtk::api_encode_bshd(&m.k_blk, k, bf16, B, S, Hkv, D, k_sb, k_ss, k_sh, 1, 64, "k")) ||
       (rc = dtk::api_encode_bshd(&m.v_blk, v, bf16, B, S, Hkv, D, v_sb, v_ss, v_sh, 1, 64, "v")))
     return rc;
-  return cuda_status(dtk::launch_attn_train_fwd_sm100(a, m, D, bf16, static_cast<cudaStream_t>(stream)), fn);
+  return cuda_status(dtk::launch_attn_train_fwd_sm100(a, m, D, bf16, sms, static_cast<cudaStream_t>(stream)), fn);
 }
 
 int dt_attn_train_backward(const void* dout, const void* q, const void* k, const void* v, const void* o,
@@ -201,6 +215,15 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
       (rc = dtk::api_encode_bshd(&m.v_blk, v, bf16, B, S, Hkv, D, a.v_sb, a.v_ss, a.v_sh, 1, 64, "v")))
     return rc;
   return cuda_status(dtk::launch_attn_train_bwd_sm100(a, m, D, bf16, sms, static_cast<cudaStream_t>(stream)), fn);
+}
+
+int64_t dt_attn_train_forward_workspace(int B, int S, int Hq, int Hkv, int D) {
+  const char* fn = "dt_attn_train_forward_workspace";
+  const int64_t s[3] = {8, 8, 8};
+  int rc = check_attn(fn, B, S, Hq, Hkv, D, s, 3, DT_DTYPE_BF16);
+  int sms = 0;
+  if (rc || (rc = need_sm100(fn, &sms))) return -rc;
+  return attn_forward_workspace(B, S, Hq, Hkv, D, sms);
 }
 
 int64_t dt_attn_train_workspace(int B, int S, int Hq, int Hkv, int D, int has_dropout) {

@@ -291,7 +291,10 @@ struct AttnTrainParams {
   void* dk;
   void* dv;
   float* delta;            // [B, Hq, S]
-  float* part;             // [splits, 2 (dv, dk), B, Hkv, S, D] partial sums when a tile of keys is split
+  // Partial sums of split tiles: [splits, B, Hq, S, D] of O (unnormalised) or dq, with part_ml
+  // [splits, B, Hq, S, 2] the forward pass's reference maximum and sum, or [splits, 2 (dv, dk), B, Hkv, S, D].
+  float* part;
+  float* part_ml;
   // Drop flags from the dq kernel for the dk, dv kernel: [groups of 32 keys, from the first
   // unpadded position rounded down to 8] x [B, Hq, S] words, or null: generated again.
   uint32_t* words;
@@ -313,10 +316,11 @@ struct AttnTrainParams {
 struct AttnTrainMaps {
   CUtensorMap q_tile, do_tile, o_tile, q_blk, do_blk, k_tile, v_tile, k_blk, v_blk;
 };
-int attn_train_splits(int B, int S, int Hkv, int R, int num_sms);
+int attn_train_splits(int B, int S, int Hkv, int R, int num_sms);      // of a tile of keys
+int attn_train_row_splits(int B, int S, int Hkv, int R, int num_sms);  // of a tile of query rows
 long long attn_train_words(int B, int S, int Hq, int D);
 cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
-                                        cudaStream_t st);
+                                        int num_sms, cudaStream_t st);
 cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
                                         int num_sms, cudaStream_t st);
 

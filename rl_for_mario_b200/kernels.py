@@ -628,9 +628,11 @@ def attn_train_forward(q: Tensor, k: Tensor, v: Tensor, pad_len: Optional[Tensor
     out = _empty_as(q)
     lse = torch.empty(B, Hq, S, dtype=torch.float32, device=dev)
     if out.numel():
+        size = _workspace("dt_attn_train_forward_workspace", dev.index, B, S, Hq, Hkv, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         _launch("dt_attn_train_forward", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                _ptr(pad_len), B, S, Hq, Hkv, D, *qs, *ks, *vs, S * Hq * D, Hq * D, D, scale or 0.0, p, _ptr(rng), site,
-                _dtype_code(q))
+                _ptr(pad_len), B, S, Hq, Hkv, D, *qs, *ks, *vs, S * Hq * D, Hq * D, D, _ptr(ws), size,
+                scale or 0.0, p, _ptr(rng), site, _dtype_code(q))
     return out, lse
 
 

@@ -14,7 +14,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     s12, a = [256, 64, 64] * 4, 4096  # any aligned non-null address: nothing is read before the device check
 
     def fwd(q=a, S=8, Hq=4, Hkv=2, D=32, strides=s12, p=0.0, rng=None, dtype=0, B=1):
-        return lib.dt_attn_train_forward(q, a, a, a, a, None, B, S, Hq, Hkv, D, *strides, 0.0, p, rng, 0, dtype, None)
+        return lib.dt_attn_train_forward(q, a, a, a, a, None, B, S, Hq, Hkv, D, *strides, None, 0, 0.0, p, rng, 0, dtype, None)
 
     cases = [(dict(q=None), "null", _lib.DT_ERR_INVALID), (dict(S=0), "positive", _lib.DT_ERR_INVALID),
              (dict(Hkv=3), "divisible", _lib.DT_ERR_INVALID), (dict(D=48), "head_dim", _lib.DT_ERR_UNSUPPORTED),

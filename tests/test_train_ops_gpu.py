@@ -116,6 +116,12 @@ ATTN = [
     (40, 130, 6, 2, 64, "each", FP16, 0.2),
     (1, 2048, 2, 1, 32, [9], BF16, 0.1),  # 64 positions for each of D: the longest whose drop flags are kept
     (1, 2055, 2, 1, 32, [9], BF16, 0.1),
+    # Few rows, long walks over the keys, cut into segments: tiles of one segment and of several, padding that
+    # leaves fewer of them, packed heads, a row whose last segment lies behind it.
+    (1, 1500, 1, 1, 64, None, FP16, 0.2),
+    (3, 1100, 3, 1, 64, [0, 517, 1099], BF16, 0.0),
+    (2, 2300, 2, 2, 32, [1203, 3], BF16, 0.1),
+    (1, 1030, 8, 2, 64, [6], FP16, 0.1),
 ]
 
 
