@@ -13,8 +13,10 @@
 // Two backward kernels: one walks the keys of a tile of query rows (delta, dq),
 // one walks the query rows behind a tile of keys (dk, dv).  Each sum has one
 // owner: no atomics, the same bits every run; the price is that S and dP are
-// formed twice.  When the tiles of keys are too few for the GPU, the rows behind
-// each are dealt out to several CTAs whose fp32 sums a third kernel adds in order.
+// formed twice.  When the tiles are too few for the GPU, the other axis of each is
+// dealt out to several CTAs, whose fp32 sums a further kernel joins in order.  The
+// dropout mask of a block is generated by the dq kernel, which hands it on as bits
+// (for contexts up to 64 positions for each of D; beyond, both generate it).
 //
 // Rounding: P and dS enter the second products in the inputs' 16-bit type, as
 // the tensor cores take both operands in one type; sums, softmax statistics
@@ -31,7 +33,8 @@
 // keys of a first block are zeroed in shared memory, so what stands there never
 // meets a product (a NaN times a zero weight would be a NaN).
 //
-// Persistent CTAs, two on each SM.  One thread loads tiles and blocks by TMA, one
+// Two CTAs on each SM, which take tile after tile until the launch has none left
+// (claim_item).  One thread loads tiles and blocks by TMA, one
 // issues the MMAs; the other warps are the element-wise part, one thread per row
 // (forward) or two (backward).  Per block of 64:
 //   forward   S = Q K^T             P -> TMEM, O += P V
@@ -48,10 +51,18 @@
 // what lets a block's scores be issued behind the products that still read the
 // previous block's weights in the same columns.
 //
-// What bounds it: an MMA of N = 64 costs about 50 cycles whatever its K, so at
-// head_dim 64 a 128 x 64 block takes 400 (forward), 600 (dq) and 800 (dk, dv)
-// tensor cycles, about as long as its element-wise part (one exponential, and
-// with dropout an eighth of a generator call, for each score).
+// What bounds it.  96 x 768, 12 / 4 heads of 64, padding up to half, bf16, p = 0.1:
+// forward 215 us, dq 241, dk and dv 272 (0.18 PFLOP of products that count: 245
+// TFLOP/s); half that batch without dropout 81, 93 and 132 us, with it 120, 136 and
+// 164.  No unit is full: the tensor pipe is busy 20 to 26 % of the time without
+// dropout (an MMA of N = 64 costs about 50 cycles whatever its K: 400, 600 and 800 for
+// a 128 x 64 block), the exponentials' unit 22 to 39 %, and 41 to 46 % of the issue
+// slots are used (with dropout 50 to 58 %: a generator call is 65 instructions for
+// eight scores).  A block is a chain from the scores over tensor memory, the
+// exponentials, tensor memory again and the next product, and two CTAs on an SM (four
+// warps a scheduler in the backward kernels) cover each other's waits only in part.
+// Four forward CTAs with a quarter of the columns each, the weights over the scores,
+// were slower (307 us): their scores wait for the product before.
 #include <utility>
 
 #include "dt_common.cuh"
@@ -580,7 +591,9 @@ struct FwdSmem {
   static_assert(kPerSm * (BYTES + 1024) <= 228 * 1024, "CTAs of an SM share its memory");
 };
 
-template <int D, bool BF16, bool DROP>
+// CUT: tiles may be cut into segments (a form of its own, as for dq: 199 us instead of
+// 187 for 2,048 x 192, 8 / 2 heads of 32, where none is cut).
+template <int D, bool BF16, bool DROP, bool CUT>
 __global__ void __launch_bounds__(kFwdThreads, kPerSm)
     attn_train_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                              const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnTrainParams p,
@@ -668,7 +681,7 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->o_empty);
-      if (fin.valid && fin.partial) {
+      if (CUT && fin.valid && fin.partial) {
         float* out = static_cast<float*>(fin.out);
 #pragma unroll
         for (int c = 0; c < D; c += 4)
@@ -692,8 +705,8 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
       uint16_t* out = static_cast<uint16_t*>(p.o) + it->out + head * p.o_sh;
       // This tile's share of the padded rows: zeros, each thread the row of its place.
       const int pz = it->tile * PT + rpos;
-      const int split = it->split;
-      const bool partial = it->per > gr.seg;
+      const int split = CUT ? it->split : 0;
+      const bool partial = CUT && it->per > gr.seg;
       if (mine && pz < pad && split == 0) {
 #pragma unroll
         for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + pz * p.o_ss + c) = make_uint4(0u, 0u, 0u, 0u);
@@ -841,7 +854,7 @@ struct BwdSmem {
   static_assert(kPerSm * (BYTES + 1024) <= 228 * 1024, "CTAs of an SM share its memory");
 };
 
-// CUT: tiles may be cut into segments (a form of its own: its registers spill, 250 us
+// CUT: tiles may be cut into segments (its registers spill: 250 us
 // instead of 241 for 96 x 768, 12 / 4 heads of 64, where none is cut).
 template <int D, bool BF16, bool DROP, bool CUT>
 __global__ void __launch_bounds__(kBwdThreads, kPerSm)
@@ -1490,10 +1503,10 @@ cudaError_t join(const AttnTrainParams& p, const Grid& gr, int num_sms, cudaStre
 }
 template <int D, bool BF16, bool DROP>
 cudaError_t run_fwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sms, cudaStream_t st) {
-  auto kern = attn_train_fwd_tc_kernel<D, BF16, DROP>;
+  const Grid gr = grid_rows(p, num_sms);
+  auto kern = gr.splits > 1 ? attn_train_fwd_tc_kernel<D, BF16, DROP, true> : attn_train_fwd_tc_kernel<D, BF16, DROP, false>;
   cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kern), FwdSmem<D>::BYTES);
   if (e != cudaSuccess) return e;
-  const Grid gr = grid_rows(p, num_sms);
   kern<<<(unsigned)gr.items, kFwdThreads, FwdSmem<D>::BYTES, st>>>(m.q_tile, m.k_blk, m.v_blk, p, gr);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   return join<D, BF16, true>(p, gr, num_sms, st);

@@ -3,7 +3,8 @@
 //   y0 = x0 cos[d] - x1 sin[d],  y1 = x1 cos[d'] + x0 sin[d'],  d' = d + D / 2,
 // so  dx0 = dy0 cos[d] + dy1 sin[d'],  dx1 = dy1 cos[d'] - dy0 sin[d].
 // One thread takes eight d of one head of one row, 16-byte accesses; bound by
-// HBM (2 bytes read and written per element).  fp32 arithmetic, one rounding.
+// HBM (2 bytes read and written per element; 96 x 768 rows, 16 heads of 64, 302 MB:
+// 53 us = 5.7 TB/s; the tables stay in L1 and L2).  fp32 arithmetic, one rounding.
 #include "dt_common.cuh"
 #include "dt_internal.h"
 
