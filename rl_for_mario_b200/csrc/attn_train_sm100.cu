@@ -125,7 +125,7 @@ struct TcShared {
 // with the most work first (longest_last: a unit's last tile has the most blocks).
 struct Grid {
   int units, tiles, items, chunks, splits;  // chunks of a group's heads; CTAs that share a tile
-  int seg;                                  // tiles of rows: key blocks of a split, at most
+  int seg;                                  // tiles of rows: key blocks of a segment
   FastDiv by_tiles, by_parts, by_kv;        // parts of a unit: chunks or splits (never both)
 };
 struct TcItem {
@@ -191,6 +191,12 @@ __device__ __forceinline__ int row_blocks(int end, int pad, int S) {
   return (min(end, S) - 1 - (pad & ~7)) / kBlk + 1;
 }
 
+// Segments of seg blocks that a tile of `all` blocks is cut into.  A last one of a single
+// block goes to the one before: the dq threads read the tile's dO and O before a
+// segment's first scores, and only its second block's scores wait for them, so the last
+// scores of a segment of one would give the tile's buffer back too early.
+__host__ __device__ __forceinline__ int segments(int all, int seg) { return all <= seg + 1 ? 1 : (all + seg - 2) / seg; }
+
 // The CTA's items: its own, then what it takes.  Taken no earlier than the loading
 // thread needs it, a few blocks before the MMAs do.
 template <class T>
@@ -230,7 +236,8 @@ struct Items {
       t.p0 = t.pad + h.tile * p.PT128;
       t.all = t.p0 < p.S ? row_blocks(t.p0 + p.PT128, t.pad, p.S) : 0;
       t.kb = (t.pad & ~7) + t.split * gr.seg * kBlk;
-      t.nblk = max(0, min(gr.seg, t.all - t.split * gr.seg));
+      const int n = segments(t.all, gr.seg);
+      t.nblk = t.split >= n ? 0 : t.split == n - 1 ? t.all - t.split * gr.seg : gr.seg;
       t.zero = t.split == 0 ? t.pad - t.kb : 0;
     } else {
       t.k0 = (t.pad & ~7) + h.tile * kRows;
@@ -706,7 +713,7 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
       // This tile's share of the padded rows: zeros, each thread the row of its place.
       const int pz = it->tile * PT + rpos;
       const int split = CUT ? it->split : 0;
-      const bool partial = CUT && it->per > gr.seg;
+      const bool partial = CUT && segments(it->per, gr.seg) > 1;
       if (mine && pz < pad && split == 0) {
 #pragma unroll
         for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + pz * p.o_ss + c) = make_uint4(0u, 0u, 0u, 0u);
@@ -1102,7 +1109,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       if (nblk > 0) {
         ++done;
         fin = true;
-        fin_partial = CUT && all > gr.seg;
+        fin_partial = CUT && segments(all, gr.seg) > 1;
         fin_out = !valid ? nullptr
                   : fin_partial
                       ? static_cast<void*>(p.part + (split * all_rows + row) * D + half * (D / 2))
@@ -1447,8 +1454,8 @@ __global__ void __launch_bounds__(256) attn_train_join_kernel(const __grid_const
     const int pad = p.pad_len ? min(max(__ldg(p.pad_len + b), 0), p.S) : 0;
     if (pos < pad) continue;
     const int all = row_blocks(pad + ((pos - pad) / p.PT128 + 1) * p.PT128, pad, p.S);
-    if (all <= seg) continue;
-    const int n = (all + seg - 1) / seg;
+    const int n = segments(all, seg);
+    if (n == 1) continue;
     float top = -INFINITY, l = 0.f;
     if constexpr (FWD)
       for (int q = 0; q < n; ++q) top = fmaxf(top, p.part_ml[2 * (q * rows + row)]);
@@ -1538,13 +1545,14 @@ cudaError_t run_bwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sm
 // causal unit has twice the average's rows, so that a few tiles are cut until there
 // are about two items for each CTA of the GPU, with eight blocks or more for each
 // (B 2, S 4000, 8 / 2 heads of 32, 128 tiles for 296 CTAs: 166 us cut in two, 120 us
-// in three, 97 us in four and in six; B 64, S 192, twelve blocks in the longest of 256
+// in three, 97 us in four and in six; B 7, S 1305, 16 / 4 heads of 32, 308 tiles: 130 us
+// whole, 76 in two and 5 for the sum; B 64, S 192, twelve blocks in the longest of 256
 // tiles: 24 us whole, 29 us with the sum cut in two).
 int attn_train_splits(int B, int S, int Hkv, int R, int num_sms) {
   if (R > 64) return 1;  // chunks of heads: not split
   const long long items = (long long)B * Hkv * ((S + kRows - 1) / kRows);
   const int pt = kBlk / R, blocks = (S + pt - 1) / pt;
-  long long n = 2LL * kPerSm * num_sms / items;
+  long long n = (2LL * kPerSm * num_sms + items / 2) / items;
   if (n > blocks / 8) n = blocks / 8;
   return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
 }

@@ -122,6 +122,8 @@ ATTN = [
     (3, 1100, 3, 1, 64, [0, 517, 1099], BF16, 0.0),
     (2, 2300, 2, 2, 32, [1203, 3], BF16, 0.1),
     (1, 1030, 8, 2, 64, [6], FP16, 0.1),
+    (1, 1500, 12, 12, 64, [9], BF16, 0.1),  # tiles of 9 and 17 blocks in segments of 8: a single block is left over
+    (1, 1500, 12, 12, 32, [9], FP16, 0.0),
 ]
 
 
