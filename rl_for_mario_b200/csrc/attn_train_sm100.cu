@@ -1019,7 +1019,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         tc_fence_after();
         const int k0 = kb + j * kBlk + 32 * half;
         const int see = valid ? pos - k0 + 1 : 32, lo = j == 0 && half == 0 ? pad - kb : 0;
-        const bool any = __any_sync(0xffffffffu, see > 0), edge = __any_sync(0xffffffffu, see < 32);
+        const bool any = __any_sync(0xffffffffu, valid && see > 0), edge = __any_sync(0xffffffffu, see < 32);
         uint32_t drop = 0;
         if constexpr (DROP) {
           if (any) {
@@ -1212,7 +1212,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     float* x_nd = reinterpret_cast<float*>(smem + SM::OFF_X + 1024) + warp * 32;          // -delta
     int* x_pos = reinterpret_cast<int*>(smem + SM::OFF_X + 2048) + warp * 32;
     const int col = 32 * half + lane, chead = col % p.HC, cpos = col / p.HC;
-    const int last_pos = min(32 * half + 31, rows - 1) / p.HC;
+    const int first_pos = 32 * half / p.HC, last_pos = min(32 * half + 31, rows - 1) / p.HC;
     int blk = 0, done = 0;
     bool ok = true;
     ItemReader items{sh, abort, p.status};
@@ -1280,8 +1280,9 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       for (int j = 0; j < nblk; ++j, ++blk) {
         const int pos = npos, q0 = pos - cpos;
         const long long row = nrow;
-        // The warp's last position against its first key: nothing to do where every query comes before every key.
-        const bool any = q0 + last_pos >= key0;
+        // The warp's last position against its first key: nothing to do where every query comes before every key
+        // (or where the warp has no query or no key).
+        const bool any = q0 + last_pos >= key0 && key0 < S && q0 + first_pos < S;
         uint32_t drop = nw;
         if constexpr (DROP && !WORDS) {
           if (any) drop = drop_word(key, (unsigned long long)row * per_row + (unsigned)(key0 >> 3), p.threshold);

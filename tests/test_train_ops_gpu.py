@@ -241,6 +241,67 @@ def test_attention_gradient_against_differences():
 
 
 @pytest.mark.gpu
+def test_attention_scratch_is_checked_on_the_host():
+    """A shape whose walks over keys are cut needs scratch in both directions: too little, none or a misaligned
+    one is refused before anything is launched, and a shape that needs none takes a null pointer."""
+    from rl_for_mario_b200 import _lib
+
+    lib = _lib.load()
+    S, D = 1500, 64
+    t = torch.zeros(1, S, 1, D, dtype=BF16, device="cuda")
+    lse = torch.zeros(1, 1, S, device="cuda")
+    need = lib.dt_attn_train_forward_workspace(1, S, 1, 1, D)
+    assert need > 0 and lib.dt_attn_train_forward_workspace(64, 192, 8, 2, 32) == 0
+    ws = torch.zeros(need + 16, dtype=torch.uint8, device="cuda")
+    out = torch.zeros_like(t)
+
+    def forward(pointer, size):
+        q = t.data_ptr()
+        return lib.dt_attn_train_forward(q, q, q, out.data_ptr(), lse.data_ptr(), None, 1, S, 1, 1, D,
+                                         *(S * D, D, D) * 4, pointer, size, 0.0, 0.0, None, 0, 0, None)
+
+    assert forward(None, need) != 0 and forward(ws.data_ptr(), need - 4) != 0 and forward(ws.data_ptr() + 4, need) != 0
+    assert forward(ws.data_ptr(), need) == 0
+    plain, drop = (lib.dt_attn_train_workspace(1, S, 1, 1, D, has) for has in (0, 1))
+    assert 0 < plain < drop
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_cut_attention_on_two_streams_and_in_a_graph():
+    """Calls whose walks are cut, at once on two streams and replayed from a graph: each has scratch of its own."""
+    _, _, dev, ddev = attn_inputs(1, 1500, 2, 2, 64, BF16, seed=21)
+    _, _, dev2, ddev2 = attn_inputs(2, 1100, 3, 1, 64, BF16, seed=22)
+    want = attn_run(dev, ddev, [9], 0.1, (3, 4, 5))[0]
+    want2 = attn_run(dev2, ddev2, [0, 77], 0.0)[0]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    runs = []
+    for _ in range(3):
+        with torch.cuda.stream(streams[0]):
+            a = attn_run(dev, ddev, [9], 0.1, (3, 4, 5))[0]
+        with torch.cuda.stream(streams[1]):
+            b = attn_run(dev2, ddev2, [0, 77], 0.0)[0]
+        runs.append((a, b))
+    torch.cuda.synchronize()
+    for a, b in runs:
+        assert all(torch.equal(x, y) for x, y in zip(want, a)) and all(torch.equal(x, y) for x, y in zip(want2, b))
+
+    from rl_for_mario_b200 import kernels
+
+    pad, rng = torch.tensor([9], dtype=torch.int32, device="cuda"), make_rng(3, 4)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = kernels.attn_train_forward(*dev, pad, p=0.1, rng=rng, site=5)
+        grads = kernels.attn_train_backward(ddev, *dev, out, lse, pad, p=0.1, rng=rng, site=5)
+    for t in (out, lse, *grads):
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(want, (out, *grads)))
+
+
+@pytest.mark.gpu
 def test_attention_two_streams_and_a_captured_graph():
     from rl_for_mario_b200 import kernels
 
