@@ -52,7 +52,7 @@
 // previous block's weights in the same columns.
 //
 // What bounds it.  96 x 768, 12 / 4 heads of 64, padding up to half, bf16, p = 0.1:
-// forward 215 us, dq 241, dk and dv 272 (0.18 PFLOP of products that count: 245
+// forward 215 us, dq 240, dk and dv 268 (0.18 PFLOP of products that count: 246
 // TFLOP/s); half that batch without dropout 81, 93 and 132 us, with it 120, 136 and
 // 164.  No unit is full: the tensor pipe is busy 20 to 26 % of the time without
 // dropout (an MMA of N = 64 costs about 50 cycles whatever its K: 400, 600 and 800 for
