@@ -179,11 +179,11 @@ class FastDTAttention(nn.Module):
         return self
 
     def dropout_state(self) -> "training.DropoutState":
-        """The module's own generator (made on its device when first asked for)."""
+        """The module's own generator (made when first asked for; it moves with the module)."""
         dev = self.q_proj.weight.device
-        if self._dropout_state is None or self._dropout_state.state.device != dev:
+        if self._dropout_state is None:
             object.__setattr__(self, "_dropout_state", training.DropoutState(self.train_seed, dev))
-        return self._dropout_state
+        return self._dropout_state.to(dev)
 
     def attend_training(self, x: Tensor, position_embeddings: Tuple[Tensor, Tensor], pad_len: Optional[Tensor],
                         rng: Optional[Tensor]) -> Tensor:

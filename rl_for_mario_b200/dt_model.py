@@ -396,11 +396,11 @@ class DTBackbone(nn.Module):
     _dropout_state: Optional[training.DropoutState] = None
 
     def dropout_state(self) -> training.DropoutState:
-        """Seed and step of the training form's dropout (made on the model's device when first asked for)."""
+        """Seed and step of the training form's dropout (made when first asked for; they move with the model)."""
         dev = self.norm.weight.device
-        if self._dropout_state is None or self._dropout_state.state.device != dev:
+        if self._dropout_state is None:
             self._dropout_state = training.DropoutState(self.train_seed, dev)
-        return self._dropout_state
+        return self._dropout_state.to(dev)
 
     def run_training(self, tokens: Tensor, pad_len: Optional[Tensor] = None):
         """embed_norm, layers and final norm (:420, :435-461) on the training operators: tokens
@@ -481,7 +481,9 @@ class MarioDT(nn.Module):
         no cache, forward() runs attention with its gradient, every residual add as one kernel with
         the dropout before it and the norm behind it, and dropout whose masks are never stored, from
         a generator of ``seed`` (model.dropout_state(), to be saved with a checkpoint).  Without
-        autograd (validation, act()) the inference kernels run as before.
+        autograd (validation, act()) the inference kernels run as before.  Ranks of a data-parallel job
+        take seeds of their own.  A forward pass that is run again for its backward pass (activation
+        checkpointing of the whole model) would draw other masks: checkpoint inside, with the same rng.
 
         Padded positions (attention_mask 0) attend to nothing and pass no gradient through the
         attention; give them action_targets of -100, as their logits mean nothing."""

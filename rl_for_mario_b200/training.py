@@ -14,6 +14,11 @@ seed and the step on the device: ``draw()`` hands out the pair for one forward
 pass and moves on, so passes have masks of their own, a backward pass sees the
 pair of its forward pass whatever was drawn since, and a captured graph draws
 anew at each replay.  ``site`` tells the places of a model apart.
+
+What follows from that: ranks of a data-parallel job take seeds of their own; a
+forward pass that is run again for its backward pass (activation checkpointing)
+has to be given the first one's pair, since a new draw() is another mask; and a
+state that two streams draw from at once is theirs to order.
 """
 from __future__ import annotations
 
@@ -40,6 +45,11 @@ class DropoutState:
         now = self.state.clone()
         self.state[1:].add_(1)
         return now
+
+    def to(self, device) -> "DropoutState":
+        """The same seed and step, held on the device."""
+        self.state = self.state.to(device)
+        return self
 
     def state_dict(self) -> dict:
         seed, step = self.state.tolist()

@@ -158,6 +158,22 @@ def test_model_step_reaches_every_parameter(dtype):
 
 
 @pytest.mark.gpu
+def test_the_generator_moves_with_its_model():
+    model = small_model(torch.float16, 0.1, 128, 4, 2).train().fuse_training(seed=11)
+    attn = model.model.layers[0].self_attn
+    for owner in (model.model, attn):
+        for _ in range(2):
+            owner.dropout_state().draw()
+    model.cpu()
+    for owner in (model.model, attn):
+        assert owner.dropout_state().state_dict() == {"seed": 11, "step": 2}
+        assert owner.dropout_state().state.device.type == "cpu"
+    model.cuda()
+    for owner in (model.model, attn):
+        assert owner.dropout_state().draw().tolist() == [11, 2] and owner.dropout_state().state.is_cuda
+
+
+@pytest.mark.gpu
 def test_every_place_drops_at_its_own_rate():
     """The embedding's, the attention's and the MLP's rate are read apart: with only one of them above zero the
     result still depends on the generator's step, and with none it does not."""
