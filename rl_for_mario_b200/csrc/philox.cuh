@@ -45,14 +45,6 @@ __device__ __forceinline__ uint4 philox7(const DropKey& k, unsigned long long bl
   return make_uint4(c0, c1, c2, c3);
 }
 
-// Whether element i of a block of words stays (i a constant): the high half of a
-// word w is >= threshold iff w >= threshold << 16, the low one is moved up first.
-template <int I>
-__device__ __forceinline__ bool stays(const uint4& w, uint32_t threshold_hi) {
-  const uint32_t x = I / 2 == 0 ? w.x : I / 2 == 1 ? w.y : I / 2 == 2 ? w.z : w.w;
-  return (I & 1 ? x : x << 16) >= threshold_hi;
-}
-
 // Drop flags of a block's eight elements in four words: bit 0 of word i is set when
 // element 2 i is dropped, bit 16 when element 2 i + 1 is.  Both halves of a word at
 // once: max(w, t) - w is 0 in a half that stays (w >= t), min with 1 makes a flag of
