@@ -498,6 +498,10 @@ DROP = [
     ((1, 1), BF16, 0.5, False), ((1, 7), FP32, 0.1, True), ((3, 8), FP16, 0.1, False), ((5, 1001), FP32, 0.25, True),
     ((192, 256), BF16, 0.1, True), ((2, 3, 5, 40), FP16, 0.9, True), ((4097, 24), BF16, 0.0, True),
     ((129, 2049), BF16, 0.1, False), ((1000, 520), FP32, 0.001, False),
+    # Odd widths: rows that begin at every place of 16 bytes, one column more or less than a warp's.
+    ((70, 247), BF16, 0.2, True), ((70, 249), FP16, 0.2, False), ((33, 1001), FP16, 0.1, True),
+    ((40, 63), BF16, 0.5, True), ((40, 65), BF16, 0.5, True), ((500, 243), FP32, 0.3, False), ((20, 4093), FP32, 0.1, True),
+    ((3, 30011), BF16, 0.0, True),
 ]
 
 
