@@ -112,6 +112,7 @@ struct alignas(16) Item {
 struct TcShared {
   uint64_t tile_full[2], tile_empty[2], blk_full[kMaxStages], blk_empty[kMaxStages];
   uint64_t s_full[2], s_read[2], dp_full, p_full, ds_full, w_done, o_empty, drain;
+  uint64_t pair[4];  // dq: the two warps that share rows have both halves of delta in place
   uint64_t item_full[kItems], item_empty[kItems];
   Item item[kItems];  // the items under way
   alignas(16) uint4 claim[2];  // answers to the requests for items, in turn
@@ -367,6 +368,7 @@ __device__ __forceinline__ void tc_init(TcShared* sh, int warps) {
     mbar_init(&sh->item_full[i], 1);
     mbar_init(&sh->item_empty[i], warps);
   }
+  for (int i = 0; i < 4; ++i) mbar_init(&sh->pair[i], 2);
   mbar_init(&sh->dp_full, 1);
   mbar_init(&sh->p_full, warps);
   mbar_init(&sh->ds_full, warps);
@@ -987,35 +989,39 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       const unsigned long long row_block = (unsigned long long)row * per_row;
       float delta = 0.f;
       float* xr = xrow + (done & 1) * 2 * kRows;  // the other half may still be read for the previous item
+      // The row's other half of delta comes from the warp of the other warpgroup, once for each item with blocks.
+      // An mbarrier, not a barrier of the block: its wait has a limit, and a warp that has left after a failed wait
+      // is not waited for without end.
+      auto exchange = [&](float mine_half) {
+        xr[half * kRows + r] = mine_half;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->pair[wq]);
+        if (!warp_wait(&sh->pair[wq], done & 1, abort, p.status)) return false;
+        delta = xr[r] + xr[kRows + r];
+        return true;
+      };
       if (nblk > 0 && all > 1) {
         // delta = O . dO: each of the row's two threads takes half of the columns.
         const int tb = done % SH::BWD_TILES;
-        if ((ok = warp_wait(&sh->tile_full[tb], (done / SH::BWD_TILES) & 1, abort, p.status))) {
-          float d = 0.f;
+        if (!(ok = warp_wait(&sh->tile_full[tb], (done / SH::BWD_TILES) & 1, abort, p.status))) break;
+        float d = 0.f;
 #pragma unroll
-          for (int c = 0; c < SH::NCH / 2; ++c) {
-            const uint32_t at = swz<SH::ROWB>(r, half * (SH::NCH / 2) + c) + tb * SH::TILE;
-            const uint4 o = *reinterpret_cast<const uint4*>(smem + SM::OFF_O + at);
-            const uint4 g = *reinterpret_cast<const uint4*>(smem + SM::OFF_B + at);
-            const uint32_t a[4] = {o.x, o.y, o.z, o.w}, y[4] = {g.x, g.y, g.z, g.w};
+        for (int c = 0; c < SH::NCH / 2; ++c) {
+          const uint32_t at = swz<SH::ROWB>(r, half * (SH::NCH / 2) + c) + tb * SH::TILE;
+          const uint4 o = *reinterpret_cast<const uint4*>(smem + SM::OFF_O + at);
+          const uint4 g = *reinterpret_cast<const uint4*>(smem + SM::OFF_B + at);
+          const uint32_t a[4] = {o.x, o.y, o.z, o.w}, y[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 fa = E::to_f2(a[e]), fy = E::to_f2(y[e]);
-              d = fmaf(fa.x, fy.x, fmaf(fa.y, fy.y, d));
-            }
+          for (int e = 0; e < 4; ++e) {
+            const float2 fa = E::to_f2(a[e]), fy = E::to_f2(y[e]);
+            d = fmaf(fa.x, fy.x, fmaf(fa.y, fy.y, d));
           }
-          xr[half * kRows + r] = d;
         }
-        ok = named_bar_and(1, 256, ok);
-        if (!ok) break;
-        delta = xr[r] + xr[kRows + r];
+        if (!(ok = exchange(d))) break;
         if (half == 0 && valid && split == 0) p.delta[row] = delta;
       }
       for (int j = 0; j < nblk; ++j, ++blk) {
-        if (!(ok = warp_wait(&sh->s_full[0], blk & 1, abort, p.status))) {
-          if (all == 1) named_bar_and(1, 256, false);  // the others may wait there
-          break;
-        }
+        if (!(ok = warp_wait(&sh->s_full[0], blk & 1, abort, p.status))) break;
         tc_fence_after();
         const int k0 = kb + j * kBlk + 32 * half;
         const int see = valid ? pos - k0 + 1 : 32, lo = j == 0 && half == 0 ? pad - kb : 0;
@@ -1066,9 +1072,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
               for (int c = 0; c < 16; ++c) s = fmaf(__uint_as_float(w[c]), __uint_as_float(d[c]), s);
             }
           }
-          xr[half * kRows + r] = s * p.inv_keep;
-          if (!(ok = named_bar_and(1, 256, true))) break;
-          delta = xr[r] + xr[kRows + r];
+          if (!(ok = exchange(s * p.inv_keep))) break;
           if (half == 0 && valid) p.delta[row] = delta;
         }
         uint32_t pk[16];

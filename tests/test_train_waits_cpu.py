@@ -1,0 +1,27 @@
+"""The waits of the attention training kernels, read from their source: what a GPU must not be made to show."""
+import re
+from pathlib import Path
+
+import rl_for_mario_b200
+
+SOURCE = Path(rl_for_mario_b200.__file__).parent / "csrc" / "attn_train_sm100.cu"
+
+
+def code():
+    return re.sub(r"//[^\n]*", "", SOURCE.read_text())
+
+
+def test_no_wait_without_a_limit():
+    """A warp leaves its loop when a wait runs out, so whoever may wait for it has to do so with a limit: inside the
+    kernels only mbarriers (mbar_wait, bounded), and barriers of the block at a kernel's entry and its end alone."""
+    text = code()
+    assert not re.search(r"\bnamed_bar|\bbar\.(sync|red|arrive)|\bbarrier\.|mbar_try_wait|__syncthreads_(and|or|count)", text)
+    for body in re.split(r"__global__", text)[1:]:
+        body = body[:body.index("\n}\n")]
+        at = [m.start() for m in re.finditer(r"__syncthreads\(\)", body)]
+        if "TcShared* sh" not in body:
+            assert not at
+            continue
+        loops = [m.start() for m in re.finditer(r"while \(true\)", body)]
+        assert len(at) == 2 and len(loops) == 1 and at[0] < loops[0] < at[1]
+        assert body.index("tmem_dealloc") > at[1]
