@@ -43,13 +43,16 @@
 // The left operand of every second product goes back to tensor memory, the
 // right one is the shared-memory tile as TMA left it, read row-major ("MN
 // major").  The next block's scores are issued as soon as this block's are in
-// registers (forward, dq: the weights have columns of their own); for dk and dv
-// the 512 columns do not hold both, so P^T lies over S^T and dS^T over dP^T, and
-// the two halves of a block alternate: while the threads form dS^T of a block,
-// dV += P^T dO and the next S^T run, and during the next exponentials
-// dK += dS^T Q and the next dP^T.  MMAs of one thread execute in order, which is
-// what lets a block's scores be issued behind the products that still read the
-// previous block's weights in the same columns.
+// registers.  The weights have columns of their own, except for dk and dv with
+// D = 64, where the columns do not hold both: there P^T lies over S^T and dS^T over
+// dP^T.  For dk and dv the two halves of a block alternate: while the threads form
+// dS^T of a block, dV += P^T dO and the next S^T run, and during the next
+// exponentials dK += dS^T Q and the next dP^T.
+//
+// Order between MMAs.  The PTX ISA promises it for those of one accumulator and
+// shape only.  So whatever is read by one MMA and written by another (weights that
+// lie where the next scores go), or by the threads, is handed on through a commit and
+// a wait on its mbarrier.
 //
 // What bounds it.  96 x 768, 12 / 4 heads of 64, padding up to half, bf16, p = 0.1:
 // forward 215 us, dq 240, dk and dv 268 (0.18 PFLOP of products that count: 246
@@ -112,6 +115,7 @@ struct alignas(16) Item {
 struct TcShared {
   uint64_t tile_full[2], tile_empty[2], blk_full[kMaxStages], blk_empty[kMaxStages];
   uint64_t s_full[2], s_read[2], dp_full, p_full, ds_full, w_done, o_empty, drain;
+  uint64_t p_taken;  // dk, dv with the weights over the scores: P^T has been read
   uint64_t pair[4];  // dq: the two warps that share rows have both halves of delta in place
   uint64_t item_full[kItems], item_empty[kItems];
   Item item[kItems];  // the items under way
@@ -370,6 +374,7 @@ __device__ __forceinline__ void tc_init(TcShared* sh, int warps) {
   }
   for (int i = 0; i < 4; ++i) mbar_init(&sh->pair[i], 2);
   mbar_init(&sh->dp_full, 1);
+  mbar_init(&sh->p_taken, 1);
   mbar_init(&sh->p_full, warps);
   mbar_init(&sh->ds_full, warps);
   mbar_init(&sh->w_done, 1);
@@ -485,9 +490,10 @@ __device__ __forceinline__ void issue_rows(TcShared* sh, int* status, Prepare pr
   warp_wait(&sh->drain, 0, nullptr, nullptr);
 }
 
-// The same for the dk, dv kernel: weights over their scores, the two halves of a
-// block in turn.
-template <int TB, int STAGES, class ScoresA, class ScoresB, class WeightsA, class WeightsB>
+// The same for the dk, dv kernel: the two halves of a block in turn.  OVER: the weights
+// lie over their scores, so the next scores wait until the product that reads them is
+// done (P^T: p_taken, dS^T: the block's blk_empty).
+template <int TB, int STAGES, bool OVER, class ScoresA, class ScoresB, class WeightsA, class WeightsB>
 __device__ __forceinline__ void issue_keys(TcShared* sh, int* status, ScoresA scores_a, ScoresB scores_b,
                                            WeightsA weights_a, WeightsB weights_b) {
   volatile int* abort = &sh->abort;
@@ -507,6 +513,7 @@ __device__ __forceinline__ void issue_keys(TcShared* sh, int* status, ScoresA sc
     }
     if (!wait && !warp_test(&sh->blk_full[st], (a_blk / STAGES) & 1)) return;
     if (!(ok = warp_wait(&sh->blk_full[st], (a_blk / STAGES) & 1, abort, status))) return;
+    if (OVER && a_blk > 0 && !(ok = warp_wait(&sh->p_taken, (a_blk - 1) & 1, abort, status))) return;
     tc_fence_after();
     scores_a(tb, st);
     commit(&sh->s_full[0]);
@@ -517,6 +524,11 @@ __device__ __forceinline__ void issue_keys(TcShared* sh, int* status, ScoresA sc
     }
   };
   auto next_b = [&]() {  // behind next_a of the same block, whose waits it shares
+    if (OVER && b_blk > 0) {
+      const int last = b_blk - 1;
+      if (!(ok = warp_wait(&sh->blk_empty[last % STAGES], (last / STAGES) & 1, abort, status))) return;
+      tc_fence_after();
+    }
     scores_b(b_tile % TB, b_blk % STAGES);
     commit(&sh->dp_full);
     ++b_blk;
@@ -531,13 +543,14 @@ __device__ __forceinline__ void issue_keys(TcShared* sh, int* status, ScoresA sc
     while (ok && !end && a_blk <= blk) next_a(true);
     if (!ok || a_blk <= blk) break;
     if (b_blk <= blk) next_b();
-    if (!(ok = warp_wait(&sh->p_full, blk & 1, abort, status))) break;
+    if (!ok || !(ok = warp_wait(&sh->p_full, blk & 1, abort, status))) break;
     if (j == 0) {
       n = sh->tile_meta[tiles & 7].x;
       if (tiles > 0 && !(ok = warp_wait(&sh->o_empty, (tiles - 1) & 1, abort, status))) break;
     }
     tc_fence_after();
     weights_a(blk % STAGES, j > 0);
+    if (OVER) commit(&sh->p_taken);
     if (!end) next_a(false);
     if (!ok || !(ok = warp_wait(&sh->ds_full, blk & 1, abort, status))) break;
     tc_fence_after();
@@ -1159,7 +1172,10 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Columns: S^T, dP^T, dV, dK, and P^T and dS^T behind them where there is room.
+  constexpr bool OVER = 2 * kBlk + 2 * D + kBlk > (int)kCols;
   const uint32_t t_s = sh->tmem, t_dp = sh->tmem + 64, t_dv = sh->tmem + 128, t_dk = sh->tmem + 128 + D;
+  const uint32_t t_p = OVER ? t_s : t_dk + D, t_ds = OVER ? t_dp : t_p + kBlk / 2, w_half = OVER ? 32 : 16;
   volatile int* abort = &sh->abort;
 
   if (warp == 8) {
@@ -1172,12 +1188,12 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     const uint32_t id_s = umma_idesc_f16(BF16, kRows, kBlk, 0, 0), id_o = umma_idesc_f16(BF16, kRows, D, 0, 1);
     auto tile_at = [](int tb) { return (uint32_t)(tb * (SH::TILE >> 4)); };
     auto blk_at = [](int st) { return (uint32_t)(st * (SH::BLK >> 4)); };
-    issue_keys<SH::BWD_TILES, SH::STAGES>(
+    issue_keys<SH::BWD_TILES, SH::STAGES, OVER>(
         sh, p.status,
         [&](int tb, int st) { issue_scores<D>(t_s, kd, tile_at(tb), qd, blk_at(st), id_s); },
         [&](int tb, int st) { issue_scores<D>(t_dp, vd, tile_at(tb), dd, blk_at(st), id_s); },
-        [&](int st, bool acc) { issue_weights<D>(t_dv, t_s, 32, dt, blk_at(st), id_o, acc); },
-        [&](int st, bool acc) { issue_weights<D>(t_dk, t_dp, 32, qt, blk_at(st), id_o, acc); });
+        [&](int st, bool acc) { issue_weights<D>(t_dv, t_p, w_half, dt, blk_at(st), id_o, acc); },
+        [&](int st, bool acc) { issue_weights<D>(t_dk, t_ds, w_half, qt, blk_at(st), id_o, acc); });
   } else if (tid == 288) {
     load_all<SH::BWD_TILES, SH::STAGES, KTile>(
         sh, p, gr,
@@ -1205,6 +1221,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     const int half = warp >> 2, wq = warp & 3;
     const uint32_t lane_off = (uint32_t)(wq * 32) << 16;
     const uint32_t ts = t_s + lane_off + 32 * half, tdp = t_dp + lane_off + 32 * half;
+    const uint32_t tp = t_p + lane_off + w_half * half, tds = t_ds + lane_off + w_half * half;
     const float c2 = p.scale * 1.4426950408889634f;
     const float2 c2v = make_float2(c2, c2), ik = make_float2(p.inv_keep, p.inv_keep);
     DropKey key{};
@@ -1338,14 +1355,14 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
                   pw[(c - c0) >> 1] = E::from_f2(w0, w1);
               }
             }
-            tmem_st8(ts + (c0 >> 1), pw);
+            tmem_st8(tp + (c0 >> 1), pw);
           }
         } else {
           uint32_t z[8];
 #pragma unroll
           for (int c = 0; c < 8; ++c) z[c] = 0u;
-          tmem_st8(ts, z);
-          tmem_st8(ts + 8, z);
+          tmem_st8(tp, z);
+          tmem_st8(tp + 8, z);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -1380,12 +1397,12 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
               }
             }
           }
-          tmem_st16(tdp, *reinterpret_cast<uint32_t(*)[16]>(s));
+          tmem_st16(tds, *reinterpret_cast<uint32_t(*)[16]>(s));
         } else {
           uint32_t z[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) z[c] = 0u;
-          tmem_st16(tdp, z);
+          tmem_st16(tds, z);
         }
         tmem_st_wait();
         tc_fence_before();
