@@ -20,7 +20,10 @@
 //
 // Rounding: P and dS enter the second products in the inputs' 16-bit type, as
 // the tensor cores take both operands in one type; sums, softmax statistics
-// and delta are fp32.  A row with a single key has a constant softmax: its dS
+// and delta are fp32.  fp16 has no exponents for P of long rows nor for dS of small
+// gradients, so there both are scaled by powers of two, which the stores take out
+// again: P of the dk, dv kernel by 2^15 (P <= 1), dS by a factor of its sample and KV
+// head (GradExponent; forward, P is relative to a running maximum).  A row with a single key has a constant softmax: its dS
 // is set to exactly zero.  Where a tile's keys are one block, delta is the sum
 // over the unrounded P dP; beyond, it is O . dO with the stored O.
 //
@@ -108,6 +111,7 @@ struct alignas(16) Item {
   int nblk, pad, heads, tile;  // blocks (-1: no more items); heads of the chunk
   int first, origin, per, split;  // rows: p0, kb; keys: q0, k0, blocks of a chunk of heads, the first block
   long long row;   // of lse, delta and the dropout rows: sample and first head, position 0
+  int lift;        // exponent of dS's factor (fp16)
   long long out, out2, part;  // element offsets of the outputs at that sample and head, position 0; rows of partial sums
 };
 
@@ -122,6 +126,7 @@ struct TcShared {
   alignas(16) uint4 claim[2];  // answers to the requests for items, in turn
   uint64_t claimed;
   int2 tile_meta[8];  // blocks and padded keys of the tiles under way (0 blocks: no more tiles)
+  float inverse[8], out_scale[2][8];  // dq, fp16: 1 / dS's factor, and scale / factor of two items in turn; each warp's own
   uint32_t tmem;
   int abort;
 };
@@ -183,12 +188,13 @@ struct QTile {
   static constexpr bool kRowTiles = true;
   int b, g, h0, heads, pad, p0, kb, nblk, tile, zero;  // zero: padded keys of the first block
   int split, all;                                      // the segment; blocks of the whole tile
+  int lift;                                            // exponent of dS's factor
 };
 // A tile of keys k0 .. k0 + 128 of KV head g and the blocks of PT positions (from
 // q0 on: earlier queries see none of these keys) x chunks of heads behind it.
 struct KTile {
   static constexpr bool kRowTiles = false;
-  int b, g, pad, k0, q0, per, nblk, tile, zero, split;  // its blocks are split, split + splits, ...
+  int b, g, pad, k0, q0, per, nblk, tile, zero, split, lift;  // its blocks are split, split + splits, ...
 };
 
 // Key blocks that the rows before position `end` of a tile see.
@@ -202,9 +208,28 @@ __device__ __forceinline__ int row_blocks(int end, int pad, int S) {
 // scores of a segment of one would give the tile's buffer back too early.
 __host__ __device__ __forceinline__ int segments(int all, int seg) { return all <= seg + 1 ? 1 : (all + seg - 2) / seg; }
 
+// fp16: the exponent of the factor of a unit's dS (attn_train_grad_max_kernel), 0 where there is no finite bound.  The
+// loading thread takes it, its load beside that of the padding: at the start of an item, in the warps that use it,
+// dq took 234 instead of 223 us for 2,048 x 192, 8 / 2 heads of 32.
+struct GradExponent {
+  const float2* part;
+  float2 m;
+  __device__ __forceinline__ GradExponent(const AttnTrainParams& p, int unit)
+      : part(reinterpret_cast<const float2*>(p.grad_max) + (long long)unit * p.grad_parts), m(__ldg(part)) {}
+  __device__ __forceinline__ int get(const AttnTrainParams& p) {
+#pragma unroll 4
+    for (int i = 1; i < p.grad_parts; ++i) {
+      const float2 o = __ldg(part + i);
+      m = make_float2(fmaxf(m.x, o.x), fmaxf(m.y, o.y));
+    }
+    const float c = 2.f * p.inv_keep * sqrtf(m.x * m.y);  // between 2^-47 and 2^56 unless 0 or infinite
+    return c > 0.f && c < INFINITY ? 14 + 127 - (int)(__float_as_uint(c) >> 23) : 0;
+  }
+};
+
 // The CTA's items: its own, then what it takes.  Taken no earlier than the loading
 // thread needs it, a few blocks before the MMAs do.
-template <class T>
+template <class T, bool LIFT>
 struct Items {
   static constexpr bool kRowTiles = T::kRowTiles;
   int claims = -1;
@@ -228,7 +253,14 @@ struct Items {
     h.b = gr.by_kv(bg);
     h.g = bg - h.b * p.Hkv;
     h.tile = it.tile;
-    h.pad = p.pad_len ? __ldg(p.pad_len + h.b) : 0;
+    if constexpr (LIFT) {
+      GradExponent e(p, bg);
+      h.pad = p.pad_len ? __ldg(p.pad_len + h.b) : 0;
+      t.lift = e.get(p);
+    } else {
+      h.pad = p.pad_len ? __ldg(p.pad_len + h.b) : 0;
+      t.lift = 0;
+    }
     t.b = h.b;
     t.g = h.g;
     t.pad = min(max(h.pad, 0), p.S);
@@ -388,11 +420,11 @@ __device__ __forceinline__ void tc_init(TcShared* sh, int warps) {
 // The loading thread, the same for the three kernels: the tiles and blocks of the
 // CTA's items in order, each into the next of TB tile buffers and STAGES stages,
 // and each item's numbers into the ring that the element-wise warps read.
-template <int TB, int STAGES, class T, class Describe, class LoadTile, class LoadBlk>
+template <int TB, int STAGES, class T, bool LIFT, class Describe, class LoadTile, class LoadBlk>
 __device__ __forceinline__ void load_all(TcShared* sh, const AttnTrainParams& p, const Grid& gr, Describe describe,
                                          LoadTile load_tile, LoadBlk load_blk) {
   volatile int* abort = &sh->abort;
-  Items<T> items;
+  Items<T, LIFT> items;
   T t;
   int blocks = 0, tiles = 0, n = 0;
   bool ok = true, more = true;
@@ -567,6 +599,76 @@ __device__ __forceinline__ void issue_keys(TcShared* sh, int* status, ScoresA sc
   warp_wait(&sh->drain, 0, nullptr, nullptr);
 }
 
+// ---------------------------------------------------------------- scale of fp16 gradients
+// |dS_j| = P_j |dP_j - delta| <= c = 2 / (1 - p) max|dO row| max|v row| (dP_j = m' dO . v_j, delta a mean of
+// them), with the maxima over the rows of a sample and KV head behind its padding.  dS is scaled by the power of
+// two that puts c into [2^14, 2^15): half of fp16's range is left for rounding, and what falls below its
+// subnormals is below 2^-39 c.  Rows of squares' sums, NaN ignored; 2 D (Hq + Hkv) S bytes a sample to read,
+// in parts of a unit that the readers join: 6 us for 1 x 5,003, 12 / 12 heads of 64, 34 for 96 x 768, 12 / 4 of 64,
+// 42 for 2,048 x 192, 8 / 2 of 32.  The dq and dk, dv kernels take 3 to 8 % longer with it (the last two cases: 223 +
+// 294 and 251 + 284 us, in bf16, which needs none of it, 208 + 288 and 244 + 272).
+constexpr int kMaxGradParts = 32;
+
+template <int D>
+__global__ void __launch_bounds__(256) attn_train_grad_max_kernel(const __grid_constant__ AttnTrainParams p) {
+  constexpr int NC = D / 8;  // threads of a row
+  __shared__ uint32_t top[2][8];
+  const int unit = blockIdx.x / p.grad_parts, part = blockIdx.x - unit * p.grad_parts;
+  const int b = unit / p.Hkv, g = unit - b * p.Hkv;
+  const int pad = p.pad_len ? min(max(__ldg(p.pad_len + b), 0), p.S) : 0;
+  const int per = (p.S - pad + p.grad_parts - 1) / p.grad_parts;
+  const int first = min(pad + part * per, p.S), count = min(per, p.S - first);
+  auto walk = [&](const void* base, long long ss, long long sh, int heads) {
+    const uint16_t* at = static_cast<const uint16_t*>(base) + first * ss;
+    // Row r is head r % heads of position r / heads; a turn's rows are stepped to without a division.  Several turns'
+    // loads are in flight together.
+    constexpr int kTurns = 4, kPerTurn = 256 / NC;
+    const int c = threadIdx.x % NC, step = kPerTurn / heads, rest = kPerTurn % heads;
+    int pos = threadIdx.x / NC / heads, head = threadIdx.x / NC % heads;
+    float most = 0.f;
+    for (long long r0 = 0; r0 < (long long)count * heads; r0 += kTurns * kPerTurn) {
+      uint4 u[kTurns];
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        u[t] = pos < count ? *reinterpret_cast<const uint4*>(at + pos * ss + head * sh + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+        pos += step;
+        head += rest;
+        if (head >= heads) head -= heads, ++pos;
+      }
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const uint32_t w[4] = {u[t].x, u[t].y, u[t].z, u[t].w};
+        float q = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = Elem<false>::to_f2(w[e]);
+          q = fmaf(f.x, f.x, fmaf(f.y, f.y, q));
+        }
+#pragma unroll
+        for (int o = NC / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+        most = fmaxf(most, q);
+      }
+    }
+    return __reduce_max_sync(0xffffffffu, __float_as_uint(most));  // of floats from 0 up, by their bits
+  };
+  const uint32_t of_do = walk(static_cast<const uint16_t*>(p.dout) + b * p.do_sb + (long long)g * p.R * p.do_sh, p.do_ss,
+                              p.do_sh, p.R);
+  const uint32_t of_v = walk(static_cast<const uint16_t*>(p.v) + b * p.v_sb + g * p.v_sh, p.v_ss, p.v_sh, 1);
+  if ((threadIdx.x & 31) == 0) {
+    top[0][threadIdx.x >> 5] = of_do;
+    top[1][threadIdx.x >> 5] = of_v;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, top[threadIdx.x][w]);
+    p.grad_max[2 * (long long)blockIdx.x + threadIdx.x] = __uint_as_float(m);
+  }
+}
+
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
 // The element-wise warps' side of the item ring.
 struct ItemReader {
   TcShared* sh;
@@ -657,7 +759,7 @@ __global__ void __launch_bounds__(kFwdThreads, kPerSm)
         },
         [&](int st, bool acc) { issue_weights<D>(t_o, t_p, 16, vd, (uint32_t)(st * (SH::BLK >> 4)), id_o, acc); });
   } else if (tid == 160) {
-    load_all<2, SH::STAGES, QTile>(
+    load_all<2, SH::STAGES, QTile, false>(
         sh, p, gr,
         [&](const QTile& t, Item& it) {
           it.nblk = t.nblk, it.pad = t.pad, it.heads = t.heads, it.tile = t.tile;
@@ -925,12 +1027,13 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         },
         [&](int st, bool acc) { issue_weights<D>(t_dq, t_ds, 16, kt, (uint32_t)(st * (SH::BLK >> 4)), id_o, acc); });
   } else if (tid == 288) {
-    load_all<SH::BWD_TILES, SH::DQ_STAGES, QTile>(
+    load_all<SH::BWD_TILES, SH::DQ_STAGES, QTile, !BF16>(
         sh, p, gr,
         [&](const QTile& t, Item& it) {
           it.nblk = t.nblk, it.pad = t.pad, it.heads = t.heads, it.tile = t.tile;
           it.first = t.p0, it.origin = t.kb, it.split = t.split, it.per = t.all;
           it.row = ((long long)t.b * p.Hq + t.h0) * S;
+          it.lift = t.lift;
           it.out = t.b * p.dq_sb + t.h0 * p.dq_sh;
         },
         [&](const QTile& t, int tb) {
@@ -963,22 +1066,29 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     bool fin = false, fin_partial = false;
     auto finish = [&]() {
       fin = false;
-      uint32_t o[D / 2];
 #pragma unroll
-      for (int c = 0; c < D / 2; c += 16)
-        tmem_ld16_u(t_dq + lane_off + half * (D / 2) + c, *reinterpret_cast<uint32_t(*)[16]>(o + c));
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->o_empty);
-      if (CUT && fin_out && fin_partial) {
-        float* out = static_cast<float*>(fin_out);
+      for (int c0 = 0; c0 < D / 2; c0 += 16) {
+        uint32_t o[16];
+        tmem_ld16_u(t_dq + lane_off + half * (D / 2) + c0, o);
+        if (c0 + 16 == D / 2) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->o_empty);
+        }
+        const float out_scale = BF16 ? p.scale : *(volatile float*)&sh->out_scale[(done - 1) & 1][warp];
+        if (CUT && fin_out && fin_partial) {
+          float* out = static_cast<float*>(fin_out) + c0;
+          if constexpr (!BF16)
 #pragma unroll
-        for (int c = 0; c < D / 2; c += 4)
-          *reinterpret_cast<uint4*>(out + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-      } else if (fin_out) {
-        uint16_t* out = static_cast<uint16_t*>(fin_out);
+            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * out_scale);
 #pragma unroll
-        for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(out + c) = pack8<BF16>(o + c, p.scale);
+          for (int c = 0; c < 16; c += 4)
+            *reinterpret_cast<uint4*>(out + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+        } else if (fin_out) {
+          uint16_t* out = static_cast<uint16_t*>(fin_out) + c0;
+#pragma unroll
+          for (int c = 0; c < 16; c += 8) *reinterpret_cast<uint4*>(out + c) = pack8<BF16>(o + c, out_scale);
+        }
       }
     };
     while (true) {
@@ -986,10 +1096,11 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       if (!ok) break;
       const int nblk = it->nblk, pad = it->pad, kb = it->origin, pos = it->first + rpos;
       if (nblk < 0) break;
+      const int lift = BF16 ? 0 : it->lift;
       const bool mine = r < rows && head < it->heads, valid = mine && pos < S;
       const long long row = it->row + (long long)head * S + pos;
       // A row with a single key (pos == pad) has no gradient: its P is taken as 0.
-      const float ls = valid && pos != pad ? __ldg(p.lse + row) : INFINITY;
+      const float ls = valid && pos != pad ? __ldg(p.lse + row) - (float)lift : INFINITY;
       uint16_t* out = static_cast<uint16_t*>(p.dq) + it->out + head * p.dq_sh + half * (D / 2);
       const int pz = it->tile * PT + rpos;
       const int split = CUT ? it->split : 0, all = CUT ? it->per : nblk;
@@ -1000,6 +1111,11 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       items.next();
       out += pos * p.dq_ss;
       const unsigned long long row_block = (unsigned long long)row * per_row;
+      // fp16: P, and so dS, is formed with dS's factor in its exponent (registers are short).
+      if constexpr (!BF16) {
+        *(volatile float*)&sh->inverse[warp] = power_of_two(-lift);
+        *(volatile float*)&sh->out_scale[done & 1][warp] = p.scale * power_of_two(-lift);
+      }
       float delta = 0.f;
       float* xr = xrow + (done & 1) * 2 * kRows;  // the other half may still be read for the previous item
       // The row's other half of delta comes from the warp of the other warpgroup, once for each item with blocks.
@@ -1085,9 +1201,9 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
               for (int c = 0; c < 16; ++c) s = fmaf(__uint_as_float(w[c]), __uint_as_float(d[c]), s);
             }
           }
-          if (!(ok = exchange(s * p.inv_keep))) break;
+          if (!(ok = exchange(s * (BF16 ? p.inv_keep : p.inv_keep * *(volatile float*)&sh->inverse[warp])))) break;
           if (half == 0 && valid) p.delta[row] = delta;
-        }
+          }
         uint32_t pk[16];
         if (any) {
           const float2 ik = make_float2(p.inv_keep, p.inv_keep), nd = make_float2(-delta, -delta);
@@ -1195,12 +1311,13 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
         [&](int st, bool acc) { issue_weights<D>(t_dv, t_p, w_half, dt, blk_at(st), id_o, acc); },
         [&](int st, bool acc) { issue_weights<D>(t_dk, t_ds, w_half, qt, blk_at(st), id_o, acc); });
   } else if (tid == 288) {
-    load_all<SH::BWD_TILES, SH::STAGES, KTile>(
+    load_all<SH::BWD_TILES, SH::STAGES, KTile, !BF16>(
         sh, p, gr,
         [&](const KTile& t, Item& it) {
           it.nblk = t.nblk, it.pad = t.pad, it.tile = t.tile;
           it.first = t.q0, it.origin = t.k0, it.per = t.per, it.split = t.split;
           it.row = ((long long)t.b * p.Hq + t.g * p.R) * S;
+          it.lift = t.lift;
           it.out = t.b * p.dv_sb + t.g * p.dv_sh;
           it.out2 = t.b * p.dk_sb + t.g * p.dk_sh;
           it.part = (((long long)t.split * 2 * p.B + t.b) * p.Hkv + t.g) * S;
@@ -1223,7 +1340,9 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     const uint32_t ts = t_s + lane_off + 32 * half, tdp = t_dp + lane_off + 32 * half;
     const uint32_t tp = t_p + lane_off + w_half * half, tds = t_ds + lane_off + w_half * half;
     const float c2 = p.scale * 1.4426950408889634f;
-    const float2 c2v = make_float2(c2, c2), ik = make_float2(p.inv_keep, p.inv_keep);
+    const float2 c2v = make_float2(c2, c2);
+    constexpr float kLift = BF16 ? 0.f : 15.f;           // of P, as a power of two
+    constexpr float kLower = BF16 ? 1.f : 1.f / 32768.f;  // and out again
     DropKey key{};
     const unsigned per_row = (unsigned)(S + 7) >> 3;
     if constexpr (DROP && !WORDS) key = drop_key(p.rng, p.site);
@@ -1241,6 +1360,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
     uint16_t* fin_out = nullptr;
     float* fin_part = nullptr;
     bool fin = false;
+    float fin_inv = 1.f;  // fp16: takes dS's factor out
     auto finish = [&]() {
       fin = false;
 #pragma unroll
@@ -1254,12 +1374,15 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
           if (lane == 0) mbar_arrive(&sh->o_empty);
         }
         if (fin_part) {
+          if constexpr (!BF16)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * (half ? fin_inv : kLower));
 #pragma unroll
           for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(fin_part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         } else if (fin_out)
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
-            *reinterpret_cast<uint4*>(fin_out + c + e) = pack8<BF16>(o + e, half ? p.scale : p.inv_keep);
+            *reinterpret_cast<uint4*>(fin_out + c + e) = pack8<BF16>(o + e, half ? (BF16 ? p.scale : p.scale * fin_inv) : p.inv_keep * kLower);
       }
     };
     while (true) {
@@ -1268,6 +1391,9 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       const int nblk = it->nblk, pad = it->pad, per = it->per;
       const int first = it->first + it->split * PT, step = gr.splits * PT;
       if (nblk < 0) break;
+      const int lift = BF16 ? 0 : it->lift;
+      const float factor = power_of_two(lift) * kLower;  // dS has P's lift as well
+      const float2 ik = make_float2(p.inv_keep * factor, p.inv_keep * factor);
       const int key0 = it->origin + wq * 32, kk = key0 + lane;  // the warp's keys, the thread's
       const int it_tile = it->tile;
       const long long row_at = it->row;
@@ -1293,8 +1419,8 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
           nrow = row_at + (long long)(j / per * p.HC + chead) * S + npos;
         }
         const bool there = j < nblk && col < rows && npos < S && (gr.chunks == 1 || j / per * p.HC + chead < p.R);
-        nl = there ? -__ldg(p.lse + nrow) : -INFINITY;
-        nd = there ? -__ldg(p.delta + nrow) : 0.f;
+        nl = there ? kLift - __ldg(p.lse + nrow) : -INFINITY;
+        nd = there ? -__ldg(p.delta + nrow) * factor : 0.f;
         if constexpr (WORDS) nw = there && npos >= key0 ? __ldg(words + nrow) : 0u;  // written where a key is seen
       };
       fetch(0);
@@ -1391,7 +1517,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
                 if constexpr (DROP)
                   d = ffma2(make_float2(drop & 1u << (c0 + c) ? 0.f : d.x, drop & 2u << (c0 + c) ? 0.f : d.y), ik, md);
                 else
-                  d = fadd2(d, md);
+                  d = BF16 ? fadd2(d, md) : ffma2(d, ik, md);
                 d = fmul2(make_float2(__uint_as_float(s[c0 + c]), __uint_as_float(s[c0 + c + 1])), d);
                 s[(c0 + c) >> 1] = E::from_f2(d.x, d.y);
               }
@@ -1413,6 +1539,7 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
       if (nblk > 0) {
         ++done;
         fin = true;
+        if constexpr (!BF16) fin_inv = power_of_two(-lift);
         const bool kept = kk >= pad && kk < S;
         fin_out = kept ? out + kk * out_ss : nullptr;
         fin_part = kept && part ? part + (long long)kk * D : nullptr;
@@ -1505,7 +1632,7 @@ __global__ void __launch_bounds__(256) attn_train_join_kernel(const __grid_const
       if (c == 0) p.lse[row] = top + log2f(l);
     } else {
       uint16_t* out = static_cast<uint16_t*>(p.dq) + b * p.dq_sb + (long long)pos * p.dq_ss + h * p.dq_sh;
-      *reinterpret_cast<uint4*>(out + c) = pack8<BF16>(s, p.scale);
+      *reinterpret_cast<uint4*>(out + c) = pack8<BF16>(s, BF16 ? p.scale : 1.f);  // fp16: scaled with the factor taken out
     }
   }
 }
@@ -1550,6 +1677,10 @@ cudaError_t run_bwd(const AttnTrainParams& p, const AttnTrainMaps& m, int num_sm
   if ((e = smem_limit_once(reinterpret_cast<const void*>(kk), BwdSmem<D, false>::BYTES)) != cudaSuccess) return e;
   const int splits = attn_train_splits(p.B, p.S, p.Hkv, p.R, num_sms);
   const Grid gk = grid_keys(p, splits);
+  if constexpr (!BF16) {
+    attn_train_grad_max_kernel<D><<<(unsigned)(p.B * p.Hkv * p.grad_parts), 256, 0, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
   kq<<<(unsigned)gq.items, kBwdThreads, BwdSmem<D, true>::BYTES, st>>>(m.q_tile, m.do_tile, m.o_tile, m.k_blk,
                                                                               m.v_blk, p, gq);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
@@ -1596,6 +1727,13 @@ int attn_train_row_splits(int B, int S, int Hkv, int R, int num_sms) {
 long long attn_train_words(int B, int S, int Hq, int D) {
   if (S > kWordsPerDim * D) return 0;
   return (long long)B * Hq * S * ((S + kBlk - 1) / kBlk * 2);
+}
+
+// Blocks that share the rows of a sample and KV head in attn_train_grad_max_kernel: about
+// eight 16-byte loads a thread.
+int attn_train_grad_parts(int S, int R, int D) {
+  const long long n = (long long)S * (R + 1) * (D / 8) / 2048;
+  return (int)(n < 1 ? 1 : n > kMaxGradParts ? kMaxGradParts : n);
 }
 
 cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,

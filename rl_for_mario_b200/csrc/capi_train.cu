@@ -91,7 +91,8 @@ int check_elem_aligned(const char* fn, int dtype, std::initializer_list<const vo
   return DT_OK;
 }
 
-// The backward pass's scratch: delta, then the partial sums of split tiles of keys, then the drop flags.
+// The backward pass's scratch: delta, then the partial sums of split tiles, then the drop flags, then (fp16) the
+// parts of the gradients' scale.
 int64_t delta_elems(int B, int S, int Hq) { return ((int64_t)B * Hq * S + 3) / 4 * 4; }
 int64_t attn_row_part_elems(int B, int S, int Hq, int Hkv, int D, int sms) {
   const int n = dtk::attn_train_row_splits(B, S, Hkv, Hq / Hkv, sms);
@@ -107,7 +108,8 @@ int64_t attn_forward_workspace(int B, int S, int Hq, int Hkv, int D, int sms) {
 }
 int64_t attn_workspace(int B, int S, int Hq, int Hkv, int D, bool drop, int sms) {
   return 4 * (delta_elems(B, S, Hq) + attn_part_elems(B, S, Hq, Hkv, D, sms) +
-              (drop ? dtk::attn_train_words(B, S, Hq, D) : 0));
+              (drop ? dtk::attn_train_words(B, S, Hq, D) : 0) +
+              (int64_t)B * Hkv * dtk::attn_train_grad_parts(S, Hq / Hkv, D) * 2);
 }
 
 constexpr int kMaxHidden = 8192;  // 32 warps of 256 columns: one block holds a row
@@ -188,8 +190,10 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
   a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
   a.delta = static_cast<float*>(workspace);
   a.part = a.delta + delta_elems(B, S, Hq);
-  if (a.threshold && dtk::attn_train_words(B, S, Hq, D))
-    a.words = reinterpret_cast<uint32_t*>(a.part + attn_part_elems(B, S, Hq, Hkv, D, sms));
+  a.grad_max = a.part + attn_part_elems(B, S, Hq, Hkv, D, sms);
+  a.grad_parts = dtk::attn_train_grad_parts(S, Hq / Hkv, D);
+  const int64_t words = a.threshold ? dtk::attn_train_words(B, S, Hq, D) : 0;
+  if (words) a.words = reinterpret_cast<uint32_t*>(a.grad_max), a.grad_max += words;
   long long* const to[24] = {&a.q_sb,  &a.q_ss,  &a.q_sh,  &a.k_sb,  &a.k_ss,  &a.k_sh,  &a.v_sb,  &a.v_ss,
                              &a.v_sh,  &a.o_sb,  &a.o_ss,  &a.o_sh,  &a.do_sb, &a.do_ss, &a.do_sh, &a.dq_sb,
                              &a.dq_ss, &a.dq_sh, &a.dk_sb, &a.dk_ss, &a.dk_sh, &a.dv_sb, &a.dv_ss, &a.dv_sh};

@@ -298,6 +298,8 @@ struct AttnTrainParams {
   // Drop flags from the dq kernel for the dk, dv kernel: [groups of 32 keys, from the first
   // unpadded position rounded down to 8] x [B, Hq, S] words, or null: generated again.
   uint32_t* words;
+  float* grad_max;  // backward, fp16: [B, Hkv, grad_parts, 2] largest squared norms of rows of dout and v
+  int grad_parts;
   const int32_t* pad_len;  // [B] or null
   long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh;
   long long do_sb, do_ss, do_sh, dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
@@ -319,6 +321,7 @@ struct AttnTrainMaps {
 int attn_train_splits(int B, int S, int Hkv, int R, int num_sms);      // of a tile of keys
 int attn_train_row_splits(int B, int S, int Hkv, int R, int num_sms);  // of a tile of query rows
 long long attn_train_words(int B, int S, int Hq, int D);
+int attn_train_grad_parts(int S, int R, int D);
 cudaError_t launch_attn_train_fwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,
                                         int num_sms, cudaStream_t st);
 cudaError_t launch_attn_train_bwd_sm100(const AttnTrainParams& p, const AttnTrainMaps& m, int D, bool bf16,

@@ -1,0 +1,117 @@
+"""The training attention's gradients away from unit scale, against the float64 restatement.
+
+Bounds are those of tests/test_train_ops_gpu.py without its absolute term for fp16: with u = 2^-11 and A the
+absolute terms of a result, u A for the one rounding of P or dS, u |y| for the result's, u of delta's terms
+beyond one block of keys, 2^-18 A for the fp32 steps.  What fp16's subnormals may add, by their half steps:
+2^-25 for the result itself.  P reaches dv scaled by 2^15 (half step 2^-40 of it), and dS reaches dq and dk
+scaled by the power of two that brings c = 2 / (1 - p) max|dO row| max|v row| of the sample and KV head, which
+no |dS| exceeds, to 2^14 or more: a half step is at most 2^-39 c there.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import train_ref as ref
+from test_train_ops_gpu import attn_inputs, attn_run, check, no_device_error  # noqa: F401
+
+FP16 = torch.float16
+U, SLACK = 2.0 ** -11, 2.0 ** -18
+
+
+def tolerances(host, dout, pads, p, keep):
+    q, k, v = (t.double() for t in host)
+    g = dout.double()
+    B, S, Hq, D = q.shape
+    Hkv = k.shape[2]
+    R = Hq // Hkv
+    r = ref.attention(q, k, v, g, pads, None, keep)
+    tol = {}
+    for name in ("dq", "dk", "dv"):
+        want, mag = r[name]
+        tol[name] = U * 1.01 * (want.abs() + mag) + SLACK * mag + 2.0 ** -25 * 1.01
+        if name != "dv":
+            off, size = r[name + "_delta"]
+            tol[name] += U * 1.01 * off + SLACK * size
+    inv = 65536 / (65536 - round(p * 65536))
+    for b in range(B):
+        lo = min(pads[b], S)
+        for h in range(Hkv):
+            mine = slice(h * R, (h + 1) * R)
+            gg, kk, qq, vv = g[b, lo:, mine], k[b, lo:, h], q[b, lo:, mine], v[b, lo:, h]
+            c = 2 * inv * gg.norm(dim=-1).max().item() * vv.norm(dim=-1).max().item() if lo < S else 0.0
+            tol["dq"][b, lo:, mine] += 2.0 ** -39 * c / math.sqrt(D) * kk.abs().sum(0)
+            tol["dk"][b, lo:, h] += 2.0 ** -39 * c / math.sqrt(D) * qq.abs().sum((0, 1))
+            tol["dv"][b, lo:, h] += 2.0 ** -40 * inv * gg.abs().sum((0, 1))
+    return r, tol
+
+
+def run(host, dout, pads, p, rng=(77, 5, 3)):
+    B, S, Hq, D = host[0].shape
+    keep = ref.keep_factor(B * Hq * S, S, p, *rng).view(B, Hq, S, S) if p > 0 else None
+    got, _ = attn_run(tuple(t.cuda() for t in host), dout.cuda(), pads, p, rng)
+    r, tol = tolerances(host, dout, pads, p, keep)
+    for name, t in zip(("dq", "dk", "dv"), got[1:]):
+        check(name, t, r[name][0], tol[name])
+    return r
+
+
+CASES = [
+    # B, S, Hq, Hkv, D, pads, p, scale of dout: one block of keys, several, walks that are cut or split
+    (2, 40, 4, 2, 64, [0, 7], 0.1, 1e-4),
+    (3, 192, 8, 2, 32, [0, 96, 191], 0.0, 1e-4),
+    (1, 1000, 4, 2, 64, [0], 0.0, 1e-2),
+    (1, 1300, 4, 2, 32, [9], 0.1, 1e-4),
+    (2, 1100, 6, 2, 64, [0, 300], 0.2, 1e-4),
+    (1, 2500, 2, 2, 64, [0], 0.0, 1e-3),
+    (1, 2055, 2, 1, 32, [5], 0.1, 1e-5),
+    (40, 130, 6, 2, 64, [(7 * b) % 130 for b in range(40)], 0.1, 1e-3),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"B{c[0]}_S{c[1]}_{c[2]}x{c[3]}_D{c[4]}_p{c[6]}_{c[7]}")
+def test_small_fp16_gradients(case):
+    B, S, Hq, Hkv, D, pads, p, size = case
+    host, dout, _, _ = attn_inputs(B, S, Hq, Hkv, D, FP16, seed=S)
+    run(host, (dout.double() * size).to(FP16), pads, p)
+
+
+@pytest.mark.gpu
+def test_fp16_gradients_of_samples_and_heads_of_different_size():
+    """Each sample's and KV head's gradients are as exact as if they stood alone."""
+    host, dout, _, _ = attn_inputs(3, 700, 4, 2, 64, FP16, seed=31)
+    size = torch.tensor([1.0, 1e-2, 1e-4]).view(3, 1, 1, 1) * torch.tensor([1.0, 1.0, 2e-2, 2e-2]).view(1, 1, 4, 1)
+    run(host, (dout.double() * size).to(FP16), [0, 3, 130], 0.1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,p", [(50, 0.0), (300, 0.1), (1100, 0.0)])
+def test_large_fp16_gradients(S, p):
+    """|dS| of up to some 1e5 is no overflow where the gradients themselves fit the type."""
+    host, dout, _, _ = attn_inputs(2, S, 4, 2, 64, FP16, seed=S)
+    host = ((host[0].double() * 0.3).to(FP16), (host[1].double() * 0.3).to(FP16), (host[2].double() * 100).to(FP16))
+    r = run(host, (dout.double() * 250).to(FP16), [0, 9], p)
+    assert max(r[n][0].abs().max().item() for n in ("dq", "dk", "dv")) < 60000
+
+
+@pytest.mark.gpu
+def test_fp16_gradients_without_any():
+    """All-zero gradients give zeros; a sample that is all padding has no row to take a maximum over."""
+    host, dout, _, _ = attn_inputs(2, 90, 4, 2, 32, FP16, seed=1)
+    got, _ = attn_run(tuple(t.cuda() for t in host), torch.zeros_like(dout).cuda(), [0, 90])
+    assert all((t == 0).all() for t in got[1:])
+    run(host, dout, [4, 90], 0.0)
+
+
+@pytest.mark.gpu
+def test_fp16_padding_does_not_set_the_scale():
+    """Infinities, NaN and huge values in padded rows change nothing."""
+    host, dout, dev, ddev = attn_inputs(2, 300, 4, 2, 64, FP16, seed=8, fused=False)
+    ddev = ddev * 1e-3
+    want, _ = attn_run(dev, ddev, [0, 70])
+    bad = [t.clone() for t in (*dev, ddev)]
+    for i, t in enumerate(bad):
+        t[1, :70] = (float("inf"), 6e4, float("nan"), 6e4)[i]
+    got, _ = attn_run(bad[:3], bad[3], [0, 70])
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
