@@ -19,8 +19,8 @@ def test_no_wait_without_a_limit():
     for body in re.split(r"__global__", text)[1:]:
         body = body[:body.index("\n}\n")]
         at = [m.start() for m in re.finditer(r"__syncthreads\(\)", body)]
-        if "TcShared* sh" not in body:
-            assert not at
+        if "TcShared* sh" not in body:  # no wait that may fail: every thread reaches every barrier
+            assert "mbar" not in body and "return;" not in body and "break;" not in body
             continue
         loops = [m.start() for m in re.finditer(r"while \(true\)", body)]
         assert len(at) == 2 and len(loops) == 1 and at[0] < loops[0] < at[1]
