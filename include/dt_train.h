@@ -41,8 +41,10 @@ extern "C" {
  * lse [B, Hq, S] fp32 receives the base-2 logarithm of each row's softmax
  * denominator (+inf for a row without keys), the backward call's input.
  * workspace: dt_attn_train_forward_workspace bytes, 16-byte aligned.  Values that
- * are not finite never leave padding; elsewhere they may reach earlier rows of
- * their block of 64 positions, as a zero weight times them is not a zero.
+ * are not finite never leave padding, their sample or their KV head.  Within those,
+ * a zero weight times them is not a zero: in k and v they may reach rows of o (and
+ * dq) up to 190 positions before them, in q and dout the dk and dv of keys up to
+ * 127 positions behind them.
  */
 int dt_attn_train_forward(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* pad_len,
                           int B, int S, int Hq, int Hkv, int D, int64_t q_sb, int64_t q_ss, int64_t q_sh,

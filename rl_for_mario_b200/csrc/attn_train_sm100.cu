@@ -1328,11 +1328,11 @@ __global__ void __launch_bounds__(kBwdThreads, kPerSm)
           tma_load_4d(smem + SM::OFF_B + tb * SH::TILE, &tmV, &sh->tile_full[tb], 0, t.g, t.k0, t.b);
         },
         [&](const KTile& t, int j, int st) {
-          const int c = gr.chunks > 1 ? j / t.per : 0, h0 = t.g * p.R + c * p.HC;
+          const int c = gr.chunks > 1 ? j / t.per : 0, h0 = c * p.HC;
           const int q0 = t.q0 + (t.split + j * gr.splits - c * t.per) * PT;
           mbar_arrive_expect_tx(&sh->blk_full[st], 2u * (uint32_t)(rows * SH::ROWB));
-          tma_load_4d(smem + SM::OFF_C + st * SH::BLK, &tmQ, &sh->blk_full[st], 0, h0, q0, t.b);
-          tma_load_4d(smem + SM::OFF_E + st * SH::BLK, &tmDO, &sh->blk_full[st], 0, h0, q0, t.b);
+          tma_load_5d(smem + SM::OFF_C + st * SH::BLK, &tmQ, &sh->blk_full[st], 0, h0, t.g, q0, t.b);
+          tma_load_5d(smem + SM::OFF_E + st * SH::BLK, &tmDO, &sh->blk_full[st], 0, h0, t.g, q0, t.b);
         });
   } else if (warp < 8) {
     const int half = warp >> 2, wq = warp & 3;

@@ -152,6 +152,21 @@ int api_device(int** status, int* cc_major, int* num_sms) {
   return DT_OK;
 }
 
+int api_encode_groups(CUtensorMap* map, const void* base, bool bf16, int B, int S, int Hkv, int R, int D, int64_t sb,
+                      int64_t ss, int64_t sh, uint32_t box_h, uint32_t box_s, const char* name) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return fail(DT_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  const cuuint64_t dims[5] = {(cuuint64_t)D, (cuuint64_t)R, (cuuint64_t)Hkv, (cuuint64_t)S, (cuuint64_t)B};
+  const cuuint64_t strides[4] = {(cuuint64_t)(2 * sh), (cuuint64_t)(2 * sh * R), (cuuint64_t)(2 * ss), (cuuint64_t)(2 * sb)};
+  const cuuint32_t box[5] = {(cuuint32_t)D, box_h, 1, box_s, 1}, estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         D == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DT_ERR_INVALID, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", name, (int)r);
+  return DT_OK;
+}
+
 int api_encode_bshd(CUtensorMap* map, const void* base, bool bf16, int B, int S, int H, int D, int64_t sb, int64_t ss,
                     int64_t sh, uint32_t box_h, uint32_t box_s, const char* name) {
   return encode_bshd(map, base, bf16, B, S, H, D, sb, ss, sh, box_h, box_s, name);

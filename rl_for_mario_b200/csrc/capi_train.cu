@@ -208,11 +208,12 @@ int dt_attn_train_backward(const void* dout, const void* q, const void* k, const
   dtk::AttnTrainMaps m;
   const uint32_t hc = (uint32_t)a.HC;
   if ((rc = dtk::api_encode_bshd(&m.q_tile, q, bf16, B, S, Hq, D, a.q_sb, a.q_ss, a.q_sh, hc, 128 / hc, "q")) ||
-      (rc = dtk::api_encode_bshd(&m.q_blk, q, bf16, B, S, Hq, D, a.q_sb, a.q_ss, a.q_sh, hc, 64 / hc, "q")) ||
+      (rc = dtk::api_encode_groups(&m.q_blk, q, bf16, B, S, Hkv, a.R, D, a.q_sb, a.q_ss, a.q_sh, hc, 64 / hc, "q")) ||
       (rc = dtk::api_encode_bshd(&m.do_tile, dout, bf16, B, S, Hq, D, a.do_sb, a.do_ss, a.do_sh, hc, 128 / hc,
                                  "dout")) ||
       (rc = dtk::api_encode_bshd(&m.o_tile, o, bf16, B, S, Hq, D, a.o_sb, a.o_ss, a.o_sh, hc, 128 / hc, "o")) ||
-      (rc = dtk::api_encode_bshd(&m.do_blk, dout, bf16, B, S, Hq, D, a.do_sb, a.do_ss, a.do_sh, hc, 64 / hc, "dout")) ||
+      (rc = dtk::api_encode_groups(&m.do_blk, dout, bf16, B, S, Hkv, a.R, D, a.do_sb, a.do_ss, a.do_sh, hc, 64 / hc,
+                                   "dout")) ||
       (rc = dtk::api_encode_bshd(&m.k_tile, k, bf16, B, S, Hkv, D, a.k_sb, a.k_ss, a.k_sh, 1, 128, "k")) ||
       (rc = dtk::api_encode_bshd(&m.k_blk, k, bf16, B, S, Hkv, D, a.k_sb, a.k_ss, a.k_sh, 1, 64, "k")) ||
       (rc = dtk::api_encode_bshd(&m.v_tile, v, bf16, B, S, Hkv, D, a.v_sb, a.v_ss, a.v_sh, 1, 128, "v")) ||

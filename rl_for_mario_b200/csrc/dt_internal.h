@@ -199,6 +199,10 @@ int api_device(int** status, int* cc_major, int* num_sms);
 // Tensor map over a 16-bit [B, S, H, D] tensor (element strides), boxes of box_s positions of box_h heads.
 int api_encode_bshd(CUtensorMap* map, const void* base, bool bf16, int B, int S, int H, int D, int64_t sb, int64_t ss,
                     int64_t sh, uint32_t box_h, uint32_t box_s, const char* name);
+// The same over a tensor whose heads come in Hkv groups of R: box_h heads of one group, of which those past the
+// group's end read as zero.
+int api_encode_groups(CUtensorMap* map, const void* base, bool bf16, int B, int S, int Hkv, int R, int D, int64_t sb,
+                      int64_t ss, int64_t sh, uint32_t box_h, uint32_t box_s, const char* name);
 
 struct DropoutParams {
   const void* x;
@@ -314,7 +318,8 @@ struct AttnTrainParams {
   float inv_keep;
 };
 // TMA maps over [B, S, H, D]: tiles of 128 rows and blocks of 64, of packed
-// (position, head) rows for q and dout, of positions of one head for k and v.
+// (position, head) rows for q and dout, of positions of one head for k and v.  The blocks of q and dout
+// are summed over (dk, dv), so theirs keep to a KV head's own query heads.
 struct AttnTrainMaps {
   CUtensorMap q_tile, do_tile, o_tile, q_blk, do_blk, k_tile, v_tile, k_blk, v_blk;
 };

@@ -115,3 +115,44 @@ def test_fp16_padding_does_not_set_the_scale():
         t[1, :70] = (float("inf"), 6e4, float("nan"), 6e4)[i]
     got, _ = attn_run(bad[:3], bad[3], [0, 70])
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,D,S", [(70, 32, 40), (65, 64, 130), (3, 64, 200)])
+def test_heads_do_not_mix(R, D, S):
+    """NaN in all of one KV head's rows (its query heads, keys, values and their gradient) leaves the other's results
+    as they were, also where the last chunk of 64 query heads is not full."""
+    _, _, dev, ddev = attn_inputs(2, S, 2 * R, 2, D, torch.bfloat16, seed=R, fused=False)
+    want, _ = attn_run(dev, ddev, [0, 5], 0.1, (5, 6, 7))
+    for g in (0, 1):
+        bad = [t.clone() for t in (*dev, ddev)]
+        for t in bad:
+            n = t.shape[2] // 2
+            t[:, :, g * n:(g + 1) * n] = float("nan")
+        got, _ = attn_run(bad[:3], bad[3], [0, 5], 0.1, (5, 6, 7))
+        for w, t in zip(want, got):
+            n = t.shape[2] // 2
+            keep = slice((1 - g) * n, (2 - g) * n)
+            assert torch.equal(w[:, :, keep], t[:, :, keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv,D,dt", [(1, 1, 64, torch.bfloat16), (4, 2, 32, FP16), (3, 1, 64, torch.bfloat16)])
+def test_how_far_values_that_are_not_finite_reach(Hq, Hkv, D, dt):
+    """A NaN in k or v: rows more than 190 positions before it keep their results; in q or dout: keys more than 127
+    positions behind it.  (fp16 gradients take one scale from a sample's finite values, which the NaN leaves.)"""
+    S, at = 700, 411
+    _, _, dev, ddev = attn_inputs(1, S, Hq, Hkv, D, dt, seed=9, fused=False)
+    want, _ = attn_run(dev, ddev, [3])
+    for which in range(4):
+        bad = [t.clone() for t in (*dev, ddev)]
+        bad[which][:, at] = float("nan")
+        got, _ = attn_run(bad[:3], bad[3], [3])
+        if which in (1, 2):
+            for w, t in zip(want[:2], got[:2]):
+                assert torch.isfinite(t[:, :at - 190]).all() and torch.isnan(t[:, at:]).all()
+                assert torch.equal(w[:, :at - 190], t[:, :at - 190]) or dt == FP16
+        else:
+            for w, t in zip(want[2:], got[2:]):
+                assert torch.isfinite(t[:, at + 128:]).all()
+                assert torch.equal(w[:, at + 128:], t[:, at + 128:]) or dt == FP16
