@@ -360,11 +360,14 @@ __global__ void __launch_bounds__(MAXT, 1) residual_norm_bwd_kernel(const __grid
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (POST) xn.p[i] = fmul2(xn.p[i], both(r_post));  // from here on the normalised x
+        // Dropped: x itself without a post norm (it counts as 0 whatever it was, in the gate's gradient as well).
+        auto drop = [&](float2& v) {
+          v.x = (m >> (2 * i)) & 1u ? v.x : 0.f;
+          v.y = (m >> (2 * i + 1)) & 1u ? v.y : 0.f;
+        };
+        if constexpr (DROP && !POST) drop(xn.p[i]);
         float2 gv = fmul2(xn.p[i], cw.p[i]);
-        if constexpr (DROP) {
-          gv.x = (m >> (2 * i)) & 1u ? gv.x : 0.f;
-          gv.y = (m >> (2 * i + 1)) & 1u ? gv.y : 0.f;
-        }
+        if constexpr (DROP && POST) drop(gv);
         h.p[i] = fmul2(fadd2(h.p[i], gv), both(r_pre));  // the normalised h
         a_pre.p[i] = ffma2(t.p[i], h.p[i], a_pre.p[i]);
         t.p[i] = fmul2(t.p[i], wpre.p[i]);

@@ -156,3 +156,27 @@ def test_how_far_values_that_are_not_finite_reach(Hq, Hkv, D, dt):
             for w, t in zip(want[2:], got[2:]):
                 assert torch.isfinite(t[:, at + 128:]).all()
                 assert torch.equal(w[:, at + 128:], t[:, at + 128:]) or dt == FP16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["none", "channel", "sample", "token"])
+@pytest.mark.parametrize("H,dt", [(264, torch.bfloat16), (130, torch.float32), (64, FP16), (1001, torch.float32)])
+def test_residual_norm_drops_whatever_the_value(gate, H, dt):
+    """NaN and infinities of x where it is dropped give what zeros there give, in every result and gradient."""
+    from test_train_ops_gpu import norm_inputs, norm_run
+
+    B, S = 3, 20
+    gates = {"none": 0, "channel": 1, "sample": B, "token": B * S}[gate]
+    shape = {"none": None, "channel": (H,), "sample": (B, 1, H), "token": (B, S, H)}[gate]
+    host = norm_inputs(B * S, H, dt, False, gates, seed=H)
+    rng = (31, 4, 2)
+    dropped = ref.keep_factor(B * S, H, 0.3, *rng) == 0
+    zero, bad = dict(host), dict(host)
+    zero["x"] = host["x"].masked_fill(dropped, 0.0)
+    odd = torch.where(torch.arange(H) % 2 == 0, float("nan"), float("inf")).to(dt)
+    bad["x"] = torch.where(dropped, odd, host["x"])
+    a, b = (norm_run(h, shape, p=0.3, rng=rng, shape=(B, S, H)) for h in (zero, bad))
+    for x, y in zip(a, b):
+        assert (x is None) == (y is None)
+        if x is not None:
+            assert torch.isfinite(y).all() and torch.equal(x, y)
