@@ -41,6 +41,16 @@ from .cache import LayerKV, dense_layer
 Tensor = torch.Tensor
 
 
+def left_padding(mask: Tensor, length: int, check: bool) -> Tensor:
+    """pad_len [B] of a [B, length] mask; with ``check`` a mask that is not zeros then ones is refused (a host read)."""
+    pad = kernels.pad_len_from_mask(mask, length)
+    if check:
+        want = torch.arange(length, device=mask.device)[None] >= pad[:, None]
+        if not torch.equal(want, mask != 0):
+            raise ValueError("attention_mask is not a left-padding mask (zeros then ones per row)")
+    return pad
+
+
 class FastDTAttention(nn.Module):
     def __init__(self, config, compute_dtype: Optional[torch.dtype] = None, check_masks: bool = False):
         super().__init__()
@@ -98,12 +108,7 @@ class FastDTAttention(nn.Module):
             return None
         if mask.dim() != 2 or mask.shape[1] != length:
             raise ValueError(f"attention_mask must be [B, {length}], got {tuple(mask.shape)}")
-        pad = kernels.pad_len_from_mask(mask, length)
-        if self.check_masks:
-            want = torch.arange(length, device=mask.device)[None] >= pad[:, None]
-            if not torch.equal(want, mask != 0):
-                raise ValueError("attention_mask is not a left-padding mask (zeros then ones per row)")
-        return pad
+        return left_padding(mask, length, self.check_masks)
 
     def set_fused_norm(self, norm: Optional[nn.Module]) -> None:
         """Fuses ``norm`` (an RMSNorm with ``weight`` and ``eps``) into the Q/K/V

@@ -22,7 +22,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import kernels, training
-from .attention import FastDTAttention
+from .attention import FastDTAttention, left_padding
 from .cache import LayerKV, PagedKVCache
 
 Tensor = torch.Tensor
@@ -383,7 +383,8 @@ class DTBackbone(nn.Module):
         if self.train_form and torch.is_grad_enabled() and past_key_values is None and not use_cache:
             pad = None
             if attention_mask is not None:
-                pad = 3 * kernels.pad_len_from_mask(attention_mask, T)
+                check = any(layer.self_attn.check_masks for layer in self.layers)
+                pad = 3 * left_padding(attention_mask, T, check)
             return self.run_training(self.embed_tokens(states, actions, returns_to_go, timesteps), pad)
         h = self.embed(states, actions, returns_to_go, timesteps)
         mask3 = None
