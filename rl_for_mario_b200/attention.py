@@ -174,7 +174,7 @@ class FastDTAttention(nn.Module):
     # ----------------------------------------------------------------- training
     def fuse_training(self, on: bool = True, seed: int = 0, site: int = 0) -> "FastDTAttention":
         """Runs forward() on the training operators whenever autograd is on and no cache takes part
-        (bf16 / fp16 compute).  ``seed``: of the module's own dropout generator; ``site``: the first of
+        (bf16 / fp16 compute: the module's type, autocast's or compute_dtype).  ``seed``: of the module's own dropout generator; ``site``: the first of
         two dropout sites (attention weights, output), which modules that share a seed keep apart.
 
         Rows of padded positions come out of the attention as zeros there and pass no gradient (the
@@ -192,11 +192,15 @@ class FastDTAttention(nn.Module):
 
     def attend_training(self, x: Tensor, position_embeddings: Tuple[Tensor, Tensor], pad_len: Optional[Tensor],
                         rng: Optional[Tensor]) -> Tensor:
-        """Projections, attention and o_proj of the training form, without the dropout of the output."""
-        kd = self._kernel_dtype(x)
-        if kd == torch.float32:
-            raise TypeError("the training form of FastDTAttention computes in bf16 or fp16: convert the model or give "
-                            "compute_dtype")
+        """Projections, attention and o_proj of the training form, without the dropout of the output.
+
+        Under autocast the projections run in autocast's type, as nn.Linear's do, and so does the attention (unless
+        compute_dtype says otherwise)."""
+        ac = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None
+        kd = self.compute_dtype or ac or x.dtype
+        if kd not in (torch.bfloat16, torch.float16):
+            raise TypeError("the training form of FastDTAttention computes in bf16 or fp16: convert the model, use "
+                            "autocast or give compute_dtype")
         if self.rope_rounding != "fp32":
             raise ValueError("the training form rotates q and k in fp32: rope_rounding must be 'fp32'")
         B, S, _ = x.shape
@@ -204,10 +208,14 @@ class FastDTAttention(nn.Module):
         cos, sin = position_embeddings
         p = self.dropout if self.training else 0.0
         ws = (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
-        if (kd == x.dtype == ws[0].dtype and D in (32, 64) and x.shape[-1] % 8 == 0 and x.data_ptr() % 16 == 0
-                and x.stride(-1) == 1 and not torch.is_autocast_enabled()
+        if ac == kd:
+            xk, ws = x.to(ac), [w.to(ac) for w in ws]
+        else:
+            xk = x
+        if (kd == xk.dtype == ws[0].dtype and ac in (None, kd) and D in (32, 64) and xk.shape[-1] % 8 == 0
+                and xk.data_ptr() % 16 == 0 and xk.stride(-1) == 1
                 and all(m.bias is None for m in (self.q_proj, self.k_proj, self.v_proj))):
-            qkv = training.qkv_rope(x, torch.cat(ws), cos, sin, (Hq + Hkv) * D, D)
+            qkv = training.qkv_rope(xk, torch.cat(tuple(ws)), cos, sin, (Hq + Hkv) * D, D)
             out = training.attention_qkv(qkv.view(B, S, Hq + 2 * Hkv, D), Hq, Hkv, pad_len, p=p, rng=rng,
                                          site=self.train_site)
         else:
@@ -220,7 +228,8 @@ class FastDTAttention(nn.Module):
             k = rotate(self.k_proj(x).view(B, S, Hkv, D))
             v = self.v_proj(x).view(B, S, Hkv, D).to(kd)
             out = training.attention(q, k, v, pad_len, p=p, rng=rng, site=self.train_site)
-        return self.o_proj(out.reshape(B, S, Hq * D).to(x.dtype))
+        out = out.reshape(B, S, Hq * D)
+        return self.o_proj(out if ac else out.to(x.dtype))
 
     # ------------------------------------------------------------------ forward
     def forward(self, x: Tensor, position_embeddings: Tuple[Tensor, Tensor],
@@ -240,6 +249,9 @@ class FastDTAttention(nn.Module):
                 x = self._fused_norm(x)
             y = self.attend_training(x, position_embeddings, self._pad_len(attention_mask, seq_len), rng)
             if p > 0:
+                if residual is not None and residual.dtype != y.dtype:  # as residual + y would (autocast)
+                    dt = torch.promote_types(residual.dtype, y.dtype)
+                    y, residual = y.to(dt), residual.to(dt)
                 return training.dropout(y, p, rng, self.train_site + 1, residual), None
             return (y if residual is None else residual + y), None
         kd = self._kernel_dtype(x)

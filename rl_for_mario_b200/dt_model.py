@@ -146,9 +146,11 @@ class DTBlock(nn.Module):
         attn, mlp, post = self.self_attn, self.mlp, self.post_attention_layernorm
         p_attn, p_mlp = self.training_rates()
         y = attn.attend_training(n, position_embeddings, pad_len, rng)
-        h, n = training.residual_norm(y, h, post.weight, post.eps, p=p_attn, rng=rng, site=attn.train_site + 1)
+        # Under autocast the products come out in its type and the stream keeps the weights'.
+        h, n = training.residual_norm(y.to(h.dtype), h, post.weight, post.eps, p=p_attn, rng=rng,
+                                      site=attn.train_site + 1)
         y = mlp.down_proj(F.silu(mlp.gate_proj(n)) * mlp.up_proj(n))
-        return training.residual_norm(y, h, next_norm.weight, next_norm.eps, p=p_mlp, rng=rng,
+        return training.residual_norm(y.to(h.dtype), h, next_norm.weight, next_norm.eps, p=p_mlp, rng=rng,
                                       site=attn.train_site + 2)
 
     def training_rates(self) -> Tuple[float, float]:
@@ -478,10 +480,10 @@ class MarioDT(nn.Module):
         return self
 
     def fuse_training(self, on: bool = True, seed: int = 0) -> "MarioDT":
-        """Trains a bf16 / fp16 model on the training operators (training.py): with autograd on and
-        no cache, forward() runs attention with its gradient, every residual add as one kernel with
-        the dropout before it and the norm behind it, and dropout whose masks are never stored, from
-        a generator of ``seed`` (model.dropout_state(), to be saved with a checkpoint).  Without
+        """Trains a model in bf16 / fp16, its own type or autocast's, on the training operators
+        (training.py): with autograd on and no cache, forward() runs attention with its gradient,
+        every residual add as one kernel with the dropout before it and the norm behind it, and
+        dropout whose masks are never stored, from a generator of ``seed`` (model.dropout_state(), to be saved with a checkpoint).  Without
         autograd (validation, act()) the inference kernels run as before.  Ranks of a data-parallel job
         take seeds of their own.  A forward pass that is run again for its backward pass (activation
         checkpointing of the whole model) would draw other masks: checkpoint inside, with the same rng.
