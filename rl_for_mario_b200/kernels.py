@@ -27,8 +27,16 @@ def _dtype_code(t: Tensor) -> int:
         raise TypeError(f"unsupported dtype {t.dtype}") from None
 
 
+# torch's own shortcuts past the objects of current_stream() and current_device() (a microsecond a call), where this
+# torch has them.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
 def _stream_ptr(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)  # current_stream(device).cuda_stream, without its objects
+    if _raw_stream is None or device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
 
 
 def _ptr(t: Optional[Tensor]) -> Optional[int]:
@@ -534,7 +542,7 @@ def _launch(name: str, dev: torch.device, *args) -> None:
     """Calls the entry point on the device's current stream (its last argument), with the device
     current: the library launches there."""
     fn = getattr(_lib.load(), name)
-    had = torch._C._cuda_getDevice()
+    had = _raw_device() if _raw_device is not None else torch.cuda.current_device()
     if had == dev.index:
         rc = fn(*args, _stream_ptr(dev))
     else:

@@ -180,3 +180,10 @@ def test_residual_norm_drops_whatever_the_value(gate, H, dt):
         assert (x is None) == (y is None)
         if x is not None:
             assert torch.isfinite(y).all() and torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_status_of_a_device_without_an_index():
+    from rl_for_mario_b200.kernels import device_status
+
+    assert device_status(torch.device("cuda")) == 0 and device_status() == 0

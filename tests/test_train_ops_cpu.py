@@ -123,3 +123,39 @@ def test_generator_words():
         c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
         k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
     assert base[0].tolist() == [h for v in c for h in (v & 0xFFFF, v >> 16)]
+
+
+def test_streams_and_devices_of_a_launch(monkeypatch):
+    """The stream of a device named with and without an index, with and without torch's private shortcuts; a launch
+    makes its tensors' device current and puts the other one back, also when the call raises."""
+    from types import SimpleNamespace
+
+    from rl_for_mario_b200 import kernels as K
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d: SimpleNamespace(cuda_stream=100 + (d.index or 0)))
+    monkeypatch.setattr(K, "_raw_stream", lambda i: 100 + i)
+    one, bare = torch.device("cuda", 1), torch.device("cuda")
+    assert K._stream_ptr(one) == 101 and K._stream_ptr(bare) == 100
+    monkeypatch.setattr(K, "_raw_stream", None)
+    assert K._stream_ptr(one) == 101 and K._stream_ptr(bare) == 100
+
+    now, seen = [0], []
+
+    def entry(*args):
+        seen.append((now[0], args))
+        if args[0] == "raise":
+            raise RuntimeError("from the call")
+        return 0
+
+    monkeypatch.setattr(K._lib, "load", lambda: SimpleNamespace(entry=entry))
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: now.__setitem__(0, d if isinstance(d, int) else d.index))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    for raw in (lambda: now[0], None):
+        monkeypatch.setattr(K, "_raw_device", raw)
+        K._launch("entry", one, "a")
+        assert seen[-1] == (1, ("a", 101)) and now[0] == 0
+        with pytest.raises(RuntimeError, match="from the call"):
+            K._launch("entry", one, "raise")
+        assert now[0] == 0
+        K._launch("entry", torch.device("cuda", 0), "b")
+        assert seen[-1] == (0, ("b", 100)) and now[0] == 0
