@@ -123,8 +123,9 @@ int dt_residual_norm_backward(const void* dh, int64_t dh_stride, const void* dn,
 /*
  * y = residual + dropout(x) (residual null: 0) over rows [rows, cols]; the
  * gradient of x is the same call on the gradient of y without a residual.
- * bf16, fp16 or fp32, any strides and alignment (contiguous 16-byte aligned
- * rows of a multiple of 8 elements run faster); y overlaps neither input.
+ * bf16, fp16 or fp32, 1 <= cols <= 2^31 - 256, any strides and alignment
+ * (contiguous 16-byte aligned rows of a multiple of 8 elements run faster); y
+ * overlaps neither input.
  */
 int dt_dropout(const void* x, int64_t x_stride, const void* residual, int64_t res_stride, void* y, int64_t y_stride,
                int64_t rows, int cols, double p, const int64_t* rng, uint32_t site, int dtype, void* stream);

@@ -112,6 +112,7 @@ int64_t attn_workspace(int B, int S, int Hq, int Hkv, int D, bool drop, int sms)
               (int64_t)B * Hkv * dtk::attn_train_grad_parts(S, Hq / Hkv, D) * 2);
 }
 
+constexpr int kMaxCols = 0x7fffff00;  // of dropout: columns are numbered in 32 bits, in pieces of 256
 constexpr int kMaxHidden = 8192;  // 32 warps of 256 columns: one block holds a row
 
 int64_t part_elems(const dtk::ResidualNormPlan& q, int H, int64_t gate_rows, bool post) {
@@ -361,6 +362,7 @@ int dt_dropout(const void* x, int64_t x_stride, const void* residual, int64_t re
   int rc = check_dtype(fn, dtype);
   if (rc) return rc;
   if ((rc = check_rows(fn, x, rows, cols, "rows", "cols"))) return rc;
+  if (cols > kMaxCols) return api_fail(DT_ERR_UNSUPPORTED, "%s: %d columns, above %d", fn, cols, kMaxCols);
   if (!y) return api_fail(DT_ERR_INVALID, "%s: null y", fn);
   if ((rc = check_elem_aligned(fn, dtype, {x, residual, y}))) return rc;
   dtk::DropoutParams a{};

@@ -703,6 +703,12 @@ def rope_grad_(g: Tensor, cos: Tensor, sin: Tensor, rope_cols: int, head_dim: in
     return g
 
 
+def _check_width(n: int) -> None:
+    """Widths go through the C ABI as 32-bit integers, which ctypes cuts without a word."""
+    if n >= 2 ** 31:
+        raise ValueError(f"rows of {n} elements are too wide: give them as more rows of fewer than 2^31 - 255")
+
+
 def _rows2d(t: Tensor) -> Tuple[Tensor, int]:
     """t as [rows, K] with a contiguous last dimension (a copy when no view exists), and its row stride."""
     K = t.shape[-1]
@@ -738,6 +744,7 @@ def _check_residual_norm(x, residual, pre_weight, post_weight, gate):
         raise ValueError("x must have a last dimension")
     if dt not in _DTYPES:
         raise TypeError(f"unsupported dtype {dt}")
+    _check_width(shape[-1])
     if residual is not None and residual.shape != shape:
         raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(shape)}")
     if pre_weight.shape != shape[-1:] or not pre_weight.is_contiguous():
@@ -830,6 +837,7 @@ def dropout_forward(x: Tensor, p: float, rng: Optional[Tensor], site: int = 0,
     dev = _same_device(x, rng, residual)
     if x.dim() < 1 or x.dtype not in _DTYPES:
         raise TypeError(f"dropout takes bf16, fp16 or fp32 tensors of one or more dimensions (got {x.dtype})")
+    _check_width(x.shape[-1])
     p = _check_dropout(p, rng, site)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have x's shape and dtype")

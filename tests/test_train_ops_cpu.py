@@ -159,3 +159,20 @@ def test_streams_and_devices_of_a_launch(monkeypatch):
         assert now[0] == 0
         K._launch("entry", torch.device("cuda", 0), "b")
         assert seen[-1] == (0, ("b", 100)) and now[0] == 0
+
+
+def test_widths_beyond_32_bits_are_refused(monkeypatch):
+    """2^32 + 8 columns would reach the library as 8; from 2^31 - 255 on the kernel's column numbers would overflow."""
+    from rl_for_mario_b200 import _lib, kernels as K
+
+    lib, a = _lib.load(), 4096
+    for cols in (2 ** 31 - 255, 2 ** 31 - 1):
+        assert lib.dt_dropout(a, 8, None, 0, a, 8, 1, cols, 0.0, None, 0, 0, None) == _lib.DT_ERR_UNSUPPORTED
+    rows = torch.empty(1, device="meta", dtype=torch.bfloat16)
+    for n in (2 ** 31, 2 ** 32 + 8):
+        wide = rows.expand(2, n)
+        with pytest.raises(ValueError, match="too wide"):
+            K._check_residual_norm(wide, None, wide[0], None, None)
+        monkeypatch.setattr(K, "_same_device", lambda *t: torch.device("cuda", 0))
+        with pytest.raises(ValueError, match="too wide"):
+            K.dropout_forward(wide, 0.0, None)
