@@ -5,6 +5,7 @@ library itself never allocates), and launches on torch's current CUDA stream.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 import struct
@@ -615,8 +616,9 @@ def _check_attn_train(q: Tensor, k: Tensor, v: Tensor, pad_len: Optional[Tensor]
             raise ValueError(f"pad_len must be [{B}] (got {tuple(pad_len.shape)})")
         if pad_len.dtype != torch.int32 or not pad_len.is_contiguous():
             pad_len = pad_len.to(torch.int32).contiguous()
-    if scale is not None and not scale > 0:
-        raise ValueError(f"scale must be positive (got {scale})")
+    # As the kernels get it: a scale that fp32 holds as 0 would mean the default one.
+    if scale is not None and not 0.0 < ctypes.c_float(scale).value < math.inf:
+        raise ValueError(f"scale must be positive and finite in fp32 (got {scale})")
     return pad_len, B, S, Hq, kshape[2], D
 
 

@@ -176,3 +176,17 @@ def test_widths_beyond_32_bits_are_refused(monkeypatch):
         monkeypatch.setattr(K, "_same_device", lambda *t: torch.device("cuda", 0))
         with pytest.raises(ValueError, match="too wide"):
             K.dropout_forward(wide, 0.0, None)
+
+
+def heads(h):
+    return torch.zeros(1, 4, h, 32, dtype=torch.bfloat16)
+
+
+def test_scales_that_fp32_does_not_hold():
+    """A scale that fp32 rounds to 0 stood for the default one."""
+    from rl_for_mario_b200 import kernels as K
+
+    for scale in (1e-50, -1.0, float("nan"), float("inf"), 1e39):
+        with pytest.raises(ValueError, match="scale"):
+            K._check_attn_train(heads(4), heads(2), heads(2), None, scale)
+    assert K._check_attn_train(heads(4), heads(2), heads(2), None, 1e-30)[1:] == (1, 4, 4, 2, 32)
