@@ -619,6 +619,8 @@ def _check_attn_train(q: Tensor, k: Tensor, v: Tensor, pad_len: Optional[Tensor]
     # As the kernels get it: a scale that fp32 holds as 0 would mean the default one.
     if scale is not None and not 0.0 < ctypes.c_float(scale).value < math.inf:
         raise ValueError(f"scale must be positive and finite in fp32 (got {scale})")
+    if Hq < 1 or kshape[2] < 1 or Hq % kshape[2]:
+        raise ValueError(f"{Hq} query heads are not a multiple of {kshape[2]} KV heads")
     return pad_len, B, S, Hq, kshape[2], D
 
 

@@ -190,3 +190,12 @@ def test_scales_that_fp32_does_not_hold():
         with pytest.raises(ValueError, match="scale"):
             K._check_attn_train(heads(4), heads(2), heads(2), None, scale)
     assert K._check_attn_train(heads(4), heads(2), heads(2), None, 1e-30)[1:] == (1, 4, 4, 2, 32)
+
+
+def test_numbers_of_heads():
+    """No query heads left dk and dv unwritten, whatever the number of KV heads."""
+    from rl_for_mario_b200 import kernels as K
+
+    for hq, hkv in ((0, 2), (4, 0), (0, 0), (3, 2), (2, 4)):
+        with pytest.raises(ValueError, match="heads"):
+            K._check_attn_train(heads(hq), heads(hkv), heads(hkv), None, None)
