@@ -246,6 +246,8 @@ class FastDTAttention(nn.Module):
             p = self.dropout if self.training else 0.0
             rng = self.dropout_state().draw() if p > 0 else None
             if raw_input:
+                if self._fused_norm is None:
+                    raise ValueError("raw_input=True needs set_fused_norm()")
                 x = self._fused_norm(x)
             y = self.attend_training(x, position_embeddings, self._pad_len(attention_mask, seq_len), rng)
             if p > 0:

@@ -124,3 +124,16 @@ def test_model_step_under_autocast_reaches_every_parameter(ac):
     # Outside autocast an fp32 model is refused as before.
     with pytest.raises(TypeError, match="training form"):
         model(**data, action_targets=targets)
+
+
+@pytest.mark.gpu
+def test_raw_input_of_a_module_without_a_norm_is_refused():
+    from rl_for_mario_b200.attention import FastDTAttention
+    from rl_for_mario_b200.dt_model import DTConfig, rope_tables
+
+    cfg = DTConfig(hidden_size=128, num_attention_heads=4, num_key_value_heads=2, context_len=8)
+    m = FastDTAttention(cfg).cuda().bfloat16()
+    x, pe = torch.zeros(1, 6, 128, device="cuda", dtype=BF16), tuple(t.cuda() for t in rope_tables(32, 6, 1e4))
+    for on in (False, True):
+        with pytest.raises(ValueError, match="set_fused_norm"):
+            m.fuse_training(on)(x, pe, raw_input=True)
