@@ -243,12 +243,12 @@ class FastDTAttention(nn.Module):
             raise ValueError("FastDTAttention runs on CUDA only (no CPU path)")
         bsz, seq_len, _ = x.shape
         if self.train_form and torch.is_grad_enabled() and past_key_value is None and not use_cache:
-            p = self.dropout if self.training else 0.0
-            rng = self.dropout_state().draw() if p > 0 else None
             if raw_input:
                 if self._fused_norm is None:
                     raise ValueError("raw_input=True needs set_fused_norm()")
                 x = self._fused_norm(x)
+            p = self.dropout if self.training else 0.0
+            rng = self.dropout_state().draw() if p > 0 else None
             y = self.attend_training(x, position_embeddings, self._pad_len(attention_mask, seq_len), rng)
             if p > 0:
                 if residual is not None and residual.dtype != y.dtype:  # as residual + y would (autocast)

@@ -137,3 +137,4 @@ def test_raw_input_of_a_module_without_a_norm_is_refused():
     for on in (False, True):
         with pytest.raises(ValueError, match="set_fused_norm"):
             m.fuse_training(on)(x, pe, raw_input=True)
+    assert m.dropout_state().state_dict()["step"] == 0  # a refused call draws nothing
