@@ -52,6 +52,14 @@ def left_padding(mask: Tensor, length: int, check: bool) -> Tensor:
 
 
 class FastDTAttention(nn.Module):
+    # Training form (fuse_training): off, the module's own generator, and the number that
+    # tells this module's dropout from other modules'.  Of the class, so that a module that
+    # was pickled without them runs as it did.
+    train_form = False
+    train_seed = 0
+    train_site = 0
+    _dropout_state: Optional["training.DropoutState"] = None
+
     def __init__(self, config, compute_dtype: Optional[torch.dtype] = None, check_masks: bool = False):
         super().__init__()
         self.num_key_value_heads = (config.num_attention_heads if config.num_key_value_heads is None
@@ -81,12 +89,6 @@ class FastDTAttention(nn.Module):
         object.__setattr__(self, "_fused_norm", None)
         object.__setattr__(self, "_fused_w", None)
         object.__setattr__(self, "_fused_key", None)
-        # Training form (fuse_training): off, the module's own generator, and the
-        # number that tells this module's dropout from other modules'.
-        self.train_form = False
-        self.train_seed = 0
-        self.train_site = 0
-        object.__setattr__(self, "_dropout_state", None)
 
     @classmethod
     def from_reference(cls, ref_attn: nn.Module, config, **kw) -> "FastDTAttention":

@@ -22,3 +22,14 @@ def test_training_form_checks_masks_where_a_layer_asks_for_it(mask):
     # A mask that is one is taken: the refusal that follows is the kernels', of CPU tensors.
     with pytest.raises(ValueError, match="CUDA"):
         m(**data, attention_mask=torch.tensor([[0, 0, 1, 1], [0, 1, 1, 1]]))
+
+
+def test_modules_pickled_before_the_training_form():
+    """A module whose state holds nothing of the training form is one that is not in it."""
+    m = model().model.layers[0].self_attn
+    for name in ("train_form", "train_seed", "train_site", "_dropout_state"):
+        m.__dict__.pop(name, None)
+    with pytest.raises(ValueError, match="CUDA"):  # past the switch: the refusal is the module's own, of CPU tensors
+        m(torch.zeros(1, 3, 128), (torch.zeros(3, 32), torch.zeros(3, 32)))
+    assert m.train_form is False and m.train_site == 0
+    assert m.dropout_state().state_dict() == {"seed": 0, "step": 0}
