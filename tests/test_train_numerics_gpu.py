@@ -187,3 +187,31 @@ def test_status_of_a_device_without_an_index():
     from rl_for_mario_b200.kernels import device_status
 
     assert device_status(torch.device("cuda")) == 0 and device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,D,dt,p", [(20, 32, torch.bfloat16, 0.0), (90, 64, torch.bfloat16, 0.2), (150, 32, FP16, 0.0)])
+def test_attention_gradient_along_itself(S, D, dt, p):
+    """The slope of the float64 forward pass along each gradient, by central differences: it is the gradient's norm.
+    An element off by t moves the kernels' slope along d by t |d|, all of them by |t| |d| = |t| at most (Cauchy and
+    Schwarz), t the elementwise bound: a few u of the norm."""
+    B, Hq, Hkv, pads, rng = 2, 4, 2, [0, 6], (77, 5, 3)
+    host, dout, _, _ = attn_inputs(B, S, Hq, Hkv, D, dt, seed=S)
+    keep = ref.keep_factor(B * Hq * S, S, p, *rng).view(B, Hq, S, S) if p > 0 else None
+    got, _ = attn_run(tuple(t.cuda() for t in host), dout.cuda(), pads, p, rng)
+    r = ref.attention(*host, dout, pads, None, keep)
+    u = torch.finfo(dt).eps / 2
+    for i, name in enumerate(("dq", "dk", "dv")):
+        want, mag = r[name]
+        tol = u * 1.01 * (want.abs() + mag) + SLACK * mag + (2.0 ** -22 if dt == FP16 else 0.0)
+        if name != "dv":
+            tol = tol + u * 1.01 * r[name + "_delta"][0] + SLACK * r[name + "_delta"][1]
+        d, e, ends = want / want.norm(), 1e-4, []
+        for sign in (1, -1):
+            moved = [t.double() for t in host]
+            moved[i] = moved[i] + sign * e * d
+            ends.append((ref.attention(*moved, dout, pads, None, keep)["out"][0] * dout.double()).sum())
+        slope = ((ends[0] - ends[1]) / (2 * e)).item()
+        bound = tol.norm().item() + 1e-6 * want.norm().item()
+        assert bound < 0.08 * want.norm().item()  # so a gradient wrong by a tenth fails
+        assert abs((got[1 + i].double().cpu() * d).sum().item() - slope) <= bound, name
