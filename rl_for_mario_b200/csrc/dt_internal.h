@@ -277,7 +277,7 @@ struct ResidualNormPlan {
   long long chunks, chunk_rows, chunks_per_span, span_rows, grid;
   int groups;  // rows of a block
 };
-// ahead: the backward kernel holds rows ahead (residual_norm_ring says which calls).
+// ring: the backward kernel's rows arrive in a ring (residual_norm_ring says which calls).
 ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, bool ring, int num_sms);
 bool residual_norm_ring(const ResidualNormParams& p, int dtype);
 cudaError_t launch_residual_norm_fwd_sm100(ResidualNormParams p, int dtype, int num_sms, cudaStream_t st);

@@ -40,9 +40,11 @@ namespace dtk {
 
 namespace {
 
-// 16-bit rows of vectors are fetched before their turn, others where they are used
-// (fp32 rows held ahead take the registers of one block in four: 21 and 30 us
-// against 16 and 27, 4,257 rows of 1,001).
+// 16-bit rows of vectors are fetched before their turn, others where they are used:
+// fp32 rows held ahead take the registers of one block in four (forward, rows of vectors,
+// both norms: 15.3 us against 18.4 for 4,257 rows of 1,024, 22.8 against 26.7 for 1,200 of
+// 4,096, but 71.0 against 67.3 for 36,864 of 768; element by element 16 against 21 for
+// 4,257 of 1,001).
 template <int DT, bool VEC>
 constexpr bool kAhead = VEC && DT != 2;
 
@@ -548,8 +550,10 @@ bool can_vector(const ResidualNormParams& p, int dtype, bool bwd) {
 // `warps` warps holds.
 static int rn_wpr(int H) { return (H + 255) / 256; }
 static int rn_groups(int H, int warps) { return rn_wpr(H) >= warps ? 1 : warps / rn_wpr(H); }
-// Warps of a block: with a ring of rows on their way one block of 16 warps fills an
-// SM, without one four blocks of 8.
+// Warps of a block of the backward pass: with a ring of rows on their way one block of
+// 16 warps fills an SM, without one two blocks of 8 (up to 128 registers a thread; planned
+// for four, the grid ran in two waves and left twice the parts: 48 x 768 fp32 rows of 768
+// 139 + 7 us instead of 125 + 4, 4,257 of 1,001 27.5 + 4.4 instead of 26 + 3.3).
 constexpr int kFwdWarps = 8;
 static int rn_bwd_warps(bool ring) { return ring ? 16 : 8; }
 
@@ -561,7 +565,7 @@ ResidualNormPlan residual_norm_plan(long long M, int H, long long gate_rows, boo
   q.groups = groups;
   q.span_rows = gate_rows > 1 ? gate_rows : M;
   const long long spans = M / q.span_rows;
-  const int fit = (ring ? 16 : 32) / warps;
+  const int fit = 16 / warps;  // blocks on an SM
   const long long want = (long long)num_sms * (fit < 1 ? 1 : fit);
   const long long most = (q.span_rows + groups - 1) / groups;
   long long per_span = want / spans;

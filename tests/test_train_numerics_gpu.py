@@ -215,3 +215,18 @@ def test_attention_gradient_along_itself(S, D, dt, p):
         bound = tol.norm().item() + 1e-6 * want.norm().item()
         assert bound < 0.08 * want.norm().item()  # so a gradient wrong by a tenth fails
         assert abs((got[1 + i].double().cpu() * d).sum().item() - slope) <= bound, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [96, 257, 1001, 4096, 5000])
+def test_residual_norm_parts_are_one_wave(H):
+    """The backward pass leaves one partial row of each weight's gradient for each block that the GPU holds at a time:
+    sixteen warps an SM, a row's ceil(H / 256) warps in blocks of eight or more."""
+    from rl_for_mario_b200 import _lib
+
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    wpr = -(-H // 256)
+    block = wpr * max(1, 8 // wpr)
+    rows = sms * max(1, 16 // block)
+    need = _lib.load().dt_residual_norm_workspace(100000, H, 0, 1)
+    assert 0 < need <= 4 * (2 * rows * (-(-H // 4) * 4) + 16)
