@@ -58,13 +58,15 @@
 // a wait on its mbarrier.
 //
 // What bounds it.  96 x 768, 12 / 4 heads of 64, padding up to half, bf16, p = 0.1:
-// forward 215 us, dq 240, dk and dv 268 (0.18 PFLOP of products that count: 246
-// TFLOP/s); half that batch without dropout 81, 93 and 132 us, with it 120, 136 and
-// 164.  No unit is full: the tensor pipe is busy 20 to 26 % of the time without
+// forward 214 us, dq 246, dk and dv 272 (0.18 PFLOP of products that count: 243
+// TFLOP/s); half that batch without dropout 80, 93 and 138 us, with it 118, 136 and
+// 166.  No unit is full: the tensor pipe is busy 20 to 27 % of the time without
 // dropout (an MMA of N = 64 costs about 50 cycles whatever its K: 400, 600 and 800 for
-// a 128 x 64 block), the exponentials' unit 22 to 39 %, and 41 to 46 % of the issue
-// slots are used (with dropout 50 to 58 %: a generator call is 65 instructions for
-// eight scores).  A block is a chain from the scores over tensor memory, the
+// a 128 x 64 block), the exponentials' unit 21 to 39 %, and 41 to 47 % of the issue
+// slots are used (with dropout 50 to 56 %: a generator call is 65 instructions for
+// eight scores).  The dk, dv kernel spills 76 to 136 bytes a thread in most forms, and
+// with D = 64 its scores' waits for the weights under them cost 132 -> 138 us of the
+// case without dropout (164 -> 166 with it).  A block is a chain from the scores over tensor memory, the
 // exponentials, tensor memory again and the next product, and two CTAs on an SM (four
 // warps a scheduler in the backward kernels) cover each other's waits only in part.
 // Four forward CTAs with a quarter of the columns each, the weights over the scores,
@@ -1711,7 +1713,10 @@ int attn_train_splits(int B, int S, int Hkv, int R, int num_sms) {
 }
 
 // Segments of the longest tile of query rows' key blocks, each its own item: the same
-// rule for the walk over keys.
+// rule for the walk over keys, but rounded down, as there are two joins to pay for
+// (rounded to the nearest, forward and dq: 3 x 1800, 8 / 2 heads of 32 43 + 47 -> 42 + 45 us
+// with the forward join, but 2 x 2000, 12 heads of 64 35 + 37 -> 45 + 43, 1 x 1100, 40 heads
+// of 64 22 + 24 -> 33 + 30, 1 x 4096, 12 heads of 64 95 + 110 -> 96 + 112).
 int attn_train_row_splits(int B, int S, int Hkv, int R, int num_sms) {
   if (R > 64) return 1;
   const int pt = kRows / R;

@@ -16,8 +16,9 @@
 // c' = mean(s x^) looks as if it had to wait for c, but s x^ = (alpha g v) D, so
 //   c' = mean(alpha g v e) - r_pre c mean(alpha g v h^),
 // and one sum over the row gives all three means.
-// h is formed again from x and residual in fp32 instead of being read back: the
-// same bytes, and the gradient does not see the rounding of the stored h.
+// h is formed again from x and residual in fp32 instead of being read back, so the
+// gradient does not see the rounding of the stored h.  With a post norm or a gate x is
+// needed anyway and the bytes are the same; without either it is one tensor more to read.
 //
 // Everything between the loads and the stores is fp32; each output is rounded
 // once, and n is the norm of the unrounded h.

@@ -230,3 +230,23 @@ def test_residual_norm_parts_are_one_wave(H):
     rows = sms * max(1, 16 // block)
     need = _lib.load().dt_residual_norm_workspace(100000, H, 0, 1)
     assert 0 < need <= 4 * (2 * rows * (-(-H // 4) * 4) + 16)
+
+
+@pytest.mark.gpu
+def test_captured_fp16_backward_scales_by_its_own_gradients():
+    """A replay takes the scale of the gradients that stand in its inputs then."""
+    from rl_for_mario_b200 import kernels
+
+    _, _, dev, ddev = attn_inputs(2, 300, 4, 2, 64, FP16, seed=12)
+    pad = torch.tensor([0, 17], dtype=torch.int32, device="cuda")
+    out, lse = kernels.attn_train_forward(*dev, pad)
+    d = ddev.clone()
+    want = [kernels.attn_train_backward(ddev * s, *dev, out, lse, pad) for s in (1.0, 2.0 ** -12, 8.0)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = kernels.attn_train_backward(d, *dev, out, lse, pad)
+    for s, w in zip((1.0, 2.0 ** -12, 8.0), want):
+        d.copy_(ddev * s)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, w))
