@@ -241,11 +241,11 @@ def _two_to(k):
 
 def _encode(x, words, bias, top, signed):
     """(codes, scales), uint8 [blocks, 256] and [blocks]: x rounded to three bits behind the leading one, down or
-    up by its word.  A block's scale is the (biased) exponent e of its largest value, 24 at least; its codes hold
+    up by its word.  A block's scale is the (biased) exponent e of its largest value, 32 at least; its codes hold
     |x| 2^(127 + top - e) with exponents from 1 - bias, subnormal numbers below; the sign is bit 7 of a signed code.
     An unsigned code is 0 for a zero alone."""
     x = x.view(-1, BLOCK)
-    e = (x.abs().view(torch.int32) >> 23).amax(1, keepdim=True).clamp_(min=24)
+    e = (x.abs().view(torch.int32) >> 23).amax(1, keepdim=True).clamp_(min=32)
     y = x.abs() * _two_to(127 + top - e)
     small = ((y * 2.0 ** (bias + 18)).to(torch.int32) + words) >> 16
     large = ((y.view(torch.int32) + (words << 4)) >> 20) - ((127 - bias) << 3)
@@ -432,7 +432,7 @@ def _rounded(x, u, lowest, top):
     come to a step or more.  The steps end at 2^lowest under a block's top binade, which is 2^top."""
     x = x.view(-1, BLOCK)
     big = torch.frexp(x.abs().amax(1, keepdim=True))[1] - 1          # 2^big <= the largest < 2^(big + 1)
-    scale = torch.ldexp(torch.ones_like(big, dtype=torch.float64), torch.clamp(big, min=24 - 127) - top)
+    scale = torch.ldexp(torch.ones_like(big, dtype=torch.float64), torch.clamp(big, min=32 - 127) - top)
     y = x.abs() / scale
     step = torch.ldexp(torch.ones_like(y), torch.clamp(torch.frexp(y)[1] - 1, min=lowest) - 3)
     return torch.floor(y / step + u.view(-1, BLOCK).double() / 65536) * step * scale * torch.sign(x), step * scale
