@@ -121,6 +121,42 @@ int dt_residual_norm_backward(const void* dh, int64_t dh_stride, const void* dn,
                               double p, const int64_t* rng, uint32_t site, int dtype, void* stream);
 
 /*
+ * The norm of every query and key head with the rotate-half RoPE in the same pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * w          x a head of q or k, w = w_q or w_k [D]
+ *   out[i] = y[i] cos[t, i] - y[i + D/2] sin[t, i],
+ *   out[i + D/2] = y[i + D/2] cos[t, i + D/2] + y[i] sin[t, i + D/2]        i < D/2
+ * at table row t = start_pos[b] + s (start_pos null: s).  q, q_out [B, S, Hq, D], k,
+ * k_out [B, S, Hkv, D], D contiguous; strides holds the (batch, position, head)
+ * element strides of q, k, q_out and k_out, 12 values.  Any head numbers; even D from 2
+ * to 256, bf16, fp16 or fp32, any strides and alignment (D a power of two from 8 on,
+ * 8-byte aligned (fp32 16-byte) heads and 16-byte aligned table rows run faster).
+ * Weights in the same type, or in fp32 with weights_fp32.  cos / sin [cos_rows, D] fp32
+ * with a common row stride.  A position outside the tables sets the device status word
+ * and its outputs to zeros.  An output may be its own input.  fp32 arithmetic, one
+ * rounding.
+ */
+int dt_head_norm_rope_forward(const void* q, const void* k, const void* w_q, const void* w_k, void* q_out, void* k_out,
+                              const float* cos_tab, const float* sin_tab, int64_t cos_stride, int cos_rows,
+                              const int32_t* start_pos, int B, int S, int Hq, int Hkv, int D, const int64_t* strides,
+                              int weights_fp32, float eps, int dtype, void* stream);
+
+/* Bytes of scratch that dt_head_norm_rope_backward needs on the current device;
+ * negative on an error. */
+int64_t dt_head_norm_rope_workspace(int B, int S, int Hq, int Hkv, int D);
+
+/*
+ * Gradient of dt_head_norm_rope_forward from dq_out and dk_out: dq, dk (which may be
+ * dq_out and dk_out themselves), dw_q, dw_k [D] in the weights' type.  strides: of q,
+ * k, dq, dk, dq_out and dk_out, 18 values.  workspace: dt_head_norm_rope_workspace
+ * bytes, 16-byte aligned.  Deterministic: sums are fp32 and in a fixed order.
+ */
+int dt_head_norm_rope_backward(const void* dq_out, const void* dk_out, const void* q, const void* k, const void* w_q,
+                               const void* w_k, void* dq, void* dk, void* dw_q, void* dw_k, const float* cos_tab,
+                               const float* sin_tab, int64_t cos_stride, int cos_rows, const int32_t* start_pos,
+                               void* workspace, int64_t workspace_bytes, int B, int S, int Hq, int Hkv, int D,
+                               const int64_t* strides, int weights_fp32, float eps, int dtype, void* stream);
+
+/*
  * y = residual + dropout(x) (residual null: 0) over rows [rows, cols]; the
  * gradient of x is the same call on the gradient of y without a residual.
  * bf16, fp16 or fp32, 1 <= cols <= 2^31 - 256, any strides and alignment

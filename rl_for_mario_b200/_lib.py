@@ -69,6 +69,11 @@ SIGNATURES = {
     "dt_residual_norm_workspace": (_L, [_L, _I, _L, _I]),
     "dt_residual_norm_backward": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                        _L, _L, _I, _F, _F, _D, _P, _U, _I, _P]),
+    "dt_head_norm_rope_forward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _P, _I, _I, _I, _I, _I, _P, _I, _F, _I,
+                                       _P]),
+    "dt_head_norm_rope_workspace": (_L, [_I, _I, _I, _I, _I]),
+    "dt_head_norm_rope_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _P, _P, _L, _I, _I, _I,
+                                        _I, _I, _P, _I, _F, _I, _P]),
     "dt_dropout": (_I, [_P, _L, _P, _L, _P, _L, _L, _I, _D, _P, _U, _I, _P]),
 }
 

@@ -123,6 +123,56 @@ int64_t part_elems(const dtk::ResidualNormPlan& q, int H, int64_t gate_rows, boo
   return n * ((H + 3) / 4 * 4) + 16;
 }
 
+constexpr int kMaxHeadDim = 256;
+
+int check_head_norm(const char* fn, int B, int S, int Hq, int Hkv, int D) {
+  if (B < 1 || S < 1 || Hq < 1 || Hkv < 1)
+    return api_fail(DT_ERR_INVALID, "%s: sizes must be positive (B=%d S=%d Hq=%d Hkv=%d)", fn, B, S, Hq, Hkv);
+  if (D < 2 || D > kMaxHeadDim || D % 2)
+    return api_fail(DT_ERR_UNSUPPORTED, "%s: head_dim %d must be even and lie in 2..%d", fn, D, kMaxHeadDim);
+  if ((long long)B * S > 0x7fffffffLL / (Hq > Hkv ? Hq : Hkv))
+    return api_fail(DT_ERR_UNSUPPORTED, "%s: too many heads (B=%d S=%d Hq=%d Hkv=%d)", fn, B, S, Hq, Hkv);
+  return DT_OK;
+}
+
+// What forward and backward share.  strides: (batch, position, head) of x and out (and the gradient) for q, then k.
+int head_norm_setup(const char* fn, dtk::HeadNormParams& a, const float* cos_tab, const float* sin_tab,
+                    int64_t cos_stride, int cos_rows, const int32_t* start_pos, int B, int S, int Hq, int Hkv, int D,
+                    const int64_t* strides, int w32, float eps, int dtype, bool bwd, int* sms) {
+  int rc = check_dtype(fn, dtype);
+  if (rc || (rc = check_head_norm(fn, B, S, Hq, Hkv, D))) return rc;
+  if (!cos_tab || !sin_tab || !strides) return api_fail(DT_ERR_INVALID, "%s: null cos/sin/strides", fn);
+  for (int i = 0; i < (bwd ? 18 : 12); ++i)
+    if (strides[i] < 0) return api_fail(DT_ERR_INVALID, "%s: stride #%d is negative", fn, i);
+  if (cos_rows < 1 || (!start_pos && cos_rows < S) || cos_stride < D ||
+      ((reinterpret_cast<uintptr_t>(cos_tab) | reinterpret_cast<uintptr_t>(sin_tab)) & 3))
+    return api_fail(DT_ERR_INVALID, "%s: cos/sin need %d rows of %d (got %d, stride %lld), 4-byte aligned", fn,
+                    start_pos ? 1 : S, D, cos_rows, (long long)cos_stride);
+  if (reinterpret_cast<uintptr_t>(start_pos) & 3)
+    return api_fail(DT_ERR_INVALID, "%s: start_pos must be 4-byte aligned", fn);
+  if (!(eps >= 0.f)) return api_fail(DT_ERR_INVALID, "%s: eps must not be negative (got %g)", fn, eps);
+  for (const dtk::HeadNormSide& s : a.side) {
+    if (!s.x || !s.w || !s.out || (bwd && (!s.grad || !s.dw))) return api_fail(DT_ERR_INVALID, "%s: null pointer", fn);
+    if ((rc = check_elem_aligned(fn, dtype, {s.x, s.grad, s.out}))) return rc;
+    if ((rc = check_elem_aligned(fn, w32 ? DT_DTYPE_FP32 : dtype, {s.w, s.dw}))) return rc;
+  }
+  if ((rc = need_sm100(fn, sms, &a.status))) return rc;
+  const int heads[2] = {Hq, Hkv};
+  for (int i = 0; i < 2; ++i) {
+    dtk::HeadNormSide& s = a.side[i];
+    const int64_t* st = strides + i * 3;
+    s.x_sb = st[0], s.x_ss = st[1], s.x_sh = st[2], s.o_sb = st[6], s.o_ss = st[7], s.o_sh = st[8];
+    if (bwd) s.g_sb = st[12], s.g_ss = st[13], s.g_sh = st[14];
+    const dtk::HeadNormSplit q = dtk::head_norm_split((long long)B * S, heads[i], heads[1 - i], D, bwd, *sms);
+    s.heads = heads[i], s.per = q.per, s.ranges = q.ranges, s.blocks = q.blocks;
+    s.by_ranges = dtk::FastDiv((uint32_t)q.ranges);
+  }
+  a.cos = cos_tab, a.sin = sin_tab, a.cs_stride = cos_stride, a.cos_rows = cos_rows, a.start = start_pos;
+  a.rows = B * S, a.S = S, a.D = D, a.by_s = dtk::FastDiv((uint32_t)S);
+  a.w32 = w32 != 0 || dtype == DT_DTYPE_FP32, a.eps = eps, a.inv_d = 1.f / (float)D;
+  return DT_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -372,6 +422,54 @@ int dt_dropout(const void* x, int64_t x_stride, const void* residual, int64_t re
   a.x = x, a.residual = residual, a.y = y, a.x_stride = x_stride, a.res_stride = res_stride, a.y_stride = y_stride;
   a.rows = rows, a.cols = cols, a.rng = reinterpret_cast<const long long*>(rng), a.site = site;
   return cuda_status(dtk::launch_dropout_sm100(a, dtype, sms, static_cast<cudaStream_t>(stream)), fn);
+}
+
+int dt_head_norm_rope_forward(const void* q, const void* k, const void* w_q, const void* w_k, void* q_out, void* k_out,
+                              const float* cos_tab, const float* sin_tab, int64_t cos_stride, int cos_rows,
+                              const int32_t* start_pos, int B, int S, int Hq, int Hkv, int D, const int64_t* strides,
+                              int weights_fp32, float eps, int dtype, void* stream) {
+  const char* fn = "dt_head_norm_rope_forward";
+  Range range(fn);
+  dtk::HeadNormParams a{};
+  a.side[0].x = q, a.side[0].w = w_q, a.side[0].out = q_out;
+  a.side[1].x = k, a.side[1].w = w_k, a.side[1].out = k_out;
+  int sms = 0;
+  const int rc = head_norm_setup(fn, a, cos_tab, sin_tab, cos_stride, cos_rows, start_pos, B, S, Hq, Hkv, D, strides,
+                                 weights_fp32, eps, dtype, false, &sms);
+  if (rc) return rc;
+  return cuda_status(dtk::launch_head_norm_sm100(a, dtype, false, static_cast<cudaStream_t>(stream)), fn);
+}
+
+int64_t dt_head_norm_rope_workspace(int B, int S, int Hq, int Hkv, int D) {
+  const char* fn = "dt_head_norm_rope_workspace";
+  int rc = check_head_norm(fn, B, S, Hq, Hkv, D), sms = 0;
+  if (rc || (rc = need_sm100(fn, &sms))) return -rc;
+  const long long rows = (long long)B * S;
+  return 4LL * D * (dtk::head_norm_split(rows, Hq, Hkv, D, true, sms).blocks +
+                    dtk::head_norm_split(rows, Hkv, Hq, D, true, sms).blocks);
+}
+
+int dt_head_norm_rope_backward(const void* dq_out, const void* dk_out, const void* q, const void* k, const void* w_q,
+                               const void* w_k, void* dq, void* dk, void* dw_q, void* dw_k, const float* cos_tab,
+                               const float* sin_tab, int64_t cos_stride, int cos_rows, const int32_t* start_pos,
+                               void* workspace, int64_t workspace_bytes, int B, int S, int Hq, int Hkv, int D,
+                               const int64_t* strides, int weights_fp32, float eps, int dtype, void* stream) {
+  const char* fn = "dt_head_norm_rope_backward";
+  Range range(fn);
+  dtk::HeadNormParams a{};
+  a.side[0].x = q, a.side[0].w = w_q, a.side[0].out = dq, a.side[0].grad = dq_out, a.side[0].dw = dw_q;
+  a.side[1].x = k, a.side[1].w = w_k, a.side[1].out = dk, a.side[1].grad = dk_out, a.side[1].dw = dw_k;
+  int sms = 0;
+  const int rc = head_norm_setup(fn, a, cos_tab, sin_tab, cos_stride, cos_rows, start_pos, B, S, Hq, Hkv, D, strides,
+                                 weights_fp32, eps, dtype, true, &sms);
+  if (rc) return rc;
+  const int64_t first = (int64_t)a.side[0].blocks * D, all = first + (int64_t)a.side[1].blocks * D;
+  if (workspace_bytes < 4 * all || !workspace || !aligned16(workspace))
+    return api_fail(DT_ERR_INVALID, "%s: workspace of %lld bytes is too small, null or not 16-byte aligned", fn,
+                    (long long)workspace_bytes);
+  a.side[0].part = static_cast<float*>(workspace);
+  a.side[1].part = a.side[0].part + first;
+  return cuda_status(dtk::launch_head_norm_sm100(a, dtype, true, static_cast<cudaStream_t>(stream)), fn);
 }
 
 }  // extern "C"

@@ -245,6 +245,39 @@ struct RopeGradParams {
 };
 cudaError_t launch_rope_grad_sm100(const RopeGradParams& p, bool bf16, int num_sms, cudaStream_t st);
 
+// One kind of head (query or key): element strides of batch, position and head.
+struct HeadNormSide {
+  const void* x;
+  const void* grad;  // backward: of the rotated heads
+  void* out;         // the rotated heads; backward: the gradient of x
+  const void* w;     // [D]
+  void* dw;
+  float* part;  // [blocks, D]
+  long long x_sb, x_ss, x_sh, g_sb, g_ss, g_sh, o_sb, o_ss, o_sh;
+  int heads, per, ranges;  // a position's heads are cut into `ranges` ranges of `per` (the last may be shorter)
+  unsigned blocks;
+  FastDiv by_ranges;
+};
+struct HeadNormParams {
+  HeadNormSide side[2];
+  const float* cos;
+  const float* sin;
+  const int32_t* start;  // [B] first position of each sample, or null: 0
+  int* status;
+  long long cs_stride;
+  int rows, S, D, cos_rows;  // rows: B S, times either side's ranges below 2^31
+  int lg;                    // log2 of the lanes that hold a head
+  FastDiv by_s;
+  bool w32;  // weights (and their gradients) in fp32
+  float eps, inv_d;
+};
+struct HeadNormSplit {
+  int per, ranges;
+  unsigned blocks;
+};
+HeadNormSplit head_norm_split(long long rows, int heads, int other_heads, int D, bool bwd, int num_sms);
+cudaError_t launch_head_norm_sm100(HeadNormParams p, int dtype, bool bwd, cudaStream_t st);
+
 struct ResidualNormParams {
   const void* x;
   const void* residual;  // or null

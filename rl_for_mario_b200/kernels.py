@@ -834,6 +834,109 @@ def residual_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], x: Tensor
     return dx, dres, dpre, dpost, dgate
 
 
+def _check_head_norm(q, k, q_weight, k_weight, eps, cos, sin, start_pos):
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("head_norm_rope takes q [B, S, Hq, D] and k [B, S, Hkv, D]")
+    B, S, Hq, D = q.shape
+    Hkv = k.shape[2]
+    dt = q.dtype
+    if k.shape != (B, S, Hkv, D):
+        raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    if dt not in _DTYPES or k.dtype != dt:
+        raise TypeError(f"q and k must share a dtype, bf16, fp16 or fp32 (got {dt} and {k.dtype})")
+    if D < 2 or D > 256 or D % 2:
+        raise ValueError(f"head_dim must be even and lie in 2..256 (got {D})")
+    if Hq < 1 or Hkv < 1:
+        raise ValueError("q and k need one head at least")
+    if B * S * max(Hq, Hkv) >= 2 ** 31:
+        raise ValueError(f"too many heads: {B} x {S} x {max(Hq, Hkv)} must stay below 2^31")
+    wt = q_weight.dtype
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.shape != (D,) or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [{D}] tensor")
+        if w.dtype != wt or wt not in (dt, torch.float32):
+            raise TypeError(f"q_weight and k_weight must have the dtype of q, or fp32 both (got {w.dtype})")
+    if not 0.0 <= ctypes.c_float(eps).value < math.inf:
+        raise ValueError(f"eps must be finite and not negative (got {eps})")
+    cos, sin = _prep_tables(cos, sin)
+    rows = cos.shape[0]
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D or rows < (S if start_pos is None else 1):
+        raise ValueError(f"cos and sin must be [{'rows' if start_pos is not None else f'>= {S}'}, {D}] tables "
+                         f"(got {tuple(cos.shape)}, {tuple(sin.shape)})")
+    if rows == 1 or cos.stride(0) < D:  # a stride that says nothing, or rows on top of each other
+        cos, sin = cos.contiguous(), sin.contiguous()
+    if start_pos is not None:
+        if start_pos.shape != (B,):
+            raise ValueError(f"start_pos must be [{B}] (got {tuple(start_pos.shape)})")
+        if start_pos.dtype != torch.int32 or not start_pos.is_contiguous():
+            start_pos = start_pos.to(torch.int32).contiguous()
+    return cos, sin, start_pos, B, S, Hq, Hkv, D
+
+
+_PACK12, _PACK18 = struct.Struct("12q"), struct.Struct("18q")
+
+
+def _dense_heads(t: Tensor) -> Tensor:
+    return t if t.stride(3) == 1 else t.contiguous()
+
+
+def head_norm_rope_forward(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, eps: float, cos: Tensor,
+                           sin: Tensor, start_pos: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """RMSNorm of every head of q [B,S,Hq,D] and k [B,S,Hkv,D] (one weight [D] for each of the two), then the
+    rotate-half RoPE, in one pass: (q_out, k_out), contiguous, in q's dtype.
+
+    Position (b, s) takes row start_pos[b] + s of cos / sin [rows, D] (start_pos [B] int32; None: row s); one
+    outside the tables gives zeros and is reported by device_status().  Any head numbers and strides, even D
+    up to 256, bf16, fp16 or fp32; weights in q's dtype or fp32.  fp32 arithmetic, one rounding.  The results
+    go to attention with apply_rope=False, in prefill, cached decode and training alike."""
+    dev = _same_device(q, k, q_weight, k_weight, cos, sin, start_pos)
+    cos, sin, start_pos, B, S, Hq, Hkv, D = _check_head_norm(q, k, q_weight, k_weight, eps, cos, sin, start_pos)
+    q, k = _dense_heads(q), _dense_heads(k)
+    qo, ko = _empty_as(q), _empty_as(k)
+    if B * S:
+        _launch("dt_head_norm_rope_forward", dev, q.data_ptr(), k.data_ptr(), q_weight.data_ptr(),
+                k_weight.data_ptr(), qo.data_ptr(), ko.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0),
+                cos.shape[0], _ptr(start_pos), B, S, Hq, Hkv, D,
+                _PACK12.pack(*q.stride()[:3], *k.stride()[:3], S * Hq * D, Hq * D, D, S * Hkv * D, Hkv * D, D),
+                int(q_weight.dtype == torch.float32), eps, _dtype_code(q))
+    return qo, ko
+
+
+def head_norm_rope_backward(dq_out: Tensor, dk_out: Tensor, q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor,
+                            eps: float, cos: Tensor, sin: Tensor, start_pos: Optional[Tensor] = None,
+                            grads: Optional[Tuple[Tensor, Tensor]] = None) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """Gradient of head_norm_rope_forward from dq_out and dk_out and the forward call's arguments: (dq, dk,
+    dq_weight, dk_weight).  ``grads``: tensors to write dq and dk into, which may be dq_out and dk_out
+    themselves (for instance the parts of one [B, S, Hq + 2 Hkv, D] gradient).  Sums are fp32 and in a fixed
+    order.  Every position counts: a NaN of q or k is a NaN of its weight's gradient even where dq_out is 0."""
+    dev = _same_device(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, start_pos)
+    cos, sin, start_pos, B, S, Hq, Hkv, D = _check_head_norm(q, k, q_weight, k_weight, eps, cos, sin, start_pos)
+    for t, like in ((dq_out, q), (dk_out, k)):
+        if t.shape != like.shape or t.dtype != like.dtype:
+            raise ValueError("dq_out and dk_out must have the shape and dtype of q and k")
+    q, k, dq_out, dk_out = (_dense_heads(t) for t in (q, k, dq_out, dk_out))
+    if grads is None:
+        dq, dk = _empty_as(q), _empty_as(k)
+    else:
+        dq, dk = grads
+        _same_device(q, dq, dk)
+        for name, t, like in (("dq", dq, q), ("dk", dk, k)):
+            if t.shape != like.shape or t.dtype != like.dtype or t.stride(3) != 1 or 0 in t.stride():
+                raise ValueError(f"{name} must be a {tuple(like.shape)} {like.dtype} tensor with contiguous D")
+    dwq, dwk = _empty_as(q_weight), _empty_as(k_weight)
+    if B * S == 0:
+        return dq, dk, dwq.zero_(), dwk.zero_()
+    size = _workspace("dt_head_norm_rope_workspace", dev.index, B, S, Hq, Hkv, D)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _launch("dt_head_norm_rope_backward", dev, dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
+            q_weight.data_ptr(), k_weight.data_ptr(), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(),
+            cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], _ptr(start_pos), ws.data_ptr(), size, B, S,
+            Hq, Hkv, D, _PACK18.pack(*q.stride()[:3], *k.stride()[:3], *dq.stride()[:3], *dk.stride()[:3],
+                                     *dq_out.stride()[:3], *dk_out.stride()[:3]),
+            int(q_weight.dtype == torch.float32), eps, _dtype_code(q))
+    return dq, dk, dwq, dwk
+
+
 def dropout_forward(x: Tensor, p: float, rng: Optional[Tensor], site: int = 0,
                     residual: Optional[Tensor] = None) -> Tensor:
     """residual + dropout(x) (residual None: dropout(x)) with a mask that is a function of rng, site
