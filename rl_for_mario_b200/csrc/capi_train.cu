@@ -163,13 +163,12 @@ int head_norm_setup(const char* fn, dtk::HeadNormParams& a, const float* cos_tab
     const int64_t* st = strides + i * 3;
     s.x_sb = st[0], s.x_ss = st[1], s.x_sh = st[2], s.o_sb = st[6], s.o_ss = st[7], s.o_sh = st[8];
     if (bwd) s.g_sb = st[12], s.g_ss = st[13], s.g_sh = st[14];
-    const dtk::HeadNormSplit q = dtk::head_norm_split((long long)B * S, heads[i], heads[1 - i], D, bwd, *sms);
-    s.heads = heads[i], s.per = q.per, s.ranges = q.ranges, s.blocks = q.blocks;
-    s.by_ranges = dtk::FastDiv((uint32_t)q.ranges);
+    s.heads = heads[i];
   }
   a.cos = cos_tab, a.sin = sin_tab, a.cs_stride = cos_stride, a.cos_rows = cos_rows, a.start = start_pos;
   a.rows = B * S, a.S = S, a.D = D, a.by_s = dtk::FastDiv((uint32_t)S);
   a.w32 = w32 != 0 || dtype == DT_DTYPE_FP32, a.eps = eps, a.inv_d = 1.f / (float)D;
+  dtk::head_norm_plan(a, dtype, bwd, *sms);
   return DT_OK;
 }
 
@@ -444,9 +443,7 @@ int64_t dt_head_norm_rope_workspace(int B, int S, int Hq, int Hkv, int D) {
   const char* fn = "dt_head_norm_rope_workspace";
   int rc = check_head_norm(fn, B, S, Hq, Hkv, D), sms = 0;
   if (rc || (rc = need_sm100(fn, &sms))) return -rc;
-  const long long rows = (long long)B * S;
-  return 4LL * D * (dtk::head_norm_split(rows, Hq, Hkv, D, true, sms).blocks +
-                    dtk::head_norm_split(rows, Hkv, Hq, D, true, sms).blocks);
+  return 4LL * D * dtk::head_norm_parts((long long)B * S, Hq, Hkv, D, sms);
 }
 
 int dt_head_norm_rope_backward(const void* dq_out, const void* dk_out, const void* q, const void* k, const void* w_q,

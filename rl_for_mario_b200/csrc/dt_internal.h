@@ -265,18 +265,16 @@ struct HeadNormParams {
   const int32_t* start;  // [B] first position of each sample, or null: 0
   int* status;
   long long cs_stride;
-  int rows, S, D, cos_rows;  // rows: B S, times either side's ranges below 2^31
+  int rows, S, D, cos_rows;  // rows: positions of all samples, times either side's heads below 2^31
   int lg;                    // log2 of the lanes that hold a head
   FastDiv by_s;
   bool w32;  // weights (and their gradients) in fp32
+  bool vec;  // whole vectors of 16 bytes
   float eps, inv_d;
 };
-struct HeadNormSplit {
-  int per, ranges;
-  unsigned blocks;
-};
-HeadNormSplit head_norm_split(long long rows, int heads, int other_heads, int D, bool bwd, int num_sms);
-cudaError_t launch_head_norm_sm100(HeadNormParams p, int dtype, bool bwd, cudaStream_t st);
+void head_norm_plan(HeadNormParams& p, int dtype, bool bwd, int num_sms);  // sets vec, lg and the sides' ranges and blocks
+long long head_norm_parts(long long rows, int Hq, int Hkv, int D, int num_sms);  // blocks of a backward pass, at most
+cudaError_t launch_head_norm_sm100(const HeadNormParams& p, int dtype, bool bwd, cudaStream_t st);
 
 struct ResidualNormParams {
   const void* x;

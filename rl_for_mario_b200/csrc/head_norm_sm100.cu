@@ -28,16 +28,18 @@ namespace dtk {
 namespace {
 
 constexpr int kThreads = 256;
+template <bool BWD>
+constexpr int kResident = BWD ? 2 : 3;  // blocks on an SM
 
-// Four pairs of a head as fp32: a[j], b[j] are elements i, i + h of the lane's pair j.
-// VEC: pairs 4 c .. 4 c + 3 of lane c (D a multiple of 8, 4 elements an access); otherwise
-// pairs c + G j, those at or past h reading as 0 and not written.
+// ---------------------------------------------------------------- any width, stride and alignment
+// Four pairs of a head as fp32: a[j], b[j] are elements i, i + h of pair i = c + G j of lane c; those at
+// or past h read as 0 and are not written.
 struct Pairs {
   float a[4], b[4];
 };
 
 // A head's elements as they stand in memory, on their way while another head is worked on.
-template <int DT, bool VEC>
+template <int DT>
 struct RawPairs {
   using T = typename TrainElem<DT>::T;
   T a[4], b[4];
@@ -56,51 +58,18 @@ struct RawPairs {
     return p;
   }
 };
-template <int DT>
-struct RawPairs<DT, true> {
-  using T = typename TrainElem<DT>::T;
-  using V = typename std::conditional<DT == 2, float4, uint2>::type;
-  V a, b;
-  __device__ __forceinline__ void load(const T* x, int c, int, int h) {
-    a = *reinterpret_cast<const V*>(x + 4 * c);
-    b = *reinterpret_cast<const V*>(x + 4 * c + h);
-  }
-  __device__ __forceinline__ Pairs get() const {
-    Pairs p;
-    if constexpr (DT == 2) {
-      p.a[0] = a.x, p.a[1] = a.y, p.a[2] = a.z, p.a[3] = a.w;
-      p.b[0] = b.x, p.b[1] = b.y, p.b[2] = b.z, p.b[3] = b.w;
-    } else {
-      using E = Elem<DT == 0>;
-      const float2 a0 = E::to_f2(a.x), a1 = E::to_f2(a.y), b0 = E::to_f2(b.x), b1 = E::to_f2(b.y);
-      p.a[0] = a0.x, p.a[1] = a0.y, p.a[2] = a1.x, p.a[3] = a1.y;
-      p.b[0] = b0.x, p.b[1] = b0.y, p.b[2] = b1.x, p.b[3] = b1.y;
-    }
-    return p;
-  }
-};
 
-template <int DT, bool VEC>
+template <int DT>
 __device__ __forceinline__ void store_pairs(typename TrainElem<DT>::T* o, int c, int lg, int h, const Pairs& p) {
-  if constexpr (VEC && DT == 2) {
-    *reinterpret_cast<float4*>(o + 4 * c) = make_float4(p.a[0], p.a[1], p.a[2], p.a[3]);
-    *reinterpret_cast<float4*>(o + 4 * c + h) = make_float4(p.b[0], p.b[1], p.b[2], p.b[3]);
-  } else if constexpr (VEC) {
-    using E = Elem<DT == 0>;
-    *reinterpret_cast<uint2*>(o + 4 * c) = make_uint2(E::from_f2(p.a[0], p.a[1]), E::from_f2(p.a[2], p.a[3]));
-    *reinterpret_cast<uint2*>(o + 4 * c + h) = make_uint2(E::from_f2(p.b[0], p.b[1]), E::from_f2(p.b[2], p.b[3]));
-  } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = c + (j << lg);
-      if (i < h) o[i] = TrainElem<DT>::from_f(p.a[j]), o[i + h] = TrainElem<DT>::from_f(p.b[j]);
-    }
+  for (int j = 0; j < 4; ++j) {
+    const int i = c + (j << lg);
+    if (i < h) o[i] = TrainElem<DT>::from_f(p.a[j]), o[i + h] = TrainElem<DT>::from_f(p.b[j]);
   }
 }
 
-template <bool VEC>
 __device__ __forceinline__ Pairs load_table(const float* row, int c, int lg, int h) {
-  RawPairs<2, VEC> t;
+  RawPairs<2> t;
   t.load(row, c, lg, h);
   return t.get();
 }
@@ -110,11 +79,50 @@ __device__ __forceinline__ float group_sum(float v, int lg) {
   return v;
 }
 
+template <int LG>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = 1 << LG >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The block's part of a weight's gradient from its warps' [warps, D], in a fixed order.
+template <int DT>
+__device__ __forceinline__ void block_sum(const HeadNormParams& p, const HeadNormSide& sd, unsigned block,
+                                          const float* sums) {
+  __syncthreads();
+  if ((int)threadIdx.x < p.D) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < kThreads / 32; ++k) t += sums[k * p.D + threadIdx.x];
+    if (sd.blocks > 1)
+      sd.part[(long long)block * p.D + threadIdx.x] = t;
+    else if (p.w32)
+      static_cast<float*>(sd.dw)[threadIdx.x] = t;
+    else
+      static_cast<typename TrainElem<DT>::T*>(sd.dw)[threadIdx.x] = TrainElem<DT>::from_f(t);
+  }
+}
+
 // Blocks below side[0].blocks take the query heads, the others the key heads.  Item n of a
-// side is the heads j per .. of row n / ranges, j = n % ranges; every group of a warp takes
-// the same number of turns, those without a head left on zeros.
-template <int DT, bool VEC, bool BWD>
-__global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) head_norm_kernel(const __grid_constant__ HeadNormParams p) {
+// side is the heads `per` j .. of position n / ranges (all samples' in a row), j = n % ranges:
+// neighbouring groups read neighbouring memory (with the same position of different samples
+// side by side, which share a table row, 96 x 768, 12 / 4 heads of 64 took 66 us, 57 so).
+// Every group of a warp takes the same number of turns, those without a head left on zeros.
+struct Item {
+  int b, s, head;
+};
+__device__ __forceinline__ Item item_of(const HeadNormParams& p, const HeadNormSide& sd, int item) {
+  Item q;
+  const int row = sd.by_ranges(item);
+  q.head = (item - row * sd.ranges) * sd.per;
+  q.b = p.by_s(row);
+  q.s = row - q.b * p.S;
+  return q;
+}
+
+template <int DT, bool BWD>
+__global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_any_kernel(const __grid_constant__ HeadNormParams p) {
   using T = typename TrainElem<DT>::T;
   const bool second = blockIdx.x >= p.side[0].blocks;
   const HeadNormSide& sd = p.side[second];
@@ -127,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) head_norm_kernel(const 
   Pairs w, acc;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int i = VEC ? 4 * c + j : c + (j << lg);
+    const int i = c + (j << lg);
     auto weight = [&](int n) {
       return p.w32 ? static_cast<const float*>(sd.w)[n] : TrainElem<DT>::to_f(static_cast<const T*>(sd.w)[n]);
     };
@@ -138,21 +146,21 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) head_norm_kernel(const 
 
   for (long long first = group - lead; first < items; first += groups) {
     const bool live = first + lead < items;
-    const int item = (int)(live ? first + lead : 0), row = sd.by_ranges(item), head = (item - row * sd.ranges) * sd.per;
-    const int b = p.by_s(row), s = row - b * p.S;
+    const Item it = item_of(p, sd, live ? (int)(first + lead) : 0);
+    const int b = it.b, s = it.s, head = it.head;
     const long long at = (p.start ? p.start[b] : 0) + (long long)s;
     const bool known = at >= 0 && at < p.cos_rows;
     if (live && !known && p.status) atomicExch(p.status, (int)kDevBadShape);
     Pairs cs{}, sn{};
     if (known) {
-      cs = load_table<VEC>(p.cos + at * p.cs_stride, c, lg, h);
-      sn = load_table<VEC>(p.sin + at * p.cs_stride, c, lg, h);
+      cs = load_table(p.cos + at * p.cs_stride, c, lg, h);
+      sn = load_table(p.sin + at * p.cs_stride, c, lg, h);
     }
     const int n = live ? min(sd.per, sd.heads - head) : 0;
     const T* x = static_cast<const T*>(sd.x) + b * sd.x_sb + s * sd.x_ss + head * sd.x_sh;
     T* o = static_cast<T*>(sd.out) + b * sd.o_sb + s * sd.o_ss + head * sd.o_sh;
     const T* g = BWD ? static_cast<const T*>(sd.grad) + b * sd.g_sb + s * sd.g_ss + head * sd.g_sh : nullptr;
-    RawPairs<DT, VEC> nx{}, ng{};
+    RawPairs<DT> nx{}, ng{};
     if (n > 0 && known) {
       nx.load(x, c, lg, h);
       if constexpr (BWD) ng.load(g, c, lg, h);
@@ -206,40 +214,249 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) head_norm_kernel(const 
       }
       if (have) {
         if (!known) out = Pairs{};
-        store_pairs<DT, VEC>(o, c, lg, h, out);
+        store_pairs<DT>(o, c, lg, h, out);
         o += sd.o_sh;
       }
     }
   }
 
   if constexpr (BWD) {
-    // The block's sum, in a fixed order: lanes of the same place, then warps.
-    __shared__ float sums[kThreads / 32][256];
+    extern __shared__ float sums[];  // [warps, D]
     for (int o = 16; o >= 1 << lg; o >>= 1)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         acc.a[j] += __shfl_xor_sync(0xffffffffu, acc.a[j], o);
         acc.b[j] += __shfl_xor_sync(0xffffffffu, acc.b[j], o);
       }
-    const int warp = threadIdx.x >> 5;
+    float* mine = sums + (threadIdx.x >> 5) * p.D;
     if ((threadIdx.x & 31) < 1 << lg)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int i = VEC ? 4 * c + j : c + (j << lg);
-        if (i < h) sums[warp][i] = acc.a[j], sums[warp][i + h] = acc.b[j];
+        const int i = c + (j << lg);
+        if (i < h) mine[i] = acc.a[j], mine[i + h] = acc.b[j];
       }
-    __syncthreads();
-    if ((int)threadIdx.x < p.D) {
-      float t = 0.f;
-#pragma unroll
-      for (int k = 0; k < kThreads / 32; ++k) t += sums[k][threadIdx.x];
-      if (sd.blocks > 1)
-        sd.part[(long long)block * p.D + threadIdx.x] = t;
-      else if (p.w32)
-        static_cast<float*>(sd.dw)[threadIdx.x] = t;
-      else
-        static_cast<T*>(sd.dw)[threadIdx.x] = TrainElem<DT>::from_f(t);
+    block_sum<DT>(p, sd, block, sums);
+  }
+}
+
+// ---------------------------------------------------------------- heads of whole vectors
+// Lane c of a group holds elements P c .. P c + P - 1 and the same from h on: two accesses of 16 bytes
+// (P = 8, fp32 4).  A head's elements are copied into the lane's own places of a ring in shared memory,
+// kDepth heads ahead and across positions, and only the lane reads them back: no barrier, and what is in
+// flight takes no registers.
+template <int DT>
+constexpr int kPairs = DT == 2 ? 4 : 8;
+constexpr int kDepth = 2;
+
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy16(uint4* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+               : "memory");
+}
+
+// A lane's half of a head as packed pairs of fp32.
+template <int DT>
+struct Half {
+  float2 p[kPairs<DT> / 2];
+  __device__ __forceinline__ void set(uint4 u) {
+    if constexpr (DT == 2) {
+      p[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+      p[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+    } else {
+      using E = Elem<DT == 0>;
+      p[0] = E::to_f2(u.x), p[1] = E::to_f2(u.y), p[2] = E::to_f2(u.z), p[3] = E::to_f2(u.w);
     }
+  }
+  __device__ __forceinline__ uint4 bits() const {
+    if constexpr (DT == 2) {
+      return make_uint4(__float_as_uint(p[0].x), __float_as_uint(p[0].y), __float_as_uint(p[1].x),
+                        __float_as_uint(p[1].y));
+    } else {
+      using E = Elem<DT == 0>;
+      return make_uint4(E::from_f2(p[0].x, p[0].y), E::from_f2(p[1].x, p[1].y), E::from_f2(p[2].x, p[2].y),
+                        E::from_f2(p[3].x, p[3].y));
+    }
+  }
+  __device__ __forceinline__ void load_f32(const float* f) {
+#pragma unroll
+    for (int i = 0; i < kPairs<DT> / 4; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(f + 4 * i);
+      p[2 * i] = make_float2(v.x, v.y);
+      p[2 * i + 1] = make_float2(v.z, v.w);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kPairs<DT> / 2; ++i) p[i] = make_float2(0.f, 0.f);
+  }
+};
+__device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.y); }
+
+// Where a group stands in its walk: the heads of its items, one after the other.
+template <typename T>
+struct Place {
+  const T* x;
+  const T* g;
+  int k, n;  // n: heads of the item, 0 behind the last one
+};
+
+template <int DT, bool BWD, int LG>
+__global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_kernel(const __grid_constant__ HeadNormParams p) {
+  using T = typename TrainElem<DT>::T;
+  constexpr int P = kPairs<DT>, N = P / 2, TENSORS = BWD ? 4 : 2;
+  extern __shared__ uint4 ring[];  // [kDepth, TENSORS, threads]
+  __shared__ __align__(16) float weights[256];
+  const bool second = blockIdx.x >= p.side[0].blocks;
+  const HeadNormSide& sd = p.side[second];
+  const unsigned block = blockIdx.x - (second ? p.side[0].blocks : 0u);
+  constexpr int lg = LG;
+  const int c = threadIdx.x & ((1 << lg) - 1), h = p.D >> 1;
+  const bool mine = c * P < h;
+  const int e = mine ? c * P : 0;  // the lane's first element
+  for (int i = threadIdx.x; i < p.D; i += kThreads)
+    weights[i] = p.w32 ? static_cast<const float*>(sd.w)[i] : TrainElem<DT>::to_f(static_cast<const T*>(sd.w)[i]);
+  __syncthreads();
+  const long long items = (long long)p.rows * sd.ranges;
+  const long long groups = (long long)sd.blocks * kThreads >> lg;
+  const long long group = ((long long)block * kThreads + threadIdx.x) >> lg, lead = (threadIdx.x & 31) >> lg;
+
+  // (Items number less than 2^31; a warp's groups take the same number of turns.)
+  long long at = group - lead;  // the warp's first item of the turn that is copied
+  Place<T> f;
+  auto enter = [&](Place<T>& q, long long first) {
+    const bool live = first + lead < items;
+    const Item it = item_of(p, sd, live ? (int)(first + lead) : 0);
+    q.n = live && mine ? min(sd.per, sd.heads - it.head) : 0;
+    q.k = 0;
+    q.x = static_cast<const T*>(sd.x) + it.b * sd.x_sb + it.s * sd.x_ss + it.head * sd.x_sh + e;
+    if constexpr (BWD) q.g = static_cast<const T*>(sd.grad) + it.b * sd.g_sb + it.s * sd.g_ss + it.head * sd.g_sh + e;
+  };
+  uint4* slots = ring + threadIdx.x;
+  auto fetch = [&](int stage) {
+    if (f.k < f.n) {
+      uint4* to = slots + stage * (TENSORS * kThreads);
+      copy16(to, f.x);
+      copy16(to + kThreads, f.x + h);
+      if constexpr (BWD) {
+        copy16(to + 2 * kThreads, f.g);
+        copy16(to + 3 * kThreads, f.g + h);
+      }
+    }
+    copies_commit();
+    f.x += sd.x_sh;
+    if constexpr (BWD) f.g += sd.g_sh;
+    if (++f.k == sd.per && at + groups < items) {
+      at += groups;
+      enter(f, at);
+    }
+  };
+  Half<DT> aa, ab;  // sums of the weight's gradient
+  aa.clear();
+  ab.clear();
+  if (at < items) {
+    enter(f, at);
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i) fetch(i);
+  }
+  int stage = 0;
+  for (long long first = group - lead; first < items; first += groups) {
+    const bool live = first + lead < items;
+    const Item it = item_of(p, sd, live ? (int)(first + lead) : 0);
+    const int b = it.b, s = it.s, head = it.head;
+    const int n = live && mine ? min(sd.per, sd.heads - head) : 0;
+    T* o = static_cast<T*>(sd.out) + b * sd.o_sb + s * sd.o_ss + head * sd.o_sh + e;
+    const long long t = (p.start ? p.start[b] : 0) + (long long)s;
+    const bool known = t >= 0 && t < p.cos_rows;
+    if (live && !known && p.status) atomicExch(p.status, (int)kDevBadShape);
+    Half<DT> ca, cb, sa, sb;  // forward: times the weights
+    const float* cos = p.cos + (known ? t : 0) * p.cs_stride + e;
+    const float* sin = p.sin + (known ? t : 0) * p.cs_stride + e;
+    ca.load_f32(cos), cb.load_f32(cos + h), sa.load_f32(sin), sb.load_f32(sin + h);
+    if constexpr (!BWD) {
+      Half<DT> wa, wb;
+      wa.load_f32(weights + e), wb.load_f32(weights + e + h);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        ca.p[i] = fmul2(ca.p[i], wa.p[i]), cb.p[i] = fmul2(cb.p[i], wb.p[i]);
+        sa.p[i] = minus(fmul2(sa.p[i], wb.p[i])), sb.p[i] = fmul2(sb.p[i], wa.p[i]);
+      }
+    }
+    for (int k = 0; k < sd.per; ++k) {
+      copies_wait<kDepth - 1>();
+      const uint4* from = slots + stage * (TENSORS * kThreads);
+      const bool have = k < n;
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      Half<DT> xa, xb, ga, gb;
+      xa.set(have ? from[0] : zero), xb.set(have ? from[kThreads] : zero);
+      if constexpr (BWD) ga.set(have ? from[2 * kThreads] : zero), gb.set(have ? from[3 * kThreads] : zero);
+      fetch(stage);
+      stage = stage + 1 == kDepth ? 0 : stage + 1;
+      float2 q = make_float2(0.f, 0.f), z = q;
+#pragma unroll
+      for (int i = 0; i < N; ++i) q = ffma2(xa.p[i], xa.p[i], ffma2(xb.p[i], xb.p[i], q));
+      if constexpr (!BWD) {
+        const float r = rsqrtf(fmaf(group_sum<LG>(both_sum(q)), p.inv_d, p.eps));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float2 a = xa.p[i], v = xb.p[i];
+          xa.p[i] = fmul2(ffma2(v, sa.p[i], fmul2(a, ca.p[i])), both(r));
+          xb.p[i] = fmul2(ffma2(a, sb.p[i], fmul2(v, cb.p[i])), both(r));
+        }
+      } else {
+        Half<DT> wa, wb;
+        wa.load_f32(weights + e), wb.load_f32(weights + e + h);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float2 a = ga.p[i], v = gb.p[i];
+          ga.p[i] = ffma2(v, sb.p[i], fmul2(a, ca.p[i]));
+          gb.p[i] = ffma2(minus(a), sa.p[i], fmul2(v, cb.p[i]));
+          wa.p[i] = fmul2(ga.p[i], wa.p[i]);
+          wb.p[i] = fmul2(gb.p[i], wb.p[i]);
+          z = ffma2(wa.p[i], xa.p[i], ffma2(wb.p[i], xb.p[i], z));
+        }
+        const float ss = group_sum<LG>(both_sum(q)), su = group_sum<LG>(both_sum(z));
+        // A head that is not there adds nothing, whatever eps makes of its zeros.
+        const float r = have && known ? rsqrtf(fmaf(ss, p.inv_d, p.eps)) : 0.f;
+        const float m = -su * r * r * p.inv_d;  // - mean(u x^) r, to be multiplied with x
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          aa.p[i] = ffma2(ga.p[i], fmul2(xa.p[i], both(r)), aa.p[i]);
+          ab.p[i] = ffma2(gb.p[i], fmul2(xb.p[i], both(r)), ab.p[i]);
+          xa.p[i] = fmul2(ffma2(xa.p[i], both(m), wa.p[i]), both(r));
+          xb.p[i] = fmul2(ffma2(xb.p[i], both(m), wb.p[i]), both(r));
+        }
+      }
+      if (have) {
+        *reinterpret_cast<uint4*>(o) = known ? xa.bits() : zero;
+        *reinterpret_cast<uint4*>(o + h) = known ? xb.bits() : zero;
+        o += sd.o_sh;
+      }
+    }
+  }
+  copies_wait<0>();
+
+  if constexpr (BWD) {
+    __syncthreads();  // (the ring's last readers are done)
+    float* sums = reinterpret_cast<float*>(ring);  // [warps, D]
+#pragma unroll
+    for (int o = 16; o >= 1 << lg; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        aa.p[i].x += __shfl_xor_sync(0xffffffffu, aa.p[i].x, o), aa.p[i].y += __shfl_xor_sync(0xffffffffu, aa.p[i].y, o);
+        ab.p[i].x += __shfl_xor_sync(0xffffffffu, ab.p[i].x, o), ab.p[i].y += __shfl_xor_sync(0xffffffffu, ab.p[i].y, o);
+      }
+    float* row = sums + (threadIdx.x >> 5) * p.D + e;
+    if ((threadIdx.x & 31) < 1 << lg && mine)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        *reinterpret_cast<float2*>(row + 2 * i) = aa.p[i];
+        *reinterpret_cast<float2*>(row + h + 2 * i) = ab.p[i];
+      }
+    block_sum<DT>(p, sd, block, sums);
   }
 }
 
@@ -264,67 +481,114 @@ __global__ void __launch_bounds__(1024) head_norm_sum_kernel(const __grid_consta
   }
 }
 
+// 16-byte accesses need every half of a head on a 16-byte boundary, in whole vectors.
 bool can_vector(const HeadNormParams& p, int dtype, bool bwd) {
-  const long long step = 4;  // elements of an access
-  const uintptr_t bytes = dtype == 2 ? 16 : 8;
-  // Whole accesses, and a power of two of lanes.
-  if (p.D % 8 || (p.D & (p.D - 1)) || p.cs_stride % 4 ||
+  const int pairs = dtype == 2 ? 4 : 8;
+  if (p.D % (2 * pairs) || p.cs_stride % 4 ||
       ((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15))
     return false;
   for (const HeadNormSide& s : p.side) {
     const void* ptrs[] = {s.x, s.out, bwd ? s.grad : nullptr};
     for (const void* q : ptrs)
-      if (reinterpret_cast<uintptr_t>(q) % bytes) return false;
+      if (reinterpret_cast<uintptr_t>(q) & 15) return false;
     const long long strides[] = {s.x_sb, s.x_ss, s.x_sh, s.o_sb, s.o_ss, s.o_sh,
                                  bwd ? s.g_sb : 0, bwd ? s.g_ss : 0, bwd ? s.g_sh : 0};
     for (long long q : strides)
-      if (q % step) return false;
+      if (q % pairs) return false;
   }
   return true;
 }
 
+int log_lanes(int D, int pairs) {  // of the group that holds a head
+  int lg = 0;
+  while ((2 * pairs << lg) < D) ++lg;
+  return lg;
+}
+
 template <int DT, bool BWD>
-cudaError_t launch(const HeadNormParams& p, bool vec, cudaStream_t st) {
+cudaError_t launch(const HeadNormParams& p, cudaStream_t st) {
   const unsigned grid = p.side[0].blocks + p.side[1].blocks;
-  if (vec)
-    head_norm_kernel<DT, true, BWD><<<grid, kThreads, 0, st>>>(p);
-  else
-    head_norm_kernel<DT, false, BWD><<<grid, kThreads, 0, st>>>(p);
+  if (p.vec) {
+    constexpr int smem = kDepth * (BWD ? 4 : 2) * kThreads * 16;
+    static_assert(!BWD || smem >= kThreads / 32 * 256 * 4, "the block's sums lie in the ring");
+    auto run = [&](auto kernel) {
+      const cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kernel), smem);
+      if (e == cudaSuccess) kernel<<<grid, kThreads, smem, st>>>(p);
+      return e;
+    };
+    cudaError_t e = cudaErrorInvalidValue;
+    switch (p.lg) {
+      case 0: e = run(head_norm_kernel<DT, BWD, 0>); break;
+      case 1: e = run(head_norm_kernel<DT, BWD, 1>); break;
+      case 2: e = run(head_norm_kernel<DT, BWD, 2>); break;
+      case 3: e = run(head_norm_kernel<DT, BWD, 3>); break;
+      case 4: e = run(head_norm_kernel<DT, BWD, 4>); break;
+      case 5: e = run(head_norm_kernel<DT, BWD, 5>); break;
+    }
+    if (e != cudaSuccess) return e;
+  } else {
+    head_norm_any_kernel<DT, BWD><<<grid, kThreads, BWD ? kThreads / 32 * p.D * 4 : 0, st>>>(p);
+  }
   cudaError_t e = cudaGetLastError();
   if (!BWD || e != cudaSuccess || (p.side[0].blocks == 1 && p.side[1].blocks == 1)) return e;
   head_norm_sum_kernel<DT><<<dim3((unsigned)(p.D + 31) / 32, 2), 1024, 0, st>>>(p);
   return cudaGetLastError();
 }
 
-int log_lanes(int D) {  // of the group that holds a head, four pairs a lane
-  int lg = 0;
-  while ((8 << lg) < D) ++lg;
-  return lg;
-}
+struct Split {
+  int per, ranges;
+  unsigned blocks;
+};
 
-}  // namespace
-
-HeadNormSplit head_norm_split(long long rows, int heads, int other_heads, int D, bool bwd, int num_sms) {
-  HeadNormSplit q;
-  const int lg = log_lanes(D);
-  const long long lanes = (long long)num_sms * 1024;  // that an SM holds of it
-  const long long per = rows * heads / ((2 * lanes) >> lg);
-  q.per = per < 1 ? 1 : per < heads ? (int)per : heads;
-  q.ranges = (heads + q.per - 1) / q.per;
-  q.per = (heads + q.ranges - 1) / q.ranges;
-  const long long want = ((rows * q.ranges << lg) + kThreads - 1) / kThreads;
-  long long cap = bwd ? (long long)num_sms * 2 * heads / (heads + other_heads) : (long long)num_sms * 32;
+// How a side's heads are spread: blocks in proportion to them, as many as the GPU holds at a time, and each
+// position's heads cut into the number of ranges that takes a group the least time: turns of (heads of a
+// range + 1), the start of an item (table row, weights) costing about as much as a head.
+Split split_heads(long long rows, int heads, int other_heads, int D, int pairs, bool bwd, int num_sms) {
+  const int lg = log_lanes(D, pairs);
+  long long cap = (long long)num_sms * (bwd ? kResident<true> : kResident<false>) * heads / (heads + other_heads);
   if (cap < 1) cap = 1;
+  const long long groups = cap * kThreads >> lg;
+  Split q{heads, 1, 1u};
+  long long best = -1;
+  for (int ranges = 1; ranges <= heads; ++ranges) {
+    const int per = (heads + ranges - 1) / ranges;
+    if ((long long)(ranges - 1) * per >= heads) continue;  // the last would be empty
+    const long long cost = (rows * ranges + groups - 1) / groups * (per + 1);
+    if (best < 0 || cost < best) best = cost, q.per = per, q.ranges = ranges;
+  }
+  const long long want = ((rows * q.ranges << lg) + kThreads - 1) / kThreads;
   q.blocks = (unsigned)(want < cap ? want : cap);
   return q;
 }
 
-cudaError_t launch_head_norm_sm100(HeadNormParams p, int dtype, bool bwd, cudaStream_t st) {
-  p.lg = log_lanes(p.D);
-  const bool vec = can_vector(p, dtype, bwd);
-  if (dtype == 0) return bwd ? launch<0, true>(p, vec, st) : launch<0, false>(p, vec, st);
-  if (dtype == 1) return bwd ? launch<1, true>(p, vec, st) : launch<1, false>(p, vec, st);
-  return bwd ? launch<2, true>(p, vec, st) : launch<2, false>(p, vec, st);
+}  // namespace
+
+void head_norm_plan(HeadNormParams& p, int dtype, bool bwd, int num_sms) {
+  p.vec = can_vector(p, dtype, bwd);
+  const int pairs = p.vec && dtype != 2 ? 8 : 4;
+  p.lg = log_lanes(p.D, pairs);
+  for (int i = 0; i < 2; ++i) {
+    HeadNormSide& s = p.side[i];
+    const Split q = split_heads(p.rows, s.heads, p.side[1 - i].heads, p.D, pairs, bwd, num_sms);
+    s.per = q.per, s.ranges = q.ranges, s.blocks = q.blocks, s.by_ranges = FastDiv((uint32_t)q.ranges);
+  }
+}
+
+// Alignment decides between two plans when the backward call comes: room for either.
+long long head_norm_parts(long long rows, int Hq, int Hkv, int D, int num_sms) {
+  long long most = 0;
+  for (int pairs = 4; pairs <= 8; pairs += 4) {
+    const long long n = (long long)split_heads(rows, Hq, Hkv, D, pairs, true, num_sms).blocks +
+                        split_heads(rows, Hkv, Hq, D, pairs, true, num_sms).blocks;
+    most = n > most ? n : most;
+  }
+  return most;
+}
+
+cudaError_t launch_head_norm_sm100(const HeadNormParams& p, int dtype, bool bwd, cudaStream_t st) {
+  if (dtype == 0) return bwd ? launch<0, true>(p, st) : launch<0, false>(p, st);
+  if (dtype == 1) return bwd ? launch<1, true>(p, st) : launch<1, false>(p, st);
+  return bwd ? launch<2, true>(p, st) : launch<2, false>(p, st);
 }
 
 }  // namespace dtk
