@@ -166,6 +166,67 @@ int dt_head_norm_rope_backward(const void* dq_out, const void* dk_out, const voi
 int dt_dropout(const void* x, int64_t x_stride, const void* residual, int64_t res_stride, void* y, int64_t y_stride,
                int64_t rows, int cols, double p, const int64_t* rng, uint32_t site, int dtype, void* stream);
 
+/*
+ * The 2-norm of many tensors taken as one: norm (fp32, one number) receives
+ * sqrt(sum of squares).  tensors: their addresses (0: left out), sizes: numbers of
+ * elements (whole tensors without gaps, any order of dimensions), kinds: dtype codes.
+ * Any alignment.  The three arrays are the host's and are read during the call.  Sums
+ * are fp64 of fp32 sums of eight squares (fp64 squares where fp32 would overflow or
+ * lose bits), in a fixed order.  workspace: dt_grad_norm_workspace bytes, 16-byte aligned.
+ */
+int dt_grad_norm(int count, const int64_t* tensors, const int64_t* sizes, const int32_t* kinds, float* norm,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of scratch that dt_grad_norm and the clipping of dt_adamw_step need for `count`
+ * tensors on the current device; negative on an error. */
+int64_t dt_grad_norm_workspace(int count);
+
+/* Hyperparameters of a group of tensors.  lr_tensor: the rate as an fp32 number on the
+ * device, read by the kernel, or null: lr. */
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_tensor;
+} DtAdamWGroup;
+
+/*
+ * One AdamW step over many tensors:
+ *   g' = g min(1, max_norm / (norm + 1e-6))      norm: of all gradients; max_norm <= 0: g' = g
+ *   m' = beta1 m + (1 - beta1) g',  v' = beta2 v + (1 - beta2) g'^2
+ *   p' = p (1 - lr weight_decay) - lr / (1 - beta1^t) m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ * params, grads: addresses of weights and gradients (gradient 0: the tensor is left alone),
+ * of the same dtype, size and order of elements, whole tensors without gaps, any
+ * alignment; sizes: numbers of elements; kinds: dtype code + 256 * group.  1 to 16 groups.
+ * The arrays are the host's and are read during the call.
+ *
+ * The averages are flat arrays: tensor i's begin at 256 times the number of blocks of 256
+ * elements of the tensors before it (the last block of each filled up), 16-byte aligned.
+ * state_bits 32: fp32.  state_bits 8: one byte an element and one for each block of 256,
+ * the biased exponent e (32 at least) of the block's largest value; exp_avg as sign, four
+ * exponent and three further bits (a number of type e4m3) times 2^(e - 134), exp_avg_sq as
+ * five exponent and three further bits (those of a half number under its sign) times
+ * 2^(e - 141).  They are rounded up or down at random: element i of the flat array goes up
+ * when the part cut off and w / 2^16 come to a step, w word i % 8 of the generator's block
+ * i / 8 (above; site 2^32 - 1, step t), for exp_avg with its two bytes turned over.  An
+ * exp_avg_sq above zero is never stored as zero.  A block with a value that is not finite
+ * reads as NaN from then on (e = 255).
+ *
+ * master: fp32 weights of the 16-bit tensors, flat in the same way, or null: then p' is
+ * computed from the weight itself and rounded.  state: (seed, steps taken), 64-bit
+ * integers; t = steps taken + 1, which the call counts.  ticket: a zero that the call
+ * leaves as one.  With max_norm the norm is written to `norm`, and where it is not finite
+ * nothing else is written and the step is not counted; workspace as dt_grad_norm's.
+ * Deterministic.  Arithmetic in fp32, the steps' powers in fp64.
+ */
+int dt_adamw_step(int count, const int64_t* params, const int64_t* grads, const int64_t* sizes, const int32_t* kinds,
+                  int ngroups, const DtAdamWGroup* groups, int state_bits, void* exp_avg, void* exp_avg_sq,
+                  uint8_t* exp_avg_scale, uint8_t* exp_avg_sq_scale, float* master, int64_t* state, uint32_t* ticket,
+                  double max_norm, float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The numbers that 8-bit averages stand for, as bf16 (which holds each of them): [256 * blocks] each. */
+int dt_adamw_moments(const uint8_t* exp_avg, const uint8_t* exp_avg_scale, const uint8_t* exp_avg_sq,
+                     const uint8_t* exp_avg_sq_scale, int64_t blocks, void* exp_avg_out, void* exp_avg_sq_out,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

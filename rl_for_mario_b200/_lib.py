@@ -75,6 +75,10 @@ SIGNATURES = {
     "dt_head_norm_rope_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _P, _P, _L, _I, _I, _I,
                                         _I, _I, _P, _I, _F, _I, _P]),
     "dt_dropout": (_I, [_P, _L, _P, _L, _P, _L, _L, _I, _D, _P, _U, _I, _P]),
+    "dt_grad_norm": (_I, [_I, _P, _P, _P, _P, _P, _L, _P]),
+    "dt_grad_norm_workspace": (_L, [_I]),
+    "dt_adamw_step": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _D, _P, _P, _L, _P]),
+    "dt_adamw_moments": (_I, [_P, _P, _P, _P, _L, _P, _P, _P]),
 }
 
 

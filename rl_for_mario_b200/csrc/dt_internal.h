@@ -276,6 +276,49 @@ void head_norm_plan(HeadNormParams& p, int dtype, bool bwd, int num_sms);  // se
 long long head_norm_parts(long long rows, int Hq, int Hkv, int D, int num_sms);  // blocks of a backward pass, at most
 cudaError_t launch_head_norm_sm100(const HeadNormParams& p, int dtype, bool bwd, cudaStream_t st);
 
+// Many tensors in one launch: their pointers and sizes are kernel arguments.
+constexpr int kMaxTensors = 960, kAdamWGroups = 16;
+struct TensorSlot {
+  void* p;        // weights
+  const void* g;  // gradient, or null: the tensor is left alone
+  long long n;
+  uint32_t end;   // units of work up to and with this tensor, of the launch's
+  uint32_t kind;  // element code, group << 8
+};
+struct GradNormParams {
+  int count;
+  uint32_t units;
+  double* parts;  // a sum of squares for each block
+  float* norm;    // the norm itself, of a launch of one block that is the only one; else null
+};
+struct AdamWGroup {
+  double lr, b1, b2, eps, wd;
+  const float* lr_ptr;  // the rate on the device, or null: lr
+};
+struct AdamWParams {
+  AdamWGroup group[kAdamWGroups];
+  void* m;  // averages, flat: fp32, or codes with a scale for each block of 256
+  void* v;
+  uint8_t* m_scale;
+  uint8_t* v_scale;
+  float* master;       // fp32 weights of 16-bit tensors, flat, or null
+  long long* state;    // seed, steps taken
+  uint32_t* ticket;    // counts the blocks that are done; null in all launches of a step but the last
+  const double* parts;  // of the gradient's norm, or null: no clipping
+  float* norm;
+  long long first;  // block of the flat arrays that the launch's first one is
+  uint32_t units;   // blocks
+  int count, ngroups, nparts;
+  float max_norm;
+};
+int grad_norm_grid(long long units, int num_sms);
+long long grad_norm_unit();  // elements of a unit of the norm's work
+cudaError_t launch_grad_norm_sm100(const TensorSlot* slots, const GradNormParams& p, int num_sms, cudaStream_t st);
+cudaError_t launch_grad_norm_sum_sm100(const double* parts, int n, float* norm, cudaStream_t st);
+cudaError_t launch_adamw_sm100(const TensorSlot* slots, const AdamWParams& p, int num_sms, cudaStream_t st);
+cudaError_t launch_adamw_moments_sm100(const uint8_t* m, const uint8_t* m_scale, const uint8_t* v, const uint8_t* v_scale,
+                                       long long blocks, void* m_out, void* v_out, int num_sms, cudaStream_t st);
+
 struct ResidualNormParams {
   const void* x;
   const void* residual;  // or null

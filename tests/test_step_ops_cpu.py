@@ -73,3 +73,90 @@ def test_head_norm_wrapper_checks():
     refused(ValueError, "tables", sin=torch.zeros(5, 32))
     refused(ValueError, "start_pos", start_pos=torch.zeros(3, dtype=torch.int32))
     assert K._check_head_norm(*ok[:7], torch.zeros(2, dtype=torch.int64))[2].dtype == torch.int32
+
+
+def test_step_entry_points_refuse_bad_arguments():
+    import math
+
+    from rl_for_mario_b200 import _lib
+    from rl_for_mario_b200.optim import _GROUP
+
+    lib = _lib.load()
+    a, INV, UNS = 4096, _lib.DT_ERR_INVALID, _lib.DT_ERR_UNSUPPORTED
+    L, I = _lib._L, _lib._I
+
+    def arrays(p, g, n, kind):
+        return (L * 1)(p), (L * 1)(g), (L * 1)(n), (I * 1)(kind)
+
+    def norm(g=a, n=8, kind=0, count=1, out=a, ws=a, size=1 << 20):
+        _, gs, ns, ks = arrays(0, g, n, kind)
+        return lib.dt_grad_norm(count, gs, ns, ks, out, ws, size, None)
+
+    for kw, code in ((dict(count=0), INV), (dict(out=None), INV), (dict(ws=None), INV), (dict(size=7), INV),
+                     (dict(g=a + 1), INV), (dict(g=a + 2, kind=2), INV), (dict(n=-1), INV), (dict(n=1 << 40), INV),
+                     (dict(kind=3), UNS), (dict(kind=256), INV), (dict(kind=-256), INV), (dict(out=a + 2), INV)):
+        assert norm(**kw) == code, kw
+    assert lib.dt_grad_norm_workspace(0) < 0
+
+    def step(count=1, p=a, g=a, n=8, kind=0, ngroups=1, group=(1e-3, 0.9, 0.999, 1e-8, 0.0, 0), bits=32, m=a, s=None,
+             master=None, state=a, ticket=a, max_norm=0.0, norm=None, ws=None, size=0):
+        ps, gs, ns, ks = arrays(p, g, n, kind)
+        return lib.dt_adamw_step(count, ps, gs, ns, ks, ngroups, _GROUP.pack(*group), bits, m, a, s, s, master, state,
+                                 ticket, max_norm, norm, ws, size, None)
+
+    bad = [dict(count=0), dict(p=0), dict(p=a + 1), dict(g=a + 1), dict(n=-1), dict(kind=256), dict(m=None), dict(m=a + 8),
+           dict(bits=8), dict(master=a + 4), dict(state=None), dict(state=a + 4), dict(ticket=None), dict(ticket=a + 2),
+           dict(max_norm=1.0), dict(max_norm=1.0, norm=a), dict(max_norm=math.nan), dict(max_norm=1e-60, norm=a, ws=a),
+           dict(max_norm=1.0, norm=a, ws=a + 8, size=1 << 20)]
+    for i, wrong in enumerate((-1.0, 1.0, 1.0, 0.0, -1.0)):  # lr, betas, eps, decay
+        group = [1e-3, 0.9, 0.999, 1e-8, 0.0, 0]
+        for w in (wrong, math.nan, math.inf):
+            group[i] = w
+            bad.append(dict(group=tuple(group)))
+    bad.append(dict(group=(1e-3, 0.9, 0.999, 1e-8, 0.0, a + 1)))
+    for kw in bad:
+        assert step(**kw) == INV, kw
+    for kw in (dict(kind=3), dict(ngroups=0), dict(ngroups=17), dict(bits=16)):
+        assert step(**kw) == UNS, kw
+    assert lib.dt_adamw_moments(a, a, a, a, 0, a, a, None) == INV
+    assert lib.dt_adamw_moments(a, a, None, a, 1, a, a, None) == INV
+    assert lib.dt_adamw_moments(a, a, a, a, 1, a + 8, a, None) == INV
+
+
+def test_optimizer_refuses_cpu_tensors():
+    from rl_for_mario_b200 import optim
+
+    with pytest.raises(ValueError, match="CUDA"):
+        optim.AdamW([torch.nn.Parameter(torch.zeros(3))])
+    with pytest.raises(ValueError, match="CUDA"):
+        optim.grad_norm([torch.zeros(3)])
+    assert optim._dense(torch.zeros(3, 4, 5).permute(2, 0, 1)) and optim._dense(torch.zeros(1, 5)[:, :5])
+    assert not optim._dense(torch.zeros(4, 4)[:, :3]) and not optim._dense(torch.zeros(1).expand(3))
+    assert optim._dense(torch.zeros(0, 3)) and optim._dense(torch.zeros(()))
+
+
+def test_rounding_at_random_of_the_restatement():
+    """The 8-bit form as the oracle states it: every code decodes to a number that is stored as itself whatever its
+    word, two neighbours come in the part's proportion, scales are powers of two from the block's largest."""
+    import numpy as np
+
+    from oracle import step_ref as ref
+
+    for kind, codes in ((ref.FIRST, np.arange(0, 120)), (ref.SECOND, np.arange(0, 240))):
+        block = np.zeros(256, np.uint8)
+        block[:len(codes)] = codes
+        block[255] = codes[-1]  # of the top binade: the block's scale is its own
+        for scale in (32, 100, 127, 254):
+            x = ref.decode(block, np.array([scale]), kind)
+            assert np.isfinite(x).all() and (np.diff(x[:len(codes)]) > 0).all()
+            assert np.array_equal(x.astype(np.float32), torch.from_numpy(x).bfloat16().float().numpy())
+            for word in (0, 65535):
+                back, e = ref.encode(x, np.full(256, word), kind)
+                assert np.array_equal(back, block) and e[0] == scale
+    x = np.zeros(256, np.float32)
+    x[0], x[1:] = 1.0, 0.3
+    up = [ref.encode(x, np.full(256, w), ref.SECOND)[0][1] for w in range(0, 65536, 64)]
+    low = min(up)
+    a, b = (float(ref.decode(np.full(256, c, np.uint8), np.array([127]), ref.SECOND)[0]) for c in (low, low + 1))
+    share = (0.3 - a) / (b - a)
+    assert a < 0.3 < b and abs(np.mean([u != low for u in up]) - share) < 2 / 1024
