@@ -7,7 +7,7 @@
 //
 // Tensors are cut into blocks of 256 elements, a warp's work; a tensor starts a new block, so
 // the averages of tensor i lie from element 256 (blocks before it) on in flat arrays of whole
-// blocks.  Pointers and sizes travel as kernel arguments (up to 960 tensors a launch): there
+// blocks.  Pointers and sizes travel as kernel arguments (up to 768 tensors a launch): there
 // is no table on the device to be built, kept or to go stale.
 //
 // Averages in 8 bits: a block of each shares a scale 2^e, e from its largest value.  m is kept as
@@ -36,7 +36,11 @@ namespace dtk {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kNormResident = 4;  // blocks on an SM
+template <bool BITS8>
+constexpr int kStepResident = BITS8 ? 3 : 2;
 constexpr int kNormUnit = 1024;      // elements of a warp's turn in the norm
+constexpr int kStepUnit = 512;       // and in the step
 constexpr uint32_t kSite = 0xffffffffu;  // the generator's site of the averages' rounding
 constexpr int kMinScale = 32;        // exponents of scales (biased): their products with any code are normal numbers
 
@@ -59,40 +63,72 @@ __device__ __forceinline__ int find_slot(const uint32_t* ends, int count, uint32
 
 __device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<unsigned long long>(p) & 15) == 0; }
 
-// Eight elements from `at` on of a tensor of element code DT; those past its end read as 0 and are not written.
-template <int DT>
-__device__ __forceinline__ void get8(const void* base, long long at, long long n, bool vec, float (&v)[8]) {
-  using T = typename TrainElem<DT>::T;
-  const T* x = static_cast<const T*>(base) + at;
+// Eight elements as they stand in memory (one 16-byte word of 16-bit ones, two of fp32), on their way while
+// others are worked on.
+struct Raw8Any {
+  uint4 u[2];
+};
+__device__ __forceinline__ Raw8Any get_raw(int code, const void* base, long long at, long long n, bool vec) {
+  Raw8Any r;
+  r.u[0] = r.u[1] = make_uint4(0u, 0u, 0u, 0u);
   if (vec && at + 8 <= n) {
-    load8<DT, true>(x, 0, 0, 8, v);
-  } else {
+    const uint4* x = reinterpret_cast<const uint4*>(static_cast<const char*>(base) + at * (code == 2 ? 4 : 2));
+    r.u[0] = x[0];
+    if (code == 2) r.u[1] = x[1];
+  } else if (at < n) {  // an address off the boundary, or the tensor's end: elements past it read as 0
+    uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = at + i < n ? TrainElem<DT>::to_f(x[i]) : 0.f;
-  }
-}
-template <int DT>
-__device__ __forceinline__ void put8(void* base, long long at, long long n, bool vec, const float (&v)[8]) {
-  using T = typename TrainElem<DT>::T;
-  T* x = static_cast<T*>(base) + at;
-  if (vec && at + 8 <= n) {
-    store8<DT, true>(x, 0, 0, 8, v);
-  } else {
+    for (int i = 0; i < 8; ++i) w[i] = 0u;
+    if (code == 2) {
+      const uint32_t* x = static_cast<const uint32_t*>(base) + at;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (at + i < n) x[i] = TrainElem<DT>::from_f(v[i]);
+      for (int i = 0; i < 8; ++i)
+        if (at + i < n) w[i] = x[i];
+    } else {
+      const uint16_t* x = static_cast<const uint16_t*>(base) + at;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (at + i < n) w[i >> 1] |= (uint32_t)x[i] << (16 * (i & 1));
+    }
+    r.u[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    r.u[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
+  return r;
 }
-// By the tensor's own code (the same for a warp).
-__device__ __forceinline__ void get8_of(int code, const void* base, long long at, long long n, bool vec, float (&v)[8]) {
-  if (code == 0) get8<0>(base, at, n, vec, v);
-  else if (code == 1) get8<1>(base, at, n, vec, v);
-  else get8<2>(base, at, n, vec, v);
+__device__ __forceinline__ void unpack(int code, const Raw8Any& r, F8& v) {
+  const uint32_t w[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v.p[i] = code == 2   ? make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]))
+             : code == 1 ? Elem<false>::to_f2(w[i])
+                         : Elem<true>::to_f2(w[i]);
 }
-__device__ __forceinline__ void put8_of(int code, void* base, long long at, long long n, bool vec, const float (&v)[8]) {
-  if (code == 0) put8<0>(base, at, n, vec, v);
-  else if (code == 1) put8<1>(base, at, n, vec, v);
-  else put8<2>(base, at, n, vec, v);
+// The elements rounded to their type; those past the tensor's end are not written.
+__device__ __forceinline__ void put8(int code, void* base, long long at, long long n, bool vec, const F8& v) {
+  if (code == 2) {
+    float* x = static_cast<float*>(base) + at;
+    if (vec && at + 8 <= n) {
+      *reinterpret_cast<float4*>(x) = make_float4(v.p[0].x, v.p[0].y, v.p[1].x, v.p[1].y);
+      *reinterpret_cast<float4*>(x + 4) = make_float4(v.p[2].x, v.p[2].y, v.p[3].x, v.p[3].y);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (at + i < n) x[i] = i & 1 ? v.p[i >> 1].y : v.p[i >> 1].x;
+    }
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = code == 1 ? Elem<false>::from_f2(v.p[i].x, v.p[i].y) : Elem<true>::from_f2(v.p[i].x, v.p[i].y);
+    uint16_t* x = static_cast<uint16_t*>(base) + at;
+    if (vec && at + 8 <= n) {
+      *reinterpret_cast<uint4*>(x) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (at + i < n) x[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
+  }
 }
 
 // The block's sum of a value of each thread, in a fixed order; every thread gets it.
@@ -108,20 +144,8 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
 }
 
 // ---------------------------------------------------------------- norm
-// Sums of eight squares are fp32 where that loses nothing, else fp64 (squares of numbers
-// beyond 2^63 overflow in fp32, those of numbers below 2^-63 lose their bits); sums of
-// those fp64.
-__device__ __forceinline__ double square8(const float (&v)[8]) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s = fmaf(v[i], v[i], s);
-  if (s >= 1e-28f && s <= 1e38f) return (double)s;
-  double d = 0.0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) d += (double)v[i] * (double)v[i];
-  return d;
-}
-
+// Sums of 32 squares are fp32 where that loses nothing, else fp64 (squares of numbers beyond
+// 2^63 overflow in fp32, those of numbers below 2^-63 lose their bits); sums of those fp64.
 template <int N>
 __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_constant__ TensorTable<N> table,
                                                              const __grid_constant__ GradNormParams p) {
@@ -135,13 +159,43 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
     const int t = find_slot(ends, p.count, u, lane);
     const TensorSlot& s = table.slot[t];
     if (!s.g) continue;
+    const int code = s.kind & 3;
     const long long first = (long long)(u - (t ? ends[t - 1] : 0u)) * kNormUnit + lane * 8;
     const bool vec = aligned16(s.g);
+    constexpr int TURNS = kNormUnit / 256;
+    Raw8Any raw[TURNS];
 #pragma unroll
-    for (int i = 0; i < kNormUnit / 256; ++i) {
-      float v[8];
-      get8_of(s.kind & 3, s.g, first + i * 256, s.n, vec, v);
-      sum += square8(v);
+    for (int i = 0; i < TURNS; ++i) raw[i] = get_raw(code, s.g, first + i * 256, s.n, vec);
+    float2 q[TURNS];
+    auto squares = [&](int code) {
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        F8 v;
+        unpack(code, raw[i], v);
+        q[i] = fmul2(v.p[0], v.p[0]);
+#pragma unroll
+        for (int j = 1; j < 4; ++j) q[i] = ffma2(v.p[j], v.p[j], q[i]);
+      }
+    };
+    if (code == 0) squares(0);
+    else if (code == 1) squares(1);
+    else squares(2);
+#pragma unroll
+    for (int i = TURNS / 2; i > 0; i >>= 1)
+#pragma unroll
+      for (int j = 0; j < i; ++j) q[j] = fadd2(q[j], q[j + i]);
+    const float f = both_sum(q[0]);
+    if (f >= 1e-28f && f <= 1e38f) {
+      sum += (double)f;
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < TURNS; ++i) {
+        F8 v;
+        unpack(code, get_raw(code, s.g, first + i * 256, s.n, vec), v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sum += (double)v.p[j].x * (double)v.p[j].x + (double)v.p[j].y * (double)v.p[j].y;
+      }
     }
   }
   sum = block_sum(sum, red);
@@ -174,58 +228,87 @@ __device__ __forceinline__ float decode_scale(int e) {
   return e == 255 ? __uint_as_float(0x7fc00000u) : scale_of(max(e, kMinScale) - TOP);
 }
 
-// Four codes of the first (second) average as fp32, without their block's scale.
-__device__ __forceinline__ void decode_first(uint32_t codes, float* v) {
+// Eight codes of the first (second) average as fp32, times f.
+__device__ __forceinline__ void decode_first(uint2 codes, float f, F8& v) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 4; ++i) {
     uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)(codes >> (16 * i))));
-    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)((i < 2 ? codes.x : codes.y) >> (16 * (i & 1)))));
+    v.p[i] = fmul2(__half22float2(*reinterpret_cast<__half2*>(&h)), both(f));
   }
 }
-__device__ __forceinline__ void decode_second(uint32_t codes, float* v) {
+__device__ __forceinline__ void decode_second(uint2 codes, float f, F8& v) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 4; ++i) {
     // Two codes, each 7 bits up in a half of its own.
-    uint32_t h = __byte_perm(codes, 0, i ? 0x4342 : 0x4140) << 7;
-    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    uint32_t h = __byte_perm(i < 2 ? codes.x : codes.y, 0, i & 1 ? 0x4342 : 0x4140) << 7;
+    v.p[i] = fmul2(__half22float2(*reinterpret_cast<__half2*>(&h)), both(f));
   }
 }
 
-// y >= 0, scaled into the codes' range (2^(TOP + 1) at most), rounded up or down by u, a 16-bit word:
-// three bits behind the leading one, from 2^(1 - BIAS) down in steps of 2^(-2 - BIAS).
-template <int BIAS>
-__device__ __forceinline__ uint32_t encode(float y, uint32_t u) {
-  const uint32_t small = ((uint32_t)__float2int_rz(y * (float)(1ull << (BIAS + 18))) + u) >> 16;
-  const uint32_t large = ((__float_as_uint(y) + (u << 4)) >> 20) - ((127u - BIAS) << 3);
-  return y < 1.f / (1 << (BIAS - 1)) ? small : large;
+// The largest of three numbers, or NaN when one of them is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
-// Stores a lane's eight values of a block; returns nothing, the block's scale goes with lane 0.
+// y >= 0, scaled into the codes' range (below 2^(TOP + 1)), rounded up or down at random to three bits behind
+// the leading one: the code comes out as the top byte.  An fp32 number shifted up by four bits has its
+// exponent's lower five bits and its three leading ones there, and 20 more below; adding the word at the
+// top of these carries into the code in the part's proportion.  The exponent's bias changes by the byte that
+// `word` has above the 16 random bits.  Numbers below 2^(1 - BIAS) have equal steps of 2^(-2 - BIAS): 2^(1 - BIAS) is
+// added first, after which they stand in the binade with that spacing, eight codes up (rounded to zero:
+// what falls off lies below the random bits).  The comparison's result as the number 1 or 0 does both on the
+// FMA pipe: the ALU, at half its rate, is what the 8-bit step runs into (selects instead: XX us).
+template <int BIAS>
+__device__ __forceinline__ uint32_t encode(float y, uint32_t word, uint32_t select) {
+  constexpr float low = 1.f / (1 << (BIAS - 1));
+  constexpr uint32_t back = (uint32_t)(-((127 - BIAS) << 3)) & 0xffu;
+  // The bits of 1.0f times this are -8 in the top byte: 127 * 2^23 * 16 mod 2^32 = -2^27.
+  constexpr uint32_t eight = 16u;
+  static_assert(0x3f800000u * eight == (uint32_t)(-8) << 24, "");
+  float small;
+  asm("set.lt.f32.f32 %0, %1, %2;" : "=f"(small) : "f"(y), "f"(low));
+  const float z = __fmaf_rz(small, low, y);
+  return __float_as_uint(z) * 16u + (__float_as_uint(small) * eight + __byte_perm(word, back, select));
+}
+
+// Stores a lane's eight values of a block, the block's scale by lane 0.  Random words: the two halves of each word,
+// the bytes of a half turned over for the signed average.
 template <int BIAS, int TOP, bool SIGNED>
-__device__ __forceinline__ void put_codes(uint8_t* codes, uint8_t* scale, const float (&x)[8], const uint4& words, int lane) {
-  uint32_t most = 0;
+__device__ __forceinline__ void put_codes(uint8_t* codes, uint8_t* scale, const F8& x, const uint4& words, int lane) {
+  float most = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-  const int e = max((int)(__reduce_max_sync(0xffffffffu, most) >> 23), kMinScale);
+  for (int i = 0; i < 4; ++i) most = max_nan(most, fabsf(x.p[i].x), fabsf(x.p[i].y));
+  const int e = max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23), kMinScale);
   const float f = scale_of(254 + TOP - min(e, 254));
   const uint32_t w[4] = {words.x, words.y, words.z, words.w};
-  uint32_t c[2] = {0u, 0u};
+  uint32_t c[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t u = i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
-    uint32_t k = encode<BIAS>(fabsf(x[i]) * f, u) & 0xffu;
-    if constexpr (SIGNED)
-      k |= __float_as_uint(x[i]) >> 24 & 0x80u;
-    else
-      k = x[i] > 0.f ? max(k, 1u) : k;
-    c[i >> 2] |= k << (8 * (i & 3));
+  for (int i = 0; i < 4; ++i) {
+    const float2 y = fmul2(x.p[i], both(f));
+    // Bytes: 0, the half's two, the bias.
+    c[2 * i] = encode<BIAS>(SIGNED ? fabsf(y.x) : y.x, w[i], SIGNED ? 0x4015 : 0x4105);
+    c[2 * i + 1] = encode<BIAS>(SIGNED ? fabsf(y.y) : y.y, w[i], SIGNED ? 0x4235 : 0x4325);
+    if constexpr (SIGNED) {
+      c[2 * i] = (c[2 * i] & 0x7fffffffu) | (__float_as_uint(y.x) & 0x80000000u);
+      c[2 * i + 1] = (c[2 * i + 1] & 0x7fffffffu) | (__float_as_uint(y.y) & 0x80000000u);
+    }
   }
-  *reinterpret_cast<uint2*>(codes) = make_uint2(c[0], c[1]);
+  uint32_t four[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    four[k] = __byte_perm(__byte_perm(c[4 * k], c[4 * k + 1], 0x0073), __byte_perm(c[4 * k + 2], c[4 * k + 3], 0x0073), 0x5410);
+    if constexpr (!SIGNED)
+      if ((four[k] - 0x01010101u) & ~four[k] & 0x80808080u)  // a zero among them: a step for what is above zero
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = j & 1 ? x.p[2 * k + (j >> 1)].y : x.p[2 * k + (j >> 1)].x;
+          if (v > 0.f && !(four[k] >> (8 * j) & 0xffu)) four[k] |= 1u << (8 * j);
+        }
+  }
+  *reinterpret_cast<uint2*>(codes) = make_uint2(four[0], four[1]);
   if (lane == 0) *scale = (uint8_t)e;
 }
 
@@ -234,11 +317,113 @@ struct GroupNow {
   float rate, root, decay, b1, c1, b2, c2, eps;
 };
 
-// Off by an ulp at most; the weights' own rounding is larger than what it does to a step.
+// Each off by an ulp or so; the weights' own rounding is larger than what that does to a step.
 __device__ __forceinline__ float fast_sqrt(float x) {
   float r;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+__device__ __forceinline__ float fast_inverse(float x) {  // of normal numbers (eps is one)
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// What a lane holds of a block of 256 elements.
+template <bool BITS8>
+struct BlockLoad {
+  Raw8Any g, w;
+  uint4 m[BITS8 ? 1 : 2], v[BITS8 ? 1 : 2];  // 8 bits: codes in x, y, the scale in z
+};
+
+// A block's place: of the lane's first element in its tensor and in the flat arrays.
+struct BlockPlace {
+  long long at, block;
+  __device__ __forceinline__ long long mine(int lane) const { return block * 256 + lane * 8; }
+};
+
+// CODE: the tensor's element code; VEC: the block is whole and stands on 16-byte boundaries.
+template <bool BITS8, bool MASTER, int CODE, bool VEC>
+__device__ __forceinline__ BlockLoad<BITS8> load_block(const AdamWParams& p, const TensorSlot& s, const BlockPlace& q, int lane) {
+  BlockLoad<BITS8> r;
+  const long long mine = q.mine(lane), end = VEC ? q.at + 8 : s.n;
+  r.g = get_raw(CODE, s.g, q.at, end, VEC || aligned16(s.g));
+  if constexpr (MASTER && CODE != 2)
+    r.w = get_raw(2, p.master, mine, mine + 8, true);
+  else
+    r.w = get_raw(CODE, s.p, q.at, end, VEC || aligned16(s.p));
+  if constexpr (BITS8) {
+    const uint2 m = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.m) + mine);
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.v) + mine);
+    r.m[0] = make_uint4(m.x, m.y, p.m_scale[q.block], 0u);
+    r.v[0] = make_uint4(v.x, v.y, p.v_scale[q.block], 0u);
+  } else {
+    const Raw8Any m = get_raw(2, p.m, mine, mine + 8, true), v = get_raw(2, p.v, mine, mine + 8, true);
+    r.m[0] = m.u[0], r.m[1] = m.u[1], r.v[0] = v.u[0], r.v[1] = v.u[1];
+  }
+  return r;
+}
+
+template <bool BITS8, bool MASTER, int CODE, bool VEC>
+__device__ __forceinline__ void step_block(const AdamWParams& p, const TensorSlot& s, const BlockPlace& place,
+                                           const BlockLoad<BITS8>& r, const GroupNow& q, float clip, const DropKey& key,
+                                           int lane) {
+  const long long mine = place.mine(lane);
+  F8 w, h, m, v;
+  unpack(CODE, r.g, h);
+  unpack(MASTER ? 2 : CODE, r.w, w);
+  // The averages times b1 and b2: in 8 bits scale and factor in one, which rounds the same.
+  if constexpr (BITS8) {
+    decode_first(make_uint2(r.m[0].x, r.m[0].y), decode_scale<7>((int)r.m[0].z) * q.b1, m);
+    decode_second(make_uint2(r.v[0].x, r.v[0].y), decode_scale<14>((int)r.v[0].z) * q.b2, v);
+  } else {
+    unpack(2, Raw8Any{r.m[0], r.m[1]}, m);
+    unpack(2, Raw8Any{r.v[0], r.v[1]}, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m.p[i] = fmul2(m.p[i], both(q.b1)), v.p[i] = fmul2(v.p[i], both(q.b2));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // Each product and sum of the averages rounded by itself (packed ones are never contracted): what is
+    // stored does not depend on the compiler.
+    h.p[i] = fmul2(h.p[i], both(clip));
+    m.p[i] = fadd2(m.p[i], fmul2(h.p[i], both(q.c1)));
+    v.p[i] = fadd2(v.p[i], fmul2(fmul2(h.p[i], h.p[i]), both(q.c2)));
+    const float2 d = make_float2(fast_inverse(fmaf(fast_sqrt(v.p[i].x), q.root, q.eps)),
+                                 fast_inverse(fmaf(fast_sqrt(v.p[i].y), q.root, q.eps)));
+    w.p[i] = ffma2(fmul2(m.p[i], both(-q.rate)), d, fmul2(w.p[i], both(q.decay)));
+  }
+  if constexpr (MASTER && CODE != 2) put8(2, p.master, mine, mine + 8, true, w);
+  put8(CODE, s.p, place.at, VEC ? place.at + 8 : s.n, VEC || aligned16(s.p), w);
+  if constexpr (BITS8) {
+    const uint4 u = philox7(key, (unsigned long long)place.block * 32 + lane);
+    put_codes<7, 7, true>(static_cast<uint8_t*>(p.m) + mine, p.m_scale + place.block, m, u, lane);
+    put_codes<15, 14, false>(static_cast<uint8_t*>(p.v) + mine, p.v_scale + place.block, v, u, lane);
+  } else {
+    put8(2, p.m, mine, mine + 8, true, m);
+    put8(2, p.v, mine, mine + 8, true, v);
+  }
+}
+
+// A warp's unit of work: two blocks, or what the tensor has left of them.
+template <bool BITS8, bool MASTER, int CODE>
+__device__ __forceinline__ void step_unit(const AdamWParams& p, const TensorSlot& s, uint32_t unit, float clip,
+                                          const GroupNow* groups, const DropKey& key, int lane) {
+  const long long first = (long long)unit * kStepUnit;
+  const BlockPlace a{first + lane * 8, p.first + s.first + (long long)unit * (kStepUnit / 256)}, b{a.at + 256, a.block + 1};
+  const GroupNow q = groups[s.kind >> 8];
+  if (first + kStepUnit <= s.n && aligned16(s.p) && aligned16(s.g)) {
+    const auto x = load_block<BITS8, MASTER, CODE, true>(p, s, a, lane), y = load_block<BITS8, MASTER, CODE, true>(p, s, b, lane);
+    step_block<BITS8, MASTER, CODE, true>(p, s, a, x, q, clip, key, lane);
+    step_block<BITS8, MASTER, CODE, true>(p, s, b, y, q, clip, key, lane);
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      const BlockPlace& c = i ? b : a;
+      if (first + i * 256 < s.n)
+        step_block<BITS8, MASTER, CODE, false>(p, s, c, load_block<BITS8, MASTER, CODE, false>(p, s, c, lane), q, clip, key, lane);
+    }
+  }
 }
 
 // x^n by squaring.
@@ -249,8 +434,8 @@ __device__ __forceinline__ double power(double x, unsigned long long n) {
   return r;
 }
 
-template <bool BITS8, int N>
-__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ TensorTable<N> table,
+template <bool BITS8, bool MASTER, int N>
+__global__ void __launch_bounds__(kThreads, kStepResident<BITS8>) adamw_kernel(const __grid_constant__ TensorTable<N> table,
                                                             const __grid_constant__ AdamWParams p) {
   __shared__ uint32_t ends[N];
   __shared__ GroupNow groups[kAdamWGroups];
@@ -277,55 +462,15 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
   const int lane = threadIdx.x & 31;
   const DropKey key{(uint32_t)seed, (uint32_t)((unsigned long long)seed >> 32), (uint32_t)step, kSite};
   if (!skip)
-    for (uint32_t b = blockIdx.x * kWarps + (threadIdx.x >> 5); b < p.units; b += gridDim.x * kWarps) {
-      const int t = find_slot(ends, p.count, b, lane);
+    for (uint32_t u = blockIdx.x * kWarps + (threadIdx.x >> 5); u < p.units; u += gridDim.x * kWarps) {
+      const int t = find_slot(ends, p.count, u, lane);
       const TensorSlot& s = table.slot[t];
       if (!s.g) continue;
+      const uint32_t unit = u - (t ? ends[t - 1] : 0u);
       const int code = s.kind & 3;
-      const GroupNow& q = groups[s.kind >> 8];
-      const long long n = s.n, at = (long long)(b - (t ? ends[t - 1] : 0u)) * 256 + lane * 8;
-      const long long block = p.first + b, mine = block * 256 + lane * 8;
-      const bool vec_p = aligned16(s.p), vec_g = aligned16(s.g), master = p.master && code != 2;
-      float w[8], g[8], m[8], v[8];
-      get8_of(code, s.g, at, n, vec_g, g);
-      if (master)
-        load8<2, true>(p.master + mine, 0, 0, 8, w);
-      else
-        get8_of(code, s.p, at, n, vec_p, w);
-      if constexpr (BITS8) {
-        const uint2 cm = *reinterpret_cast<const uint2*>(static_cast<uint8_t*>(p.m) + mine);
-        const uint2 cv = *reinterpret_cast<const uint2*>(static_cast<uint8_t*>(p.v) + mine);
-        const float fm = decode_scale<7>(p.m_scale[block]), fv = decode_scale<14>(p.v_scale[block]);
-        decode_first(cm.x, m), decode_first(cm.y, m + 4);
-        decode_second(cv.x, v), decode_second(cv.y, v + 4);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m[i] *= fm, v[i] *= fv;
-      } else {
-        load8<2, true>(static_cast<float*>(p.m) + mine, 0, 0, 8, m);
-        load8<2, true>(static_cast<float*>(p.v) + mine, 0, 0, 8, v);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // Each product and sum of the averages rounded by itself: what is stored does not depend on how a
-        // compiler contracts them.
-        const float h = __fmul_rn(g[i], clip);
-        m[i] = __fadd_rn(__fmul_rn(m[i], q.b1), __fmul_rn(h, q.c1));
-        v[i] = __fadd_rn(__fmul_rn(v[i], q.b2), __fmul_rn(__fmul_rn(h, h), q.c2));
-        w[i] = w[i] * q.decay - q.rate * __fdividef(m[i], fmaf(fast_sqrt(v[i]), q.root, q.eps));
-      }
-      if (master) store8<2, true>(p.master + mine, 0, 0, 8, w);
-      put8_of(code, s.p, at, n, vec_p, w);
-      if constexpr (BITS8) {
-        const uint4 u = philox7(key, (unsigned long long)block * 32 + lane);
-        // One word for both averages, its bytes turned over for the first.
-        const uint4 r = make_uint4(__byte_perm(u.x, 0, 0x2301), __byte_perm(u.y, 0, 0x2301),
-                                   __byte_perm(u.z, 0, 0x2301), __byte_perm(u.w, 0, 0x2301));
-        put_codes<7, 7, true>(static_cast<uint8_t*>(p.m) + mine, p.m_scale + block, m, r, lane);
-        put_codes<15, 14, false>(static_cast<uint8_t*>(p.v) + mine, p.v_scale + block, v, u, lane);
-      } else {
-        store8<2, true>(static_cast<float*>(p.m) + mine, 0, 0, 8, m);
-        store8<2, true>(static_cast<float*>(p.v) + mine, 0, 0, 8, v);
-      }
+      if (code == 0) step_unit<BITS8, MASTER, 0>(p, s, unit, clip, groups, key, lane);
+      else if (code == 1) step_unit<BITS8, MASTER, 1>(p, s, unit, clip, groups, key, lane);
+      else step_unit<BITS8, MASTER, 2>(p, s, unit, clip, groups, key, lane);
     }
   // The last block to come here counts the step; every block has read it by then.
   if (threadIdx.x == 0 && p.ticket && !skip) {
@@ -344,15 +489,11 @@ __global__ void __launch_bounds__(kThreads) adamw_moments_kernel(const uint8_t* 
   const int lane = threadIdx.x & 31;
   for (long long b = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); b < blocks; b += (long long)gridDim.x * kWarps) {
     const long long at = b * 256 + lane * 8;
-    const uint2 cm = *reinterpret_cast<const uint2*>(m + at), cv = *reinterpret_cast<const uint2*>(v + at);
-    const float fm = decode_scale<7>(m_scale[b]), fv = decode_scale<14>(v_scale[b]);
-    float x[8], y[8];
-    decode_first(cm.x, x), decode_first(cm.y, x + 4);
-    decode_second(cv.x, y), decode_second(cv.y, y + 4);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= fm, y[i] *= fv;
-    store8<0, true>(m_out + at, 0, 0, 8, x);
-    store8<0, true>(v_out + at, 0, 0, 8, y);
+    F8 x, y;
+    decode_first(*reinterpret_cast<const uint2*>(m + at), decode_scale<7>(m_scale[b]), x);
+    decode_second(*reinterpret_cast<const uint2*>(v + at), decode_scale<14>(v_scale[b]), y);
+    put8(0, m_out, at, at + 8, true, x);
+    put8(0, v_out, at, at + 8, true, y);
   }
 }
 
@@ -380,10 +521,11 @@ unsigned grid_for(long long units, int num_sms, int resident) {
 
 }  // namespace
 
-constexpr int kNormResident = 8, kStepResident = 4;
+
 
 int grad_norm_grid(long long units, int num_sms) { return (int)grid_for(units, num_sms, kNormResident); }
 long long grad_norm_unit() { return kNormUnit; }
+long long adamw_unit() { return kStepUnit; }
 
 cudaError_t launch_grad_norm_sm100(const TensorSlot* slots, const GradNormParams& p, int num_sms, cudaStream_t st) {
   const unsigned grid = (unsigned)grad_norm_grid(p.units, num_sms);
@@ -399,12 +541,12 @@ cudaError_t launch_grad_norm_sum_sm100(const double* parts, int n, float* norm, 
 }
 
 cudaError_t launch_adamw_sm100(const TensorSlot* slots, const AdamWParams& p, int num_sms, cudaStream_t st) {
-  const unsigned grid = grid_for(p.units, num_sms, kStepResident);
+  const unsigned grid = grid_for(p.units, num_sms, p.m_scale ? kStepResident<true> : kStepResident<false>);
   with_tables(slots, p.count, [&](const auto& t) {
-    if (p.m_scale)
-      adamw_kernel<true><<<grid, kThreads, 0, st>>>(t, p);
-    else
-      adamw_kernel<false><<<grid, kThreads, 0, st>>>(t, p);
+    if (p.m_scale && p.master) adamw_kernel<true, true><<<grid, kThreads, 0, st>>>(t, p);
+    else if (p.m_scale) adamw_kernel<true, false><<<grid, kThreads, 0, st>>>(t, p);
+    else if (p.master) adamw_kernel<false, true><<<grid, kThreads, 0, st>>>(t, p);
+    else adamw_kernel<false, false><<<grid, kThreads, 0, st>>>(t, p);
   });
   return cudaGetLastError();
 }

@@ -21,8 +21,8 @@ struct Range {
   Range& operator=(const Range&) = delete;
 };
 
-constexpr int64_t kMaxUnits = 0x7fffffffLL;  // of a launch
-constexpr int64_t kMaxSize = 1LL << 38;      // elements of a tensor: fewer blocks than a launch takes
+constexpr int64_t kMaxBlocks = 0x3fffffffLL;  // of 256 elements, of a launch
+constexpr int64_t kMaxSize = 1LL << 37;      // elements of a tensor: fewer blocks than a launch takes
 
 int cuda_status(cudaError_t e, const char* what) {
   return e == cudaSuccess ? DT_OK : api_fail(DT_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
@@ -52,8 +52,8 @@ int check_tensor(const char* fn, int i, int64_t p, int64_t g, int64_t n, int kin
   return DT_OK;
 }
 
-// Walks through the tensors in launches of up to kMaxTensors and kMaxUnits units: f(slots, count, units, first
-// unit of all, last launch).  Tensors' units: their elements in units of `unit`, rounded up.
+// Walks through the tensors in launches of up to kMaxTensors tensors and kMaxBlocks blocks: f(slots, count, units, first
+// block of all, last launch).  Tensors' units: their elements in units of `unit`, rounded up; blocks: of 256.
 template <typename F>
 int in_launches(int count, const int64_t* params, const int64_t* grads, const int64_t* sizes, const int32_t* kinds,
                 int64_t unit, F f) {
@@ -61,17 +61,18 @@ int in_launches(int count, const int64_t* params, const int64_t* grads, const in
   int64_t first = 0;
   for (int i = 0; i < count;) {
     int n = 0;
-    int64_t units = 0;
+    int64_t units = 0, blocks = 0;
     for (; i < count && n < dtk::kMaxTensors; ++i, ++n) {
-      const int64_t more = (sizes[i] + unit - 1) / unit;
-      if (units + more > kMaxUnits && n) break;
+      const int64_t more = (sizes[i] + unit - 1) / unit, b = (sizes[i] + 255) / 256;
+      if (blocks + b > kMaxBlocks && n) break;
       units += more;
-      slots[n] = TensorSlot{params ? reinterpret_cast<void*>(params[i]) : nullptr,
-                            reinterpret_cast<const void*>(grads[i]), sizes[i], (uint32_t)units, (uint32_t)kinds[i]};
+      slots[n] = TensorSlot{params ? reinterpret_cast<void*>(params[i]) : nullptr, reinterpret_cast<const void*>(grads[i]),
+                            sizes[i], (uint32_t)units, (uint32_t)blocks, (uint32_t)kinds[i]};
+      blocks += b;
     }
     const int rc = f(slots, n, (uint32_t)units, first, i == count);
     if (rc) return rc;
-    first += units;
+    first += blocks;
   }
   return DT_OK;
 }
@@ -93,9 +94,9 @@ int launch_norm(const char* fn, int count, const int64_t* grads, const int64_t* 
 }
 
 int64_t norm_parts(int count, int num_sms) {
-  // A launch ends at kMaxTensors tensors or before a tensor that would pass kMaxUnits: at most one for each of them.
+  // A launch ends at kMaxTensors tensors, or before one that would pass kMaxBlocks: 2^38 elements, which no GPU holds.
   const int64_t launches = (count + dtk::kMaxTensors - 1) / dtk::kMaxTensors;
-  return launches * dtk::grad_norm_grid(kMaxUnits, num_sms);
+  return launches * dtk::grad_norm_grid(kMaxBlocks, num_sms);
 }
 
 }  // namespace
@@ -186,7 +187,7 @@ int dt_adamw_step(int count, const int64_t* params, const int64_t* grads, const 
   p.ngroups = ngroups, p.m = exp_avg, p.v = exp_avg_sq, p.master = master;
   if (state_bits == 8) p.m_scale = exp_avg_scale, p.v_scale = exp_avg_sq_scale;
   p.state = reinterpret_cast<long long*>(state);
-  return in_launches(count, params, grads, sizes, kinds, 256,
+  return in_launches(count, params, grads, sizes, kinds, dtk::adamw_unit(),
                      [&](const TensorSlot* slots, int n, uint32_t units, int64_t first, bool last) {
                        p.count = n, p.units = units, p.first = first, p.ticket = last ? ticket : nullptr;
                        return cuda_status(dtk::launch_adamw_sm100(slots, p, sms, st), fn);

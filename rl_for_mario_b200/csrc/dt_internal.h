@@ -277,13 +277,14 @@ long long head_norm_parts(long long rows, int Hq, int Hkv, int D, int num_sms); 
 cudaError_t launch_head_norm_sm100(const HeadNormParams& p, int dtype, bool bwd, cudaStream_t st);
 
 // Many tensors in one launch: their pointers and sizes are kernel arguments.
-constexpr int kMaxTensors = 960, kAdamWGroups = 16;
+constexpr int kMaxTensors = 768, kAdamWGroups = 16;
 struct TensorSlot {
   void* p;        // weights
   const void* g;  // gradient, or null: the tensor is left alone
   long long n;
-  uint32_t end;   // units of work up to and with this tensor, of the launch's
-  uint32_t kind;  // element code, group << 8
+  uint32_t end;    // units of work up to and with this tensor, of the launch's
+  uint32_t first;  // blocks of 256 elements of the launch's tensors before it
+  uint32_t kind;   // element code, group << 8
 };
 struct GradNormParams {
   int count;
@@ -307,12 +308,13 @@ struct AdamWParams {
   const double* parts;  // of the gradient's norm, or null: no clipping
   float* norm;
   long long first;  // block of the flat arrays that the launch's first one is
-  uint32_t units;   // blocks
+  uint32_t units;
   int count, ngroups, nparts;
   float max_norm;
 };
 int grad_norm_grid(long long units, int num_sms);
 long long grad_norm_unit();  // elements of a unit of the norm's work
+long long adamw_unit();      // and of the step's
 cudaError_t launch_grad_norm_sm100(const TensorSlot* slots, const GradNormParams& p, int num_sms, cudaStream_t st);
 cudaError_t launch_grad_norm_sum_sm100(const double* parts, int n, float* norm, cudaStream_t st);
 cudaError_t launch_adamw_sm100(const TensorSlot* slots, const AdamWParams& p, int num_sms, cudaStream_t st);

@@ -14,6 +14,7 @@ import ctypes
 import math
 import struct
 from array import array
+from operator import attrgetter
 from typing import Dict, Iterable, List, Optional, Tuple, Union
 
 import torch
@@ -39,6 +40,12 @@ def _dense(t: Tensor) -> bool:
     return True
 
 
+# Each of these looks at one property of many tensors without an interpreted loop: a model has a hundred
+# tensors, and a microsecond for each would be more than the kernels take.
+_data_ptr, _numel, _contiguous, _on = (getattr(Tensor, n) for n in ("data_ptr", "numel", "is_contiguous", "get_device"))
+_dtype_of, _grad_of = attrgetter("dtype"), attrgetter("grad")
+
+
 def _address(values: array) -> int:
     return values.buffer_info()[0]
 
@@ -49,20 +56,24 @@ def grad_norm(tensors: Iterable[Optional[Tensor]]) -> Tensor:
     ts = [t for t in tensors if t is not None]
     if not ts:
         raise ValueError("grad_norm needs one tensor at least")
-    dev = ts[0].device
-    kinds = array("i")
-    for i, t in enumerate(ts):
-        if t.device != dev or dev.type != "cuda":
-            kernels._same_device(*ts)
-        if t.layout is not torch.strided:
-            raise TypeError("grad_norm takes dense tensors")
-        kinds.append(kernels._dtype_code(t))
-        if not _dense(t):
-            ts[i] = t.contiguous()
+    dev, dt = ts[0].device, ts[0].dtype
+    if (dev.type == "cuda" and dt in kernels._DTYPES and set(map(_dtype_of, ts)) == {dt}
+            and set(map(_on, ts)) == {dev.index} and all(map(_contiguous, ts))):
+        kinds = array("i", [kernels._DTYPES[dt]]) * len(ts)
+    else:
+        kinds = array("i")
+        for i, t in enumerate(ts):
+            if t.device != dev or dev.type != "cuda":
+                kernels._same_device(*ts)
+            if t.layout is not torch.strided:
+                raise TypeError("grad_norm takes dense tensors")
+            kinds.append(kernels._dtype_code(t))
+            if not _dense(t):
+                ts[i] = t.contiguous()
     norm = torch.empty((), dtype=torch.float32, device=dev)
     size = kernels._workspace("dt_grad_norm_workspace", dev.index, len(ts))
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    at, n = array("q", [t.data_ptr() for t in ts]), array("q", [t.numel() for t in ts])
+    at, n = array("q", map(_data_ptr, ts)), array("q", map(_numel, ts))
     kernels._launch("dt_grad_norm", dev, len(ts), _address(at), _address(n), _address(kinds), norm.data_ptr(),
                     ws.data_ptr(), size)
     return norm
@@ -102,7 +113,7 @@ class AdamW(torch.optim.Optimizer):
         self.seed = int(seed) - 2 ** 64 if int(seed) >= 2 ** 63 else int(seed)
         self._order: List[Tensor] = []  # parameters as they were added: the order of the flat arrays
         self._buffers: Dict[str, Tensor] = {}
-        self._built = 0
+        self._built = 0  # parameters that the arrays are made for
         self.norm: Optional[Tensor] = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
@@ -191,6 +202,10 @@ class AdamW(torch.optim.Optimizer):
         self._strides = [None if p.is_contiguous() else p.stride() for p in ps]
         self._sizes = array("q", self._numels)
         self._kinds = array("i", [kernels._dtype_code(p) + 256 * group[id(p)] for p in ps])
+        self._plain = all(st is None for st in self._strides)
+        self._seen: Optional[array] = None
+        self._held: List[Tensor] = []
+        self._packed = [(None, b"")] * len(self.param_groups)
 
     def _ready(self) -> None:
         if not self._order:
@@ -225,31 +240,19 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         self._ready()
-        ps, keep = self._order, []
-        buf = self._buffers
+        ps, buf = self._order, self._buffers
         dev = buf["count"].device
-        index, at, to, some = dev.index, [], [], False
-        for i, (p, dt, n, st) in enumerate(zip(ps, self._dtypes, self._numels, self._strides)):
-            g = p.grad
-            if (g is not None and st is None and p.dtype is dt and g.dtype is dt and p.numel() == n == g.numel()
-                    and p.is_contiguous() and g.is_contiguous() and p.get_device() == index == g.get_device()):
-                at.append(p.data_ptr())
-                to.append(g.data_ptr())
-                some = True
-            else:
-                a, b = self._odd(i, keep)
-                at.append(a)
-                to.append(b)
-                some = some or b != 0
-        if not some:
+        at, to, keep = self._addresses(ps, dev.index)
+        if to is None:
             return loss
         size, ws, norm = 0, None, None
         if self.max_norm is not None:
             size = kernels._workspace("dt_grad_norm_workspace", dev.index, len(ps))
-            ws = torch.empty(size, dtype=torch.uint8, device=dev)
+            ws = buf.get("parts")
+            if ws is None or ws.numel() < size:
+                ws = buf["parts"] = torch.empty(size, dtype=torch.uint8, device=dev)
             norm = self.norm = torch.empty((), dtype=torch.float32, device=dev)
-        groups = b"".join([self._pack_group(g, dev) for g in self.param_groups])
-        at, to = array("q", at), array("q", to)
+        groups = b"".join([self._group_bytes(i, g, dev) for i, g in enumerate(self.param_groups)])
         kernels._launch("dt_adamw_step", dev, len(ps), _address(at), _address(to), _address(self._sizes),
                         _address(self._kinds), len(self.param_groups), groups, self.state_bits,
                         buf["exp_avg"].data_ptr(), buf["exp_avg_sq"].data_ptr(), kernels._ptr(buf.get("exp_avg_scale")),
@@ -257,6 +260,60 @@ class AdamW(torch.optim.Optimizer):
                         buf["count"].data_ptr(), buf["ticket"].data_ptr(), self.max_norm or 0.0, kernels._ptr(norm),
                         kernels._ptr(ws), size)
         return loss
+
+    def _addresses(self, ps: List[Tensor], index: int):
+        """(addresses of the parameters, of their gradients, tensors to be held until the launch); the second None
+        without any gradient.  Every parameter and gradient is looked at in every step."""
+        grads = list(map(_grad_of, ps))
+        live = [g for g in grads if g is not None]
+        if not live:
+            return None, None, live
+        at = array("q", map(_data_ptr, ps))
+        if (len(live) == len(ps) and self._plain and all(map(_contiguous, ps)) and all(map(_contiguous, grads))
+                and list(map(_dtype_of, grads)) == self._dtypes and list(map(_numel, grads)) == self._numels
+                and set(map(_on, grads)) == {index}):
+            # A parameter at its address of the last look is the same memory: that is held meanwhile.
+            if at != self._seen:
+                for i in range(len(ps)):
+                    self._same(i)
+                self._held, self._seen = [p.detach() for p in ps], at
+            return at, array("q", map(_data_ptr, grads)), grads
+        keep: List[Tensor] = []
+        to = array("q", [self._gradient(i, g, keep) for i, g in enumerate(grads)])
+        return at, to, keep
+
+    def _same(self, i: int) -> Tensor:
+        """Parameter i, whose type, size, order of memory and device have to be those of the flat arrays."""
+        p = self._order[i]
+        if (p.dtype != self._dtypes[i] or p.numel() != self._numels[i] or p.device != self._buffers["count"].device
+                or (None if p.is_contiguous() else p.stride()) != self._strides[i]):
+            raise ValueError(f"parameter {i} has changed its type, size, strides or device")
+        return p
+
+    def _gradient(self, i: int, g: Optional[Tensor], keep: List[Tensor]) -> int:
+        """The address of parameter i's gradient in the parameter's order of memory; 0 without one."""
+        p = self._same(i)
+        if g is None:
+            return 0
+        if g.layout is not torch.strided:
+            raise TypeError("AdamW takes dense gradients")
+        if g.dtype != p.dtype or g.shape != p.shape or g.device != p.device:
+            raise ValueError(f"the gradient of parameter {i} does not match it")
+        if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+            g = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
+            keep.append(g)
+        return g.data_ptr()
+
+    def _group_bytes(self, i: int, g: dict, dev: torch.device) -> bytes:
+        """_pack_group of group i, taken again when one of its numbers has changed."""
+        key = (g["lr"], g["betas"], g["eps"], g["weight_decay"])
+        if isinstance(key[0], Tensor):
+            return self._pack_group(g, dev)
+        was, packed = self._packed[i]
+        if was != key:
+            packed = self._pack_group(g, dev)
+            self._packed[i] = key, packed
+        return packed
 
     # -------------------------------------------------------------------------- state
     def steps(self) -> Tensor:
@@ -291,7 +348,7 @@ class AdamW(torch.optim.Optimizer):
         number = {id(p): i for i, p in enumerate(p for g in self.param_groups for p in g["params"])}
         groups = [{**{k: v for k, v in g.items() if k != "params"}, "params": [number[id(p)] for p in g["params"]]}
                   for g in self.param_groups]
-        state = {k: v for k, v in self._buffers.items() if k not in ("count", "ticket")}
+        state = {k: v for k, v in self._buffers.items() if k not in ("count", "ticket", "parts")}
         return {"state": {"seed": self.seed, "step": self._buffers["count"][1], **state}, "param_groups": groups}
 
     @torch.no_grad()
@@ -300,7 +357,7 @@ class AdamW(torch.optim.Optimizer):
         state, groups = state_dict["state"], state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the state has other groups of parameters")
-        mine = {k: v for k, v in self._buffers.items() if k not in ("count", "ticket")}
+        mine = {k: v for k, v in self._buffers.items() if k not in ("count", "ticket", "parts")}
         if set(mine) | {"seed", "step"} != set(state):
             raise ValueError(f"the state has {sorted(state)}, this optimizer {sorted(mine)}, seed and step")
         for k, t in mine.items():

@@ -52,8 +52,9 @@ def test_norm(sizes, types):
     want = math.sqrt(sum(t.double().pow(2).sum().item() for t in ts))
     got = optim.grad_norm([t.cuda() for t in ts])
     assert got.dtype == FP32 and got.dim() == 0
-    # Eight squares in fp32: 9 e on a sum of positive terms, halved by the root; one rounding.
-    assert abs(got.item() - want) <= want * 6 * E
+    # 32 squares in fp32: a product, three sums of a pair, two of four, one of two make 8 e on a sum of positive terms,
+    # halved by the root; one rounding.
+    assert abs(got.item() - want) <= want * 5 * E
 
 
 def test_norm_of_any_layout_and_size_of_number():
@@ -63,12 +64,12 @@ def test_norm_of_any_layout_and_size_of_number():
     views = [x, x.permute(2, 0, 1), x[:, ::2], x[3:, 5:, 7:], x[:1].expand(7, 30, 20), None,
              torch.randn(10001, device="cuda").bfloat16()[1:]]
     want = math.sqrt(sum(t.double().pow(2).sum().item() for t in views if t is not None))
-    assert abs(optim.grad_norm(views).item() - want) <= want * 6 * E
+    assert abs(optim.grad_norm(views).item() - want) <= want * 5 * E
     for size in (1e30, 1e18, 1e-19, 1e-25, 1e-38):
         y = torch.randn(5000, device="cuda").mul_(size)
         want = y.double().pow(2).sum().sqrt().item()
         got = optim.grad_norm([y, torch.zeros(3000, device="cuda")]).item()
-        assert abs(got - want) <= want * 6 * E + 2.0 ** -149, size
+        assert abs(got - want) <= want * 5 * E + 2.0 ** -149, size
     assert optim.grad_norm([torch.zeros(0, device="cuda")]).item() == 0
     assert math.isnan(optim.grad_norm([x, torch.tensor([math.nan], device="cuda")]).item())
     assert optim.grad_norm([x, torch.tensor([-math.inf], device="cuda").half()]).item() == math.inf
@@ -155,7 +156,7 @@ def test_steps(dtypes, bits, master, max_norm, lr, betas, eps, wd):
         clip = 1.0
         if max_norm is not None:
             norm = math.sqrt(sum(x.double().pow(2).sum().item() for x in grads if x is not None))
-            assert abs(opt.norm.item() - norm) <= norm * 6 * E
+            assert abs(opt.norm.item() - norm) <= norm * 5 * E
             clip = min(1.0, max_norm / (norm + 1e-6))
             clip32 = np.minimum(np.float32(1), np.float32(max_norm) / (np.float32(opt.norm.item()) + np.float32(1e-6)))
         if bits == 8:
@@ -252,7 +253,7 @@ def test_many_tensors_and_layouts():
     opt = adamw(ps, lr=0.01, weight_decay=0.5, max_norm=3.0)
     opt.step()
     norm = math.sqrt(sum(x.double().pow(2).sum().item() for x in gs))
-    assert abs(opt.norm.item() - norm) <= norm * 6 * E
+    assert abs(opt.norm.item() - norm) <= norm * 5 * E
     new = pool.cpu()
     touched = torch.zeros(60000, dtype=torch.bool)
     for p, x in zip(ps, gs):
