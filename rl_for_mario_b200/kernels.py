@@ -838,10 +838,11 @@ def _check_head_norm(q, k, q_weight, k_weight, eps, cos, sin, start_pos):
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("head_norm_rope takes q [B, S, Hq, D] and k [B, S, Hkv, D]")
     B, S, Hq, D = q.shape
-    Hkv = k.shape[2]
-    dt = q.dtype
-    if k.shape != (B, S, Hkv, D):
-        raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    kshape = k.shape
+    Hkv = kshape[2]
+    dt, wt = q.dtype, q_weight.dtype
+    if kshape != (B, S, Hkv, D):
+        raise ValueError(f"k {tuple(kshape)} does not match q {tuple(q.shape)}")
     if dt not in _DTYPES or k.dtype != dt:
         raise TypeError(f"q and k must share a dtype, bf16, fp16 or fp32 (got {dt} and {k.dtype})")
     if D < 2 or D > 256 or D % 2:
@@ -850,21 +851,19 @@ def _check_head_norm(q, k, q_weight, k_weight, eps, cos, sin, start_pos):
         raise ValueError("q and k need one head at least")
     if B * S * max(Hq, Hkv) >= 2 ** 31:
         raise ValueError(f"too many heads: {B} x {S} x {max(Hq, Hkv)} must stay below 2^31")
-    wt = q_weight.dtype
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.shape != (D,) or not w.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous [{D}] tensor")
-        if w.dtype != wt or wt not in (dt, torch.float32):
-            raise TypeError(f"q_weight and k_weight must have the dtype of q, or fp32 both (got {w.dtype})")
-    if not 0.0 <= ctypes.c_float(eps).value < math.inf:
+    if q_weight.shape != (D,) or k_weight.shape != (D,) or not (q_weight.is_contiguous() and k_weight.is_contiguous()):
+        raise ValueError(f"q_weight and k_weight must be contiguous [{D}] tensors")
+    if k_weight.dtype != wt or (wt != dt and wt != torch.float32):
+        raise TypeError(f"q_weight and k_weight must have the dtype of q, or fp32 both (got {wt} and {k_weight.dtype})")
+    if not 0.0 <= eps <= _MOST_FP32:
         raise ValueError(f"eps must be finite and not negative (got {eps})")
-    cos, sin = _prep_tables(cos, sin)
-    rows = cos.shape[0]
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D or rows < (S if start_pos is None else 1):
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D or cos.shape[0] < (S if start_pos is None else 1):
         raise ValueError(f"cos and sin must be [{'rows' if start_pos is not None else f'>= {S}'}, {D}] tables "
                          f"(got {tuple(cos.shape)}, {tuple(sin.shape)})")
-    if rows == 1 or cos.stride(0) < D:  # a stride that says nothing, or rows on top of each other
-        cos, sin = cos.contiguous(), sin.contiguous()
+    if not (cos.is_contiguous() and sin.is_contiguous() and cos.dtype == sin.dtype == torch.float32):
+        cos, sin = _prep_tables(cos, sin)
+        if cos.shape[0] == 1 or cos.stride(0) < D:  # a stride that says nothing, or rows on top of each other
+            cos, sin = cos.contiguous(), sin.contiguous()
     if start_pos is not None:
         if start_pos.shape != (B,):
             raise ValueError(f"start_pos must be [{B}] (got {tuple(start_pos.shape)})")
@@ -873,6 +872,7 @@ def _check_head_norm(q, k, q_weight, k_weight, eps, cos, sin, start_pos):
     return cos, sin, start_pos, B, S, Hq, Hkv, D
 
 
+_MOST_FP32 = torch.finfo(torch.float32).max
 _PACK12, _PACK18 = struct.Struct("12q"), struct.Struct("18q")
 
 
@@ -895,7 +895,7 @@ def head_norm_rope_forward(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Ten
     qo, ko = _empty_as(q), _empty_as(k)
     if B * S:
         _launch("dt_head_norm_rope_forward", dev, q.data_ptr(), k.data_ptr(), q_weight.data_ptr(),
-                k_weight.data_ptr(), qo.data_ptr(), ko.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0),
+                k_weight.data_ptr(), qo.data_ptr(), ko.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0) if cos.shape[0] > 1 else D,
                 cos.shape[0], _ptr(start_pos), B, S, Hq, Hkv, D,
                 _PACK12.pack(*q.stride()[:3], *k.stride()[:3], S * Hq * D, Hq * D, D, S * Hkv * D, Hkv * D, D),
                 int(q_weight.dtype == torch.float32), eps, _dtype_code(q))
@@ -930,7 +930,7 @@ def head_norm_rope_backward(dq_out: Tensor, dk_out: Tensor, q: Tensor, k: Tensor
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     _launch("dt_head_norm_rope_backward", dev, dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
             q_weight.data_ptr(), k_weight.data_ptr(), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(),
-            cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], _ptr(start_pos), ws.data_ptr(), size, B, S,
+            cos.data_ptr(), sin.data_ptr(), cos.stride(0) if cos.shape[0] > 1 else D, cos.shape[0], _ptr(start_pos), ws.data_ptr(), size, B, S,
             Hq, Hkv, D, _PACK18.pack(*q.stride()[:3], *k.stride()[:3], *dq.stride()[:3], *dk.stride()[:3],
                                      *dq_out.stride()[:3], *dk_out.stride()[:3]),
             int(q_weight.dtype == torch.float32), eps, _dtype_code(q))

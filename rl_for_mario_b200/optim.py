@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+import sys
 from array import array
 from operator import attrgetter
 from typing import Dict, Iterable, List, Optional, Tuple, Union
@@ -203,7 +204,7 @@ class AdamW(torch.optim.Optimizer):
         self._sizes = array("q", self._numels)
         self._kinds = array("i", [kernels._dtype_code(p) + 256 * group[id(p)] for p in ps])
         self._plain = all(st is None for st in self._strides)
-        self._seen: Optional[array] = None
+        self._seen: Optional[List[int]] = None
         self._held: List[Tensor] = []
         self._packed = [(None, b"")] * len(self.param_groups)
 
@@ -233,8 +234,18 @@ class AdamW(torch.optim.Optimizer):
             keep.append(own)
         return p.data_ptr(), g.data_ptr()
 
-    @torch.no_grad()
     def step(self, closure=None):
+        # torch wraps an optimizer's step to run its hooks and mark it for the profiler, which takes 15 us; that
+        # wrapper is used where there is a hook or a profiler to serve.
+        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or any(map(len, _GLOBAL_HOOKS))
+                or _profiling()):
+            return _hooked_step(self, closure)
+        return self._step(closure)
+
+    step.hooked = True  # (tells torch not to wrap it again)
+
+    @torch.no_grad()
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -268,7 +279,7 @@ class AdamW(torch.optim.Optimizer):
         live = [g for g in grads if g is not None]
         if not live:
             return None, None, live
-        at = array("q", map(_data_ptr, ps))
+        at = list(map(_data_ptr, ps))
         if (len(live) == len(ps) and self._plain and all(map(_contiguous, ps)) and all(map(_contiguous, grads))
                 and list(map(_dtype_of, grads)) == self._dtypes and list(map(_numel, grads)) == self._numels
                 and set(map(_on, grads)) == {index}):
@@ -276,11 +287,11 @@ class AdamW(torch.optim.Optimizer):
             if at != self._seen:
                 for i in range(len(ps)):
                     self._same(i)
-                self._held, self._seen = [p.detach() for p in ps], at
-            return at, array("q", map(_data_ptr, grads)), grads
+                self._held, self._seen, self._at = [p.detach() for p in ps], at, array("q", at)
+            return self._at, array("q", map(_data_ptr, grads)), grads
         keep: List[Tensor] = []
         to = array("q", [self._gradient(i, g, keep) for i, g in enumerate(grads)])
-        return at, to, keep
+        return array("q", at), to, keep
 
     def _same(self, i: int) -> Tensor:
         """Parameter i, whose type, size, order of memory and device have to be those of the flat arrays."""
@@ -379,3 +390,10 @@ class AdamW(torch.optim.Optimizer):
 
     def __getstate__(self) -> dict:
         return self.__dict__.copy()
+
+
+_hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)
+# Where this torch does not have them under these names, every step goes through torch's wrapper.
+_GLOBAL_HOOKS = tuple(getattr(sys.modules[torch.optim.Optimizer.__module__], "_global_optimizer_" + n, (None,))
+                      for n in ("pre_hooks", "post_hooks"))
+_profiling = getattr(torch.autograd, "_profiler_enabled", lambda: True)

@@ -334,6 +334,39 @@ def test_captured_step_reads_rate_number_and_gradient_anew():
             assert all(torch.equal(x, y) for x, y in zip(a.moments(), b.moments()))
 
 
+def test_hooks_closure_and_scheduler():
+    ps, qs = make_params([FP32]), make_params([FP32])
+    a, b = adamw(ps, lr=0.1), adamw(qs, lr=0.1)
+    seen = []
+    handles = [a.register_step_pre_hook(lambda *x: seen.append("pre")), a.register_step_post_hook(lambda *x: seen.append("post"))]
+    half = torch.optim.lr_scheduler.LambdaLR(a, lambda t: 0.5 ** t)
+
+    def closure():
+        seen.append(torch.is_grad_enabled())
+        set_grads(ps, 1)
+        return 7.0
+
+    assert a.step(closure) == 7.0 and seen == ["pre", True, "post"]
+    half.step()
+    assert a.param_groups[0]["lr"] == 0.05
+    for h in handles:
+        h.remove()
+    set_grads(ps, 2)
+    assert a.step() is None and len(seen) == 3
+    set_grads(qs, 1)
+    b.step()
+    b.param_groups[0]["lr"] = 0.05
+    set_grads(qs, 2)
+    b.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q)
+    c = copy.deepcopy(a)
+    assert c.param_groups[0]["params"][0] is not ps[0] and int(c.steps()) == 2
+    with torch.no_grad():
+        ps[0].add_(1.0)
+    assert not torch.equal(c.param_groups[0]["params"][0], ps[0])
+
+
 def test_another_stream():
     ps, qs = make_params([FP32]), make_params([FP32])
     a, b = adamw(ps, max_norm=1.0), adamw(qs, max_norm=1.0)
