@@ -23,6 +23,10 @@ throughout) unless ``compute_dtype`` selects bf16/fp16 tensor-core compute, in
 which case Q/K/V are cast for the kernels and the result is cast back.  There
 is no CPU path: CPU inputs raise.
 
+``config.qk_norm`` puts an RMSNorm on every query and key head before the rotation (weights q_norm.weight
+and k_norm.weight [head_dim]; the reference has none), which bounds the attention's scores in 16-bit training:
+one kernel for both norms and the RoPE, in prefill, cached decode and training.
+
 The kernels above have no gradient.  ``fuse_training()`` switches forward() to
 the training operators (training.py) whenever autograd is on and no cache takes
 part: same projections and RoPE, attention with its gradient, and dropout on
@@ -51,6 +55,15 @@ def left_padding(mask: Tensor, length: int, check: bool) -> Tensor:
     return pad
 
 
+class HeadNorm(nn.Module):
+    """The weight of the norm of every query (or key) head, run by kernels.head_norm_rope_forward."""
+
+    def __init__(self, dim: int, eps: float):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim))
+
+
 class FastDTAttention(nn.Module):
     # Training form (fuse_training): off, the module's own generator, and the number that
     # tells this module's dropout from other modules'.  Of the class, so that a module that
@@ -76,6 +89,9 @@ class FastDTAttention(nn.Module):
         self.k_proj = nn.Linear(config.hidden_size, self.n_local_kv_heads * self.head_dim, bias=False)
         self.v_proj = nn.Linear(config.hidden_size, self.n_local_kv_heads * self.head_dim, bias=False)
         self.o_proj = nn.Linear(self.n_local_heads * self.head_dim, config.hidden_size, bias=False)
+        if getattr(config, "qk_norm", False):  # (read by _head_norms: modules pickled without them have none)
+            eps = getattr(config, "rms_norm_eps", 1e-5)
+            self.q_norm, self.k_norm = HeadNorm(self.head_dim, eps), HeadNorm(self.head_dim, eps)
         self.attn_dropout = nn.Dropout(self.dropout)
         self.resid_dropout = nn.Dropout(self.dropout)
         self.compute_dtype = compute_dtype
@@ -104,6 +120,18 @@ class FastDTAttention(nn.Module):
         if kd not in (torch.bfloat16, torch.float16, torch.float32):
             raise TypeError(f"unsupported compute dtype {kd}")
         return kd
+
+    def _head_norms(self, kd: torch.dtype) -> Optional[Tuple[Tensor, Tensor, float]]:
+        """(q weight, k weight, eps) of the norms of query and key heads as the kernel takes them for kd, or None."""
+        q_norm = getattr(self, "q_norm", None)
+        if q_norm is None:
+            return None
+        if self.rope_rounding != "fp32":
+            raise ValueError("norms of query and key heads rotate in fp32: rope_rounding must be 'fp32'")
+        ws = [m.weight if m.weight.dtype in (kd, torch.float32) else m.weight.float() for m in (q_norm, self.k_norm)]
+        if ws[0].dtype != ws[1].dtype:
+            ws = [w.float() for w in ws]
+        return ws[0], ws[1], q_norm.eps
 
     def _pad_len(self, mask: Optional[Tensor], length: int) -> Optional[Tensor]:
         if mask is None:
@@ -151,6 +179,9 @@ class FastDTAttention(nn.Module):
         projections and the RoPE of q / k (rows s of the position tables)."""
         bsz, seq_len, _ = x.shape
         Hq, Hkv, D = self.n_local_heads, self.n_local_kv_heads, self.head_dim
+        norms = self._head_norms(kd)
+        if norms is not None:
+            return self._project_normed(x, kd, raw_input, pe, norms)
         if raw_input:
             if self._fused_norm is None:
                 raise ValueError("raw_input=True needs set_fused_norm()")
@@ -172,6 +203,33 @@ class FastDTAttention(nn.Module):
         xk = self.k_proj(x).view(bsz, seq_len, Hkv, D).to(kd)
         xv = self.v_proj(x).view(bsz, seq_len, Hkv, D).to(kd)
         return xq, xk, xv, False
+
+    def _project_normed(self, x: Tensor, kd: torch.dtype, raw_input: bool, pe: Tuple[Tensor, Tensor], norms):
+        """_project with the norms of query and key heads: the projections, then norm and RoPE of q and k in one
+        kernel."""
+        bsz, seq_len, _ = x.shape
+        Hq, Hkv, D = self.n_local_heads, self.n_local_kv_heads, self.head_dim
+        half = x.dtype in (torch.bfloat16, torch.float16) and kd == x.dtype
+        if raw_input:
+            if self._fused_norm is None:
+                raise ValueError("raw_input=True needs set_fused_norm()")
+            if not half:
+                x = self._fused_norm(x)
+        if half and raw_input:
+            qkv = kernels.rmsnorm_qkv(x, self._fused_weight(x.dtype), self._fused_norm.eps)
+        elif half and self._qkv_rope_ok(x):
+            qkv = nn.functional.linear(x, self._cat_weight(x.dtype))
+        else:
+            qkv = None
+        if qkv is not None:
+            xq, xk, xv = qkv.view(bsz, seq_len, Hq + 2 * Hkv, D).split([Hq, Hkv, Hkv], 2)
+        else:
+            xq = self.q_proj(x).view(bsz, seq_len, Hq, D).to(kd)
+            xk = self.k_proj(x).view(bsz, seq_len, Hkv, D).to(kd)
+            xv = self.v_proj(x).view(bsz, seq_len, Hkv, D).to(kd)
+        with torch.no_grad():  # as the attention kernels behind it: no gradient in this form
+            xq, xk = kernels.head_norm_rope_forward(xq, xk, *norms, *pe)
+        return xq, xk, xv, True
 
     # ----------------------------------------------------------------- training
     def fuse_training(self, on: bool = True, seed: int = 0, site: int = 0) -> "FastDTAttention":
@@ -209,6 +267,7 @@ class FastDTAttention(nn.Module):
         Hq, Hkv, D = self.n_local_heads, self.n_local_kv_heads, self.head_dim
         cos, sin = position_embeddings
         p = self.dropout if self.training else 0.0
+        norms = self._head_norms(kd)
         ws = (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
         if ac == kd:
             xk, ws = x.to(ac), [w.to(ac) for w in ws]
@@ -217,17 +276,26 @@ class FastDTAttention(nn.Module):
         if (kd == xk.dtype == ws[0].dtype and ac in (None, kd) and D in (32, 64) and xk.shape[-1] % 8 == 0
                 and xk.data_ptr() % 16 == 0 and xk.stride(-1) == 1
                 and all(m.bias is None for m in (self.q_proj, self.k_proj, self.v_proj))):
-            qkv = training.qkv_rope(xk, torch.cat(tuple(ws)), cos, sin, (Hq + Hkv) * D, D)
-            out = training.attention_qkv(qkv.view(B, S, Hq + 2 * Hkv, D), Hq, Hkv, pad_len, p=p, rng=rng,
-                                         site=self.train_site)
+            if norms is not None:
+                qkv = nn.functional.linear(xk, torch.cat(tuple(ws))).view(B, S, Hq + 2 * Hkv, D)
+                out = training.attention_qk_norm(qkv, Hq, Hkv, *norms, cos, sin, pad_len, p=p, rng=rng,
+                                                 site=self.train_site)
+            else:
+                qkv = training.qkv_rope(xk, torch.cat(tuple(ws)), cos, sin, (Hq + Hkv) * D, D)
+                out = training.attention_qkv(qkv.view(B, S, Hq + 2 * Hkv, D), Hq, Hkv, pad_len, p=p, rng=rng,
+                                             site=self.train_site)
         else:
             def rotate(t):
                 t = t.float()
                 half = torch.cat((-t[..., D // 2:], t[..., :D // 2]), -1)
                 return (t * cos[:S, None].float() + half * sin[:S, None].float()).to(kd)
 
-            q = rotate(self.q_proj(x).view(B, S, Hq, D))
-            k = rotate(self.k_proj(x).view(B, S, Hkv, D))
+            if norms is not None:
+                q, k = training.head_norm_rope(self.q_proj(x).view(B, S, Hq, D).to(kd),
+                                               self.k_proj(x).view(B, S, Hkv, D).to(kd), *norms, cos, sin)
+            else:
+                q = rotate(self.q_proj(x).view(B, S, Hq, D))
+                k = rotate(self.k_proj(x).view(B, S, Hkv, D))
             v = self.v_proj(x).view(B, S, Hkv, D).to(kd)
             out = training.attention(q, k, v, pad_len, p=p, rng=rng, site=self.train_site)
         out = out.reshape(B, S, Hq * D)

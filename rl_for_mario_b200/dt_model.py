@@ -21,7 +21,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import kernels, training
+from . import kernels, optim, training
 from .attention import FastDTAttention, left_padding
 from .cache import LayerKV, PagedKVCache
 
@@ -47,6 +47,7 @@ class DTConfig:
     rope_theta: float = 10000.0
     flash_attn: bool = True
     label_smoothing: float = 0.1
+    qk_norm: bool = False  # norms of query and key heads (not in the reference)
     max_position_embeddings: int = field(init=False)
 
     def __post_init__(self):
@@ -56,7 +57,7 @@ class DTConfig:
     @classmethod
     def from_reference(cls, ref_cfg) -> "DTConfig":
         names = [f for f in cls.__dataclass_fields__ if f != "max_position_embeddings"]
-        return cls(**{n: getattr(ref_cfg, n) for n in names})
+        return cls(**{n: getattr(ref_cfg, n) for n in names if n != "qk_norm" or hasattr(ref_cfg, n)})
 
 
 class RMSNorm(nn.Module):
@@ -496,6 +497,13 @@ class MarioDT(nn.Module):
         for i, layer in enumerate(self.model.layers):
             layer.self_attn.fuse_training(on, seed, 1 + 3 * i)  # three sites a block; 0 is the embedding's
         return self
+
+    def adamw(self, lr: float = 1e-3, weight_decay: float = 1e-2, **kw) -> optim.AdamW:
+        """AdamW over the model's parameters that train (optim.AdamW: further arguments go there); weights of
+        products, convolutions and embeddings decay, norms' weights and biases do not."""
+        ps = [p for p in self.parameters() if p.requires_grad]
+        groups = [{"params": [p for p in ps if p.dim() > 1]}, {"params": [p for p in ps if p.dim() < 2], "weight_decay": 0.0}]
+        return optim.AdamW([g for g in groups if g["params"]], lr=lr, weight_decay=weight_decay, **kw)
 
     def reference_rounding(self, on: bool = True) -> "MarioDT":
         """Evaluates a 16-bit model at the reference's own rounding points, so its

@@ -3,8 +3,9 @@
 The reference trains this model with dropout (trainer/train_pretrain.py:121-129;
 model/model_decision_transformer.py:153-163, :256-271, :420): ``attention`` /
 ``attention_qkv`` are the causal GQA attention with its gradient, ``qkv_rope``
-the Q/K/V projection with RoPE and its gradient, ``residual_norm`` the residual
-add with the norms before and after it, its gate and dropout, ``dropout`` the
+the Q/K/V projection with RoPE and its gradient, ``head_norm_rope`` the norm of every
+query and key head with the RoPE behind it (``attention_qk_norm``: with the attention
+behind that), ``residual_norm`` the residual add with the norms before and after it, its gate and dropout, ``dropout`` the
 plain one.  ``MarioDT.fuse_training()`` and ``FastDTAttention.fuse_training()``
 run a model on them.
 
@@ -135,6 +136,64 @@ class _QKVRope(torch.autograd.Function):
 def qkv_rope(x: Tensor, w: Tensor, cos: Tensor, sin: Tensor, rope_cols: int, head_dim: int) -> Tensor:
     """Differentiable kernels.qkv_rope: x [B, S, K] @ w^T with the RoPE of its first rope_cols columns."""
     return _QKVRope.apply(x, w, cos, sin, rope_cols, head_dim)
+
+
+class _HeadNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, eps, cos, sin, start_pos):
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, start_pos)
+        ctx.eps = eps
+        return kernels.head_norm_rope_forward(q, k, q_weight, k_weight, eps, cos, sin, start_pos)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, cos, sin, start_pos = ctx.saved_tensors
+        dq, dk, dwq, dwk = kernels.head_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, ctx.eps, cos, sin,
+                                                           start_pos)
+        return dq, dk, dwq, dwk, None, None, None, None
+
+
+def head_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, eps: float, cos: Tensor, sin: Tensor,
+                   start_pos: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """Differentiable kernels.head_norm_rope_forward: q [B,S,Hq,D] and k [B,S,Hkv,D] with every head normalised and
+    rotated."""
+    return _HeadNormRope.apply(q, k, q_weight, k_weight, eps, cos, sin, start_pos)
+
+
+class _AttentionQKNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, q_weight, k_weight, heads, kv_heads, eps, cos, sin, pad_len, scale, p, rng, site):
+        q, k, v = qkv.split([heads, kv_heads, kv_heads], 2)
+        q, k = kernels.head_norm_rope_forward(q, k, q_weight, k_weight, eps, cos, sin)
+        out, lse = kernels.attn_train_forward(q, k, v, pad_len, scale, p, rng, site)
+        ctx.save_for_backward(qkv, q, k, q_weight, k_weight, cos, sin, out, lse, pad_len, rng)
+        ctx.how = (heads, kv_heads, eps, scale, p, site)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        qkv, q, k, q_weight, k_weight, cos, sin, out, lse, pad_len, rng = ctx.saved_tensors
+        heads, kv_heads, eps, scale, p, site = ctx.how
+        parts = [heads, kv_heads, kv_heads]
+        xq, xk, v = qkv.split(parts, 2)
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        dq, dk, dv = dqkv.split(parts, 2)
+        kernels.attn_train_backward(dout, q, k, v, out, lse, pad_len, scale, p, rng, site, grads=(dq, dk, dv))
+        _, _, dwq, dwk = kernels.head_norm_rope_backward(dq, dk, xq, xk, q_weight, k_weight, eps, cos, sin,
+                                                         grads=(dq, dk))
+        return dqkv, dwq, dwk, None, None, None, None, None, None, None, None, None, None
+
+
+def attention_qk_norm(qkv: Tensor, heads: int, kv_heads: int, q_weight: Tensor, k_weight: Tensor, eps: float,
+                      cos: Tensor, sin: Tensor, pad_len: Optional[Tensor] = None, scale: Optional[float] = None,
+                      p: float = 0.0, rng: Optional[Tensor] = None, site: int = 0) -> Tensor:
+    """attention_qkv() on a projection output whose query and key heads are normalised and rotated first (rows 0 .. S - 1
+    of the tables); the gradient of the projection is written as one tensor, the heads' in place."""
+    if qkv.dim() != 4 or qkv.shape[2] != heads + 2 * kv_heads:
+        raise ValueError(f"qkv must be [B, S, {heads + 2 * kv_heads}, D] (got {tuple(qkv.shape)})")
+    return _AttentionQKNorm.apply(qkv, q_weight, k_weight, heads, kv_heads, eps, cos, sin, pad_len, scale, p, rng, site)
 
 
 class _ResidualNorm(torch.autograd.Function):

@@ -33,6 +33,32 @@ def test_head_norm_entry_points_refuse_bad_arguments():
     assert lib.dt_head_norm_rope_workspace(1, 8, 4, 2, 31) < 0 and lib.dt_head_norm_rope_workspace(0, 8, 4, 2, 32) < 0
 
 
+@pytest.mark.parametrize("D", [2, 6, 32])
+def test_head_norm_gradient_against_differences(D):
+    """The oracle's gradient against central differences of its forward pass: with h = 2^-17 they are off by h^2 times
+    a third derivative (sizes here: some tens) and by 2^-52 / h of the sum."""
+    from oracle import step_ref as ref
+
+    g = torch.Generator().manual_seed(D)
+    x, w = torch.randn(2, 3, 2, D, generator=g, dtype=torch.float64), 1 + 0.3 * torch.randn(D, generator=g, dtype=torch.float64)
+    cos, sin, d = (torch.randn(*s, generator=g, dtype=torch.float64) for s in ((5, D), (5, D), x.shape))
+    pos = torch.tensor([[0, 3, 4], [1, 2, 2]])
+    r = ref.head_norm_rope(x, w, cos, sin, 1e-2, pos, d)
+    h = 2.0 ** -17
+
+    def value(x, w):
+        return (ref.head_norm_rope(x, w, cos, sin, 1e-2, pos)["out"][0] * d).sum().item()
+
+    for n, t in (("dx", x), ("dw", w)):
+        for i in range(0, t.numel(), max(1, t.numel() // 40)):
+            e = torch.zeros_like(t).view(-1)
+            e[i] = h
+            e = e.view_as(t)
+            args = [(x + e, w), (x - e, w)] if n == "dx" else [(x, w + e), (x, w - e)]
+            diff = (value(*args[0]) - value(*args[1])) / (2 * h)
+            assert abs(diff - r[n][0].view(-1)[i].item()) < 1e-6 * (1 + abs(diff)), (n, i)
+
+
 def test_head_norm_wrapper_checks():
     from rl_for_mario_b200 import kernels as K
 
