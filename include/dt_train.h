@@ -181,8 +181,9 @@ int dt_grad_norm(int count, const int64_t* tensors, const int64_t* sizes, const 
  * tensors on the current device; negative on an error. */
 int64_t dt_grad_norm_workspace(int count);
 
-/* Hyperparameters of a group of tensors.  lr_tensor: the rate as an fp32 number on the
- * device, read by the kernel, or null: lr. */
+/* Hyperparameters of a group of tensors: betas in [0, 1), eps a normal fp32 number, the
+ * others not negative.  lr_tensor: the rate as an fp32 number on the device, read by the
+ * kernel, or null: lr. */
 typedef struct {
   double lr, beta1, beta2, eps, weight_decay;
   const float* lr_tensor;

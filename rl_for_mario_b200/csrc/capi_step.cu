@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <nvtx3/nvToolsExt.h>
 
+#include <cfloat>
 #include <cmath>
 
 #include "../../include/dt_attn.h"
@@ -82,12 +83,12 @@ int launch_norm(const char* fn, int count, const int64_t* grads, const int64_t* 
                 double* parts, int64_t room, float* norm, int num_sms, cudaStream_t st, int* total) {
   *total = 0;
   return in_launches(count, nullptr, grads, sizes, kinds, dtk::grad_norm_unit(),
-                     [&](const TensorSlot* slots, int n, uint32_t units, int64_t first, bool last) {
+                     [&](const TensorSlot* slots, int n, uint32_t units, int64_t, bool) {
                        const int grid = dtk::grad_norm_grid(units, num_sms);
                        if (*total + grid > room) return api_fail(DT_ERR_INVALID, "%s: the workspace is too small", fn);
                        dtk::GradNormParams p{};
                        p.count = n, p.units = units, p.parts = parts + *total;
-                       p.norm = first == 0 && last && grid == 1 ? norm : nullptr;
+                       p.norm = n == count && grid == 1 ? norm : nullptr;
                        *total += grid;
                        return cuda_status(dtk::launch_grad_norm_sm100(slots, p, num_sms, st), fn);
                      });
@@ -154,7 +155,7 @@ int dt_adamw_step(int count, const int64_t* params, const int64_t* grads, const 
   for (int i = 0; i < ngroups; ++i) {
     const DtAdamWGroup& g = groups[i];
     if (!(g.beta1 >= 0 && g.beta1 < 1 && g.beta2 >= 0 && g.beta2 < 1 && g.lr >= 0 && g.lr < INFINITY &&
-          g.weight_decay >= 0 && g.weight_decay < INFINITY && (float)g.eps > 0.f && (float)g.eps < INFINITY) ||
+          g.weight_decay >= 0 && g.weight_decay < INFINITY && (float)g.eps >= FLT_MIN && (float)g.eps < INFINITY) ||
         !aligned(g.lr_tensor, 4))
       return api_fail(DT_ERR_INVALID, "%s: group %d: lr %g, betas %g %g, eps %g, weight_decay %g", fn, i, g.lr, g.beta1,
                       g.beta2, g.eps, g.weight_decay);

@@ -27,6 +27,7 @@ Tensor = torch.Tensor
 BLOCK = 256  # elements of a parameter that share a scale; each parameter starts a new block
 _MOST_GROUPS = 16
 _GROUP = struct.Struct("5dQ")
+_LEAST_FP32, _MOST_FP32 = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 def _dense(t: Tensor) -> bool:
@@ -90,7 +91,8 @@ class AdamW(torch.optim.Optimizer):
     rounded up or down at random (by ``seed``, the step and the element), so that they follow the gradients
     as those in 32 bits do: v to about 10 % of its root, m to about 8 %.
     ``master``: fp32 weights are kept beside 16-bit parameters; without them a step smaller than half a unit
-    in the last place of a 16-bit weight is lost.
+    in the last place of a 16-bit weight is lost.  They are what a step starts from: reset_master() after the
+    parameters were changed from outside.
     ``max_norm``: the gradient is scaled so that its norm over all parameters is at most this; the norm of
     each step is in ``norm``.  A step whose norm is not finite changes nothing and is not counted.
 
@@ -156,8 +158,8 @@ class AdamW(torch.optim.Optimizer):
         if not (0.0 <= lr < math.inf and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and 0.0 <= wd < math.inf):
             raise ValueError(f"lr and weight_decay must not be negative, betas lie in [0, 1) (got lr {lr}, betas "
                              f"{(b1, b2)}, weight_decay {wd})")
-        if not 0.0 < ctypes.c_float(eps).value < math.inf:
-            raise ValueError(f"eps must be positive and finite in fp32 (got {eps})")
+        if not _LEAST_FP32 <= eps <= _MOST_FP32:
+            raise ValueError(f"eps must be a normal number in fp32 (got {eps})")
         return _GROUP.pack(lr, b1, b2, eps, wd, at)
 
     def _overlap(self) -> None:
@@ -181,12 +183,7 @@ class AdamW(torch.optim.Optimizer):
                 new[k + "_scale"] = torch.full((total,), 32, dtype=torch.uint8, device=dev)
         if self.keeps_master:
             new["master"] = torch.zeros(total * BLOCK, dtype=torch.float32, device=dev)
-            at = 0
-            for i, (p, n) in enumerate(zip(ps, blocks)):
-                if i >= self._built:
-                    flat = new["master"][at * BLOCK:at * BLOCK + p.numel()]
-                    flat.copy_(torch.as_strided(p.detach(), (p.numel(),), (1,)))
-                at += n
+            self._fill_master(new["master"], self._built)
         for k, t in old.items():
             if k in new:
                 new[k][:t.numel()].copy_(t)
@@ -207,6 +204,21 @@ class AdamW(torch.optim.Optimizer):
         self._seen: Optional[List[int]] = None
         self._held: List[Tensor] = []
         self._packed = [(None, b"")] * len(self.param_groups)
+
+    def _fill_master(self, master: Tensor, first: int) -> None:
+        at = 0
+        for i, p in enumerate(self._order):
+            if i >= first and p.dtype != torch.float32:
+                master[at:at + p.numel()].copy_(torch.as_strided(p.detach(), (p.numel(),), (1,)))
+            at += (p.numel() + BLOCK - 1) // BLOCK * BLOCK
+
+    @torch.no_grad()
+    def reset_master(self) -> None:
+        """Takes the fp32 weights from the 16-bit parameters anew: after these were changed from outside (weights loaded
+        into the model, say), which the next step would otherwise undo."""
+        self._ready()
+        if self.keeps_master:
+            self._fill_master(self._buffers["master"], 0)
 
     def _ready(self) -> None:
         if not self._order:
@@ -255,6 +267,7 @@ class AdamW(torch.optim.Optimizer):
         dev = buf["count"].device
         at, to, keep = self._addresses(ps, dev.index)
         if to is None:
+            self.norm = None
             return loss
         size, ws, norm = 0, None, None
         if self.max_norm is not None:
@@ -287,6 +300,7 @@ class AdamW(torch.optim.Optimizer):
             if at != self._seen:
                 for i in range(len(ps)):
                     self._same(i)
+                self._overlap()
                 self._held, self._seen, self._at = [p.detach() for p in ps], at, array("q", at)
             return self._at, array("q", map(_data_ptr, grads)), grads
         keep: List[Tensor] = []

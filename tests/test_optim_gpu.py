@@ -40,7 +40,8 @@ def near(name, got, want, tol):
 
 # ------------------------------------------------------------------------------------------- norm
 NORMS = [([1], [FP32]), ([0, 3, 0], [BF16]), ([255, 256, 257, 1023, 1024, 1025], [BF16, FP32, FP16]),
-         ([1 << 20, 7, 300001], [FP32, BF16]), ([5] * 959 + [4097] * 3, [FP16, FP32]), ([3] * 2000, [BF16])]
+         ([1 << 20, 7, 300001], [FP32, BF16]), ([5] * 959 + [4097] * 3, [FP16, FP32]), ([3] * 2000, [BF16]),
+         ([0] * 800 + [5], [FP32]), ([7] + [0] * 1600, [BF16])]
 
 
 @pytest.mark.parametrize("sizes,types", NORMS)
@@ -299,6 +300,30 @@ def test_group_added_later_and_state_across_optimizers():
             adamw(qs, [dict(params=qs[:4]), dict(params=qs[4:])], state_bits=40 - bits).load_state_dict(one.state_dict())
 
 
+def test_fp32_weights_taken_anew():
+    ps = make_params([BF16, FP32])
+    opt = adamw(ps, master=True, lr=0.0, weight_decay=0.0)
+    set_grads(ps, 1)
+    opt.step()
+    with torch.no_grad():
+        for p in ps:
+            p.mul_(3.0)
+    now = [p.detach().clone() for p in ps]
+    opt.reset_master()
+    set_grads(ps, 2)
+    opt.step()  # a rate of zero: the weights are what they were set to
+    for p, q in zip(ps, now):
+        assert torch.equal(p, q)
+    at = blocks_of(ps)
+    for i, p in enumerate(ps):
+        want = torch.zeros(p.numel(), device="cuda") if p.dtype == FP32 else memory(p).float()
+        assert torch.equal(part(opt.master, at[i], p), want)
+    for p in ps:
+        p.grad = None
+    opt.step()
+    assert int(opt.steps()) == 2
+
+
 def test_captured_step_reads_rate_number_and_gradient_anew():
     for bits in (32, 8):
         lr = torch.full((), 0.01, device="cuda")
@@ -413,7 +438,7 @@ def test_refusals():
     ok = dict(params=[p])
     for kw, match in ((dict(state_bits=16), "state_bits"), (dict(max_norm=0.0), "max_norm"), (dict(max_norm=math.nan), "max_norm"),
                       (dict(seed=2 ** 64), "seed"), (dict(lr=-1.0), "lr"), (dict(lr=math.nan), "lr"), (dict(betas=(1.0, 0.9)), "betas"),
-                      (dict(betas=(0.9, -0.1)), "betas"), (dict(eps=0.0), "eps"), (dict(eps=1e-60), "eps"),
+                      (dict(betas=(0.9, -0.1)), "betas"), (dict(eps=0.0), "eps"), (dict(eps=1e-60), "eps"), (dict(eps=1e-40), "eps"),
                       (dict(weight_decay=-0.1), "weight_decay"), (dict(lr=torch.zeros(2, device="cuda")), "lr tensor"),
                       (dict(lr=torch.zeros(())), "lr tensor")):
         with pytest.raises(ValueError, match=match):

@@ -139,6 +139,7 @@ def test_step_entry_points_refuse_bad_arguments():
         for w in (wrong, math.nan, math.inf):
             group[i] = w
             bad.append(dict(group=tuple(group)))
+    bad += [dict(group=(1e-3, 0.9, 0.999, eps, 0.0, 0)) for eps in (1e-40, 1e39, -1e-8)]
     bad.append(dict(group=(1e-3, 0.9, 0.999, 1e-8, 0.0, a + 1)))
     for kw in bad:
         assert step(**kw) == INV, kw
