@@ -36,12 +36,12 @@ namespace dtk {
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kNormResident = 4;  // blocks on an SM
-template <bool BITS8>
-constexpr int kStepResident = BITS8 ? 3 : 2;
+constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kNormResident = 8;  // blocks on an SM
+template <bool BITS8, bool MASTER = false>
+constexpr int kStepResident = BITS8 && !MASTER ? 5 : 4;
 constexpr int kNormUnit = 1024;      // elements of a warp's turn in the norm
-constexpr int kStepUnit = 512;       // and in the step
+constexpr int kPair = 512;           // of two blocks, whose loads are in flight together in the step
 constexpr uint32_t kSite = 0xffffffffu;  // the generator's site of the averages' rounding
 constexpr int kMinScale = 32;        // exponents of scales (biased): their products with any code are normal numbers
 
@@ -272,10 +272,10 @@ __device__ __forceinline__ uint32_t encode(float y, uint32_t word, uint32_t sele
   return __float_as_uint(z) * 16u + (__float_as_uint(small) * eight + __byte_perm(word, back, select));
 }
 
-// Stores a lane's eight values of a block, the block's scale by lane 0.  Random words: the two halves of each word,
+// Stores a lane's eight values of a block; returns the block's scale.  Random words: the two halves of each word,
 // the bytes of a half turned over for the signed average.
 template <int BIAS, int TOP, bool SIGNED>
-__device__ __forceinline__ void put_codes(uint8_t* codes, uint8_t* scale, const F8& x, const uint4& words, int lane) {
+__device__ __forceinline__ int put_codes(uint8_t* codes, const F8& x, const uint4& words) {
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) most = max_nan(most, fabsf(x.p[i].x), fabsf(x.p[i].y));
@@ -307,7 +307,7 @@ __device__ __forceinline__ void put_codes(uint8_t* codes, uint8_t* scale, const 
         }
   }
   *reinterpret_cast<uint2*>(codes) = make_uint2(four[0], four[1]);
-  if (lane == 0) *scale = (uint8_t)e;
+  return e;
 }
 
 // ---------------------------------------------------------------- step
@@ -336,7 +336,14 @@ __device__ __forceinline__ float fast_inverse(float x) {  // of normal numbers (
 template <bool BITS8>
 struct BlockLoad {
   Raw8Any g, w;
-  uint4 m[BITS8 ? 1 : 2], v[BITS8 ? 1 : 2];  // 8 bits: codes in x, y, the scale in z
+  uint4 m[BITS8 ? 1 : 2], v[BITS8 ? 1 : 2];  // 8 bits: codes in x, y
+};
+
+// The scales of a unit's blocks: lane i holds those of block i, so that a unit reads and writes them in one
+// access each.  (Byte by byte with each block, 81 M bf16 weights took 205 us: loads and stores of neighbouring
+// bytes by many warps get in each other's way.)
+struct Scales {
+  int m, v;
 };
 
 // A block's place: of the lane's first element in its tensor and in the flat arrays.
@@ -358,8 +365,8 @@ __device__ __forceinline__ BlockLoad<BITS8> load_block(const AdamWParams& p, con
   if constexpr (BITS8) {
     const uint2 m = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.m) + mine);
     const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.v) + mine);
-    r.m[0] = make_uint4(m.x, m.y, p.m_scale[q.block], 0u);
-    r.v[0] = make_uint4(v.x, v.y, p.v_scale[q.block], 0u);
+    r.m[0] = make_uint4(m.x, m.y, 0u, 0u);
+    r.v[0] = make_uint4(v.x, v.y, 0u, 0u);
   } else {
     const Raw8Any m = get_raw(2, p.m, mine, mine + 8, true), v = get_raw(2, p.v, mine, mine + 8, true);
     r.m[0] = m.u[0], r.m[1] = m.u[1], r.v[0] = v.u[0], r.v[1] = v.u[1];
@@ -368,17 +375,17 @@ __device__ __forceinline__ BlockLoad<BITS8> load_block(const AdamWParams& p, con
 }
 
 template <bool BITS8, bool MASTER, int CODE, bool VEC>
-__device__ __forceinline__ void step_block(const AdamWParams& p, const TensorSlot& s, const BlockPlace& place,
-                                           const BlockLoad<BITS8>& r, const GroupNow& q, float clip, const DropKey& key,
-                                           int lane) {
+__device__ __forceinline__ void step_block(const AdamWParams& p, const TensorSlot& s, const BlockPlace& place, int number,
+                                           Scales& scales, const BlockLoad<BITS8>& r, const GroupNow& q, float clip,
+                                           const DropKey& key, int lane) {
   const long long mine = place.mine(lane);
   F8 w, h, m, v;
   unpack(CODE, r.g, h);
   unpack(MASTER ? 2 : CODE, r.w, w);
   // The averages times b1 and b2: in 8 bits scale and factor in one, which rounds the same.
   if constexpr (BITS8) {
-    decode_first(make_uint2(r.m[0].x, r.m[0].y), decode_scale<7>((int)r.m[0].z) * q.b1, m);
-    decode_second(make_uint2(r.v[0].x, r.v[0].y), decode_scale<14>((int)r.v[0].z) * q.b2, v);
+    decode_first(make_uint2(r.m[0].x, r.m[0].y), decode_scale<7>(__shfl_sync(0xffffffffu, scales.m, number)) * q.b1, m);
+    decode_second(make_uint2(r.v[0].x, r.v[0].y), decode_scale<14>(__shfl_sync(0xffffffffu, scales.v, number)) * q.b2, v);
   } else {
     unpack(2, Raw8Any{r.m[0], r.m[1]}, m);
     unpack(2, Raw8Any{r.v[0], r.v[1]}, v);
@@ -387,11 +394,12 @@ __device__ __forceinline__ void step_block(const AdamWParams& p, const TensorSlo
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    // Each product and sum of the averages rounded by itself (packed ones are never contracted): what is
-    // stored does not depend on the compiler.
+    // Each product and sum of the averages is rounded by itself, so that what is stored is one well-defined number.
+    // (The sums are written as a product with one plus the other: a packed product and the sum behind it would be
+    // contracted for all their .rn, and `one` is an argument that the compiler does not know.)
     h.p[i] = fmul2(h.p[i], both(clip));
-    m.p[i] = fadd2(m.p[i], fmul2(h.p[i], both(q.c1)));
-    v.p[i] = fadd2(v.p[i], fmul2(fmul2(h.p[i], h.p[i]), both(q.c2)));
+    m.p[i] = ffma2(fmul2(h.p[i], both(q.c1)), both(p.one), m.p[i]);
+    v.p[i] = ffma2(fmul2(fmul2(h.p[i], h.p[i]), both(q.c2)), both(p.one), v.p[i]);
     const float2 d = make_float2(fast_inverse(fmaf(fast_sqrt<BITS8>(v.p[i].x), q.root, q.eps)),
                                  fast_inverse(fmaf(fast_sqrt<BITS8>(v.p[i].y), q.root, q.eps)));
     w.p[i] = ffma2(fmul2(m.p[i], both(-q.rate)), d, fmul2(w.p[i], both(q.decay)));
@@ -400,33 +408,48 @@ __device__ __forceinline__ void step_block(const AdamWParams& p, const TensorSlo
   put8(CODE, s.p, place.at, VEC ? place.at + 8 : s.n, VEC || aligned16(s.p), w);
   if constexpr (BITS8) {
     const uint4 u = philox7(key, (unsigned long long)place.block * 32 + lane);
-    put_codes<7, 7, true>(static_cast<uint8_t*>(p.m) + mine, p.m_scale + place.block, m, u, lane);
-    put_codes<15, 14, false>(static_cast<uint8_t*>(p.v) + mine, p.v_scale + place.block, v, u, lane);
+    const int em = put_codes<7, 7, true>(static_cast<uint8_t*>(p.m) + mine, m, u);
+    const int ev = put_codes<15, 14, false>(static_cast<uint8_t*>(p.v) + mine, v, u);
+    if (lane == number) scales = Scales{em, ev};
   } else {
     put8(2, p.m, mine, mine + 8, true, m);
     put8(2, p.v, mine, mine + 8, true, v);
   }
 }
 
-// A warp's unit of work: two blocks, or what the tensor has left of them.
+// A warp's unit of work: pairs of blocks, or what the tensor has left of them.
 template <bool BITS8, bool MASTER, int CODE>
 __device__ __forceinline__ void step_unit(const AdamWParams& p, const TensorSlot& s, uint32_t unit, float clip,
                                           const GroupNow* groups, const DropKey& key, int lane) {
-  const long long first = (long long)unit * kStepUnit;
-  const BlockPlace a{first + lane * 8, p.first + s.first + (long long)unit * (kStepUnit / 256)}, b{a.at + 256, a.block + 1};
   const GroupNow q = groups[s.kind >> 8];
-  if (first + kStepUnit <= s.n && aligned16(s.p) && aligned16(s.g)) {
-    const auto x = load_block<BITS8, MASTER, CODE, true>(p, s, a, lane), y = load_block<BITS8, MASTER, CODE, true>(p, s, b, lane);
-    step_block<BITS8, MASTER, CODE, true>(p, s, a, x, q, clip, key, lane);
-    step_block<BITS8, MASTER, CODE, true>(p, s, b, y, q, clip, key, lane);
-  } else {
+  const bool vec = aligned16(s.p) && aligned16(s.g);
+  const int pairs = BITS8 ? p.pairs : 1;
+  long long first = (long long)unit * pairs * kPair;
+  BlockPlace a{first + lane * 8, p.first + s.first + first / 256};
+  const long long block = a.block;
+  const bool scaled = BITS8 && lane < 2 * pairs && first + lane * 256 < s.n;  // of the lane's block
+  Scales scales{0, 0};
+  if (scaled) scales = Scales{p.m_scale[block + lane], p.v_scale[block + lane]};
 #pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-      const BlockPlace& c = i ? b : a;
-      if (first + i * 256 < s.n)
-        step_block<BITS8, MASTER, CODE, false>(p, s, c, load_block<BITS8, MASTER, CODE, false>(p, s, c, lane), q, clip, key, lane);
+  for (int k = 0; k < pairs && first < s.n; ++k, first += kPair) {
+    const BlockPlace b{a.at + 256, a.block + 1};
+    if (vec && first + kPair <= s.n) {
+      const auto x = load_block<BITS8, MASTER, CODE, true>(p, s, a, lane), y = load_block<BITS8, MASTER, CODE, true>(p, s, b, lane);
+      step_block<BITS8, MASTER, CODE, true>(p, s, a, 2 * k, scales, x, q, clip, key, lane);
+      step_block<BITS8, MASTER, CODE, true>(p, s, b, 2 * k + 1, scales, y, q, clip, key, lane);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        const BlockPlace& c = i ? b : a;
+        if (first + i * 256 < s.n)
+          step_block<BITS8, MASTER, CODE, false>(p, s, c, 2 * k + i, scales,
+                                                 load_block<BITS8, MASTER, CODE, false>(p, s, c, lane), q, clip, key, lane);
+      }
     }
+    a.at += kPair;
+    a.block += 2;
   }
+  if (scaled) p.m_scale[block + lane] = (uint8_t)scales.m, p.v_scale[block + lane] = (uint8_t)scales.v;
 }
 
 // x^n by squaring.
@@ -438,7 +461,7 @@ __device__ __forceinline__ double power(double x, unsigned long long n) {
 }
 
 template <bool BITS8, bool MASTER, int N>
-__global__ void __launch_bounds__(kThreads, kStepResident<BITS8>) adamw_kernel(const __grid_constant__ TensorTable<N> table,
+__global__ void __launch_bounds__(kThreads, kStepResident<BITS8, MASTER>) adamw_kernel(const __grid_constant__ TensorTable<N> table,
                                                             const __grid_constant__ AdamWParams p) {
   __shared__ uint32_t ends[N];
   __shared__ GroupNow groups[kAdamWGroups];
@@ -528,7 +551,10 @@ unsigned grid_for(long long units, int num_sms, int resident) {
 
 int grad_norm_grid(long long units, int num_sms) { return (int)grid_for(units, num_sms, kNormResident); }
 long long grad_norm_unit() { return kNormUnit; }
-long long adamw_unit() { return kStepUnit; }
+int adamw_pairs(long long blocks, int state_bits, int num_sms) {
+  const long long warps = (long long)num_sms * kWarps * kStepResident<true>;
+  return state_bits == 8 && blocks / 8 >= 3 * warps ? 4 : 1;
+}
 
 cudaError_t launch_grad_norm_sm100(const TensorSlot* slots, const GradNormParams& p, int num_sms, cudaStream_t st) {
   const unsigned grid = (unsigned)grad_norm_grid(p.units, num_sms);
@@ -544,7 +570,7 @@ cudaError_t launch_grad_norm_sum_sm100(const double* parts, int n, float* norm, 
 }
 
 cudaError_t launch_adamw_sm100(const TensorSlot* slots, const AdamWParams& p, int num_sms, cudaStream_t st) {
-  const unsigned grid = grid_for(p.units, num_sms, p.m_scale ? kStepResident<true> : kStepResident<false>);
+  const unsigned grid = grid_for(p.units, num_sms, !p.m_scale ? kStepResident<false> : p.master ? kStepResident<true, true> : kStepResident<true>);
   with_tables(slots, p.count, [&](const auto& t) {
     if (p.m_scale && p.master) adamw_kernel<true, true><<<grid, kThreads, 0, st>>>(t, p);
     else if (p.m_scale) adamw_kernel<true, false><<<grid, kThreads, 0, st>>>(t, p);

@@ -185,10 +185,14 @@ int dt_adamw_step(int count, const int64_t* params, const int64_t* grads, const 
     const DtAdamWGroup& g = groups[i];
     p.group[i] = dtk::AdamWGroup{g.lr, g.beta1, g.beta2, g.eps, g.weight_decay, g.lr_tensor};
   }
+  p.one = 1.f;
   p.ngroups = ngroups, p.m = exp_avg, p.v = exp_avg_sq, p.master = master;
   if (state_bits == 8) p.m_scale = exp_avg_scale, p.v_scale = exp_avg_sq_scale;
   p.state = reinterpret_cast<long long*>(state);
-  return in_launches(count, params, grads, sizes, kinds, dtk::adamw_unit(),
+  int64_t blocks = 0;
+  for (int i = 0; i < count; ++i) blocks += (sizes[i] + 255) / 256;
+  p.pairs = dtk::adamw_pairs(blocks, state_bits, sms);
+  return in_launches(count, params, grads, sizes, kinds, 512LL * p.pairs,
                      [&](const TensorSlot* slots, int n, uint32_t units, int64_t first, bool last) {
                        p.count = n, p.units = units, p.first = first, p.ticket = last ? ticket : nullptr;
                        return cuda_status(dtk::launch_adamw_sm100(slots, p, sms, st), fn);

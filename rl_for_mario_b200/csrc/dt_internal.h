@@ -308,13 +308,15 @@ struct AdamWParams {
   const double* parts;  // of the gradient's norm, or null: no clipping
   float* norm;
   long long first;  // block of the flat arrays that the launch's first one is
-  uint32_t units;
+  uint32_t units;   // of `pairs` pairs of blocks
+  int pairs;
   int count, ngroups, nparts;
   float max_norm;
+  float one;  // 1, which keeps sums from being contracted
 };
 int grad_norm_grid(long long units, int num_sms);
 long long grad_norm_unit();  // elements of a unit of the norm's work
-long long adamw_unit();      // and of the step's
+int adamw_pairs(long long blocks, int state_bits, int num_sms);  // pairs of blocks in a unit of the step's
 cudaError_t launch_grad_norm_sm100(const TensorSlot* slots, const GradNormParams& p, int num_sms, cudaStream_t st);
 cudaError_t launch_grad_norm_sum_sm100(const double* parts, int n, float* norm, cudaStream_t st);
 cudaError_t launch_adamw_sm100(const TensorSlot* slots, const AdamWParams& p, int num_sms, cudaStream_t st);

@@ -201,8 +201,7 @@ class AdamW(torch.optim.Optimizer):
         self._sizes = array("q", self._numels)
         self._kinds = array("i", [kernels._dtype_code(p) + 256 * group[id(p)] for p in ps])
         self._plain = all(st is None for st in self._strides)
-        self._seen: Optional[List[int]] = None
-        self._held: List[Tensor] = []
+        self._look(list(map(_data_ptr, ps)))
         self._packed = [(None, b"")] * len(self.param_groups)
 
     def _fill_master(self, master: Tensor, first: int) -> None:
@@ -301,11 +300,15 @@ class AdamW(torch.optim.Optimizer):
                 for i in range(len(ps)):
                     self._same(i)
                 self._overlap()
-                self._held, self._seen, self._at = [p.detach() for p in ps], at, array("q", at)
+                self._look(at)
             return self._at, array("q", map(_data_ptr, grads)), grads
         keep: List[Tensor] = []
         to = array("q", [self._gradient(i, g, keep) for i, g in enumerate(grads)])
         return array("q", at), to, keep
+
+    def _look(self, at: List[int]) -> None:
+        """Notes where the parameters are, and holds the memory there."""
+        self._seen, self._at, self._held = at, array("q", at), [p.detach() for p in self._order]
 
     def _same(self, i: int) -> Tensor:
         """Parameter i, whose type, size, order of memory and device have to be those of the flat arrays."""

@@ -202,6 +202,54 @@ def test_steps(dtypes, bits, master, max_norm, lr, betas, eps, wd):
                 assert np.array_equal(value, ref.decode(codes, scales, kind))
 
 
+@pytest.mark.parametrize("dtype,master", [(BF16, False), (FP16, True), (FP32, False)])
+def test_large_units_of_8_bit_averages(dtype, master):
+    """Enough elements for units of eight blocks: whole ones, ones that a tensor ends in, tensors of less than one, an
+    address off the boundary.  Codes, scales and weights of windows of each against the restatement."""
+    sizes = [24_000_003, 5, 256 * 9, 700_001, 2048, 1]
+    g = torch.Generator(device="cuda").manual_seed(0)
+    pool = torch.randn(sum(sizes) + 64, generator=g, device="cuda").mul_(0.05).to(dtype)
+    ps, at = [], 0
+    for i, n in enumerate(sizes):
+        at += 1 if i == 3 else (-at) % 8
+        ps.append(torch.nn.Parameter(pool[at:at + n]))
+        at += n
+    opt = adamw(ps, lr=1e-2, state_bits=8, master=master, weight_decay=0.1, seed=7)
+    starts = blocks_of(ps)
+    for t in (1, 2):
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=g, device="cuda").mul_(1e-3).to(dtype)
+        old = [p.detach().cpu() for p in ps]
+        state = {k: v.cpu().clone() for k, v in opt.state_dict()["state"].items() if isinstance(v, torch.Tensor)}
+        opt.step()
+        after = {k: v.cpu() for k, v in opt.state_dict()["state"].items() if isinstance(v, torch.Tensor)}
+        for i, (p, n) in enumerate(zip(ps, sizes)):
+            blocks = (n + 255) // 256
+            for b0 in sorted({0, max(0, blocks // 2 - 8), max(0, blocks - 24)}):
+                b1 = min(blocks, b0 + 24)
+                lo, hi = b0 * 256, min(n, b1 * 256)
+                first = starts[i] // 256 + b0
+                sl, sb = slice(first * 256, (first + b1 - b0) * 256), slice(first, first + b1 - b0)
+                m0 = ref.decode(state["exp_avg"][sl].numpy(), state["exp_avg_scale"][sb].numpy(), ref.FIRST)
+                v0 = ref.decode(state["exp_avg_sq"][sl].numpy(), state["exp_avg_sq_scale"][sb].numpy(), ref.SECOND)
+                x = p.grad[lo:hi].cpu()
+                m1, v1 = ref.averages_f32(m0, v0, np.pad(x.float().numpy(), (0, len(m0) - len(x))), 0.9, 0.999)
+                block = np.arange(first * 32, (first + b1 - b0) * 32, dtype=np.uint64)
+                w = ref.philox_words(block, 7, t, ref.SITE).reshape(-1).astype(np.int64)
+                for name, y, words, kind in (("exp_avg", m1, (w >> 8) | ((w & 255) << 8), ref.FIRST), ("exp_avg_sq", v1, w, ref.SECOND)):
+                    codes, scales = ref.encode(y, words, kind)
+                    assert np.array_equal(after[name][sl].numpy(), codes) and np.array_equal(after[name + "_scale"][sb].numpy(), scales)
+                kept = master and dtype != FP32
+                r = ref.adamw(state["master"][sl][:hi - lo] if kept else old[i][lo:hi], x, torch.from_numpy(m0[:hi - lo]),
+                              torch.from_numpy(v0[:hi - lo]), t, 1e-2, 0.9, 0.999, 1e-8, 0.1)
+                want, (ap, au) = r["p"]
+                tol, u = 4 * E * ap + 40 * E * au + E * want.abs(), 0 if kept or dtype == FP32 else torch.finfo(dtype).eps / 2
+                near("p", after["master"][sl][:hi - lo] if kept else p[lo:hi], want, tol * (1 + u) + u * want.abs())
+                if kept:
+                    assert torch.equal(p[lo:hi].cpu(), after["master"][sl][:hi - lo].to(dtype))
+    assert int(opt.steps()) == 2
+
+
 def test_a_step_that_is_not_finite_changes_nothing():
     for bits in (8, 32):
         ps = make_params([BF16])
