@@ -22,8 +22,11 @@
 //    of 1 / (1 - b2) = 1,000 steps would carry noise of 80 % of itself; so it is about 20 %, 10 % in its root.
 // A v above zero never becomes zero, so that no m is divided by eps alone.
 //
-// Bound by HBM: bytes an element, bf16 weights: 22 with 32-bit averages, 10 with 8-bit ones, 28 with
-// fp32 weights beside them.
+// Bound by HBM: an element of a bf16 weight costs 22 bytes with 32-bit averages, 10 with 8-bit ones, 28 with 32-bit
+// averages and fp32 weights beside it.  81.3 M weights in 125 tensors, inputs cold: 32-bit averages 292 us in bf16
+// (6.1 TB/s), 383 in fp32 (28 bytes, 5.9), 386 in bf16 with fp32 weights (5.9); 8-bit ones 216 us with fp32 weights
+// beside bf16 ones (16 bytes, 6.0), 212 in fp32 (6.1), 171 to 175 in bf16 alone (4.7 TB/s): there the codes' integer
+// work, some 50 issue slots an element, takes as long as the bytes (issue slots 60 % in use, the ALU pipe 45 %).
 #include <cstring>
 #include <type_traits>
 
@@ -37,7 +40,10 @@ namespace dtk {
 namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
-constexpr int kNormResident = 8;  // blocks on an SM
+// Blocks on an SM.  Norm, 81.3 M bf16 numbers: 41 us with 8, 45 with 6, 45 with 12 (spills).  Step: what leaves the loads of
+// two blocks their registers; 32-bit averages, bf16 weights: 292 us with 4, 300 with 6; 8-bit ones 175 with 5, 184
+// to 187 with 6 (spills), 192 to 197 with 4.
+constexpr int kNormResident = 8;
 template <bool BITS8, bool MASTER = false>
 constexpr int kStepResident = BITS8 && !MASTER ? 5 : 4;
 constexpr int kNormUnit = 1024;      // elements of a warp's turn in the norm
@@ -258,7 +264,7 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 // `word` has above the 16 random bits.  Numbers below 2^(1 - BIAS) have equal steps of 2^(-2 - BIAS): 2^(1 - BIAS) is
 // added first, after which they stand in the binade with that spacing, eight codes up (rounded to zero:
 // what falls off lies below the random bits).  The comparison's result as the number 1 or 0 does both on the
-// FMA pipe: the ALU, at half its rate, is what the 8-bit step runs into (selects instead: XX us).
+// FMA pipe: the ALU, at half its rate, is what the 8-bit step runs into.
 template <int BIAS>
 __device__ __forceinline__ uint32_t encode(float y, uint32_t word, uint32_t select) {
   constexpr float low = 1.f / (1 << (BIAS - 1));
@@ -552,8 +558,12 @@ unsigned grid_for(long long units, int num_sms, int resident) {
 int grad_norm_grid(long long units, int num_sms) { return (int)grid_for(units, num_sms, kNormResident); }
 long long grad_norm_unit() { return kNormUnit; }
 int adamw_pairs(long long blocks, int state_bits, int num_sms) {
+  // 8 bits: units of four pairs have their scales in one access, units of one leave more warps something to do.  bf16
+  // weights in eight tensors, one pair against four: 1 M 11.3 us and 15.4, 5 M 21 and 21.5, 10 M 31.8 and 29.7, 18 M
+  // 52 and 46, 80 M 206 and 171 (two pairs 183, eight 183, sixteen 204); so four from one and a half for each warp on.
+  // 32 bits: one (two pairs 2 to 4 % slower, four 4 %: neighbouring warps then read further apart).
   const long long warps = (long long)num_sms * kWarps * kStepResident<true>;
-  return state_bits == 8 && blocks / 8 >= 3 * warps ? 4 : 1;
+  return state_bits == 8 && blocks >= 12 * warps ? 4 : 1;
 }
 
 cudaError_t launch_grad_norm_sm100(const TensorSlot* slots, const GradNormParams& p, int num_sms, cudaStream_t st) {
