@@ -108,9 +108,11 @@ class FastDTAttention(nn.Module):
 
     @classmethod
     def from_reference(cls, ref_attn: nn.Module, config, **kw) -> "FastDTAttention":
-        """Builds the fast module with the weights of a reference DecisionTransformerAttention."""
+        """Builds the fast module with the weights of a reference DecisionTransformerAttention (which has no norms of
+        heads: with config.qk_norm theirs are ones)."""
         m = cls(config, **kw)
-        m.load_state_dict(ref_attn.state_dict())
+        ones = {n: t for n, t in m.state_dict().items() if n in ("q_norm.weight", "k_norm.weight")}
+        m.load_state_dict({**ones, **ref_attn.state_dict()})
         p = next(ref_attn.parameters())
         return m.to(device=p.device, dtype=p.dtype)
 

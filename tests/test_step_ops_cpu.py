@@ -187,3 +187,36 @@ def test_rounding_at_random_of_the_restatement():
     a, b = (float(ref.decode(np.full(256, c, np.uint8), np.array([127]), ref.SECOND)[0]) for c in (low, low + 1))
     share = (0.3 - a) / (b - a)
     assert a < 0.3 < b and abs(np.mean([u != low for u in up]) - share) < 2 / 1024
+
+
+def test_head_norms_of_a_swapped_module():
+    from types import SimpleNamespace
+
+    from rl_for_mario_b200.attention import FastDTAttention, swap_attention
+
+    def config(**kw):
+        return SimpleNamespace(hidden_size=64, num_attention_heads=2, num_key_value_heads=1, dropout=0.0, **kw)
+
+    class Reference(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            for n, k in (("q", 64), ("k", 32), ("v", 32), ("o", 64)):
+                setattr(self, n + "_proj", torch.nn.Linear(64, k, bias=False))
+
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.self_attn = Reference()
+
+    block, ref = Block(), None
+    ref = block.self_attn
+    assert swap_attention(block, config(qk_norm=True, rms_norm_eps=1e-6)) == 1
+    m = block.self_attn
+    assert torch.equal(m.k_proj.weight, ref.k_proj.weight) and (m.q_norm.weight == 1).all() and m.k_norm.eps == 1e-6
+    assert {"q_norm.weight", "k_norm.weight"} <= set(m.state_dict())
+    again = FastDTAttention.from_reference(m, config(qk_norm=True))
+    assert again.k_norm.eps == 1e-5
+    plain = FastDTAttention(config())
+    assert set(plain.state_dict()) == {f"{n}_proj.weight" for n in "qkvo"} and plain._head_norms(torch.float32) is None
+    with pytest.raises(RuntimeError):
+        FastDTAttention.from_reference(m, config())
