@@ -89,7 +89,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits`` 32: averages in fp32.  8: in one byte an element with a power of two for each 256 elements,
     rounded up or down at random (by ``seed``, the step and the element), so that they follow the gradients
-    as those in 32 bits do: v to about 10 % of its root, m to about 8 %.
+    as those in 32 bits do: v to about 10 % of its root, m to about 8 %.  Ranks that hold copies of the same
+    parameters take the same seed, which keeps the copies the same.
     ``master``: fp32 weights are kept beside 16-bit parameters; without them a step smaller than half a unit
     in the last place of a 16-bit weight is lost.  They are what a step starts from: reset_master() after the
     parameters were changed from outside.
@@ -265,7 +266,7 @@ class AdamW(torch.optim.Optimizer):
         ps, buf = self._order, self._buffers
         dev = buf["count"].device
         at, to, keep = self._addresses(ps, dev.index)
-        if to is None:
+        if to is None or not self._blocks:
             self.norm = None
             return loss
         size, ws, norm = 0, None, None

@@ -499,6 +499,11 @@ def test_refusals():
         optim.AdamW([torch.nn.Parameter(torch.zeros(4, 4, device="cuda")[:, ::2])])
     with pytest.raises(ValueError, match="16 groups"):
         optim.AdamW([dict(params=[torch.nn.Parameter(torch.zeros(1, device="cuda"))]) for _ in range(17)])
+    none = torch.nn.Parameter(torch.zeros(0, 3, device="cuda"))
+    none.grad = torch.zeros(0, 3, device="cuda")
+    opt = optim.AdamW([none], state_bits=8, max_norm=1.0)
+    opt.step()
+    assert int(opt.steps()) == 0 and opt.moments()[0].numel() == 0
     q = torch.zeros(20, device="cuda")
     opt = optim.AdamW([torch.nn.Parameter(q[:12]), torch.nn.Parameter(q[11:])])
     with pytest.raises(ValueError, match="share memory"):
