@@ -170,8 +170,8 @@ int dt_dropout(const void* x, int64_t x_stride, const void* residual, int64_t re
  * The 2-norm of many tensors taken as one: norm (fp32, one number) receives
  * sqrt(sum of squares).  tensors: their addresses (0: left out), sizes: numbers of
  * elements (whole tensors without gaps, any order of dimensions), kinds: dtype codes.
- * Any alignment.  The three arrays are the host's and are read during the call.  Sums
- * are fp64 of fp32 sums of eight squares (fp64 squares where fp32 would overflow or
+ * Any alignment.  The three arrays are the host's and are read during the call.  Pairs
+ * of squares are added in fp32, the rest in fp64 (all of it where fp32 would overflow or
  * lose bits), in a fixed order.  workspace: dt_grad_norm_workspace bytes, 16-byte aligned.
  */
 int dt_grad_norm(int count, const int64_t* tensors, const int64_t* sizes, const int32_t* kinds, float* norm,

@@ -553,9 +553,10 @@ unsigned grid_for(long long units, int num_sms, int resident) {
 
 }  // namespace
 
-
-
-int grad_norm_grid(long long units, int num_sms) { return (int)grid_for(units, num_sms, kNormResident); }
+// (What four warps take in four turns is one block's, which needs no second launch for the sum.)
+int grad_norm_grid(long long units, int num_sms) {
+  return units <= 4 * kWarps ? 1 : (int)grid_for(units, num_sms, kNormResident);
+}
 long long grad_norm_unit() { return kNormUnit; }
 int adamw_pairs(long long blocks, int state_bits, int num_sms) {
   // 8 bits: units of four pairs have their scales in one access, units of one leave more warps something to do.  bf16

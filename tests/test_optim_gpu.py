@@ -53,8 +53,7 @@ def test_norm(sizes, types):
     want = math.sqrt(sum(t.double().pow(2).sum().item() for t in ts))
     got = optim.grad_norm([t.cuda() for t in ts])
     assert got.dtype == FP32 and got.dim() == 0
-    # 32 squares in fp32: a product, three sums of a pair, two of four, one of two make 8 e on a sum of positive terms,
-    # halved by the root; one rounding.
+    # Two squares and their sum in fp32, 3 e on positive terms, halved by the root; fp64 behind them; one rounding.
     assert abs(got.item() - want) <= want * 5 * E
 
 
