@@ -128,8 +128,9 @@ int dt_residual_norm_backward(const void* dh, int64_t dh_stride, const void* dn,
  * at table row t = start_pos[b] + s (start_pos null: s).  q, q_out [B, S, Hq, D], k,
  * k_out [B, S, Hkv, D], D contiguous; strides holds the (batch, position, head)
  * element strides of q, k, q_out and k_out, 12 values.  Any head numbers; even D from 2
- * to 256, bf16, fp16 or fp32, any strides and alignment (D a power of two from 8 on,
- * 8-byte aligned (fp32 16-byte) heads and 16-byte aligned table rows run faster).
+ * to 256, bf16, fp16 or fp32, any strides and alignment (D a multiple of 16, or of 8 in
+ * fp32, with 16-byte aligned heads and table rows runs fastest; 16-bit heads of a multiple
+ * of 8 on 8-byte boundaries come next).
  * Weights in the same type, or in fp32 with weights_fp32.  cos / sin [cos_rows, D] fp32
  * with a common row stride.  A position outside the tables sets the device status word
  * and its outputs to zeros.  An output may be its own input.  fp32 arithmetic, one

@@ -269,7 +269,7 @@ struct HeadNormParams {
   int lg;                    // log2 of the lanes that hold a head
   FastDiv by_s;
   bool w32;  // weights (and their gradients) in fp32
-  bool vec;  // whole vectors of 16 bytes
+  int vec;   // elements of an access: 8, 4, or 0 for element by element
   float eps, inv_d;
 };
 void head_norm_plan(HeadNormParams& p, int dtype, bool bwd, int num_sms);  // sets vec, lg and the sides' ranges and blocks

@@ -245,12 +245,12 @@ __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_any_kernel
 
 // ---------------------------------------------------------------- heads of whole vectors
 // Lane c of a group holds elements P c .. P c + P - 1 and the same from h on: two accesses of 16 bytes
-// (P = 8, fp32 4).  A head's elements are copied into the lane's own places of a ring in shared memory,
+// (P = 8, fp32 4), or of 8 for 16-bit heads whose halves are not whole 16-byte vectors (P = 4).  A head's elements are copied into the lane's own places of a ring in shared memory,
 // kDepth heads ahead and across positions, and only the lane reads them back: no barrier, and what is in
 // flight takes no registers (one head ahead in registers: 107 + 178 us where this took 66 + 99).  Two heads ahead: with
 // four, and three, 61 + 94 us instead of 57 + 90, as the ring's memory is L1's, which holds table rows.
-template <int DT>
-constexpr int kPairs = DT == 2 ? 4 : 8;
+template <int DT, int P>
+using Vec = typename std::conditional<P * (DT == 2 ? 4 : 2) == 16, uint4, uint2>::type;
 constexpr int kDepth = 2;
 
 template <int N>
@@ -258,37 +258,48 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copy16(uint4* to, const void* from) {
+__device__ __forceinline__ void copy_vec(uint4* to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void copy_vec(uint2* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
                : "memory");
 }
 
 // A lane's half of a head as packed pairs of fp32.
-template <int DT>
+template <int DT, int P>
 struct Half {
-  float2 p[kPairs<DT> / 2];
+  float2 p[P / 2];
   __device__ __forceinline__ void set(uint4 u) {
     if constexpr (DT == 2) {
       p[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
       p[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
     } else {
       using E = Elem<DT == 0>;
-      p[0] = E::to_f2(u.x), p[1] = E::to_f2(u.y), p[2] = E::to_f2(u.z), p[3] = E::to_f2(u.w);
+      p[0] = E::to_f2(u.x), p[1] = E::to_f2(u.y), p[P / 2 - 2] = E::to_f2(u.z), p[P / 2 - 1] = E::to_f2(u.w);
     }
   }
-  __device__ __forceinline__ uint4 bits() const {
+  __device__ __forceinline__ void set(uint2 u) {
+    using E = Elem<DT == 0>;
+    p[0] = E::to_f2(u.x), p[1] = E::to_f2(u.y);
+  }
+  __device__ __forceinline__ Vec<DT, P> bits() const {
     if constexpr (DT == 2) {
       return make_uint4(__float_as_uint(p[0].x), __float_as_uint(p[0].y), __float_as_uint(p[1].x),
                         __float_as_uint(p[1].y));
     } else {
       using E = Elem<DT == 0>;
-      return make_uint4(E::from_f2(p[0].x, p[0].y), E::from_f2(p[1].x, p[1].y), E::from_f2(p[2].x, p[2].y),
-                        E::from_f2(p[3].x, p[3].y));
+      if constexpr (P == 4)
+        return make_uint2(E::from_f2(p[0].x, p[0].y), E::from_f2(p[1].x, p[1].y));
+      else
+        return make_uint4(E::from_f2(p[0].x, p[0].y), E::from_f2(p[1].x, p[1].y), E::from_f2(p[2].x, p[2].y),
+                          E::from_f2(p[3].x, p[3].y));
     }
   }
   __device__ __forceinline__ void load_f32(const float* f) {
 #pragma unroll
-    for (int i = 0; i < kPairs<DT> / 4; ++i) {
+    for (int i = 0; i < P / 4; ++i) {
       const float4 v = *reinterpret_cast<const float4*>(f + 4 * i);
       p[2 * i] = make_float2(v.x, v.y);
       p[2 * i + 1] = make_float2(v.z, v.w);
@@ -296,7 +307,7 @@ struct Half {
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < kPairs<DT> / 2; ++i) p[i] = make_float2(0.f, 0.f);
+    for (int i = 0; i < P / 2; ++i) p[i] = make_float2(0.f, 0.f);
   }
 };
 __device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.y); }
@@ -309,11 +320,13 @@ struct Place {
   int k, n;  // n: heads of the item, 0 behind the last one
 };
 
-template <int DT, bool BWD, int LG>
+template <int DT, int P, bool BWD, int LG>
 __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_kernel(const __grid_constant__ HeadNormParams p) {
   using T = typename TrainElem<DT>::T;
-  constexpr int P = kPairs<DT>, N = P / 2, TENSORS = BWD ? 4 : 2;
-  extern __shared__ uint4 ring[];  // [kDepth, TENSORS, threads]
+  using V = Vec<DT, P>;
+  constexpr int N = P / 2, TENSORS = BWD ? 4 : 2;
+  extern __shared__ uint4 ring_bytes[];
+  V* ring = reinterpret_cast<V*>(ring_bytes);  // [kDepth, TENSORS, threads]
   __shared__ __align__(16) float weights[256];
   const bool second = blockIdx.x >= p.side[0].blocks;
   const HeadNormSide& sd = p.side[second];
@@ -340,15 +353,15 @@ __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_kernel(con
     q.x = static_cast<const T*>(sd.x) + it.b * sd.x_sb + it.s * sd.x_ss + it.head * sd.x_sh + e;
     if constexpr (BWD) q.g = static_cast<const T*>(sd.grad) + it.b * sd.g_sb + it.s * sd.g_ss + it.head * sd.g_sh + e;
   };
-  uint4* slots = ring + threadIdx.x;
+  V* slots = ring + threadIdx.x;
   auto fetch = [&](int stage) {
     if (f.k < f.n) {
-      uint4* to = slots + stage * (TENSORS * kThreads);
-      copy16(to, f.x);
-      copy16(to + kThreads, f.x + h);
+      V* to = slots + stage * (TENSORS * kThreads);
+      copy_vec(to, f.x);
+      copy_vec(to + kThreads, f.x + h);
       if constexpr (BWD) {
-        copy16(to + 2 * kThreads, f.g);
-        copy16(to + 3 * kThreads, f.g + h);
+        copy_vec(to + 2 * kThreads, f.g);
+        copy_vec(to + 3 * kThreads, f.g + h);
       }
     }
     copies_commit();
@@ -359,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_kernel(con
       enter(f, at);
     }
   };
-  Half<DT> aa, ab;  // sums of the weight's gradient
+  Half<DT, P> aa, ab;  // sums of the weight's gradient
   aa.clear();
   ab.clear();
   if (at < items) {
@@ -377,12 +390,12 @@ __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_kernel(con
     const long long t = (p.start ? p.start[b] : 0) + (long long)s;
     const bool known = t >= 0 && t < p.cos_rows;
     if (live && !known && p.status) atomicExch(p.status, (int)kDevBadShape);
-    Half<DT> ca, cb, sa, sb;  // forward: times the weights
+    Half<DT, P> ca, cb, sa, sb;  // forward: times the weights
     const float* cos = p.cos + (known ? t : 0) * p.cs_stride + e;
     const float* sin = p.sin + (known ? t : 0) * p.cs_stride + e;
     ca.load_f32(cos), cb.load_f32(cos + h), sa.load_f32(sin), sb.load_f32(sin + h);
     if constexpr (!BWD) {
-      Half<DT> wa, wb;
+      Half<DT, P> wa, wb;
       wa.load_f32(weights + e), wb.load_f32(weights + e + h);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -392,10 +405,10 @@ __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_kernel(con
     }
     for (int k = 0; k < sd.per; ++k) {
       copies_wait<kDepth - 1>();
-      const uint4* from = slots + stage * (TENSORS * kThreads);
+      const V* from = slots + stage * (TENSORS * kThreads);
       const bool have = k < n;
-      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-      Half<DT> xa, xb, ga, gb;
+      const V zero{};
+      Half<DT, P> xa, xb, ga, gb;
       xa.set(have ? from[0] : zero), xb.set(have ? from[kThreads] : zero);
       if constexpr (BWD) ga.set(have ? from[2 * kThreads] : zero), gb.set(have ? from[3 * kThreads] : zero);
       fetch(stage);
@@ -412,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_kernel(con
           xb.p[i] = fmul2(ffma2(a, sb.p[i], fmul2(v, cb.p[i])), both(r));
         }
       } else {
-        Half<DT> wa, wb;
+        Half<DT, P> wa, wb;
         wa.load_f32(weights + e), wb.load_f32(weights + e + h);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -436,8 +449,8 @@ __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_kernel(con
         }
       }
       if (have) {
-        *reinterpret_cast<uint4*>(o) = known ? xa.bits() : zero;
-        *reinterpret_cast<uint4*>(o + h) = known ? xb.bits() : zero;
+        *reinterpret_cast<V*>(o) = known ? xa.bits() : zero;
+        *reinterpret_cast<V*>(o + h) = known ? xb.bits() : zero;
         o += sd.o_sh;
       }
     }
@@ -446,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_kernel(con
 
   if constexpr (BWD) {
     __syncthreads();  // (the ring's last readers are done)
-    float* sums = reinterpret_cast<float*>(ring);  // [warps, D]
+    float* sums = reinterpret_cast<float*>(ring_bytes);  // [warps, D]
 #pragma unroll
     for (int o = 16; o >= 1 << lg; o >>= 1)
 #pragma unroll
@@ -486,22 +499,24 @@ __global__ void __launch_bounds__(1024) head_norm_sum_kernel(const __grid_consta
   }
 }
 
-// 16-byte accesses need every half of a head on a 16-byte boundary, in whole vectors.
-bool can_vector(const HeadNormParams& p, int dtype, bool bwd) {
-  const int pairs = dtype == 2 ? 4 : 8;
-  if (p.D % (2 * pairs) || p.cs_stride % 4 ||
-      ((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15))
-    return false;
-  for (const HeadNormSide& s : p.side) {
-    const void* ptrs[] = {s.x, s.out, bwd ? s.grad : nullptr};
-    for (const void* q : ptrs)
-      if (reinterpret_cast<uintptr_t>(q) & 15) return false;
-    const long long strides[] = {s.x_sb, s.x_ss, s.x_sh, s.o_sb, s.o_ss, s.o_sh,
-                                 bwd ? s.g_sb : 0, bwd ? s.g_ss : 0, bwd ? s.g_sh : 0};
-    for (long long q : strides)
-      if (q % pairs) return false;
+// Elements of an access of the vector kernel: every half of a head has to be whole vectors on boundaries of their size.
+// 0: there is no such size.  (96 x 768, 8 / 2 heads of 40, bf16: 45 + 73 us with accesses of 8 bytes, 82 + 124 element by
+// element.)
+int vector_pairs(const HeadNormParams& p, int dtype, bool bwd) {
+  if (p.cs_stride % 4 || ((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15)) return 0;
+  for (int pairs = dtype == 2 ? 4 : 8; pairs >= 4; pairs /= 2) {
+    const uintptr_t bytes = (uintptr_t)pairs * (dtype == 2 ? 4 : 2);
+    bool fits = p.D % (2 * pairs) == 0;
+    for (const HeadNormSide& s : p.side) {
+      const void* ptrs[] = {s.x, s.out, bwd ? s.grad : nullptr};
+      for (const void* q : ptrs) fits = fits && reinterpret_cast<uintptr_t>(q) % bytes == 0;
+      const long long strides[] = {s.x_sb, s.x_ss, s.x_sh, s.o_sb, s.o_ss, s.o_sh,
+                                   bwd ? s.g_sb : 0, bwd ? s.g_ss : 0, bwd ? s.g_sh : 0};
+      for (long long q : strides) fits = fits && q % pairs == 0;
+    }
+    if (fits) return pairs;
   }
-  return true;
+  return 0;
 }
 
 int log_lanes(int D, int pairs) {  // of the group that holds a head
@@ -510,31 +525,38 @@ int log_lanes(int D, int pairs) {  // of the group that holds a head
   return lg;
 }
 
+template <int DT, int P, bool BWD>
+cudaError_t launch_vector(const HeadNormParams& p, unsigned grid, cudaStream_t st) {
+  constexpr int ring = kDepth * (BWD ? 4 : 2) * kThreads * (int)sizeof(Vec<DT, P>), sums = kThreads / 32 * 256 * 4;
+  constexpr int smem = BWD && sums > ring ? sums : ring;  // (the block's sums lie in the ring)
+  auto run = [&](auto kernel) {
+    const cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kernel), smem);
+    if (e == cudaSuccess) kernel<<<grid, kThreads, smem, st>>>(p);
+    return e;
+  };
+  switch (p.lg) {
+    case 0: return run(head_norm_kernel<DT, P, BWD, 0>);
+    case 1: return run(head_norm_kernel<DT, P, BWD, 1>);
+    case 2: return run(head_norm_kernel<DT, P, BWD, 2>);
+    case 3: return run(head_norm_kernel<DT, P, BWD, 3>);
+    case 4: return run(head_norm_kernel<DT, P, BWD, 4>);
+    case 5: return run(head_norm_kernel<DT, P, BWD, 5>);
+  }
+  return cudaErrorInvalidValue;
+}
+
 template <int DT, bool BWD>
 cudaError_t launch(const HeadNormParams& p, cudaStream_t st) {
   const unsigned grid = p.side[0].blocks + p.side[1].blocks;
-  if (p.vec) {
-    constexpr int smem = kDepth * (BWD ? 4 : 2) * kThreads * 16;
-    static_assert(!BWD || smem >= kThreads / 32 * 256 * 4, "the block's sums lie in the ring");
-    auto run = [&](auto kernel) {
-      const cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kernel), smem);
-      if (e == cudaSuccess) kernel<<<grid, kThreads, smem, st>>>(p);
-      return e;
-    };
-    cudaError_t e = cudaErrorInvalidValue;
-    switch (p.lg) {
-      case 0: e = run(head_norm_kernel<DT, BWD, 0>); break;
-      case 1: e = run(head_norm_kernel<DT, BWD, 1>); break;
-      case 2: e = run(head_norm_kernel<DT, BWD, 2>); break;
-      case 3: e = run(head_norm_kernel<DT, BWD, 3>); break;
-      case 4: e = run(head_norm_kernel<DT, BWD, 4>); break;
-      case 5: e = run(head_norm_kernel<DT, BWD, 5>); break;
-    }
-    if (e != cudaSuccess) return e;
+  cudaError_t e = cudaSuccess;
+  if (p.vec == 8) {
+    if constexpr (DT != 2) e = launch_vector<DT, 8, BWD>(p, grid, st);
+  } else if (p.vec == 4) {
+    e = launch_vector<DT, 4, BWD>(p, grid, st);
   } else {
     head_norm_any_kernel<DT, BWD><<<grid, kThreads, BWD ? kThreads / 32 * p.D * 4 : 0, st>>>(p);
   }
-  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaGetLastError();
   if (!BWD || e != cudaSuccess || (p.side[0].blocks == 1 && p.side[1].blocks == 1)) return e;
   head_norm_sum_kernel<DT><<<dim3((unsigned)(p.D + 31) / 32, 2), 1024, 0, st>>>(p);
   return cudaGetLastError();
@@ -569,8 +591,8 @@ Split split_heads(long long rows, int heads, int other_heads, int D, int pairs, 
 }  // namespace
 
 void head_norm_plan(HeadNormParams& p, int dtype, bool bwd, int num_sms) {
-  p.vec = can_vector(p, dtype, bwd);
-  const int pairs = p.vec && dtype != 2 ? 8 : 4;
+  p.vec = vector_pairs(p, dtype, bwd);
+  const int pairs = p.vec ? p.vec : 4;
   p.lg = log_lanes(p.D, pairs);
   for (int i = 0; i < 2; ++i) {
     HeadNormSide& s = p.side[i];

@@ -108,10 +108,10 @@ def test_heads_and_gradients(B, S, Hq, Hkv, D, dt, wdt, start):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("D,dt", [(32, BF16), (64, FP32), (42, FP16)])
-def test_any_strides_and_alignment(D, dt):
-    """Heads before positions, odd strides, an offset of one element, a table that is a slice of a wider one,
-    expanded gradients."""
+@pytest.mark.parametrize("D,dt,off", [(32, BF16, 1), (64, FP32, 1), (42, FP16, 1), (64, BF16, 4), (128, FP16, 4), (96, FP32, 4)])
+def test_any_strides_and_alignment(D, dt, off):
+    """Heads before positions, gaps, an offset of one element or four (16-bit heads on 8-byte boundaries), a table that
+    is a slice of a wider one, expanded gradients."""
     from rl_for_mario_b200 import kernels
 
     B, S, Hq, Hkv = 3, 9, 4, 2
@@ -119,15 +119,16 @@ def test_any_strides_and_alignment(D, dt):
     hq, hk, _ = qkv.split([Hq, Hkv, Hkv], 2)
     cos, sin = tables(S, D, 5)
     pos = torch.arange(S).expand(B, S)
-    wide = torch.zeros(S, 2 * D + 1, device="cuda")
-    wide[:, 1:D + 1], wide[:, D + 1:] = cos.cuda(), sin.cuda()
-    how = (wq.cuda(), wk.cuda(), EPS, wide[:, 1:D + 1], wide[:, D + 1:])
+    wide = torch.zeros(S, 2 * D + off, device="cuda")
+    wide[:, off:D + off], wide[:, D + off:] = cos.cuda(), sin.cuda()
+    how = (wq.cuda(), wk.cuda(), EPS, wide[:, off:D + off], wide[:, D + off:])
 
     def moved(t):
-        """The same numbers: one element off the boundary, [B, H, S, D] in memory with gaps."""
+        """The same numbers: off the boundary, [B, H, S, D] in memory with gaps."""
         b, s, n, d = t.shape
-        buf = torch.full((b * n * s * (d + 3) + 1,), float("nan"), dtype=t.dtype, device="cuda")
-        v = buf[1:].view(b, n, s, d + 3)[..., :d].permute(0, 2, 1, 3)
+        gap = 3 if off == 1 else off
+        buf = torch.full((b * n * s * (d + gap) + off,), float("nan"), dtype=t.dtype, device="cuda")
+        v = buf[off:].view(b, n, s, d + gap)[..., :d].permute(0, 2, 1, 3)
         v.copy_(t)
         return v
 
