@@ -505,6 +505,11 @@ class MarioDT(nn.Module):
         groups = [{"params": [p for p in ps if p.dim() > 1]}, {"params": [p for p in ps if p.dim() < 2], "weight_decay": 0.0}]
         return optim.AdamW([g for g in groups if g["params"]], lr=lr, weight_decay=weight_decay, **kw)
 
+    def weights_changed(self) -> None:
+        """Says that the parameters were written where PyTorch did not see it: by a replay of a captured training step.
+        The weights that fused blocks and attention modules derive from them are then taken anew."""
+        torch.autograd.graph.increment_version(list(self.parameters()))
+
     def reference_rounding(self, on: bool = True) -> "MarioDT":
         """Evaluates a 16-bit model at the reference's own rounding points, so its
         logits track the reference's 16-bit execution (model.to(torch.bfloat16))

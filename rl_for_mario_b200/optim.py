@@ -283,7 +283,16 @@ class AdamW(torch.optim.Optimizer):
                         kernels._ptr(buf.get("exp_avg_sq_scale")), kernels._ptr(buf.get("master")),
                         buf["count"].data_ptr(), buf["ticket"].data_ptr(), self.max_norm or 0.0, kernels._ptr(norm),
                         kernels._ptr(ws), size)
+        # The launch writes through addresses: PyTorch has to be told, as autograd's check of saved tensors and every
+        # weight derived from these (a model's folded norms) go by the version.  (7 us for 125 tensors.)
+        torch.autograd.graph.increment_version([p for p, g in zip(ps, to) if g])
         return loss
+
+    def weights_changed(self) -> None:
+        """Tells PyTorch that the parameters were written, which step() does by itself.  A replay of a captured step runs
+        no Python: call this after it, before the model is used outside the graph, as what is derived from the
+        weights (MarioDT.fuse_norms, FastDTAttention) is taken anew when their version has changed."""
+        torch.autograd.graph.increment_version(self._order)
 
     def _addresses(self, ps: List[Tensor], index: int):
         """(addresses of the parameters, of their gradients, tensors to be held until the launch); the second None

@@ -1,0 +1,67 @@
+"""The optimizer's host side on CPU tensors: its launch is replaced by writes through the addresses that the entry
+point gets, as the kernel's are.  (AdamW refuses CPU parameters; the check is taken out here.)"""
+import ctypes
+
+import pytest
+import torch
+
+from rl_for_mario_b200 import kernels, optim
+
+
+class Calls(list):
+    """The arguments of the launches: a dict of each."""
+
+    def __call__(self, name, dev, count, at, to, sizes, kinds, ngroups, groups, bits, *rest):
+        assert name == "dt_adamw_step"
+
+        def longs(p):
+            return list((ctypes.c_int64 * count).from_address(p))
+
+        call = dict(count=count, at=longs(at), to=longs(to), sizes=longs(sizes), ngroups=ngroups,
+                    groups=[optim._GROUP.unpack_from(groups, i * optim._GROUP.size) for i in range(ngroups)])
+        for p, g, n in zip(call["at"], call["to"], call["sizes"]):
+            if g:  # fp32 weights: p -= g
+                for i in range(n):
+                    w = ctypes.c_float.from_address(p + 4 * i)
+                    w.value -= ctypes.c_float.from_address(g + 4 * i).value
+        self.append(call)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    c = Calls()
+    monkeypatch.setattr(optim.AdamW, "_check_param", lambda self, p: None)
+    monkeypatch.setattr(kernels, "_launch", c)
+    return c
+
+
+def params(*shapes):
+    return [torch.nn.Parameter(torch.ones(s)) for s in shapes]
+
+
+def test_a_step_raises_the_versions_of_what_it_wrote(calls):
+    ps = params(3, (2, 5), 4)
+    opt = optim.AdamW(ps)
+    ps[0].grad, ps[2].grad = torch.full((3,), 0.5), torch.full((4,), 0.25)
+    was = [p._version for p in ps]
+    opt.step()
+    assert len(calls) == 1 and (ps[0] == 0.5).all() and (ps[1] == 1).all() and (ps[2] == 0.75).all()
+    now = [p._version for p in ps]
+    assert now[0] > was[0] and now[1] == was[1] and now[2] > was[2]
+    for p in ps:
+        p.grad = None
+    opt.step()  # no gradient: no step
+    assert len(calls) == 1 and [p._version for p in ps] == now
+    opt.weights_changed()
+    assert all(p._version > v for p, v in zip(ps, now))
+
+
+def test_a_step_between_a_forward_pass_and_its_backward_pass_is_an_error(calls):
+    ps = params((4, 3))
+    opt = optim.AdamW(ps)
+    ps[0].grad = torch.ones(4, 3)
+    x = torch.ones(2, 3, requires_grad=True)
+    y = torch.nn.functional.linear(x, ps[0]).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
