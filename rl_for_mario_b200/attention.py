@@ -45,6 +45,19 @@ from .cache import LayerKV, dense_layer
 Tensor = torch.Tensor
 
 
+def remade(old: Optional[Tensor], make) -> Tuple[Tensor, bool]:
+    """(make(), whether it is to be kept): a weight derived from parameters, in the memory of the ``old`` one where it
+    fits, so that a captured graph that reads that finds the new one in its place.  One that is made inside a capture is
+    the graph's own, made anew at each replay, and not kept: it holds nothing until then."""
+    with torch.inference_mode(False), torch.no_grad():  # (a tensor of inference mode could not be written outside it)
+        new = make()
+        if new.is_cuda and torch.cuda.is_current_stream_capturing():
+            return new, False
+        if old is not None and old.shape == new.shape and old.dtype == new.dtype and old.device == new.device:
+            new = old.copy_(new)
+        return new, True
+
+
 def left_padding(mask: Tensor, length: int, check: bool) -> Tensor:
     """pad_len [B] of a [B, length] mask; with ``check`` a mask that is not zeros then ones is refused (a host read)."""
     pad = kernels.pad_len_from_mask(mask, length)
@@ -152,7 +165,9 @@ class FastDTAttention(nn.Module):
         ps = (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight, self._fused_norm.weight)
         key = tuple((p.data_ptr(), p._version) for p in ps) + (dtype,)
         if self._fused_w is None or self._fused_key != key:
-            w = kernels.fold_norm_weight(*ps, dtype=dtype)
+            w, kept = remade(self._fused_w, lambda: kernels.fold_norm_weight(*ps, dtype=dtype))
+            if not kept:
+                return w
             object.__setattr__(self, "_fused_w", w)
             object.__setattr__(self, "_fused_key", key)
         return self._fused_w
@@ -171,7 +186,10 @@ class FastDTAttention(nn.Module):
         ps = (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
         key = tuple((p.data_ptr(), p._version) for p in ps) + (dtype,)
         if getattr(self, "_cat_key", None) != key:
-            object.__setattr__(self, "_cat_w", torch.cat([p.to(dtype) for p in ps], dim=0).contiguous())
+            w, kept = remade(getattr(self, "_cat_w", None), lambda: torch.cat([p.to(dtype) for p in ps], dim=0).contiguous())
+            if not kept:
+                return w
+            object.__setattr__(self, "_cat_w", w)
             object.__setattr__(self, "_cat_key", key)
         return self._cat_w
 

@@ -22,7 +22,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import kernels, optim, training
-from .attention import FastDTAttention, left_padding
+from .attention import FastDTAttention, left_padding, remade
 from .cache import LayerKV, PagedKVCache
 
 Tensor = torch.Tensor
@@ -126,7 +126,10 @@ class DTBlock(nn.Module):
         ps = (self.mlp.gate_proj.weight, self.mlp.up_proj.weight, self.post_attention_layernorm.weight)
         key = tuple((p.data_ptr(), p._version) for p in ps) + (dtype,)
         if getattr(self, "_swiglu_w", None) is None or self._swiglu_key != key:
-            self._swiglu_w = kernels.fold_swiglu_weight(*ps, dtype=dtype)
+            w, kept = remade(getattr(self, "_swiglu_w", None), lambda: kernels.fold_swiglu_weight(*ps, dtype=dtype))
+            if not kept:
+                return w
+            self._swiglu_w = w
             self._swiglu_key = key
         return self._swiglu_w
 

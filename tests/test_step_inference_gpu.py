@@ -127,3 +127,35 @@ def test_a_step_between_a_forward_pass_and_its_backward_pass_is_an_error():
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_a_captured_inference_after_a_step():
+    """The graph reads derived weights where they were at its capture: they are renewed in their place.  A capture that
+    finds old ones makes its own at each replay."""
+    m = make(True).fuse_training().fuse_norms()
+    opt = m.adamw(lr=0.05)
+    b = batch(m)
+    infer(m, b), infer(m, b)
+
+    def step():
+        m(**b).loss.backward()
+        opt.step()
+        opt.zero_grad(set_to_none=True)
+
+    def captured():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph), torch.no_grad():
+            out = m(**b).action_logits
+        return graph, out
+
+    warm = captured()
+    step()
+    cold = captured()  # the derived weights are those of before the step
+    for _ in range(2):
+        want = infer(make(True, copy.deepcopy(m.state_dict())).fuse_norms(), b)
+        cold[0].replay()
+        assert torch.equal(cold[1], want)
+        assert torch.equal(infer(m, b), want)
+        warm[0].replay()
+        assert torch.equal(warm[1], want)
+        step()
