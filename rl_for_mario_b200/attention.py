@@ -172,6 +172,13 @@ class FastDTAttention(nn.Module):
             object.__setattr__(self, "_fused_key", key)
         return self._fused_w
 
+    def renew_derived(self) -> None:
+        """Brings the weights derived from the parameters up to them, in place."""
+        if self._fused_w is not None:
+            self._fused_weight(self._fused_w.dtype)
+        if getattr(self, "_cat_w", None) is not None:
+            self._cat_weight(self._cat_w.dtype)
+
     def _qkv_rope_ok(self, x: Tensor) -> bool:
         """The one-GEMM q | k | v + RoPE path: 16-bit x [B, S, H] with a contiguous last
         dimension, no projection biases, head_dim 32 / 64, sizes multiples of 8."""

@@ -501,6 +501,14 @@ class MarioDT(nn.Module):
             layer.self_attn.fuse_training(on, seed, 1 + 3 * i)  # three sites a block; 0 is the embedding's
         return self
 
+    def renew_derived(self) -> None:
+        """Brings the weights that fused blocks and attention modules derive from the parameters up to them, in place, for
+        a captured graph that reads them (forward() does so by itself)."""
+        for layer in self.model.layers:
+            layer.self_attn.renew_derived()
+            if getattr(layer, "_swiglu_w", None) is not None:
+                layer._swiglu_weight(layer._swiglu_w.dtype)
+
     def adamw(self, lr: float = 1e-3, weight_decay: float = 1e-2, **kw) -> optim.AdamW:
         """AdamW over the model's parameters that train (optim.AdamW: further arguments go there); weights of
         products, convolutions and embeddings decay, norms' weights and biases do not."""

@@ -18,6 +18,7 @@ reference steps all environments with one action array, :408).
 """
 from __future__ import annotations
 
+from operator import attrgetter
 from typing import Optional
 
 import torch
@@ -27,6 +28,8 @@ from .cache import PagedKVCache
 from .dt_model import MarioDT
 
 Tensor = torch.Tensor
+
+_version_of = attrgetter("_version")
 
 
 def shard_range(num_envs: int, rank: int, world: int):
@@ -66,6 +69,9 @@ class DTRollout:
     t and replays it; later episodes only replay.  Cache lengths and the RoPE
     rows a step uses depend on the step index, hence one graph per index; the
     graphs share one memory pool and are always replayed in capture order.
+    They read the model's weights in place; weights derived from these (fused
+    norms) are renewed in place before a step when a parameter's version has
+    changed (MarioDT.weights_changed says so for writes PyTorch did not see).
     The all-gather of the logits, the action choice and the host's cache
     bookkeeping stay outside the graphs.  Inputs are copied into static
     buffers (``frame_buffer`` can be written in place by the environment to
@@ -100,6 +106,8 @@ class DTRollout:
         self._graphs = {}   # step index -> (CUDAGraph, host cache lengths after the step)
         self._pool = None
         self._static = None
+        self._params = [p for p in model.parameters() if not p.is_inference()]  # (those have no version)
+        self._versions = None  # theirs at the last step through a graph
 
     def reset(self) -> None:
         self.cache.reset()
@@ -155,7 +163,12 @@ class DTRollout:
         if self.episodes == 0:
             # First episode: eager, which also initialises every kernel and library.
             self._body(st, t == 0)
-        elif t not in self._graphs:
+            return st["logits"]
+        versions = list(map(_version_of, self._params))
+        if versions != self._versions:
+            self.model.renew_derived()
+            self._versions = versions
+        if t not in self._graphs:
             if self._pool is None:
                 self._pool = torch.cuda.graph_pool_handle()
             g = torch.cuda.CUDAGraph()
