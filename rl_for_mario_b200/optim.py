@@ -10,6 +10,7 @@ each replay.
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 import math
 import struct
@@ -402,16 +403,24 @@ class AdamW(torch.optim.Optimizer):
             if state[k].numel() != t.numel() or state[k].dtype != t.dtype:
                 raise ValueError(f"{k} of the state does not match: {tuple(state[k].shape)} {state[k].dtype}, "
                                  f"{tuple(t.shape)} {t.dtype} here")
-        packed = [{**{k: v for k, v in new.items() if k != "params"}, "params": g["params"]}
+        dev = self._buffers["count"].device
+        # What is loaded becomes this optimizer's own; a rate on the device keeps its place, where captured steps read it.
+        loaded = [{**copy.deepcopy({k: v for k, v in new.items() if k != "params"}), "params": g["params"]}
                   for g, new in zip(self.param_groups, groups)]
-        for g in packed:
-            self._pack_group(g, self._buffers["count"].device)
+        for new in loaded:
+            if isinstance(new["lr"], Tensor):
+                new["lr"] = new["lr"].to(dev)
+            self._pack_group(new, dev)
         for k, t in mine.items():
             t.copy_(state[k].reshape(-1))
         self.seed = int(state["seed"])
         self._buffers["count"][0].fill_(self.seed)
         self._buffers["count"][1].copy_(torch.as_tensor(state["step"], dtype=torch.int64))
-        for g, new in zip(self.param_groups, packed):
+        for g, new in zip(self.param_groups, loaded):
+            lr = g["lr"]
+            if isinstance(lr, Tensor):
+                lr.copy_(new["lr"].reshape(lr.shape)) if isinstance(new["lr"], Tensor) else lr.fill_(new["lr"])
+                new["lr"] = lr
             g.clear()
             g.update(new)
 
