@@ -345,9 +345,9 @@ class AdamW(torch.optim.Optimizer):
 
     def _group_bytes(self, i: int, g: dict, dev: torch.device) -> bytes:
         """_pack_group of group i, taken again when one of its numbers has changed."""
-        key = (g["lr"], g["betas"], g["eps"], g["weight_decay"])
-        if isinstance(key[0], Tensor):
+        if isinstance(g["lr"], Tensor):
             return self._pack_group(g, dev)
+        key = (g["lr"], *g["betas"], g["eps"], g["weight_decay"])  # (numbers: a list of betas may be changed in place)
         was, packed = self._packed[i]
         if was != key:
             packed = self._pack_group(g, dev)

@@ -65,3 +65,26 @@ def test_a_step_between_a_forward_pass_and_its_backward_pass_is_an_error(calls):
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("make", [list, tuple])
+def test_every_step_takes_the_groups_numbers_as_they_are(calls, make):
+    ps = params(3, 4)
+    ps[0].grad, ps[1].grad = torch.ones(3), torch.ones(4)
+    opt = optim.AdamW([dict(params=[ps[0]], betas=make((0.9, 0.99))), dict(params=[ps[1]])], betas=make((0.8, 0.98)))
+    opt.step()
+    group = opt.param_groups[0]
+    if make is list:
+        group["betas"][0] = 0.5
+    else:
+        group["betas"] = (0.5, 0.99)
+    opt.step()
+    group["lr"], group["eps"], group["weight_decay"] = 0.25, 1e-3, 0.125
+    opt.step()
+    first = [c["groups"][0][:5] for c in calls]
+    assert first == [(1e-3, 0.9, 0.99, 1e-8, 1e-2), (1e-3, 0.5, 0.99, 1e-8, 1e-2), (0.25, 0.5, 0.99, 1e-3, 0.125)]
+    assert all(c["groups"][1][:5] == (1e-3, 0.8, 0.98, 1e-8, 1e-2) for c in calls)
+    group["betas"] = make((1.0, 0.99))
+    with pytest.raises(ValueError, match="betas"):
+        opt.step()
+    assert len(calls) == 3
