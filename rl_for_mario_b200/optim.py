@@ -119,6 +119,7 @@ class AdamW(torch.optim.Optimizer):
         self._order: List[Tensor] = []  # parameters as they were added: the order of the flat arrays
         self._buffers: Dict[str, Tensor] = {}
         self._built = 0  # parameters that the arrays are made for
+        self._packed: List[Tuple[Optional[tuple], bytes]] = []  # of each group: its numbers, and these as bytes
         self.norm: Optional[Tensor] = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
@@ -136,6 +137,7 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
         self._order.extend(group["params"])
+        self._packed.append((None, b""))
 
     def _check_param(self, p: Tensor) -> None:
         if not p.is_cuda:
@@ -204,7 +206,6 @@ class AdamW(torch.optim.Optimizer):
         self._kinds = array("i", [kernels._dtype_code(p) + 256 * group[id(p)] for p in ps])
         self._plain = all(st is None for st in self._strides)
         self._look(list(map(_data_ptr, ps)))
-        self._packed = [(None, b"")] * len(self.param_groups)
 
     def _fill_master(self, master: Tensor, first: int) -> None:
         at = 0

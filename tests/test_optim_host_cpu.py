@@ -88,3 +88,17 @@ def test_every_step_takes_the_groups_numbers_as_they_are(calls, make):
     with pytest.raises(ValueError, match="betas"):
         opt.step()
     assert len(calls) == 3
+
+
+def test_a_group_without_parameters_added_later(calls):
+    ps = params(3, 4)
+    ps[0].grad, ps[1].grad = torch.ones(3), torch.ones(4)
+    opt = optim.AdamW([ps[0]])
+    opt.step()
+    opt.add_param_group(dict(params=[], lr=0.5))
+    opt.step()
+    assert [c["ngroups"] for c in calls] == [1, 2] and calls[1]["groups"][1][0] == 0.5
+    opt.add_param_group(dict(params=[ps[1]], lr=0.25))
+    opt.step()
+    assert calls[2]["ngroups"] == 3 and calls[2]["sizes"] == [3, 4] and calls[2]["groups"][2][0] == 0.25
+    assert [len(g["params"]) for g in opt.state_dict()["param_groups"]] == [1, 0, 1]
