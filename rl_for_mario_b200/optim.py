@@ -304,19 +304,19 @@ class AdamW(torch.optim.Optimizer):
         if not live:
             return None, None, live
         at = list(map(_data_ptr, ps))
+        # A parameter at its address of the last look is the same memory: that is held meanwhile.
+        if at != self._seen:
+            for i in range(len(ps)):
+                self._same(i)
+            self._overlap()
+            self._look(at)
         if (len(live) == len(ps) and self._plain and all(map(_contiguous, ps)) and all(map(_contiguous, grads))
                 and list(map(_dtype_of, grads)) == self._dtypes and list(map(_numel, grads)) == self._numels
                 and set(map(_on, grads)) == {index}):
-            # A parameter at its address of the last look is the same memory: that is held meanwhile.
-            if at != self._seen:
-                for i in range(len(ps)):
-                    self._same(i)
-                self._overlap()
-                self._look(at)
             return self._at, array("q", map(_data_ptr, grads)), grads
         keep: List[Tensor] = []
         to = array("q", [self._gradient(i, g, keep) for i, g in enumerate(grads)])
-        return array("q", at), to, keep
+        return self._at, to, keep
 
     def _look(self, at: List[int]) -> None:
         """Notes where the parameters are, and holds the memory there."""

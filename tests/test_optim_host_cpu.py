@@ -102,3 +102,29 @@ def test_a_group_without_parameters_added_later(calls):
     opt.step()
     assert calls[2]["ngroups"] == 3 and calls[2]["sizes"] == [3, 4] and calls[2]["groups"][2][0] == 0.25
     assert [len(g["params"]) for g in opt.state_dict()["param_groups"]] == [1, 0, 1]
+
+
+@pytest.mark.parametrize("how", ["all gradients", "one missing", "another order of memory"])
+def test_moved_parameters_that_share_memory_are_refused(calls, how):
+    ps = params(6, 5, 4)
+    if how == "another order of memory":
+        ps.append(torch.nn.Parameter(torch.ones(2, 3, 4, 5).to(memory_format=torch.channels_last)))
+    opt = optim.AdamW(ps)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    if how == "one missing":
+        ps[2].grad = None
+    pool = torch.zeros(64)
+    for p, at in zip(ps, (0, 5, 32)):  # the last element of the first is the first of the second
+        p.data = pool[at:at + p.numel()]
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
+    assert len(calls) == 1
+    for p, at in zip(ps, (0, 6, 32)):
+        p.data = pool[at:at + p.numel()]
+    opt.step()
+    assert len(calls) == 2 and calls[1]["at"][:3] == [pool.data_ptr() + 4 * n for n in (0, 6, 32)]
+    ps[1].data = torch.zeros(7)
+    with pytest.raises(ValueError, match="changed"):
+        opt.step()
