@@ -46,7 +46,7 @@ def _dense(t: Tensor) -> bool:
 # Each of these looks at one property of many tensors without an interpreted loop: a model has a hundred
 # tensors, and a microsecond for each would be more than the kernels take.
 _data_ptr, _numel, _contiguous, _on = (getattr(Tensor, n) for n in ("data_ptr", "numel", "is_contiguous", "get_device"))
-_dtype_of, _grad_of = attrgetter("dtype"), attrgetter("grad")
+_dtype_of, _grad_of, _bytes = attrgetter("dtype"), attrgetter("grad"), attrgetter("nbytes")
 
 
 def _address(values: array) -> int:
@@ -201,6 +201,7 @@ class AdamW(torch.optim.Optimizer):
         group = {id(p): i for i, g in enumerate(self.param_groups) for p in g["params"]}
         self._dtypes = [p.dtype for p in ps]
         self._numels = [p.numel() for p in ps]
+        self._nbytes = list(map(_bytes, ps))
         self._strides = [None if p.is_contiguous() else p.stride() for p in ps]
         self._sizes = array("q", self._numels)
         self._kinds = array("i", [kernels._dtype_code(p) + 256 * group[id(p)] for p in ps])
@@ -287,7 +288,7 @@ class AdamW(torch.optim.Optimizer):
                         kernels._ptr(ws), size)
         # The launch writes through addresses: PyTorch has to be told, as autograd's check of saved tensors and every
         # weight derived from these (a model's folded norms) go by the version.  (7 us for 125 tensors.)
-        torch.autograd.graph.increment_version([p for p, g in zip(ps, to) if g])
+        torch.autograd.graph.increment_version(ps if 0 not in to else [p for p, g in zip(ps, to) if g])
         return loss
 
     def weights_changed(self) -> None:
@@ -304,13 +305,14 @@ class AdamW(torch.optim.Optimizer):
         if not live:
             return None, None, live
         at = list(map(_data_ptr, ps))
-        # A parameter at its address of the last look is the same memory: that is held meanwhile.
+        # Nothing is held of a parameter's memory: other memory may stand at its address of the last look.
         if at != self._seen:
             for i in range(len(ps)):
                 self._same(i)
             self._overlap()
             self._look(at)
-        if (len(live) == len(ps) and self._plain and all(map(_contiguous, ps)) and all(map(_contiguous, grads))
+        if (len(live) == len(ps) and self._plain and list(map(_bytes, ps)) == self._nbytes
+                and all(map(_contiguous, ps)) and all(map(_contiguous, grads))
                 and list(map(_dtype_of, grads)) == self._dtypes and list(map(_numel, grads)) == self._numels
                 and set(map(_on, grads)) == {index}):
             return self._at, array("q", map(_data_ptr, grads)), grads
@@ -319,8 +321,8 @@ class AdamW(torch.optim.Optimizer):
         return self._at, to, keep
 
     def _look(self, at: List[int]) -> None:
-        """Notes where the parameters are, and holds the memory there."""
-        self._seen, self._at, self._held = at, array("q", at), [p.detach() for p in self._order]
+        """Notes where the parameters are."""
+        self._seen, self._at = at, array("q", at)
 
     def _same(self, i: int) -> Tensor:
         """Parameter i, whose type, size, order of memory and device have to be those of the flat arrays."""

@@ -128,3 +128,36 @@ def test_moved_parameters_that_share_memory_are_refused(calls, how):
     ps[1].data = torch.zeros(7)
     with pytest.raises(ValueError, match="changed"):
         opt.step()
+
+
+def test_memory_that_a_parameter_left_is_given_back(calls):
+    import weakref
+
+    ps = params(6, 5)
+    opt = optim.AdamW(ps)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    old = weakref.ref(ps[0].data.untyped_storage())
+    assert old() is not None
+    ps[0].data = torch.zeros(6)  # as a model that is moved elsewhere
+    assert old() is None
+
+
+@pytest.mark.parametrize("how", ["smaller", "larger type"])
+def test_a_parameter_of_another_size_at_its_old_address_is_refused(calls, how, monkeypatch):
+    """What was there may have been given back and handed out anew: an address alone says nothing."""
+    pool = torch.ones(64)
+    p = torch.nn.Parameter(pool[:8] if how == "smaller" else pool[:8].view(torch.bfloat16)[:8])
+    opt = optim.AdamW([p])
+    p.grad = torch.ones_like(p)
+    monkeypatch.setattr(optim, "_on", lambda t: None)  # (a CPU tensor's index is not None)
+    opt._ready()
+    opt._addresses(opt._order, None)
+    g = p.grad
+    p.grad = None
+    p.data = pool[:4] if how == "smaller" else pool[:8]
+    monkeypatch.setattr(optim, "_grad_of", lambda t: g)
+    assert p.data_ptr() == pool.data_ptr()
+    with pytest.raises(ValueError, match="changed"):
+        opt._addresses(opt._order, None)
