@@ -230,25 +230,6 @@ class AdamW(torch.optim.Optimizer):
             self._build()
 
     # --------------------------------------------------------------------------- step
-    def _odd(self, i: int, keep: list) -> Tuple[int, int]:
-        """Addresses of parameter i and its gradient where they are not both as they mostly are."""
-        p, g = self._order[i], self._order[i].grad
-        if p.dtype != self._dtypes[i] or p.numel() != self._numels[i] or not p.is_cuda or \
-                p.device != self._buffers["count"].device or \
-                (None if p.is_contiguous() else p.stride()) != self._strides[i]:
-            raise ValueError(f"parameter {i} has changed its type, size, strides or device")
-        if g is None:
-            return p.data_ptr(), 0
-        if g.layout is not torch.strided:
-            raise TypeError("AdamW takes dense gradients")
-        if g.dtype != p.dtype or g.shape != p.shape or g.device != p.device:
-            raise ValueError(f"the gradient of parameter {i} does not match it")
-        if g.stride() != p.stride():
-            own = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device)
-            g = own.copy_(g)
-            keep.append(own)
-        return p.data_ptr(), g.data_ptr()
-
     def step(self, closure=None):
         # torch wraps an optimizer's step to run its hooks and mark it for the profiler, which takes 15 us; that
         # wrapper is used where there is a hook or a profiler to serve.
