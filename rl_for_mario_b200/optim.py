@@ -367,15 +367,30 @@ class AdamW(torch.optim.Optimizer):
 
     def state_dict(self) -> dict:
         """{"state": seed, step and the flat arrays themselves, "param_groups": as torch's}."""
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
         self._ready()
         number = {id(p): i for i, p in enumerate(p for g in self.param_groups for p in g["params"])}
         groups = [{**{k: v for k, v in g.items() if k != "params"}, "params": [number[id(p)] for p in g["params"]]}
                   for g in self.param_groups]
         state = {k: v for k, v in self._buffers.items() if k not in ("count", "ticket", "parts")}
-        return {"state": {"seed": self.seed, "step": self._buffers["count"][1], **state}, "param_groups": groups}
+        result = {"state": {"seed": self.seed, "step": self._buffers["count"][1], **state}, "param_groups": groups}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            other = hook(self, result)
+            result = result if other is None else other
+        return result
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        state_dict = dict(state_dict)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            other = hook(self, state_dict)
+            state_dict = state_dict if other is None else other
+        self._load(state_dict)
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     @torch.no_grad()
-    def load_state_dict(self, state_dict: dict) -> None:
+    def _load(self, state_dict: dict) -> None:
         self._ready()
         state, groups = state_dict["state"], state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:

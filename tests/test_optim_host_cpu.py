@@ -161,3 +161,21 @@ def test_a_parameter_of_another_size_at_its_old_address_is_refused(calls, how, m
     assert p.data_ptr() == pool.data_ptr()
     with pytest.raises(ValueError, match="changed"):
         opt._addresses(opt._order, None)
+
+
+def test_hooks_of_saving_and_loading_are_called(calls):
+    ps = params(3)
+    opt = optim.AdamW(ps, lr=0.5)
+    seen = []
+    handles = [opt.register_state_dict_pre_hook(lambda o: seen.append(("save", o))),
+               opt.register_state_dict_post_hook(lambda o, s: {**s, "more": 7}),
+               opt.register_load_state_dict_pre_hook(lambda o, s: {k: v for k, v in s.items() if k != "more"}),
+               opt.register_load_state_dict_pre_hook(lambda o, s: s["param_groups"][0].update(lr=0.125)),
+               opt.register_load_state_dict_post_hook(lambda o: seen.append(("load", o)))]
+    saved = opt.state_dict()
+    assert saved["more"] == 7 and seen == [("save", opt)]
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 0.125 and seen == [("save", opt), ("load", opt)] and saved["more"] == 7
+    for h in handles:
+        h.remove()
+    assert "more" not in opt.state_dict() and len(seen) == 2
