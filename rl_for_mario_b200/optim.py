@@ -424,7 +424,10 @@ class AdamW(torch.optim.Optimizer):
             g.update(new)
 
     def __getstate__(self) -> dict:
-        return self.__dict__.copy()
+        """All but hooks and a step() that a scheduler put in the class's place, which belong to this object: a copy
+        starts without them, as a copy of torch's optimizers does."""
+        return {k: v for k, v in self.__dict__.items()
+                if k != "step" and not (k.startswith("_optimizer_") and k.endswith("_hooks"))}
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

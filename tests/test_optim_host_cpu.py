@@ -1,6 +1,8 @@
 """The optimizer's host side on CPU tensors: its launch is replaced by writes through the addresses that the entry
 point gets, as the kernel's are.  (AdamW refuses CPU parameters; the check is taken out here.)"""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -179,3 +181,35 @@ def test_hooks_of_saving_and_loading_are_called(calls):
     for h in handles:
         h.remove()
     assert "more" not in opt.state_dict() and len(seen) == 2
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_a_copy_is_an_optimizer_of_its_own(calls, how):
+    """With a scheduler, which replaces step() of the object, and hooks that cannot be pickled."""
+    ps = params(6, 5)
+    opt = optim.AdamW([dict(params=[ps[0]], betas=[0.9, 0.99]), dict(params=[ps[1]])], lr=0.5)
+    torch.optim.lr_scheduler.LambdaLR(opt, lambda t: 1.0)
+    seen = []
+    opt.register_step_post_hook(lambda *x: seen.append("step"))
+    opt.register_state_dict_pre_hook(lambda *x: seen.append("save"))
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    other = copy.deepcopy(opt) if how == "deepcopy" else pickle.loads(pickle.dumps(opt))
+    qs = [p for g in other.param_groups for p in g["params"]]
+    assert seen == ["step"] and len(calls) == 1
+    for q in qs:
+        assert all(q is not p for p in ps)
+        q.grad = torch.full_like(q, 0.5)
+    other.param_groups[0]["betas"][0] = 0.75
+    other.step()
+    assert seen == ["step"] and len(calls) == 2
+    assert calls[1]["at"] == [q.data_ptr() for q in qs] and calls[1]["groups"][0][1] == 0.75
+    assert all((p == 0).all() for p in ps) and all((q == -0.5).all() for q in qs)
+    other.state_dict()
+    opt.step()
+    assert seen == ["step", "step"] and calls[2]["at"] == [p.data_ptr() for p in ps]
+    assert calls[2]["groups"][0][1] == 0.9
+    with torch.no_grad():
+        other.moments()[0].fill_(3.0)
+    assert not (opt.moments()[0] == 3).any()
