@@ -23,10 +23,11 @@
 // A v above zero never becomes zero, so that no m is divided by eps alone.
 //
 // Bound by HBM: an element of a bf16 weight costs 22 bytes with 32-bit averages, 10 with 8-bit ones, 28 with 32-bit
-// averages and fp32 weights beside it.  81.3 M weights in 125 tensors, inputs cold: 32-bit averages 292 us in bf16
-// (6.1 TB/s), 383 in fp32 (28 bytes, 5.9), 386 in bf16 with fp32 weights (5.9); 8-bit ones 216 us with fp32 weights
-// beside bf16 ones (16 bytes, 6.0), 212 in fp32 (6.1), 171 to 175 in bf16 alone (4.7 TB/s): there the codes' integer
-// work, some 50 issue slots an element, takes as long as the bytes (issue slots 60 % in use, the ALU pipe 45 %).
+// averages and fp32 weights beside it.  81.3 M weights in 125 tensors, inputs cold: 32-bit averages 293 us in bf16
+// (6.1 TB/s), 385 in fp32 (28 bytes, 5.9), 387 in bf16 with fp32 weights (5.9); 8-bit ones 215 us with fp32 weights
+// beside bf16 ones (16 bytes, 6.0), 213 in fp32 (6.1), 174 in bf16 alone (4.7 TB/s): there the codes' work, 375 warp
+// instructions a block of 256 elements, takes 63 % of the issue slots and 50 % of the ALU pipe with 18 warps on an SM,
+// and a warp waits for its loads in 2.1 of the 7 cycles between two of its instructions.
 #include <cstring>
 #include <type_traits>
 
@@ -41,8 +42,8 @@ namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 // Blocks on an SM.  Norm, 81.3 M bf16 numbers: 41 us with 8, 45 with 6, 45 with 12 (spills).  Step: what leaves the loads of
-// two blocks their registers; 32-bit averages, bf16 weights: 292 us with 4, 300 with 6; 8-bit ones 175 with 5, 184
-// to 187 with 6 (spills), 192 to 197 with 4.
+// two blocks their registers; 32-bit averages, bf16 weights: 292 us with 4, 300 with 6; 8-bit ones 175 with 5 (12 bytes
+// of spills), 184 to 187 with 6 (more), 192 to 197 with 4.
 constexpr int kNormResident = 8;
 template <bool BITS8, bool MASTER = false>
 constexpr int kStepResident = BITS8 && !MASTER ? 5 : 4;

@@ -16,9 +16,9 @@
 // one.  A head is held by a group of G lanes (a power of two), a few pairs (i, i + h) a lane,
 // so that the rotation needs no exchange; the row sums are log2 G shuffles.  A group walks
 // through some heads of one position with the position's table row in registers.
-// 96 x 768 positions of 12 / 4 heads of 64, inputs cold: bf16 53 us forward (302 MB, 5.7
-// TB/s) and 85 backward (453 MB, 5.3 TB/s), half the batch in fp32 49 and 73 (6.2 TB/s).  In
-// 16 bits 55 % of the issue slots are in use and warps wait for the table rows.
+// 96 x 768 positions of 12 / 4 heads of 64, inputs cold: bf16 51 us forward (302 MB, 5.9
+// TB/s) and 82 backward (453 MB, 5.5 TB/s), half the batch in fp32 47 and 70 (6.4 TB/s).  In
+// 16 bits 55 % of the issue slots are in use, and most of what a warp waits for are loads from memory.
 #include <type_traits>
 
 #include "dt_common.cuh"
@@ -30,8 +30,9 @@ namespace dtk {
 namespace {
 
 constexpr int kThreads = 256;
-// Blocks on an SM: as many as the registers allow without spilling (forward with 2: 67 us instead of 61, 4: 84; backward
-// with 3: 199 instead of 94).
+// Blocks on an SM.  96 x 768, 12 / 4 heads of 64, bf16: forward 51 us with 3, 55 with 2, 76 with 4; backward 82 with 2, 96
+// with 1, 193 with 3.  (With 2 the 16-bit gradients of 16-byte accesses spill 8 to 12 bytes a thread, those of single
+// elements 12; nothing else does.)
 template <bool BWD>
 constexpr int kResident = BWD ? 2 : 3;
 
@@ -247,8 +248,9 @@ __global__ void __launch_bounds__(kThreads, kResident<BWD>) head_norm_any_kernel
 // Lane c of a group holds elements P c .. P c + P - 1 and the same from h on: two accesses of 16 bytes
 // (P = 8, fp32 4), or of 8 for 16-bit heads whose halves are not whole 16-byte vectors (P = 4).  A head's elements are copied into the lane's own places of a ring in shared memory,
 // kDepth heads ahead and across positions, and only the lane reads them back: no barrier, and what is in
-// flight takes no registers (one head ahead in registers: 107 + 178 us where this took 66 + 99).  Two heads ahead: with
-// four, and three, 61 + 94 us instead of 57 + 90, as the ring's memory is L1's, which holds table rows.
+// flight takes no registers (one head ahead in registers: 107 + 178 us at 96 x 768, 12 / 4 heads of 64, bf16, when a
+// first ring took 66 + 99).  Two heads ahead: 51 + 82 us there, half the batch in fp32 47 + 70; one 59 + 86 and 51 + 80;
+// three and four 51 + 82 and 47 + 72.
 template <int DT, int P>
 using Vec = typename std::conditional<P * (DT == 2 ? 4 : 2) == 16, uint4, uint2>::type;
 constexpr int kDepth = 2;

@@ -269,7 +269,7 @@ class AdamW(torch.optim.Optimizer):
                         kernels._ptr(ws), size)
         # The launch writes through addresses: PyTorch has to be told, as autograd's check of saved tensors and every
         # weight derived from these (a model's folded norms) go by the version.  (7 us for 125 tensors.)
-        torch.autograd.graph.increment_version(ps if 0 not in to else [p for p, g in zip(ps, to) if g])
+        torch.autograd.graph.increment_version(ps if all(to) else [p for p, g in zip(ps, to) if g])
         return loss
 
     def weights_changed(self) -> None:
@@ -296,7 +296,7 @@ class AdamW(torch.optim.Optimizer):
                 and all(map(_contiguous, ps)) and all(map(_contiguous, grads))
                 and list(map(_dtype_of, grads)) == self._dtypes and list(map(_numel, grads)) == self._numels
                 and set(map(_on, grads)) == {index}):
-            return self._at, array("q", map(_data_ptr, grads)), grads
+            return self._at, array("q", list(map(_data_ptr, grads))), grads
         keep: List[Tensor] = []
         to = array("q", [self._gradient(i, g, keep) for i, g in enumerate(grads)])
         return self._at, to, keep
@@ -381,6 +381,8 @@ class AdamW(torch.optim.Optimizer):
         return result
 
     def load_state_dict(self, state_dict: dict) -> None:
+        """Takes copies of what state_dict() gave, from any device; a group's rate that is a tensor here takes the loaded
+        value where it is.  Nothing is changed where the state does not fit."""
         state_dict = dict(state_dict)
         for hook in self._optimizer_load_state_dict_pre_hooks.values():
             other = hook(self, state_dict)
@@ -410,11 +412,12 @@ class AdamW(torch.optim.Optimizer):
             if isinstance(new["lr"], Tensor):
                 new["lr"] = new["lr"].to(dev)
             self._pack_group(new, dev)
+        seed, step = int(state["seed"]), torch.as_tensor(state["step"], dtype=torch.int64).reshape(())
         for k, t in mine.items():
             t.copy_(state[k].reshape(-1))
-        self.seed = int(state["seed"])
-        self._buffers["count"][0].fill_(self.seed)
-        self._buffers["count"][1].copy_(torch.as_tensor(state["step"], dtype=torch.int64))
+        self.seed = seed
+        self._buffers["count"][0].fill_(seed)
+        self._buffers["count"][1].copy_(step)
         for g, new in zip(self.param_groups, loaded):
             lr = g["lr"]
             if isinstance(lr, Tensor):
