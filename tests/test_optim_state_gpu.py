@@ -91,3 +91,45 @@ def test_a_rate_that_is_refused_changes_nothing():
         with pytest.raises(ValueError, match="lr"):
             a.load_state_dict(saved)
         assert a.param_groups[0]["lr"] == 0.1 and not (a.moments()[0] == 7).any()
+
+
+def pair(*lr, **kw):
+    """An optimizer of two groups with these rates (one: shared)."""
+    from rl_for_mario_b200 import optim
+
+    ps = [torch.nn.Parameter(torch.ones(5, device="cuda")) for _ in range(2)]
+    if len(lr) == 1:
+        return optim.AdamW([dict(params=[p]) for p in ps], lr=lr[0])
+    return optim.AdamW([dict(params=[p], lr=x) for p, x in zip(ps, lr)])
+
+
+@pytest.mark.parametrize("where", ["cuda", "cpu"])
+def test_groups_that_share_a_rate(where):
+    def rates(o):
+        return [round(float(g["lr"]), 4) for g in o.param_groups]
+
+    def saved(o):
+        s = o.state_dict()
+        if where == "cpu":
+            f = io.BytesIO()
+            torch.save(s, f)
+            f.seek(0)
+            s = torch.load(f, map_location="cpu")
+        return s
+
+    shared, apart = saved(pair(rate(0.125))), saved(pair(rate(0.25), rate(0.5)))
+    for make in (lambda: pair(0.75), lambda: pair(rate(0.75))):
+        o = make()
+        o.load_state_dict(shared)
+        assert rates(o) == [0.125, 0.125]
+        o.param_groups[0]["lr"].fill_(0.0625)  # one rate still
+        assert rates(o) == [0.0625, 0.0625]
+        o = make()
+        o.load_state_dict(apart)
+        assert rates(o) == [0.25, 0.5]
+        o.param_groups[0]["lr"].fill_(1.0)
+        assert rates(o) == [1.0, 0.5]
+    o = pair(rate(0.75), rate(1.0))
+    own = [g["lr"] for g in o.param_groups]
+    o.load_state_dict(shared)
+    assert rates(o) == [0.125, 0.125] and all(g["lr"] is t for g, t in zip(o.param_groups, own))
